@@ -24,23 +24,12 @@ from typing import Optional
 
 import torch
 
-_PKG = os.path.dirname(os.path.abspath(__file__))
-LIB_PATH = os.path.join(_PKG, "libgdn_b200.so")
+from .native import GDN_DTYPE_BF16, GDN_DTYPE_F32, LIB_PATH, SYMBOLS, GdnError, _check, _check_cuda, _DT, load_library  # noqa: F401
 
-GDN_DTYPE_F32, GDN_DTYPE_BF16 = 0, 1
 IMPLS = {"auto": 0, "chunk": 1, "recurrent": 2, "segmented": 3, "chunk_cluster": 4, "chunk_single": 5, "chunk_split": 6}
 IMPL_NAMES = {1: "chunk", 2: "recurrent", 3: "segmented", 4: "chunk_cluster", 5: "chunk_single", 6: "chunk_split"}
 # impl values whose calls may need a workspace (gdn_prefill_workspace_bytes), allocated per call
 _WORKSPACE_IMPLS = ("auto", "segmented", "chunk_split")
-_DT = {torch.float32: GDN_DTYPE_F32, torch.bfloat16: GDN_DTYPE_BF16}
-
-
-class GdnError(RuntimeError):
-    """A gdn_status error returned by the native library."""
-
-    def __init__(self, status: int, msg: str):
-        super().__init__(f"gdn_b200 error {status}: {msg}")
-        self.status = status
 
 
 class Strides(ctypes.Structure):
@@ -149,8 +138,8 @@ class EpilogueBwdArgs(ctypes.Structure):
 
 GDN_PROLOGUE_CLAMP_LA = 1
 
-# Every symbol include/gdn_b200.h declares, with its ctypes signature.
-SYMBOLS = {
+# The gated-DeltaNet symbols of include/gdn_b200.h, with their ctypes signatures.
+SYMBOLS.update({
     "gdn_prefill_fwd": ([ctypes.POINTER(PrefillArgs), ctypes.c_void_p], ctypes.c_int),
     "gdn_decode_step": ([ctypes.POINTER(DecodeArgs), ctypes.c_void_p], ctypes.c_int),
     "gdn_prefill_workspace_bytes": ([ctypes.POINTER(PrefillArgs), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
@@ -167,33 +156,7 @@ SYMBOLS = {
     "gdn_prefill_bwd": ([ctypes.POINTER(BackwardArgs), ctypes.c_void_p], ctypes.c_int),
     "gdn_layer_prologue_bwd": ([ctypes.POINTER(PrologueBwdArgs), ctypes.c_void_p], ctypes.c_int),
     "gdn_layer_epilogue_bwd": ([ctypes.POINTER(EpilogueBwdArgs), ctypes.c_void_p], ctypes.c_int),
-}
-
-_LIB = None
-
-
-def load_library(path: str = LIB_PATH):
-    """Load libgdn_b200.so (built by ``python -m archbench_b200.build``); raises if absent."""
-    global _LIB
-    if _LIB is not None and path == LIB_PATH:
-        return _LIB
-    if not os.path.exists(path):
-        raise FileNotFoundError(f"{path} is missing: build it with `python -m archbench_b200.build`")
-    lib = ctypes.CDLL(path)
-    for name, (argtypes, restype) in SYMBOLS.items():
-        fn = getattr(lib, name)
-        fn.argtypes = argtypes
-        fn.restype = restype
-    if path == LIB_PATH:
-        _LIB = lib
-    return lib
-
-
-def _check(status: int):
-    if status != 0:
-        msg = load_library().gdn_status_string(status)
-        raise GdnError(status, msg.decode() if msg else "?")
-
+})
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
@@ -218,12 +181,6 @@ def _prep_token(t: torch.Tensor, name: str, dtype: torch.dtype) -> torch.Tensor:
     if t.stride(-1) != 1 or not _aligned16(t):
         t = t.contiguous()
     return t
-
-
-def _check_cuda(*ts):
-    for t in ts:
-        if t is not None and not t.is_cuda:
-            raise ValueError("archbench_b200 ops run on CUDA tensors only (no CPU path)")
 
 
 def prefill_args(q, k, v, la, beta=None, u=None, initial_state=None, output_final_state=False, out_dtype=None, impl="auto"):
@@ -988,3 +945,7 @@ class NsgdnMixerTrain(torch.autograd.Function):
         dconv = None if conv_w is None else torch.cat([w.t() for w in dws], 0).to(conv_w.dtype)
         return (dproj, dconv, dA.to(A_log.dtype), ddt.to(dt_bias.dtype), None if dbb is None else dbb.to(b_bias.dtype),
                 dnorm.to(norm_w.dtype), dlam, None)
+
+
+# Operators of the selective-state-space mixer; their modules add their entry points to SYMBOLS.
+from .ssm_ops import causal_conv, causal_conv_step, selective_scan, selective_scan_step  # noqa: E402,F401

@@ -1,0 +1,349 @@
+"""Operators of a selective-state-space mixer on the library's CUDA kernels (``include/gdn_b200.h``): the depthwise
+causal convolution, the selective scan and their one-token forms.
+
+  causal_conv(x, weight, bias=None, activation=None, initial_state=None, output_final_state=False, lengths=None)
+      -> (y, final_state | None)
+  causal_conv_step(x, weight, state, bias=None, activation=None) -> y                      (state in place)
+  selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None,
+                 output_final_state=False, lengths=None) -> (y, final_state | None)
+  selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False) -> y  (state in place)
+
+All are reachable as ``archbench_b200.ops.<name>``.  CUDA tensors only, bf16 or fp32 token tensors with any strides;
+states and sums are fp32.  Calls that need gradients run the backward kernels through autograd (first order).  Under
+``torch.compile`` the calls run eagerly between compiled regions."""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .native import SYMBOLS, _check, _check_cuda, _DT, load_library
+
+ACT = {None: 0, "silu": 1, "gelu": 2}
+SCAN_CKPT = 16  # GDN_SCAN_CKPT
+
+
+class ConvArgs(ctypes.Structure):
+    """Mirror of gdn_conv_args (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "state_in", "state_out", "y", "lengths")] + \
+               [(n, ctypes.c_int64) for n in ("sx_b", "sx_t", "sy_b", "sy_t", "B", "T", "C")] + \
+               [(n, ctypes.c_int32) for n in ("width", "act", "dtype", "w_dtype")]
+
+
+class ConvBwdArgs(ctypes.Structure):
+    """Mirror of gdn_conv_bwd_args (include/gdn_b200.h)."""
+
+    _fields_ = [("fwd", ConvArgs), ("dy", ctypes.c_void_p), ("sdy_b", ctypes.c_int64), ("sdy_t", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("dstate_out", "dx", "dstate_in", "dweight", "dbias", "workspace")] + \
+               [("workspace_bytes", ctypes.c_uint64)]
+
+
+class ScanArgs(ctypes.Structure):
+    """Mirror of gdn_scan_args (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "dt", "Bm", "Cm", "z", "A", "Dskip", "dt_bias", "h0", "lengths",
+                                                 "y", "h_out", "ckpt")] + \
+               [(n, ctypes.c_int64) for n in ("sx_b", "sx_t", "sdt_b", "sdt_t", "sB_b", "sB_t", "sB_g", "sC_b", "sC_t", "sC_g",
+                                                "sz_b", "sz_t", "sy_b", "sy_t", "B", "T", "D", "N", "G")] + \
+               [("dtype", ctypes.c_int32), ("softplus", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ScanBwdArgs(ctypes.Structure):
+    """Mirror of gdn_scan_bwd_args (include/gdn_b200.h)."""
+
+    _fields_ = [("fwd", ScanArgs), ("dy", ctypes.c_void_p), ("sdy_b", ctypes.c_int64), ("sdy_t", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("dh_out", "dx", "ddt", "dB", "dC", "dz", "dA", "dDskip", "ddt_bias", "dh0")]
+
+
+_P, _SZ = ctypes.POINTER, ctypes.POINTER(ctypes.c_size_t)
+SYMBOLS.update({
+    "gdn_conv_fwd": ([_P(ConvArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdn_conv_step": ([_P(ConvArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdn_conv_bwd_workspace_bytes": ([_P(ConvBwdArgs), _SZ], ctypes.c_int),
+    "gdn_conv_bwd": ([_P(ConvBwdArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdn_scan_workspace_bytes": ([_P(ScanArgs), _SZ], ctypes.c_int),
+    "gdn_scan_fwd": ([_P(ScanArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdn_scan_step": ([_P(ScanArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdn_scan_bwd_workspace_bytes": ([_P(ScanBwdArgs), _SZ], ctypes.c_int),
+    "gdn_scan_bwd": ([_P(ScanBwdArgs), ctypes.c_void_p], ctypes.c_int),
+})
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def launch(name: str, args, device: torch.device, need=None) -> None:
+    """Run a library entry point on ``device``'s current stream; ``need`` names the entry point that sizes the workspace
+    of ``args`` (or of its ``fwd`` member), taken from torch's allocator for the call."""
+    lib = load_library()
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return launch(name, args, device, need)
+    ws = None
+    if need is not None:
+        n = ctypes.c_size_t(0)
+        _check(getattr(lib, need)(ctypes.byref(args), ctypes.byref(n)))
+        if n.value:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+            holder = args if hasattr(args, "workspace") else args.fwd
+            holder.workspace, holder.workspace_bytes = ws.data_ptr(), n.value
+    status = getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        _check(status)
+
+
+def _token(t: torch.Tensor, name: str, shape, dtype, device) -> torch.Tensor:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _dense(t: Optional[torch.Tensor], name: str, shape, dtype, device) -> Optional[torch.Tensor]:
+    return None if t is None else _token(t, name, shape, dtype, device).contiguous()
+
+
+def _dtype_of(x: torch.Tensor, name: str):
+    _check_cuda(x)
+    if x.dtype not in _DT:
+        raise ValueError(f"{name} must be float32 or bfloat16, got {x.dtype}")
+    return x.dtype
+
+
+def _lengths(lengths, B: int, device) -> Optional[torch.Tensor]:
+    if lengths is None:
+        return None
+    if lengths.is_floating_point() or tuple(lengths.shape) != (B,) or lengths.device != device:
+        raise ValueError(f"lengths must be an integer tensor of shape ({B},) on {device}")
+    return lengths.to(torch.int32).contiguous()
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ---- causal convolution -----------------------------------------------------------------------
+
+
+def _conv_args(x, weight, bias, state, act, lengths, y=None, state_out=None) -> ConvArgs:
+    tok = x.dim() == 3
+    B, T, C = x.shape if tok else (x.shape[0], 1, x.shape[1])
+    st = lambda t: (t.stride(0), t.stride(1) if tok else 0) if t is not None else (0, 0)
+    return ConvArgs(_p(x), _p(weight), _p(bias), _p(state), _p(state_out), _p(y), _p(lengths), *st(x), *st(y), B, T, C,
+                    weight.shape[1], act, _DT[x.dtype], _DT[weight.dtype])
+
+
+def _conv_forward(x, weight, bias, state, act, want_state, lengths):
+    B, T, C = x.shape
+    y = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
+    out = torch.empty(B, C, weight.shape[1] - 1, device=x.device, dtype=x.dtype) if want_state else None
+    launch("gdn_conv_fwd", _conv_args(x, weight, bias, state, act, lengths, y, out), x.device)
+    return y, out
+
+
+class _Conv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, act, want_state, lengths):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.act = act
+        return _conv_forward(x, weight, bias, state, act, want_state, lengths)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        B, T, C = x.shape
+        if dy is None and dlast is None:
+            return (None,) * 7
+        if x.numel() == 0:
+            dstate = None if state is None else torch.zeros_like(state) if dlast is None else dlast
+            return torch.zeros_like(x), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate, None, None, None
+        dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.device)
+        dlast = None if dlast is None else dlast.contiguous()
+        dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
+        dw = torch.empty_like(weight)
+        db = None if bias is None else torch.empty_like(bias)
+        ds = None if state is None else torch.empty_like(state)
+        a = ConvBwdArgs(_conv_args(x, weight, bias, state, ctx.act, lengths), _p(dy), dy.stride(0), dy.stride(1), _p(dlast), _p(dx),
+                        _p(ds), _p(dw), _p(db), None, 0)
+        launch("gdn_conv_bwd", a, x.device, need="gdn_conv_bwd_workspace_bytes")
+        return dx, dw, db, ds, None, None, None
+
+
+def _conv_params(weight, bias, C, device):
+    if weight.dim() == 3 and weight.shape[1] == 1:
+        weight = weight[:, 0]  # nn.Conv1d's (C, 1, W)
+    if weight.dim() != 2 or weight.shape[0] != C:
+        raise ValueError(f"weight must be ({C}, W) or ({C}, 1, W), got {tuple(weight.shape)}")
+    if not 2 <= weight.shape[1] <= 4:
+        raise ValueError(f"the convolution kernels serve widths 2 to 4, got {weight.shape[1]}")
+    if weight.dtype not in _DT:
+        raise ValueError(f"weight must be float32 or bfloat16, got {weight.dtype}")
+    weight = _dense(weight, "weight", weight.shape, weight.dtype, device)
+    return weight, _dense(bias, "bias", (C,), weight.dtype, device)
+
+
+def _act(activation, allowed):
+    if activation not in allowed:
+        raise ValueError(f"activation must be one of {allowed}, got {activation!r}")
+    return ACT[activation]
+
+
+@torch.compiler.disable
+def causal_conv(x, weight, bias=None, activation=None, initial_state=None, output_final_state=False, lengths=None):
+    """Depthwise causal convolution: y_t = act(bias + sum_w weight[:, w] x_{t-W+1+w}).
+
+    x (B, T, C); weight (C, W) or (C, 1, W), W 2 to 4; bias (C); activation None or "silu"; initial_state (B, C, W - 1),
+    the inputs before the first token (zeros if None); lengths (B): tokens of each right-padded row (y is 0 past them).
+    Returns (y, final_state or None), final_state the last W - 1 inputs, in x's dtype."""
+    dt = _dtype_of(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"x must be (B, T, C), got {tuple(x.shape)}")
+    B, T, C = x.shape
+    act = _act(activation, (None, "silu"))
+    x = _token(x, "x", x.shape, dt, x.device)
+    weight, bias = _conv_params(weight, bias, C, x.device)
+    state = _dense(initial_state, "initial_state", (B, C, weight.shape[1] - 1), dt, x.device)
+    lengths = _lengths(lengths, B, x.device)
+    if _wants_grad(x, weight, bias, state):
+        return _Conv.apply(x, weight, bias, state, act, bool(output_final_state), lengths)
+    return _conv_forward(x, weight, bias, state, act, bool(output_final_state), lengths)
+
+
+@torch.compiler.disable
+def causal_conv_step(x, weight, state, bias=None, activation=None):
+    """One token of ``causal_conv``: x (B, C), state (B, C, W - 1) contiguous, in x's dtype, advanced in place.  No
+    autograd."""
+    dt = _dtype_of(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x must be (B, C), got {tuple(x.shape)}")
+    B, C = x.shape
+    act = _act(activation, (None, "silu"))
+    x = _token(x, "x", x.shape, dt, x.device)
+    weight, bias = _conv_params(weight, bias, C, x.device)
+    if tuple(state.shape) != (B, C, weight.shape[1] - 1) or state.dtype != dt or not state.is_contiguous() or state.device != x.device:
+        raise ValueError(f"state must be a contiguous {(B, C, weight.shape[1] - 1)} {dt} tensor on {x.device}: it is updated in place")
+    y = torch.empty(B, C, device=x.device, dtype=dt)
+    launch("gdn_conv_step", _conv_args(x, weight, bias, state, act, None, y), x.device)
+    return y
+
+
+# ---- selective scan ---------------------------------------------------------------------------
+
+
+def _scan_args(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y=None, h_out=None, ckpt=None) -> ScanArgs:
+    tok = x.dim() == 3
+    st = lambda t: (t.stride(0), t.stride(1) if tok else 0) if t is not None else (0, 0)
+    st3 = lambda t: (t.stride(0), t.stride(1) if tok else 0, t.stride(-2))
+    return ScanArgs(_p(x), _p(dt), _p(Bm), _p(Cm), _p(z), _p(A), _p(D), _p(bias), _p(h0), _p(lengths), _p(y), _p(h_out), _p(ckpt),
+                    *st(x), *st(dt), *st3(Bm), *st3(Cm), *st(z), *st(y), x.shape[0], x.shape[1] if tok else 1, x.shape[-1],
+                    A.shape[1], Bm.shape[-2], _DT[x.dtype], int(softplus), None, 0)
+
+
+def _scan_forward(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, want_state, train):
+    B, T, Dm = x.shape
+    N = A.shape[1]
+    y = torch.empty(B, T, Dm, device=x.device, dtype=x.dtype)
+    h = torch.empty(B, Dm, N, device=x.device, dtype=torch.float32) if want_state else None
+    ckpt = torch.empty(B, (T + SCAN_CKPT - 1) // SCAN_CKPT, Dm, N, device=x.device, dtype=torch.float32) if train else None
+    launch("gdn_scan_fwd", _scan_args(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y, h, ckpt), x.device,
+           need="gdn_scan_workspace_bytes")
+    return y, h, ckpt
+
+
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, want_state):
+        ctx.set_materialize_grads(False)
+        y, h, ckpt = _scan_forward(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, want_state, True)
+        ctx.save_for_backward(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ckpt)
+        ctx.softplus = softplus
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ckpt = ctx.saved_tensors
+        if dy is None and dh is None:
+            return (None,) * 12
+        new = lambda t: None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+        if x.numel() == 0:
+            zero = [None if t is None else torch.zeros_like(t) for t in (x, dt, A, Bm, Cm, D, z, bias)]
+            return (*zero, None if h0 is None else torch.zeros_like(h0) if dh is None else dh, None, None, None)
+        dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.device)
+        dh = None if dh is None else dh.contiguous()
+        dx, ddt, dA, dB, dC, dD, dz, db, dh0 = (new(t) for t in (x, dt, A, Bm, Cm, D, z, bias, h0))
+        a = ScanBwdArgs(_scan_args(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ctx.softplus, ckpt=ckpt), _p(dy), dy.stride(0), dy.stride(1),
+                        _p(dh), _p(dx), _p(ddt), _p(dB), _p(dC), _p(dz), _p(dA), _p(dD), _p(db), _p(dh0))
+        launch("gdn_scan_bwd", a, x.device, need="gdn_scan_bwd_workspace_bytes")
+        return dx, ddt, dA, dB, dC, dD, dz, db, dh0, None, None, None
+
+
+def _scan_inputs(x, dt, A, B, C, D, z, dt_bias):
+    """Checked inputs: token tensors in x's dtype with unit last strides, B and C (..., G, N), parameters fp32."""
+    ty, dev, tok, Dm = _dtype_of(x, "x"), x.device, x.shape[:-1], x.shape[-1]
+    if A.dim() != 2 or A.shape[0] != Dm:
+        raise ValueError(f"A must be ({Dm}, N), got {tuple(A.shape)}")
+    N = A.shape[1]
+    if not 1 <= N <= 64:
+        raise ValueError(f"the scan kernels serve 1 to 64 states per channel, got {N}")
+    if B.dim() == x.dim():
+        B = B.unsqueeze(-2)
+    if C.dim() == x.dim():
+        C = C.unsqueeze(-2)
+    G = B.shape[-2] if B.dim() == x.dim() + 1 else 0
+    if G < 1 or Dm % G:
+        raise ValueError(f"B must be {(*tok, N)} or {(*tok, 'G', N)} with G a divisor of {Dm}, got {tuple(B.shape)}")
+    x = _token(x, "x", x.shape, ty, dev)
+    dt = _token(dt, "dt", x.shape, ty, dev)
+    B, C = _token(B, "B", (*tok, G, N), ty, dev), _token(C, "C", (*tok, G, N), ty, dev)
+    z = None if z is None else _token(z, "z", x.shape, ty, dev)
+    A = _dense(A, "A", (Dm, N), torch.float32, dev)
+    return x, dt, A, B, C, _dense(D, "D", (Dm,), torch.float32, dev), z, _dense(dt_bias, "dt_bias", (Dm,), torch.float32, dev)
+
+
+@torch.compiler.disable
+def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None, output_final_state=False,
+                   lengths=None):
+    """Selective state space scan over a block of tokens.
+
+        s_t = softplus(dt_t + dt_bias) (or dt_t + dt_bias);  h_t = exp(s_t A) h_{t-1} + s_t x_t B_t
+        y_t = (C_t . h_t + D x_t) silu(z_t)
+
+    x, dt, z (B, T, D); A (D, N), usually negative; B, C (B, T, N) or (B, T, G, N), group g serving D / G consecutive
+    channels; D, dt_bias (D); initial_state (B, D, N) fp32 (zeros if None); lengths (B): tokens of each right-padded row
+    (past them y is 0 and the state stays).  N <= 64.  Returns (y, final_state or None): y in x's dtype, the state fp32.
+    Training keeps one state per 16 tokens."""
+    if x.dim() != 3:
+        raise ValueError(f"x must be (B, T, D), got {tuple(x.shape)}")
+    x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
+    h0 = _dense(initial_state, "initial_state", (x.shape[0], x.shape[2], A.shape[1]), torch.float32, x.device)
+    lengths = _lengths(lengths, x.shape[0], x.device)
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
+        return _Scan.apply(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus), bool(output_final_state))
+    return _scan_forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus), bool(output_final_state), False)[:2]
+
+
+@torch.compiler.disable
+def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False):
+    """One token of ``selective_scan``: x, dt, z (B, D), B, C (B, N) or (B, G, N), state (B, D, N) fp32 contiguous,
+    advanced in place.  No autograd."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be (B, D), got {tuple(x.shape)}")
+    x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
+    want = (x.shape[0], x.shape[1], A.shape[1])
+    if tuple(state.shape) != want or state.dtype != torch.float32 or not state.is_contiguous() or state.device != x.device:
+        raise ValueError(f"state must be a contiguous {want} float32 tensor on {x.device}: it is updated in place")
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    launch("gdn_scan_step", _scan_args(x, dt, A, B, C, D, z, dt_bias, None, None, dt_softplus, y, state), x.device)
+    return y

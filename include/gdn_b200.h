@@ -418,6 +418,104 @@ const char* gdn_status_string(int status);
 /* GDN_B200_ABI_VERSION of the loaded library. */
 int gdn_abi_version(void);
 
+/* ---- selective state space mixer: short convolution, scan, single tokens -------------------- */
+
+/*
+ * Depthwise causal convolution, channels last, with an optional bias and SiLU:
+ *     p_t = bias + sum_{w < width} weight[:, w] x_{t - width + 1 + w},   y_t = act(p_t)
+ * x_{t < 0} comes from state_in (zeros when NULL): (B, C, width - 1), oldest first.  state_out gets the
+ * last width - 1 inputs.  With `lengths`, row b has min(max(lengths[b], 0), T) tokens: y is 0 past them and
+ * state_out ends at the last of them.  x and y have a unit channel stride; weight (C, width), bias (C) and the
+ * states are contiguous.  Any alignment; 16-byte aligned rows with C a multiple of the 16-byte vector are faster.
+ */
+typedef enum { GDN_ACT_NONE = 0, GDN_ACT_SILU = 1, GDN_ACT_GELU = 2 } gdn_act;
+
+typedef struct gdn_conv_args {
+  const void* x;        /* (B, T, C), dtype */
+  const void* weight;   /* (C, width), w_dtype */
+  const void* bias;     /* (C), w_dtype, or NULL */
+  const void* state_in; /* (B, C, width - 1), dtype, or NULL */
+  void* state_out;      /* (B, C, width - 1), dtype, or NULL; may not overlap state_in */
+  void* y;              /* (B, T, C), dtype */
+  const int32_t* lengths; /* (B) or NULL */
+  int64_t sx_b, sx_t, sy_b, sy_t;
+  int64_t B, T, C;
+  int32_t width;        /* 2, 3 or 4 */
+  int32_t act;          /* GDN_ACT_NONE or GDN_ACT_SILU */
+  int32_t dtype, w_dtype;
+} gdn_conv_args;
+
+int gdn_conv_fwd(const gdn_conv_args* args, void* stream);
+
+/* One token: x and y are (B, C) (sx_b, sy_b), state_in is advanced in place; T, lengths and state_out unused. */
+int gdn_conv_step(const gdn_conv_args* args, void* stream);
+
+/*
+ * Backward: `fwd` as in the forward (y and state_out unused); dy (B, T, C) with strides; dx contiguous.
+ * dweight and dbias are written in w_dtype from fp32 sums in a fixed order.
+ */
+typedef struct gdn_conv_bwd_args {
+  gdn_conv_args fwd;
+  const void* dy;          /* dtype */
+  int64_t sdy_b, sdy_t;
+  const void* dstate_out;  /* (B, C, width - 1), dtype, or NULL: gradient of state_out */
+  void* dx;                /* (B, T, C), dtype */
+  void* dstate_in;         /* (B, C, width - 1), dtype, or NULL */
+  void* dweight;           /* (C, width), w_dtype */
+  void* dbias;             /* (C), w_dtype, or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+} gdn_conv_bwd_args;
+
+int gdn_conv_bwd_workspace_bytes(const gdn_conv_bwd_args* args, size_t* bytes);
+int gdn_conv_bwd(const gdn_conv_bwd_args* args, void* stream);
+
+/*
+ * Selective scan.  Per row b, channel d with N states (fp32), group g = d / (D / G):
+ *     s_t = softplus(dt_t + dt_bias)  (or dt_t + dt_bias),   h_t = exp(s_t A) h_{t-1} + s_t x_t B_t[g]
+ *     y_t = (C_t[g] . h_t + Dskip x_t) silu(z_t)
+ * A (D, N), Dskip (D), dt_bias (D), h0 and h_out (B, D, N) are contiguous fp32; token tensors have a unit
+ * last stride.  `lengths` as for the convolution: y is 0 and the state stays past a row's tokens.
+ * `ckpt`, when not NULL, receives the state before every GDN_SCAN_CKPT-th token, (B, ceil(T / GDN_SCAN_CKPT),
+ * D, N), which the backward needs.  1 <= N <= 64, D a multiple of G.
+ */
+#define GDN_SCAN_CKPT 16
+
+typedef struct gdn_scan_args {
+  const void *x, *dt, *Bm, *Cm, *z; /* z may be NULL */
+  const float *A, *Dskip, *dt_bias, *h0; /* Dskip, dt_bias, h0 may be NULL */
+  const int32_t* lengths;
+  void* y;
+  float* h_out; /* may be NULL */
+  float* ckpt;  /* may be NULL */
+  int64_t sx_b, sx_t, sdt_b, sdt_t, sB_b, sB_t, sB_g, sC_b, sC_t, sC_g, sz_b, sz_t, sy_b, sy_t;
+  int64_t B, T, D, N, G;
+  int32_t dtype, softplus;
+  void* workspace; /* gdn_scan_workspace_bytes: few rows are split over time */
+  uint64_t workspace_bytes;
+} gdn_scan_args;
+
+int gdn_scan_workspace_bytes(const gdn_scan_args* args, size_t* bytes);
+int gdn_scan_fwd(const gdn_scan_args* args, void* stream);
+
+/* One token: x, dt, z, y are (B, D), Bm and Cm (B, G, N) (the _t strides unused); the state h_out is advanced in
+ * place (h0, ckpt, lengths unused). */
+int gdn_scan_step(const gdn_scan_args* args, void* stream);
+
+/* Backward: `fwd` as in the forward with `ckpt` filled and `workspace` of gdn_scan_bwd_workspace_bytes (y, h_out unused).  Gradients are contiguous; those of
+ * token tensors in dtype, the others fp32 sums in a fixed order. */
+typedef struct gdn_scan_bwd_args {
+  gdn_scan_args fwd;
+  const void* dy; /* (B, T, D), dtype */
+  int64_t sdy_b, sdy_t;
+  const float* dh_out; /* (B, D, N) or NULL: gradient of h_out */
+  void *dx, *ddt, *dB, *dC, *dz; /* dz NULL when z is */
+  float *dA, *dDskip, *ddt_bias, *dh0; /* the last three may be NULL */
+} gdn_scan_bwd_args;
+
+int gdn_scan_bwd_workspace_bytes(const gdn_scan_bwd_args* args, size_t* bytes);
+int gdn_scan_bwd(const gdn_scan_bwd_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
