@@ -161,14 +161,16 @@ int gdn_device_status(int* status, int reset) {
   if (!status) return GDN_ERR_NULL;
   int st = check_device();
   if (st != GDN_OK) return st;
-  int single = 0, pair = 0, prep = 0;
+  int single = 0, pair = 0, prep = 0, lin = 0;
   st = gdn_chunk_read_status(&single, reset);
   if (st != GDN_OK) return st;
   st = gdn_chunk_pair_read_status(&pair, reset);
   if (st != GDN_OK) return st;
   st = gdn_chunk_prep_read_status(&prep, reset);
   if (st != GDN_OK) return st;
-  *status = single != 0 ? single : (pair != 0 ? pair : prep);
+  st = gdn_linear_read_status(&lin, reset);
+  if (st != GDN_OK) return st;
+  *status = single != 0 ? single : pair != 0 ? pair : prep != 0 ? prep : lin;
   return GDN_OK;
 }
 

@@ -106,6 +106,7 @@ int gdn_chunk_pair_read_status(int* out, int reset);
 size_t gdn_chunk_prep_bytes(const gdn_prefill_args* a);
 int gdn_launch_chunk_prep(const gdn_prefill_args* a, void* prod, cudaStream_t stream);
 int gdn_chunk_prep_read_status(int* out, int reset);
+int gdn_linear_read_status(int* out, int reset);
 bool gdn_chunk_split_supported(const gdn_prefill_args* a);
 int gdn_launch_chunk_split(const gdn_prefill_args* a, const void* prod, int mode, int nseg, int seg_len, float* ws,
                            int ws_stride, cudaStream_t stream);

@@ -1,0 +1,694 @@
+// Matrix product with its epilogue, y = act(x W^T + b) + r, and its backward (bf16 operands, fp32 accumulation).
+//
+// One tcgen05 kernel serves the three products of a training step, C[M, N] = sum_k A[m, k] B[n, k] with either operand
+// stored k-contiguous or with its other index contiguous (K- or MN-major tiles):
+//   forward  y  = x W^T      A = x   (M, K)  k-contiguous     B = W (N, K)  k-contiguous
+//   backward dx = dp W       A = dp  (M, N)  k-contiguous     B = W (N, K)  contiguous along the output
+//            dW = dp^T x     A = dp  (M, N)  along the output  B = x (M, K)  along the output
+//
+// A persistent block computes 128 x BN tiles: one warp issues the TMA loads of 64-deep k blocks into a ring of stages,
+// one warp issues the MMAs, four warps read finished accumulators from tensor memory and run the epilogue while the
+// MMAs of the next tile go on (two accumulators).  Operands that TMA cannot address (rows not 16-byte aligned) are
+// written to the same shared-memory layout by four more warps with plain loads.
+#include "gdn_tiles.cuh"
+#include "sm100_ptx.cuh"
+#include "ssm_common.cuh"
+
+namespace gdn {
+namespace linear {
+
+constexpr int BM = 128, BK = 64;
+constexpr int LOAD_WARPS = 4;                       // plain loaders, present only when an operand needs them
+constexpr int BASE_THREADS = 192, LOAD_THREADS = 32 * LOAD_WARPS;
+constexpr long long WAIT_CYCLES = 4000000000ll;     // ~2 s: a wait that runs this long gives up
+
+__device__ int g_status = 0;
+
+using bf16 = __nv_bfloat16;
+
+struct Operand {  // a row-major matrix, `rows` rows of `cols` contiguous values
+  const bf16* p;
+  int64_t ld;
+  int64_t rows, cols;
+  int tma;  // addressed by its tensor map, else by plain loads
+};
+
+struct GemmP {
+  Operand a, b;
+  int64_t M, N, K;
+  int tiles_m, tiles_n, splits, kblocks;  // k blocks of 64 in all
+  // epilogue (splits == 1)
+  bf16* y;
+  int64_t ldy;
+  bf16* pre;  // (M, N) contiguous, or NULL
+  const bf16* bias;
+  const bf16* res;
+  int64_t ldr;
+  int act, vec;
+  float* part;  // splits > 1: (splits, M, N) sums
+};
+
+template <int BN>
+struct Cfg {
+  static constexpr int STAGE = (BM + BN) * BK * 2;
+  static constexpr int STAGES = 196608 / STAGE;  // 4, 6, 8 for BN = 256, 128, 64
+  static constexpr int SMEM = STAGES * STAGE + 1024 /* alignment */ + 256 /* barriers */;
+};
+
+__device__ __forceinline__ float act_fwd(float p, int act) {
+  if (act == GDN_ACT_SILU) return ssm::silu(p);
+  if (act == GDN_ACT_GELU) return 0.5f * p * (1.f + erff(p * 0.70710678118654752440f));
+  return p;
+}
+__device__ __forceinline__ float act_grad(float p, int act) {
+  if (act == GDN_ACT_SILU) return ssm::dsilu(p);
+  if (act == GDN_ACT_GELU)
+    return 0.5f * (1.f + erff(p * 0.70710678118654752440f)) + p * 0.39894228040143267794f * __expf(-0.5f * p * p);
+  return 1.f;
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          ptx::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// A box of `nrow` rows x 64 values starting at (row, col), zero outside, into the 128-byte-swizzled tile at `dst`:
+// 16-byte chunk j of row r sits at chunk j ^ (r % 8).  64 x 8 chunks by 128 threads.
+__device__ __forceinline__ void load_box(char* dst, const Operand& o, int64_t row, int64_t col, int nrow, int tid) {
+  for (int i = tid; i < nrow * 8; i += LOAD_THREADS) {
+    const int r = i / 8, j = i % 8;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    bf16* e = reinterpret_cast<bf16*>(&raw);
+    if (row + r < o.rows) {
+      const bf16* p = o.p + (row + r) * o.ld + col + j * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col + j * 8 + k < o.cols) e[k] = p[k];
+    }
+    *reinterpret_cast<uint4*>(dst + r * 128 + ((j ^ (r & 7)) << 4)) = raw;
+  }
+}
+
+// One operand's part of a stage: ROWS output indices x 64 k.  k-contiguous: one box of ROWS rows; else ROWS / 64 boxes
+// of 64 k rows.
+template <int ROWS, bool MN>
+__device__ __forceinline__ void stage_tma(char* dst, const CUtensorMap* map, uint64_t* bar, int idx0, int k0) {
+  if (!MN) {
+    tma_load_2d(dst, map, bar, k0, idx0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < ROWS / 64; ++i) tma_load_2d(dst + i * 8192, map, bar, idx0 + i * 64, k0);
+  }
+}
+template <int ROWS, bool MN>
+__device__ __forceinline__ void stage_plain(char* dst, const Operand& o, int64_t idx0, int64_t k0, int tid) {
+  if (!MN) {
+    load_box(dst, o, idx0, k0, ROWS, tid);
+  } else {
+    for (int i = 0; i < ROWS / 64; ++i) load_box(dst + i * 8192, o, k0, idx0 + i * 64, 64, tid);
+  }
+}
+
+// Operand descriptor of k step s (16 deep) in a stage part at shared address `base`.
+template <bool MN>
+__device__ __forceinline__ uint64_t step_desc(uint32_t base, int s) {
+  return MN ? ptx::sdesc_sw128(base + s * 2048, 8192, 1024) : ptx::sdesc_sw128(base + s * 32, 16, 1024);
+}
+
+// 32 consecutive columns of one row of the result.
+__device__ __forceinline__ void epilogue32(const GemmP& p, int64_t row, int64_t col, float (&v)[32]) {
+  const bool full = p.vec && col + 32 <= p.N;
+  const int n = (int)(p.N - col < 32 ? p.N - col : 32);
+  if (p.bias) {
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e[8];
+        load_vec<8>(p.bias + col + i * 8, e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i * 8 + k] += e[k];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < n) v[i] += to_f32(p.bias[col + i]);
+    }
+  }
+  auto put = [&](bf16* q) {
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = v[i * 8 + k];
+        ssm::store_vec<8>(q + i * 8, e);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < n) q[i] = __float2bfloat16_rn(v[i]);
+    }
+  };
+  if (p.pre) put(p.pre + row * p.N + col);
+  if (p.act != GDN_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], p.act);
+  }
+  if (p.res) {
+    const bf16* r = p.res + row * p.ldr + col;
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e[8];
+        load_vec<8>(r + i * 8, e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i * 8 + k] += e[k];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < n) v[i] += to_f32(r[i]);
+    }
+  }
+  put(p.y + row * p.ldy + col);
+}
+
+template <int BN, bool AMN, bool BMN>
+__global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const GemmP p) {
+  using C = Cfg<BN>;
+  constexpr int ST = C::STAGES, A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+  extern __shared__ char raw_smem[];
+  char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + ST * C::STAGE);
+  uint64_t* empty = full + ST;
+  uint64_t* tfull = empty + ST;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const bool plain = !p.a.tma || !p.b.tma;
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      ptx::mbar_init(full + i, 1 + (plain ? LOAD_WARPS : 0));
+      ptx::mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(tfull + i, 1);
+      ptx::mbar_init(tempty + i, 4);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, 2 * BN);
+    ptx::tmem_relinquish();
+  }
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int items = p.tiles_m * p.tiles_n * p.splits;
+  const int per = (p.kblocks + p.splits - 1) / p.splits;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return ptx::mbar_wait_abortable(bar, parity, WAIT_CYCLES, abort_flag); };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t bytes = (p.a.tma ? A_BYTES : 0) + (p.b.tma ? B_BYTES : 0);
+      uint32_t n = 0;  // k blocks issued
+      bool ok = true;
+      for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        const int tile = it / p.splits, sp = it % p.splits;
+        const int m0 = tile % p.tiles_m * BM, n0 = tile / p.tiles_m * BN;
+        const int kb1 = min((sp + 1) * per, p.kblocks);
+        for (int kb = sp * per; kb < kb1; ++kb, ++n) {
+          const int s = n % ST;
+          if (!wait(empty + s, ((n / ST) & 1) ^ 1)) { ok = false; break; }
+          char* st = tiles + s * C::STAGE;
+          ptx::mbar_arrive_expect_tx(full + s, bytes);
+          if (p.a.tma) stage_tma<BM, AMN>(st, &ma, full + s, m0, kb * BK);
+          if (p.b.tma) stage_tma<BN, BMN>(st + A_BYTES, &mb, full + s, n0, kb * BK);
+        }
+      }
+      if (!ok)  // leave no copy in flight: each outstanding stage's own barrier, with a limit
+        for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i) ptx::mbar_wait_bounded(full + i % ST, (i / ST) & 1, WAIT_CYCLES / 8);
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = ptx::idesc_bf16_f32(BM, BN, AMN, BMN);
+    uint32_t n = 0, acc = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x, ++acc) {
+      const int sp = it % p.splits;
+      const int kb0 = sp * per, kb1 = min((sp + 1) * per, p.kblocks);
+      const uint32_t buf = acc & 1;
+      if (!wait(tempty + buf, ((acc >> 1) & 1) ^ 1)) break;
+      ptx::tc_fence_after();
+      for (int kb = kb0; kb < kb1; ++kb, ++n) {
+        const int s = n % ST;
+        if (!wait(full + s, (n / ST) & 1)) { ok = false; break; }
+        ptx::tc_fence_after();
+        const uint32_t a = ptx::smem_u32(tiles + s * C::STAGE), b = a + A_BYTES;
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          ptx::mma_f16_ss_elect(tmem + buf * BN, step_desc<AMN>(a, k), step_desc<BMN>(b, k), idesc, kb > kb0 || k > 0);
+        ptx::mma_commit_elect(empty + s);
+      }
+      ptx::mma_commit_elect(tfull + buf);
+      if (!ok) ptx::mbar_wait_bounded(tfull + buf, (acc >> 1) & 1, WAIT_CYCLES / 8);  // no MMA left in flight
+    }
+  } else if (warp < 6) {
+    const int quarter = warp % 4;  // tensor-memory lanes this warp can read
+    uint32_t acc = 0;
+    for (int it = blockIdx.x; it < items; it += gridDim.x, ++acc) {
+      const int tile = it / p.splits, sp = it % p.splits;
+      const int64_t row = (int64_t)(tile % p.tiles_m) * BM + quarter * 32 + lane, n0 = (int64_t)(tile / p.tiles_m) * BN;
+      const uint32_t buf = acc & 1;
+      if (!wait(tfull + buf, (acc >> 1) & 1)) break;
+      ptx::tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        if (n0 + c >= p.N) break;
+        float v[32];
+        ptx::tmem_ld32(tmem + (uint32_t)(quarter * 32 << 16) + buf * BN + c, v);
+        ptx::tc_wait_ld();
+        if (row >= p.M) {
+          // padding of the tile
+        } else if (p.splits > 1) {
+          float* q = p.part + ((int64_t)sp * p.M + row) * p.N + n0 + c;
+          if (p.N % 4 == 0 && n0 + c + 32 <= p.N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(q + i * 4) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (n0 + c + i < p.N) q[i] = v[i];
+          }
+        } else {
+          epilogue32(p, row, n0 + c, v);
+        }
+        __syncwarp();  // the next load is warp-wide
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(tempty + buf);
+    }
+  } else if (plain) {
+    const int ltid = tid - BASE_THREADS;
+    uint32_t n = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
+      const int tile = it / p.splits, sp = it % p.splits;
+      const int64_t m0 = (int64_t)(tile % p.tiles_m) * BM, n0 = (int64_t)(tile / p.tiles_m) * BN;
+      const int kb1 = min((sp + 1) * per, p.kblocks);
+      for (int kb = sp * per; kb < kb1; ++kb, ++n) {
+        const int s = n % ST;
+        if (!wait(empty + s, ((n / ST) & 1) ^ 1)) { ok = false; break; }
+        char* st = tiles + s * C::STAGE;
+        if (!p.a.tma) stage_plain<BM, AMN>(st, p.a, m0, (int64_t)kb * BK, ltid);
+        if (!p.b.tma) stage_plain<BN, BMN>(st + A_BYTES, p.b, n0, (int64_t)kb * BK, ltid);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(full + s);
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicExch(&g_status, GDN_ERR_TIMEOUT);
+  if (warp == 1) ptx::tmem_dealloc(tmem, 2 * BN);
+}
+
+// The splits' sums, in order, and the epilogue; 4 columns per thread.
+__global__ void __launch_bounds__(256) split_epilogue_kernel(const GemmP p) {
+  const int64_t cols = (p.N + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.M * cols) return;
+  const int64_t row = i / cols, col = i % cols * 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (col + k >= p.N) break;
+    float v = 0.f;
+    for (int s = 0; s < p.splits; ++s) v += p.part[((int64_t)s * p.M + row) * p.N + col + k];
+    if (p.bias) v += to_f32(p.bias[col + k]);
+    if (p.pre) p.pre[row * p.N + col + k] = __float2bfloat16_rn(v);
+    v = act_fwd(v, p.act);
+    if (p.res) v += to_f32(p.res[row * p.ldr + col + k]);
+    p.y[row * p.ldy + col + k] = __float2bfloat16_rn(v);
+  }
+}
+
+// Few rows (M <= 16 MT): the weight is streamed once, straight into MMA fragments.  A block owns 8 columns of y and its
+// 8 warps share the contraction; lane (g, q) reads 8 consecutive k of weight row g and of x rows g, g + 8 and the
+// fragments take them in that order -- the contraction runs over the same permuted k on both sides.  The warps' sums
+// are added in order in shared memory.
+template <int MT, bool VEC>
+__global__ void __launch_bounds__(256) few_rows_kernel(const GemmP p) {
+  __shared__ float sums[8][MT * 16][8];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 8, n = n0 + g;
+  float acc[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
+  auto load8 = [&](const bf16* base, int64_t ld, int64_t r, int64_t rows, int64_t k) {
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const bf16* s = base + r * ld + k;
+      if (VEC) {
+        if (k < p.K) raw = *reinterpret_cast<const uint4*>(s);
+      } else {
+        bf16* e = reinterpret_cast<bf16*>(&raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < p.K) e[i] = s[i];
+      }
+    }
+    return raw;
+  };
+#pragma unroll 4
+  for (int64_t k = warp * 32 + q * 8; k - q * 8 < p.K; k += 256) {
+    const uint4 w = load8(p.b.p, p.b.ld, n, p.N, k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const uint4 x0 = load8(p.a.p, p.a.ld, m * 16 + g, p.M, k), x1 = load8(p.a.p, p.a.ld, m * 16 + g + 8, p.M, k);
+      float(&d)[4] = acc[m];
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                   : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                   : "r"(x0.x), "r"(x1.x), "r"(x0.y), "r"(x1.y), "r"(w.x), "r"(w.y));
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                   : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                   : "r"(x0.z), "r"(x1.z), "r"(x0.w), "r"(x1.w), "r"(w.z), "r"(w.w));
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[warp][m * 16 + g + i / 2 * 8][q * 2 + i % 2] = acc[m][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * 128; i += 256) {
+    const int64_t row = i / 8, col = n0 + i % 8;
+    if (row >= p.M || col >= p.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += sums[w][row][i % 8];
+    if (p.bias) v += to_f32(p.bias[col]);
+    if (p.pre) p.pre[row * p.N + col] = __float2bfloat16_rn(v);
+    v = act_fwd(v, p.act);
+    if (p.res) v += to_f32(p.res[row * p.ldr + col]);
+    p.y[row * p.ldy + col] = __float2bfloat16_rn(v);
+  }
+}
+
+// dp = dy act'(pre), with rows padded to a multiple of 8 values (zeros) so that TMA can address them, and the column
+// sums of each block's DP_ROWS rows.
+constexpr int DP_ROWS = 128;
+__global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, const bf16* pre, bf16* dp, int64_t ldp, int64_t M, int64_t N,
+                                                 int act, float* colsum) {
+  // 32 lanes x 2 columns, 8 row groups
+  const int lane = threadIdx.x % 32, rg = threadIdx.x / 32;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane * 2, r0 = (int64_t)blockIdx.y * DP_ROWS;
+  float s0 = 0.f, s1 = 0.f;
+  for (int64_t r = r0 + rg; r < min(r0 + DP_ROWS, M); r += 8) {
+    float d[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (col + i < N) {
+        d[i] = to_f32(dy[r * ldd + col + i]);
+        if (act != GDN_ACT_NONE) d[i] *= act_grad(to_f32(pre[r * N + col + i]), act);
+      }
+    if (dp && col < ldp) *reinterpret_cast<__nv_bfloat162*>(dp + r * ldp + col) = __floats2bfloat162_rn(d[0], d[1]);
+    s0 += d[0];
+    s1 += d[1];
+  }
+  if (!colsum) return;
+  __shared__ float2 part[8][32];
+  part[rg][lane] = make_float2(s0, s1);
+  __syncthreads();
+  if (rg) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    s0 += part[i][lane].x;
+    s1 += part[i][lane].y;
+  }
+  if (col < N) colsum[blockIdx.y * N + col] = s0;
+  if (col + 1 < N) colsum[blockIdx.y * N + col + 1] = s1;
+}
+
+__global__ void __launch_bounds__(256) colsum_kernel(const float* part, int64_t rows, int64_t N, bf16* out) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (i >= N) return;
+  float a = 0.f;
+  for (int64_t r = threadIdx.x % 32; r < rows; r += 32) a += part[r * N + i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (threadIdx.x % 32 == 0) out[i] = __float2bfloat16_rn(a);
+}
+
+// ---- host -------------------------------------------------------------------------------------
+
+int sm_count() {
+  static std::atomic<int> cached[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64) {
+    const int c = cached[dev].load(std::memory_order_relaxed);
+    if (c) return c;
+  }
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+  if (dev >= 0 && dev < 64) cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+bool rows16(const void* p, int64_t ld) { return ssm::aligned16(p) && ld % 8 == 0 && ld > 0; }
+
+Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols) {
+  return {static_cast<const bf16*>(p), ld, rows, cols, rows16(p, ld) ? 1 : 0};
+}
+
+// (cols, rows) map with boxes of 64 columns x box_rows rows, 128-byte swizzle, zeros outside.
+bool make_map2(CUtensorMap* m, const Operand& o, int box_rows) {
+  if (!o.tma) {
+    memset(m, 0, sizeof(*m));
+    return true;
+  }
+  auto fn = tiles::encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
+  cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<bf16*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan {
+  int bn, splits;
+  size_t part;  // bytes
+};
+
+// Tile width and splits of the contraction: the widest tile that still gives every SM one, else 64-wide tiles with the
+// contraction split until they do (at least 4 k blocks each).
+Plan plan(int64_t M, int64_t N, int64_t K) {
+  const int sms = sm_count();
+  const int64_t tm = (M + BM - 1) / BM;
+  Plan r = {64, 1, 0};
+  for (int bn : {256, 128})
+    if (tm * ((N + bn - 1) / bn) >= sms) {
+      r.bn = bn;
+      return r;
+    }
+  const int64_t t = tm * ((N + 63) / 64), kb = (K + BK - 1) / BK;
+  int64_t s = t < sms ? sms / t : 1;
+  if (s > kb / 4) s = kb / 4;
+  if (s > 16) s = 16;
+  if (s > 1) {
+    const int64_t per = (kb + s - 1) / s;
+    r.splits = (int)((kb + per - 1) / per);
+    r.part = (size_t)r.splits * M * N * sizeof(float);
+  }
+  return r;
+}
+
+template <int BN, bool AMN, bool BMN>
+int launch_gemm(const GemmP& p, cudaStream_t s) {
+  static std::atomic<unsigned long long> opted{0};
+  auto k = gemm_kernel<BN, AMN, BMN>;
+  if (!opt_in_smem(opted, {{(const void*)k, Cfg<BN>::SMEM}})) return GDN_ERR_LAUNCH;
+  CUtensorMap ma, mb;
+  if (!make_map2(&ma, p.a, AMN ? BK : BM) || !make_map2(&mb, p.b, BMN ? BK : BN)) return GDN_ERR_LAUNCH;
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int grid = (int)(items < sm_count() ? items : sm_count());
+  const bool plain = !p.a.tma || !p.b.tma;
+  k<<<grid, BASE_THREADS + (plain ? LOAD_THREADS : 0), Cfg<BN>::SMEM, s>>>(ma, mb, p);
+  return ssm::launched();
+}
+
+// C[M, N] = sum_k A B with the epilogue of p; `ws` holds plan().part bytes.
+template <bool AMN, bool BMN>
+int gemm(GemmP p, void* ws, cudaStream_t s) {
+  const Plan pl = plan(p.M, p.N, p.K);
+  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + pl.bn - 1) / pl.bn;
+  if (tm * tn * pl.splits > 0x7fffffff) return GDN_ERR_SHAPE;
+  p.tiles_m = (int)tm;
+  p.tiles_n = (int)tn;
+  p.splits = pl.splits;
+  p.kblocks = (int)((p.K + BK - 1) / BK);
+  p.part = static_cast<float*>(ws);
+  p.vec = rows16(p.y, p.ldy) && (!p.bias || ssm::aligned16(p.bias)) && (!p.res || rows16(p.res, p.ldr)) && (!p.pre || rows16(p.pre, p.N));
+  int st = pl.bn == 256 ? launch_gemm<256, AMN, BMN>(p, s) : pl.bn == 128 ? launch_gemm<128, AMN, BMN>(p, s) : launch_gemm<64, AMN, BMN>(p, s);
+  if (st != GDN_OK || p.splits == 1) return st;
+  const int64_t g = (p.M * ((p.N + 3) / 4) + 255) / 256;
+  if (g > 0x7fffffff) return GDN_ERR_SHAPE;
+  split_epilogue_kernel<<<(unsigned)g, 256, 0, s>>>(p);
+  return ssm::launched();
+}
+
+constexpr int64_t FEW_ROWS = 64;
+
+int launch_few(const GemmP& p, cudaStream_t s) {
+  const unsigned g = (unsigned)((p.N + 7) / 8);
+  const bool v = p.a.tma && p.b.tma && p.K % 8 == 0;
+  if (p.M <= 16)
+    v ? few_rows_kernel<1, true><<<g, 256, 0, s>>>(p) : few_rows_kernel<1, false><<<g, 256, 0, s>>>(p);
+  else if (p.M <= 32)
+    v ? few_rows_kernel<2, true><<<g, 256, 0, s>>>(p) : few_rows_kernel<2, false><<<g, 256, 0, s>>>(p);
+  else
+    v ? few_rows_kernel<4, true><<<g, 256, 0, s>>>(p) : few_rows_kernel<4, false><<<g, 256, 0, s>>>(p);
+  return ssm::launched();
+}
+
+int check_sizes(int64_t M, int64_t N, int64_t K, int act) {
+  if (M < 0 || N < 1 || K < 1 || M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return GDN_ERR_SHAPE;
+  if (act != GDN_ACT_NONE && act != GDN_ACT_SILU && act != GDN_ACT_GELU) return GDN_ERR_UNSUPPORTED;
+  return GDN_OK;
+}
+
+struct BwdPlan {
+  int64_t ldp;       // row length of dp, 0 when dy itself serves
+  size_t dp, colsum, part, total;
+};
+
+BwdPlan bwd_plan(const gdn_linear_bwd_args* a) {
+  BwdPlan w = {};
+  const bool copy = a->act != GDN_ACT_NONE || !rows16(a->dy, a->sdy);
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  if (copy) {
+    w.ldp = (a->N + 7) / 8 * 8;
+    w.dp = up((size_t)a->M * w.ldp * 2);
+  }
+  if (a->dbias) w.colsum = up((size_t)((a->M + DP_ROWS - 1) / DP_ROWS) * a->N * 4);
+  if (a->dx) w.part = plan(a->M, a->K, a->N).part;
+  if (a->dweight) {
+    const size_t q = plan(a->N, a->K, a->M).part;
+    if (q > w.part) w.part = q;
+  }
+  w.total = w.dp + w.colsum + w.part;
+  return w;
+}
+
+}  // namespace linear
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::linear;
+
+int gdn_linear_read_status(int* out, int reset) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, gdn::linear::g_status, sizeof(int)) != cudaSuccess) return GDN_ERR_LAUNCH;
+  if (reset) {
+    const int z = 0;
+    if (cudaMemcpyToSymbol(gdn::linear::g_status, &z, sizeof(int)) != cudaSuccess) return GDN_ERR_LAUNCH;
+  }
+  *out = v;
+  return GDN_OK;
+}
+
+extern "C" {
+
+int gdn_linear_workspace_bytes(const gdn_linear_args* a, size_t* bytes) {
+  if (!a || !bytes) return GDN_ERR_NULL;
+  const int st = check_sizes(a->M, a->N, a->K, a->act);
+  if (st != GDN_OK) return st;
+  *bytes = a->M <= FEW_ROWS ? 0 : plan(a->M, a->N, a->K).part;
+  return GDN_OK;
+}
+
+int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
+  size_t need = 0;
+  int st = gdn_linear_workspace_bytes(a, &need);
+  if (st != GDN_OK) return st;
+  if (a->M == 0) return GDN_OK;
+  if (!a->x || !a->weight || !a->y) return GDN_ERR_NULL;
+  if (a->sx < 0 || a->sw < 0 || a->sr < 0 || a->sy < 0) return GDN_ERR_SHAPE;
+  if (need && (!a->workspace || a->workspace_bytes < need)) return GDN_ERR_WORKSPACE;
+  if (!ssm::device_ok()) return GDN_ERR_DEVICE;
+  GemmP p = {};
+  p.a = operand(a->x, a->sx, a->M, a->K);
+  p.b = operand(a->weight, a->sw, a->N, a->K);
+  p.M = a->M; p.N = a->N; p.K = a->K;
+  p.y = static_cast<bf16*>(a->y); p.ldy = a->sy; p.pre = static_cast<bf16*>(a->pre);
+  p.bias = static_cast<const bf16*>(a->bias); p.res = static_cast<const bf16*>(a->residual); p.ldr = a->sr;
+  p.act = a->act;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.M <= FEW_ROWS) return launch_few(p, s);
+  return gemm<false, false>(p, a->workspace, s);
+}
+
+int gdn_linear_bwd_workspace_bytes(const gdn_linear_bwd_args* a, size_t* bytes) {
+  if (!a || !bytes) return GDN_ERR_NULL;
+  const int st = check_sizes(a->M, a->N, a->K, a->act);
+  if (st != GDN_OK) return st;
+  *bytes = bwd_plan(a).total;
+  return GDN_OK;
+}
+
+int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
+  size_t need = 0;
+  int st = gdn_linear_bwd_workspace_bytes(a, &need);
+  if (st != GDN_OK) return st;
+  if (a->M == 0) return GDN_ERR_SHAPE;  // nothing flowed; the caller zeroes the gradients
+  if (!a->dy || (a->act != GDN_ACT_NONE && !a->pre) || (a->dx && !a->weight) || (a->dweight && !a->x)) return GDN_ERR_NULL;
+  if (a->sx < 0 || a->sw < 0 || a->sdy < 0) return GDN_ERR_SHAPE;
+  if (need && (!a->workspace || a->workspace_bytes < need)) return GDN_ERR_WORKSPACE;
+  if (!ssm::device_ok()) return GDN_ERR_DEVICE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const BwdPlan w = bwd_plan(a);
+  char* ws = static_cast<char*>(a->workspace);
+  bf16* dp = w.ldp ? reinterpret_cast<bf16*>(ws) : nullptr;
+  float* colsum = a->dbias ? reinterpret_cast<float*>(ws + w.dp) : nullptr;
+  void* part = ws + w.dp + w.colsum;
+  if (dp || colsum) {
+    const int64_t gx = ((dp ? w.ldp : a->N) + 63) / 64, gy = (a->M + DP_ROWS - 1) / DP_ROWS;
+    if (gy > 65535) return GDN_ERR_SHAPE;
+    dp_kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, s>>>(static_cast<const bf16*>(a->dy), a->sdy, static_cast<const bf16*>(a->pre), dp,
+                                                               w.ldp, a->M, a->N, a->act, colsum);
+    if (colsum) colsum_kernel<<<(unsigned)((a->N + 7) / 8), 256, 0, s>>>(colsum, gy, a->N, static_cast<bf16*>(a->dbias));
+    st = ssm::launched();
+    if (st != GDN_OK) return st;
+  }
+  const Operand d = dp ? operand(dp, w.ldp, a->M, a->N) : operand(a->dy, a->sdy, a->M, a->N);
+  GemmP p = {};
+  p.act = GDN_ACT_NONE;
+  if (a->dx) {  // (M, K) = dp (M, N) W (N, K)
+    p.a = d;
+    p.b = operand(a->weight, a->sw, a->N, a->K);
+    p.M = a->M; p.N = a->K; p.K = a->N;
+    p.y = static_cast<bf16*>(a->dx); p.ldy = a->K;
+    st = gemm<false, true>(p, part, s);
+    if (st != GDN_OK) return st;
+  }
+  if (a->dweight) {  // (N, K) = dp^T (N, M) x (M, K)
+    p.a = d;
+    p.b = operand(a->x, a->sx, a->M, a->K);
+    p.M = a->N; p.N = a->K; p.K = a->M;
+    p.y = static_cast<bf16*>(a->dweight); p.ldy = a->K;
+    st = gemm<true, true>(p, part, s);
+  }
+  return st;
+}
+
+}  // extern "C"

@@ -1,0 +1,114 @@
+"""The matrix product with its epilogue, ``linear(x, weight, bias=None, activation=None, residual=None)``, on the library's
+tcgen05 kernel (``include/gdn_b200.h``), forward and backward.  Reachable as ``archbench_b200.ops.linear``."""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .native import SYMBOLS, _check_cuda
+from .ssm_ops import _P, _SZ, _act, _p, _wants_grad, launch
+
+
+class LinearArgs(ctypes.Structure):
+    """Mirror of gdn_linear_args (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "residual", "y", "pre")] + \
+               [(n, ctypes.c_int64) for n in ("sx", "sw", "sr", "sy", "M", "N", "K")] + \
+               [("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    """Mirror of gdn_linear_bwd_args (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "pre", "dy", "dx", "dweight", "dbias")] + \
+               [(n, ctypes.c_int64) for n in ("sx", "sw", "sdy", "M", "N", "K")] + \
+               [("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+SYMBOLS.update({
+    "gdn_linear_workspace_bytes": ([_P(LinearArgs), _SZ], ctypes.c_int),
+    "gdn_linear_fwd": ([_P(LinearArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdn_linear_bwd_workspace_bytes": ([_P(LinearBwdArgs), _SZ], ctypes.c_int),
+    "gdn_linear_bwd": ([_P(LinearBwdArgs), ctypes.c_void_p], ctypes.c_int),
+})
+
+
+def _forward(x, weight, bias, residual, act, want_pre):
+    M, K = x.shape
+    N = weight.shape[0]
+    y = torch.empty(M, N, device=x.device, dtype=x.dtype)
+    pre = torch.empty(M, N, device=x.device, dtype=x.dtype) if want_pre and act else None
+    a = LinearArgs(_p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(pre), x.stride(0), weight.stride(0),
+                   0 if residual is None else residual.stride(0), N, M, N, K, act, 0, None, 0)
+    launch("gdn_linear_fwd", a, x.device, need="gdn_linear_workspace_bytes")
+    return y, pre
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        y, pre = _forward(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, bias, pre)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, pre = ctx.saved_tensors
+        (M, K), N = x.shape, weight.shape[0]
+        need = ctx.needs_input_grad
+        new = lambda want, *s: torch.empty(*s, device=x.device, dtype=x.dtype) if want else None
+        if M == 0:
+            return x.new_zeros(M, K), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dy, None
+        if dy.stride(-1) != 1:
+            dy = dy.contiguous()
+        dx, dw, db = new(need[0], M, K), new(need[1], N, K), new(bias is not None and need[2], N)
+        if dx is not None or dw is not None or db is not None:
+            a = LinearBwdArgs(_p(x), _p(weight), _p(pre), _p(dy), _p(dx), _p(dw), _p(db), x.stride(0), weight.stride(0), dy.stride(0),
+                              M, N, K, ctx.act, 0, None, 0)
+            launch("gdn_linear_bwd", a, x.device, need="gdn_linear_bwd_workspace_bytes")
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def _rows(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+    """A bf16 tensor as rows with a unit last stride."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+@torch.compiler.disable
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """y = act(x weight^T + bias) + residual, in one kernel where one tile pass serves it.
+
+    x (..., K), weight (N, K), bias (N), residual (..., N), all bf16 with any strides; activation None, "silu" or "gelu"
+    (the exact, erf form).  fp32 accumulation and epilogue, one rounding at the end.  Differentiable in x, weight, bias
+    and residual; with an activation, training keeps x weight^T + bias in bf16."""
+    _check_cuda(x)
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or not weight.numel():
+        raise ValueError(f"x must be (..., K) and weight (N, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
+    act = _act(activation, (None, "silu", "gelu"))
+    lead, N = x.shape[:-1], weight.shape[0]
+    rows = _rows(x, "x", x.shape, x.device) if x.dim() > 1 else _rows(x[None], "x", (1, *x.shape), x.device)
+    w = _rows(weight, "weight", weight.shape, x.device)
+    if bias is not None:
+        if tuple(bias.shape) != (N,) or bias.dtype != torch.bfloat16 or bias.device != x.device:
+            raise ValueError(f"bias must be a bfloat16 ({N},) tensor on {x.device}")
+        bias = bias.contiguous()
+    if residual is not None:
+        residual = _rows(residual, "residual", (*lead, N), x.device) if lead else _rows(residual[None], "residual", (1, N), x.device)
+    if _wants_grad(rows, w, bias, residual):
+        y = _Linear.apply(rows, w, bias, residual, act)
+    else:
+        y = _forward(rows, w, bias, residual, act, False)[0]
+    return y if len(lead) == 1 else y.reshape(*lead, N)

@@ -947,5 +947,7 @@ class NsgdnMixerTrain(torch.autograd.Function):
                 dnorm.to(norm_w.dtype), dlam, None)
 
 
-# Operators of the selective-state-space mixer; their modules add their entry points to SYMBOLS.
+# Operators of the selective-state-space mixer and the fused linear layer; their modules add their entry points to
+# SYMBOLS.
+from .linear_ops import linear  # noqa: E402,F401
 from .ssm_ops import causal_conv, causal_conv_step, selective_scan, selective_scan_step  # noqa: E402,F401

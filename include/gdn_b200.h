@@ -516,6 +516,41 @@ typedef struct gdn_scan_bwd_args {
 int gdn_scan_bwd_workspace_bytes(const gdn_scan_bwd_args* args, size_t* bytes);
 int gdn_scan_bwd(const gdn_scan_bwd_args* args, void* stream);
 
+/* ---- matrix product with its epilogue ------------------------------------------------------- */
+
+/*
+ * y = act(x weight^T + bias) + residual; x (M, K), weight (N, K), y and residual (M, N), bias (N), all bf16 with
+ * unit last strides and fp32 accumulation, one rounding at the end.  `pre`, when not NULL, receives
+ * x weight^T + bias (the backward's input; contiguous).  Any strides and alignment; 16-byte aligned rows are faster.
+ */
+typedef struct gdn_linear_args {
+  const void *x, *weight, *bias, *residual; /* bias, residual may be NULL */
+  void *y, *pre;                            /* pre may be NULL */
+  int64_t sx, sw, sr, sy;                   /* row strides in elements */
+  int64_t M, N, K;
+  int32_t act, reserved;
+  void* workspace; /* gdn_linear_workspace_bytes */
+  uint64_t workspace_bytes;
+} gdn_linear_args;
+
+int gdn_linear_workspace_bytes(const gdn_linear_args* args, size_t* bytes);
+int gdn_linear_fwd(const gdn_linear_args* args, void* stream);
+
+/* Backward: dp = dy act'(pre); dx = dp weight, dweight = dp^T x, dbias = sum_m dp.  dx, dweight, dbias are
+ * contiguous bf16 and may be NULL. */
+typedef struct gdn_linear_bwd_args {
+  const void *x, *weight, *pre, *dy; /* pre may be NULL without an activation */
+  void *dx, *dweight, *dbias;
+  int64_t sx, sw, sdy;
+  int64_t M, N, K;
+  int32_t act, reserved;
+  void* workspace; /* gdn_linear_bwd_workspace_bytes */
+  uint64_t workspace_bytes;
+} gdn_linear_bwd_args;
+
+int gdn_linear_bwd_workspace_bytes(const gdn_linear_bwd_args* args, size_t* bytes);
+int gdn_linear_bwd(const gdn_linear_bwd_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
