@@ -56,15 +56,36 @@ __device__ __forceinline__ void store_param(void* p, int64_t i, int dtype, float
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// Hardware 2^x (about 2 units in the last place; 0 below 2^-126) and reciprocal (1 unit).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 // d silu(x) / dx
 __device__ __forceinline__ float dsilu(float x) {
   const float g = sigmoid(x);
   return g * fmaf(x, 1.f - g, 1.f);
 }
-// log(1 + e^v) without cancellation for negative v; e^-|v| lies in (0, 1].
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
+// log(1 + e^v) = max(v, 0) + log(1 + e) with e = e^-|v| in (0, 1]; log(1 + e) = 2 artanh(w), w = e / (2 + e) <= 1/3, by a
+// polynomial in w^2 of relative error 4e-9 (a least-maximum fit), so small e keeps its relative precision.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = ex2(-LOG2E * fabsf(v)), w = e * rcp(2.f + e), q = w * w;
+  float r = fmaf(q, 0.2817838788032532f, 0.2796059250831604f);
+  r = fmaf(q, r, 0.4002491235733032f);
+  r = fmaf(q, r, 0.6666631698608398f);
+  r = fmaf(q, r, 2.0f);
+  return fmaf(w, r, fmaxf(v, 0.f));
+}
 
 // Tokens of row b.
 __device__ __forceinline__ int row_tokens(const int32_t* lengths, int b, int T) {

@@ -9,39 +9,58 @@
 namespace gdn {
 namespace ssm {
 
-constexpr int TT = 32;  // tokens per tile
+constexpr int TT = 32;  // tokens per tile of the local pass; segments are whole tiles
 
-// One (row, channel block, segment) per block of 128 threads.
-template <typename T, int NL>
-__global__ void __launch_bounds__(SCAN_THREADS) scan_fwd_kernel(ScanP p) {
-  constexpr int CH = SCAN_THREADS / NL, NP = NL * SPL, PER = TT * CH / SCAN_THREADS;
-  __shared__ float2 sS[TT][CH];   // step size, step size * x
-  __shared__ float sY[TT][CH + 1];
+// One (row, channel block, segment) per block of 128 threads.  Each tile is staged by the threads in their
+// per-token role (CV channels of some tokens): raw values of the next tile are already in registers while this one is
+// computed, so no load is waited for.  In their per-state role the threads read (s, s, s x, s x) of their channel and
+// the B and C of their four states, and leave their part of C . h in shared memory; the per-token role adds the parts.
+template <typename T, int NL, int CV>
+__global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p) {
+  constexpr int TT = NL == 2 ? 16 : 32;  // tokens per tile (shared memory)
+  constexpr int CH = SCAN_THREADS / NL, NP = NL * SPL;
+  constexpr int TSTEP = SCAN_THREADS * CV / CH, PER = TT / TSTEP;  // tokens covered at once, tokens per thread
+  constexpr int QUADS = TT * NL / SCAN_THREADS > 0 ? TT * NL / SCAN_THREADS : 1;
+  __shared__ __align__(16) float4 sS[TT][CH];
+  __shared__ __align__(16) float sY[TT][SCAN_THREADS];
   __shared__ __align__(16) float sB[TT][NP], sC[TT][NP];
-  const int tid = threadIdx.x, lane = tid % 32;
+  const int tid = threadIdx.x;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
   const int seg = blockIdx.y, b = blockIdx.z;
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
-  const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T);
+  const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T), lim = min(tend, len);
 
   // per-state role
   const int hc = tid / NL, n0 = (tid % NL) * SPL;
   const bool live = hc < nch;
-  float h[SPL], A2[SPL];
-#pragma unroll
-  for (int i = 0; i < SPL; ++i) {
-    const bool ok = live && n0 + i < p.N;
-    const int64_t at = (int64_t)(d0 + hc) * p.N + n0 + i;
-    A2[i] = ok ? p.A[at] * LOG2E : 0.f;
+  f32x2 h[2], A2[2];
+  {
+    float hv[SPL], av[SPL];
     const float* from = p.nseg > 1 ? p.carry + ((int64_t)b * p.nseg + seg) * p.D * p.N : p.h0 ? p.h0 + (int64_t)b * p.D * p.N : nullptr;
-    h[i] = ok && from ? from[at] : 0.f;
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+      const bool ok = live && n0 + i < p.N;
+      const int64_t at = (int64_t)(d0 + hc) * p.N + n0 + i;
+      av[i] = ok ? p.A[at] * LOG2E : 0.f;
+      hv[i] = ok && from ? from[at] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      h[i] = pack2(hv[2 * i], hv[2 * i + 1]);
+      A2[i] = pack2(av[2 * i], av[2 * i + 1]);
+    }
   }
-  // per-token role: one channel, tokens ct0, ct0 + NL, ...
-  const int cc = tid % CH, ct0 = tid / CH;
-  const bool cok = cc < nch;
+  // per-token role: channels cc .. cc + CV, tokens ct0, ct0 + TSTEP, ...
+  const int cc = tid % (CH / CV) * CV, ct0 = tid / (CH / CV);
+  const bool cok = cc < nch;  // CV divides nch
   const int d = d0 + (cok ? cc : 0);
-  const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
+  float bias[CV], skip[CV];
+#pragma unroll
+  for (int k = 0; k < CV; ++k) {
+    bias[k] = p.dt_bias ? p.dt_bias[d + k] : 0.f;
+    skip[k] = p.Dskip ? p.Dskip[d + k] : 0.f;
+  }
   const T* xp = static_cast<const T*>(p.x) + b * p.sx_b + d;
   const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt_b + d;
   const T* zp = p.z ? static_cast<const T*>(p.z) + b * p.sz_b + d : nullptr;
@@ -50,76 +69,398 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_fwd_kernel(ScanP p) {
   const T* Cp = static_cast<const T*>(p.Cm) + b * p.sC_b + grp * p.sC_g;
   const int nck = (p.T + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT;
 
-  for (int t0 = tbeg; t0 < tend; t0 += TT) {
-    float xr[PER], zr[PER];
+  Raw<T, CV> xr[PER], dr[PER], zr[PER];
+  Quad<T> qb[QUADS], qc[QUADS];
+  auto fetch = [&](int t0) {  // places past the row's tokens read its last one; their values are dropped
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int r = ct0 + i * NL, t = t0 + r;
-      float s = 0.f;
-      xr[i] = zr[i] = 0.f;
-      if (cok && t < len && t < tend) {
-        xr[i] = to_f32(xp[t * p.sx_t]);
-        s = to_f32(dtp[t * p.sdt_t]) + bias;
+      const int64_t t = min(t0 + ct0 + i * TSTEP, lim - 1);
+      xr[i] = load_raw<T, CV>(xp + t * p.sx_t);
+      dr[i] = load_raw<T, CV>(dtp + t * p.sdt_t);
+      if (zp) zr[i] = load_raw<T, CV>(zp + t * p.sz_t);
+    }
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      const int k = tid + i * SCAN_THREADS;
+      if (TT * NL >= SCAN_THREADS || k < TT * NL) {
+        const int64_t t = min(t0 + k / NL, lim - 1);
+        qb[i] = load_quad(Bp + t * p.sB_t, k % NL * 4, p.N, p.quads);
+        qc[i] = load_quad(Cp + t * p.sC_t, k % NL * 4, p.N, p.quads);
+      }
+    }
+  };
+  if (tbeg < lim) fetch(tbeg);
+  int t0 = tbeg;
+  for (; t0 < lim; t0 += TT) {
+    float x[PER][CV], z[PER][CV];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = ct0 + i * TSTEP;
+      const bool on = t0 + r < lim;
+#pragma unroll
+      for (int k = 0; k < CV; ++k) {
+        float s = to_f32(dr[i].v[k]) + bias[k];
         if (p.softplus) s = softplus(s);
-        if (zp) zr[i] = to_f32(zp[t * p.sz_t]);
+        s = on ? s : 0.f;
+        x[i][k] = to_f32(xr[i].v[k]);
+        z[i][k] = zp ? to_f32(zr[i].v[k]) : 0.f;
+        const float u = on ? s * x[i][k] : 0.f;
+        sS[r][cc + k] = make_float4(s, s, u, u);
       }
-      sS[r][cc] = make_float2(s, s * xr[i]);
     }
-    for (int i = tid; i < TT * NP; i += SCAN_THREADS) {
-      const int r = i / NP, n = i % NP, t = t0 + r;
-      const bool ok = n < p.N && t < len && t < tend;
-      sB[r][n] = ok ? to_f32(Bp[t * p.sB_t + n]) : 0.f;
-      sC[r][n] = ok ? to_f32(Cp[t * p.sC_t + n]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      const int k = tid + i * SCAN_THREADS;
+      if (TT * NL >= SCAN_THREADS || k < TT * NL) {
+        const bool on = t0 + k / NL < lim;
+        *reinterpret_cast<float4*>(&sB[k / NL][k % NL * 4]) = quad_f32(qb[i], on);
+        *reinterpret_cast<float4*>(&sC[k / NL][k % NL * 4]) = quad_f32(qc[i], on);
+      }
     }
     __syncthreads();
-    const int rows = min(TT, tend - t0);
+    if (t0 + TT < lim) fetch(t0 + TT);
 #pragma unroll 1
-    for (int r0 = 0; r0 < TT; r0 += 16) {
-      if (r0 >= rows) break;
+    for (int r0 = 0; r0 < TT; r0 += GDN_SCAN_CKPT) {
+      if (t0 + r0 >= lim) break;
       if (p.ckpt && live) {
+        float* c = p.ckpt + (((int64_t)b * nck + (t0 + r0) / GDN_SCAN_CKPT) * p.D + d0 + hc) * p.N + n0;
+        const float2 lo = unpack2(h[0]), hi = unpack2(h[1]);
+        if (p.N % 4 == 0) {
+          if (n0 < p.N) *reinterpret_cast<float4*>(c) = make_float4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          const float hv[SPL] = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-        for (int i = 0; i < SPL; ++i)
-          if (n0 + i < p.N)
-            p.ckpt[(((int64_t)b * nck + (t0 + r0) / GDN_SCAN_CKPT) * p.D + d0 + hc) * p.N + n0 + i] = h[i];
+          for (int i = 0; i < SPL; ++i)
+            if (n0 + i < p.N) c[i] = hv[i];
+        }
       }
 #pragma unroll
-      for (int q = 0; q < 16; q += NL) {
-        float acc[NL];
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const int r = r0 + q + j;
-          const float2 ss = sS[r][hc];
-          const float4 bv = *reinterpret_cast<const float4*>(&sB[r][n0]);
-          const float4 cv = *reinterpret_cast<const float4*>(&sC[r][n0]);
-          const float bb[4] = {bv.x, bv.y, bv.z, bv.w}, cq[4] = {cv.x, cv.y, cv.z, cv.w};
-          float a = 0.f;
-#pragma unroll
-          for (int i = 0; i < SPL; ++i) {
-            h[i] = fmaf(ex2(ss.x * A2[i]), h[i], ss.y * bb[i]);
-            a = fmaf(cq[i], h[i], a);
-          }
-          acc[j] = a;
-        }
-        const int j = spread_sum<NL, NL, 1>(acc, lane);
-        sY[r0 + q + j][hc] = acc[0];
+      for (int q = 0; q < GDN_SCAN_CKPT; ++q) {
+        const int r = r0 + q;
+        const ulonglong2 su = *reinterpret_cast<const ulonglong2*>(&sS[r][hc]);
+        const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sB[r][n0]);
+        const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sC[r][n0]);
+        h[0] = fma2(exp2_2(mul2(su.x, A2[0])), h[0], mul2(su.y, bv.x));
+        h[1] = fma2(exp2_2(mul2(su.x, A2[1])), h[1], mul2(su.y, bv.y));
+        sY[r][tid] = sum2(fma2(cv.y, h[1], mul2(cv.x, h[0])));
       }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int r = ct0 + i * NL, t = t0 + r;
+      const int r = ct0 + i * TSTEP, t = t0 + r;
       if (!cok || t >= tend) continue;
-      float y = fmaf(skip, xr[i], sY[r][cc]);
-      if (zp) y *= silu(zr[i]);
-      store_as(yp + t * p.sy_t, t < len ? y : 0.f);
+      float o[CV];
+#pragma unroll
+      for (int k = 0; k < CV; ++k) {
+        float y = 0.f;
+        const float* part = &sY[r][(cc + k) * NL];
+#pragma unroll
+        for (int j = 0; j < NL; j += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(part + j);
+          y += v.x + v.y;
+        }
+        y = fmaf(skip[k], x[i][k], y);
+        if (zp) y *= silu(z[i][k]);
+        o[k] = t < lim ? y : 0.f;
+      }
+      store_raw<T, CV>(yp + t * p.sy_t, o);
     }
     // sS, sB and sC are rewritten only after every thread passed the barrier above; sY only after the next one
   }
+  // past the row's tokens
+  const float zero[CV] = {};
+  for (int t = t0 + ct0; t < tend; t += TSTEP)
+    if (cok) store_raw<T, CV>(yp + (int64_t)t * p.sy_t, zero);
   if (p.h_out && seg == p.nseg - 1 && live) {
+    const float2 lo = unpack2(h[0]), hi = unpack2(h[1]);
+    const float hv[SPL] = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
     for (int i = 0; i < SPL; ++i)
-      if (n0 + i < p.N) p.h_out[((int64_t)b * p.D + d0 + hc) * p.N + n0 + i] = h[i];
+      if (n0 + i < p.N) p.h_out[((int64_t)b * p.D + d0 + hc) * p.N + n0 + i] = hv[i];
   }
+}
+
+// The same pass for rows that 16-byte copies can take; one warp per block.  A lane holds SL states of two channels.
+// What bounds it beside the exponentials is shared memory's 128 bytes a clock into registers (a broadcast saves nothing
+// there), so a lane's B and C serve two channels: (s, u) of both, B and C are 48 bytes for eight states; with one
+// channel per lane the recurrence alone cost 386 us at 8 x 4096 tokens, 2048 channels, 16 states.  A warp by itself needs
+// no barrier, and 16 channels per block balance the 148 SMs better than 32.  Raw tiles of 16 tokens come in by
+// asynchronous copies; a thread runs the recurrence of tile k, forms the step sizes of tile k + 1 and finishes the
+// outputs of tile k - 1 in one straight piece of code, so that their latencies overlap.
+template <typename T, int NL, int SL>
+struct Tiled {
+  static constexpr int TT = 16, CH = 64 / NL, NP = NL * SL, ES = (int)sizeof(T), RING = 4;
+  static constexpr int ROW = CH * ES, BROW = NP * ES;           // bytes of a token's channels, states
+  static constexpr int RAW = TT * (3 * ROW + 2 * BROW);         // x, dt, z, B, C of a tile
+  static constexpr int S_OFF = RING * RAW, S_BYTES = TT * CH * 8;
+  static constexpr int Y_OFF = S_OFF + 2 * S_BYTES, Y_BYTES = TT * 32 * 8;
+  static constexpr int BC_OFF = Y_OFF + 2 * Y_BYTES, BC_BYTES = 2 * TT * NP * 4;
+  static constexpr int SMEM = BC_OFF + 2 * BC_BYTES;
+  static constexpr int XCH = ROW / 16, BCH = BROW / 16;         // 16-byte chunks per row
+  static constexpr int CHUNKS = TT * (3 * XCH + 2 * BCH), COPIES = (CHUNKS + 31) / 32;
+};
+
+template <typename T, int NL, int SL>
+__global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
+  using K = Tiled<T, NL, SL>;
+  constexpr int TT = K::TT, CH = K::CH, NP = K::NP, PAIRS = SL / 2;
+  constexpr int PER = TT / NL;           // (token, channel pair) items per lane
+  constexpr int QUADS = TT * NP / 64;    // four-state groups of B and C per lane
+  constexpr int GT = 2, GROUPS = TT / GT;  // tokens whose loads go together
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x;
+  const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
+  const int seg = blockIdx.y, b = blockIdx.z;
+  const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
+  const int len = row_tokens(p.lengths, b, p.T);
+  const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T), lim = min(tend, len);
+  const int ntile = lim > tbeg ? (lim - tbeg + TT - 1) / TT : 0;
+
+  // this lane's copies of a tile: destination in the ring slot, source and its step from tile to tile
+  const char* src[K::COPIES];
+  int64_t step[K::COPIES];
+  uint32_t dst[K::COPIES];
+  int tok[K::COPIES];  // token in the tile, or a large one for zeros
+  constexpr int NONE = 1 << 29;
+#pragma unroll
+  for (int i = 0; i < K::COPIES; ++i) {
+    int c = lane + i * 32;
+    tok[i] = NONE;
+    src[i] = static_cast<const char*>(p.x);
+    step[i] = 0;
+    dst[i] = c * 16;
+    const void* base;
+    int64_t sb, st, off;
+    int r, j, bytes;
+    if (c < 3 * TT * K::XCH) {
+      const int which = c / (TT * K::XCH);
+      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = d0;
+      base = which == 0 ? p.x : which == 1 ? p.dt : p.z;
+      sb = which == 0 ? p.sx_b : which == 1 ? p.sdt_b : p.sz_b;
+      st = which == 0 ? p.sx_t : which == 1 ? p.sdt_t : p.sz_t;
+    } else {
+      c -= 3 * TT * K::XCH;
+      const int which = c / (TT * K::BCH);
+      r = c / K::BCH % TT; j = c % K::BCH; bytes = which < 2 ? p.N * K::ES : 0;
+      base = which ? p.Cm : p.Bm;
+      sb = which ? p.sC_b : p.sB_b;
+      st = which ? p.sC_t : p.sB_t;
+      off = grp * (which ? p.sC_g : p.sB_g);
+    }
+    if (base && j * 16 < bytes) {
+      tok[i] = r;
+      src[i] = static_cast<const char*>(base) + (b * sb + (tbeg + r) * st + off) * K::ES + j * 16;
+      step[i] = st * TT * K::ES;
+    }
+  }
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  auto fetch = [&](int k) {  // tile k into slot k % RING; an empty group past the last tile keeps the counts equal
+    if (k < ntile) {
+#pragma unroll
+      for (int i = 0; i < K::COPIES; ++i) {
+        if (K::CHUNKS % 32 == 0 || lane + i * 32 < K::CHUNKS)
+          copy16(ring + (k & (K::RING - 1)) * K::RAW + dst[i], src[i], tbeg + k * TT + tok[i] < lim);
+        src[i] += step[i];
+      }
+    }
+    copies_commit();
+  };
+
+  // per-state role: channels hc, hc + 1
+  const int hc = lane / NL * 2, n0 = lane % NL * SL;
+  const bool live = hc < nch && n0 < p.N;
+  f32x2 h[2][PAIRS];
+  float A2[2][SL];
+  const float* from = p.nseg > 1 ? p.carry + ((int64_t)b * p.nseg + seg) * p.D * p.N : p.h0 ? p.h0 + (int64_t)b * p.D * p.N : nullptr;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float hv[SL];
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const bool ok = live && n0 + i < p.N;
+      const int64_t at = (int64_t)(d0 + hc + c) * p.N + n0 + i;
+      A2[c][i] = ok ? p.A[at] * LOG2E : 0.f;
+      hv[i] = ok && from ? from[at] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) h[c][i] = pack2(hv[2 * i], hv[2 * i + 1]);
+  }
+  auto put_states = [&](float* to) {  // rows of N (a multiple of 4) states at channel d0
+    if (!live) return;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < PAIRS; i += 2)
+        if (n0 + 2 * i < p.N)
+          *reinterpret_cast<ulonglong2*>(to + (int64_t)(hc + c) * p.N + n0 + 2 * i) = make_ulonglong2(h[c][i], h[c][i + 1]);
+  };
+  // per-token role: channels cc, cc + 1, tokens ct0, ct0 + NL, ...
+  const int cc = lane % (CH / 2) * 2, ct0 = lane / (CH / 2);
+  const bool cok = cc < nch;
+  const int d = d0 + (cok ? cc : 0);
+  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], p.dt_bias[d + 1]) : both(0.f);
+  const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], p.Dskip[d + 1]) : both(0.f);
+  T* yp = static_cast<T*>(p.y) + b * p.sy_b + d;
+  const int nck = (p.T + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT;
+
+  // The three pieces of work of an item, each as loads, arithmetic and stores apart: shared memory's stores and loads
+  // keep their order, so a load behind a store would wait for all that the store waits for.
+  struct Stage {  // (s, u) of a channel pair at a token of tile k
+    f32x2 dt, x;
+  };
+  auto stage_load = [&](int k, int i) {
+    const char* raw = smem + (k & (K::RING - 1)) * K::RAW + (ct0 + i * NL) * K::ROW + cc * K::ES;
+    return Stage{load_pair(reinterpret_cast<const T*>(raw + TT * K::ROW)), load_pair(reinterpret_cast<const T*>(raw))};
+  };
+  auto stage_make = [&](int k, int i, const Stage& g) {
+    f32x2 s = add2(g.dt, bias);
+    s = p.softplus ? softplus2(s) : s;
+    const float2 uv = unpack2(mul2(s, g.x)), sv = unpack2(s);
+    const bool on = tbeg + k * TT + ct0 + i * NL < lim;
+    return on ? make_float4(sv.x, uv.x, sv.y, uv.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  auto stage_store = [&](int k, int i, const float4& v) {
+    *(reinterpret_cast<float4*>(smem + K::S_OFF + (k & 1) * K::S_BYTES) + ((ct0 + i * NL) * CH + cc) / 2) = v;
+  };
+  auto bc_load = [&](int k, int i) {  // four states of B or C in fp32 (zeros past the tokens and the states)
+    const T* raw = reinterpret_cast<const T*>(smem + (k & (K::RING - 1)) * K::RAW + 3 * TT * K::ROW) + (lane + i * 32) * 4;
+    return make_ulonglong2(load_pair(raw), load_pair(raw + 2));
+  };
+  auto bc_store = [&](int k, int i, const ulonglong2& v) {
+    *reinterpret_cast<ulonglong2*>(smem + K::BC_OFF + (k & 1) * K::BC_BYTES + (lane + i * 32) * 16) = v;
+  };
+  struct Finish {  // the outputs of a channel pair at a token of tile k
+    f32x2 core, x, z;
+  };
+  auto finish_load = [&](int k, int i) {
+    const int r = ct0 + i * NL;
+    // the pair's parts from its NL lanes; odd lanes start with the second half, or half the banks would idle
+    const char* part = smem + K::Y_OFF + (k & 1) * K::Y_BYTES + (r * 32 + cc / 2 * NL) * 8;
+    f32x2 a[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const char* q = part + ((e ^ lane) & 1) * NL * 4;
+      if (NL == 2) {
+        a[e] = *reinterpret_cast<const f32x2*>(q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NL / 2; j += 2) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(q + j * 8);
+          a[e] = j ? add2(a[e], add2(v.x, v.y)) : add2(v.x, v.y);
+        }
+      }
+    }
+    const char* raw = smem + (k & (K::RING - 1)) * K::RAW + r * K::ROW + cc * K::ES;
+    return Finish{add2(a[0], a[1]), load_pair(reinterpret_cast<const T*>(raw)), load_pair(reinterpret_cast<const T*>(raw + 2 * TT * K::ROW))};
+  };
+  auto finish_store = [&](int k, int i, const Finish& g) {
+    const int t = tbeg + k * TT + ct0 + i * NL;
+    const f32x2 gate = p.z ? mul2(g.z, sigmoid2(g.z)) : both(1.f);
+    const float2 v = unpack2(mul2(fma2(skip, g.x, g.core), gate));
+    const float out[2] = {t < lim ? v.x : 0.f, t < lim ? v.y : 0.f};
+    if (cok && t >= tbeg && t < tend) store_raw<T, 2>(yp + t * p.sy_t, out);
+  };
+  struct Tokens {  // what GT tokens of the recurrence read
+    float4 su[GT], b[GT][SL / 4];
+    ulonglong2 c[GT][SL / 4];
+  };
+  auto tokens_load = [&](int k, int r0) {
+    Tokens g;
+    const float4* sS = reinterpret_cast<const float4*>(smem + K::S_OFF + (k & 1) * K::S_BYTES) + hc / 2;
+    const float* sB = reinterpret_cast<const float*>(smem + K::BC_OFF + (k & 1) * K::BC_BYTES) + n0;
+#pragma unroll
+    for (int q = 0; q < GT; ++q) {
+      g.su[q] = sS[(r0 + q) * (CH / 2)];
+#pragma unroll
+      for (int i = 0; i < SL / 4; ++i) {
+        g.b[q][i] = *reinterpret_cast<const float4*>(sB + (r0 + q) * NP + 4 * i);
+        g.c[q][i] = *reinterpret_cast<const ulonglong2*>(sB + (TT + r0 + q) * NP + 4 * i);
+      }
+    }
+    return g;
+  };
+
+  fetch(0);
+  fetch(1);
+  if (ntile > 0) {
+    copies_wait<1>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) stage_store(0, i, stage_make(0, i, stage_load(0, i)));
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) bc_store(0, i, bc_load(0, i));
+  }
+#pragma unroll 1
+  for (int k = 0; k < ntile; ++k) {
+    copies_wait<0>();  // tile k + 1, issued one iteration ago
+    __syncwarp();
+    fetch(k + 2);
+    f32x2* sY = reinterpret_cast<f32x2*>(smem + K::Y_OFF + (k & 1) * K::Y_BYTES) + lane;
+    if (p.ckpt) put_states(p.ckpt + (((int64_t)b * nck + (tbeg + k * TT) / GDN_SCAN_CKPT) * p.D + d0) * p.N);
+    // no branches from here on: past the last tile the staged values go unused, before the first one the stores are off
+    Tokens cur = tokens_load(k, 0);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      constexpr int SI = (PER + GROUPS - 1) / GROUPS, QI = (QUADS + GROUPS - 1) / GROUPS;
+      Stage st[SI];
+      Finish fi[SI];
+      ulonglong2 bc[QI];
+      float4 made[SI];
+      const int i0 = g * PER / GROUPS, i1 = (g + 1) * PER / GROUPS, q0 = g * QUADS / GROUPS, q1 = (g + 1) * QUADS / GROUPS;
+#pragma unroll
+      for (int i = i0; i < i1; ++i) {
+        st[i - i0] = stage_load(k + 1, i);
+        fi[i - i0] = finish_load(k - 1, i);
+      }
+#pragma unroll
+      for (int i = q0; i < q1; ++i) bc[i - q0] = bc_load(k + 1, i);
+      Tokens nxt = cur;
+      if (g + 1 < GROUPS) nxt = tokens_load(k, (g + 1) * GT);
+      if (p.ckpt && g > 0 && g * GT % GDN_SCAN_CKPT == 0 && tbeg + k * TT + g * GT < lim)
+        put_states(p.ckpt + (((int64_t)b * nck + (tbeg + k * TT + g * GT) / GDN_SCAN_CKPT) * p.D + d0) * p.N);
+      f32x2 y[GT];
+#pragma unroll
+      for (int q = 0; q < GT; ++q) {
+        const float4 su = cur.su[q];
+        f32x2 y0, y1;
+#pragma unroll
+        for (int i = 0; i < PAIRS; i += 2) {
+          const float4 bv = cur.b[q][i / 2];
+          const ulonglong2 cv = cur.c[q][i / 2];
+          h[0][i] = fma2(pack2(ex2(su.x * A2[0][2 * i]), ex2(su.x * A2[0][2 * i + 1])), h[0][i], pack2(su.y * bv.x, su.y * bv.y));
+          h[1][i] = fma2(pack2(ex2(su.z * A2[1][2 * i]), ex2(su.z * A2[1][2 * i + 1])), h[1][i], pack2(su.w * bv.x, su.w * bv.y));
+          h[0][i + 1] = fma2(pack2(ex2(su.x * A2[0][2 * i + 2]), ex2(su.x * A2[0][2 * i + 3])), h[0][i + 1], pack2(su.y * bv.z, su.y * bv.w));
+          h[1][i + 1] = fma2(pack2(ex2(su.z * A2[1][2 * i + 2]), ex2(su.z * A2[1][2 * i + 3])), h[1][i + 1], pack2(su.w * bv.z, su.w * bv.w));
+          y0 = fma2(cv.y, h[0][i + 1], i ? fma2(cv.x, h[0][i], y0) : mul2(cv.x, h[0][i]));
+          y1 = fma2(cv.y, h[1][i + 1], i ? fma2(cv.x, h[1][i], y1) : mul2(cv.x, h[1][i]));
+        }
+        y[q] = pack2(sum2(y0), sum2(y1));
+      }
+#pragma unroll
+      for (int i = i0; i < i1; ++i) made[i - i0] = stage_make(k + 1, i, st[i - i0]);
+#pragma unroll
+      for (int i = i0; i < i1; ++i) {
+        finish_store(k - 1, i, fi[i - i0]);
+        stage_store(k + 1, i, made[i - i0]);
+      }
+#pragma unroll
+      for (int i = q0; i < q1; ++i) bc_store(k + 1, i, bc[i - q0]);
+#pragma unroll
+      for (int q = 0; q < GT; ++q) sY[(g * GT + q) * 32] = y[q];
+      cur = nxt;
+    }
+  }
+  __syncwarp();
+  if (ntile > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) finish_store(ntile - 1, i, finish_load(ntile - 1, i));
+  }
+  // past the row's tokens
+  const float zero[2] = {0.f, 0.f};
+  if (cok)
+    for (int t = tbeg + ntile * TT + ct0; t < tend; t += NL) store_raw<T, 2>(yp + t * p.sy_t, zero);
+  if (p.h_out && seg == p.nseg - 1) put_states(p.h_out + ((int64_t)b * p.D + d0) * p.N);
 }
 
 // Local pass over one segment from a zero state: its end state and the sum of its step sizes (the segment's decay is
@@ -277,11 +618,26 @@ SegPlan scan_segments(int64_t B, int64_t T, int64_t blocks_per_row) {
   return {(int)((T + len - 1) / len), (int)len};
 }
 
+// Two channels per load and store: even group widths and rows aligned to a pair.
+bool scan_pairs(const ScanP& p, int es, bool bwd) {
+  auto ok = [&](const void* q, int64_t sb, int64_t st) { return (uintptr_t)q % (2 * es) == 0 && sb % 2 == 0 && st % 2 == 0; };
+  if ((p.D / p.G) % 2 || !ok(p.x, p.sx_b, p.sx_t) || !ok(p.dt, p.sdt_b, p.sdt_t) || (p.z && !ok(p.z, p.sz_b, p.sz_t))) return false;
+  return bwd ? ok(p.dy, p.sdy_b, p.sdy_t) : ok(p.y, p.sy_b, p.sy_t);
+}
+
+// Rows of x, dt, z, B and C (and pairs of y) that 16-byte copies can take.
+bool scan_rows16(const ScanP& p, int es) {
+  const int v = 16 / es;
+  auto ok = [&](const void* q, int64_t sb, int64_t st) { return aligned16(q) && sb % v == 0 && st % v == 0; };
+  return (p.D / p.G) % v == 0 && p.N % v == 0 && ok(p.x, p.sx_b, p.sx_t) && ok(p.dt, p.sdt_b, p.sdt_t) && (!p.z || ok(p.z, p.sz_b, p.sz_t)) &&
+         ok(p.Bm, p.sB_b, p.sB_t) && p.sB_g % v == 0 && ok(p.Cm, p.sC_b, p.sC_t) && p.sC_g % v == 0;
+}
+
 int scan_check(const gdn_scan_args* a, bool step) {
   if (!a) return GDN_ERR_NULL;
   if (a->B < 0 || a->T < 0 || a->D < 1 || a->N < 1 || a->G < 1) return GDN_ERR_SHAPE;
   if (a->N > 64) return GDN_ERR_UNSUPPORTED;
-  if (a->D % a->G || a->B > 65535 || a->T > (1 << 30) || a->D > (1 << 24)) return GDN_ERR_SHAPE;
+  if (a->D % a->G || a->B > 65535 || a->T > (1 << 29) || a->D > (1 << 24)) return GDN_ERR_SHAPE;
   if (!elem_size(a->dtype)) return GDN_ERR_DTYPE;
   if (!a->A) return GDN_ERR_NULL;
   const int64_t st[] = {a->sx_b, a->sx_t, a->sdt_b, a->sdt_t, a->sB_b, a->sB_t, a->sB_g, a->sC_b, a->sC_t, a->sC_g, a->sz_b, a->sz_t, a->sy_b, a->sy_t};
@@ -301,6 +657,9 @@ ScanP scan_params(const gdn_scan_args* a) {
   p.sC_b = a->sC_b; p.sC_t = a->sC_t; p.sC_g = a->sC_g; p.sz_b = a->sz_b; p.sz_t = a->sz_t; p.sy_b = a->sy_b; p.sy_t = a->sy_t;
   p.B = (int)a->B; p.T = (int)a->T; p.D = (int)a->D; p.N = (int)a->N; p.G = (int)a->G;
   p.softplus = a->softplus != 0;
+  const int es = elem_size(a->dtype);
+  auto quad = [&](const void* q, int64_t sb, int64_t st, int64_t sg) { return (uintptr_t)q % (4 * es) == 0 && sb % 4 == 0 && st % 4 == 0 && sg % 4 == 0; };
+  p.quads = a->N % 4 == 0 && a->N == scan_lanes(a->N) * SPL && quad(a->Bm, a->sB_b, a->sB_t, a->sB_g) && quad(a->Cm, a->sC_b, a->sC_t, a->sC_g);
   p.dblocks = scan_dblocks(a->D, a->G, a->N);
   const SegPlan sp = scan_segments(a->B > 0 ? a->B : 1, a->T, (int64_t)p.dblocks * a->G);
   p.nseg = sp.nseg;
@@ -331,13 +690,28 @@ int scan_launch_carry(const ScanP& p, int dtype, bool reverse, cudaStream_t s) {
   return launched();
 }
 
+template <typename T, int NL, int SL>
+int launch_tiled(ScanP p, cudaStream_t s) {
+  using K = Tiled<T, NL, SL>;
+  static std::atomic<unsigned long long> opted{0};
+  auto k = scan_fwd_tiled_kernel<T, NL, SL>;
+  if (!opt_in_smem(opted, {{(const void*)k, K::SMEM}})) return GDN_ERR_LAUNCH;
+  p.dblocks = (p.D / p.G + K::CH - 1) / K::CH;
+  k<<<dim3(p.dblocks * p.G, p.nseg, p.B), 32, K::SMEM, s>>>(p);
+  return launched();
+}
 template <typename T>
+int launch_tiled(const ScanP& p, cudaStream_t s) {
+  return p.N <= 8 ? launch_tiled<T, 2, 4>(p, s) : p.N <= 16 ? launch_tiled<T, 4, 4>(p, s) : p.N <= 32 ? launch_tiled<T, 8, 4>(p, s) : launch_tiled<T, 8, 8>(p, s);
+}
+
+template <typename T, int CV>
 void launch_fwd(const ScanP& p, int nl, cudaStream_t s) {
   const dim3 g(p.dblocks * p.G, p.nseg, p.B);
-  if (nl == 2) scan_fwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 4) scan_fwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 8) scan_fwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 16) scan_fwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 2) scan_fwd_kernel<T, 2, CV><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 4) scan_fwd_kernel<T, 4, CV><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 8) scan_fwd_kernel<T, 8, CV><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 16) scan_fwd_kernel<T, 16, CV><<<g, SCAN_THREADS, 0, s>>>(p);
 }
 
 template <typename T>
@@ -390,7 +764,12 @@ int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
     if (st != GDN_OK) return st;
   }
   const int nl = scan_lanes(p.N);
-  a->dtype == GDN_DTYPE_F32 ? launch_fwd<float>(p, nl, s) : launch_fwd<__nv_bfloat16>(p, nl, s);
+  if (scan_rows16(p, elem_size(a->dtype)) && scan_pairs(p, elem_size(a->dtype), false))
+    return a->dtype == GDN_DTYPE_F32 ? launch_tiled<float>(p, s) : launch_tiled<__nv_bfloat16>(p, s);
+  if (scan_pairs(p, elem_size(a->dtype), false))
+    a->dtype == GDN_DTYPE_F32 ? launch_fwd<float, 2>(p, nl, s) : launch_fwd<__nv_bfloat16, 2>(p, nl, s);
+  else
+    a->dtype == GDN_DTYPE_F32 ? launch_fwd<float, 1>(p, nl, s) : launch_fwd<__nv_bfloat16, 1>(p, nl, s);
   return launched();
 }
 

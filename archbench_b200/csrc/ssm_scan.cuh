@@ -15,7 +15,6 @@ namespace ssm {
 
 constexpr int SCAN_THREADS = 128;
 constexpr int SPL = 4;  // states per lane
-constexpr float LOG2E = 1.44269504088896340736f;
 
 struct ScanP {
   const void *x, *dt, *Bm, *Cm, *z, *dy;
@@ -31,14 +30,130 @@ struct ScanP {
   int64_t sx_b, sx_t, sdt_b, sdt_t, sB_b, sB_t, sB_g, sC_b, sC_t, sC_g, sz_b, sz_t, sy_b, sy_t, sdy_b, sdy_t;
   int B, T, D, N, G;
   int softplus;
+  int quads;  // rows of B and C can be loaded four states at a time
   int nseg, seg_len;  // segments of seg_len tokens (a multiple of GDN_SCAN_CKPT)
   int dblocks;        // channel blocks per group
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// Two fp32 values in one 64-bit register: Blackwell multiplies and adds both with one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
+  const float2 v = unpack2(x);
+  return pack2(ex2(v.x), ex2(v.y));
+}
+__device__ __forceinline__ float sum2(f32x2 v) {
+  const float2 e = unpack2(v);
+  return e.x + e.y;
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
+// softplus and the sigmoid of two values (see ssm_common.cuh for the formulas).
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
+  const float2 e = unpack2(add2(exp2_2(mul2(x, both(-LOG2E))), both(1.f)));
+  return pack2(rcp(e.x), rcp(e.y));
+}
+__device__ __forceinline__ f32x2 softplus2(f32x2 v) {
+  const float2 a = unpack2(v);
+  const f32x2 e = exp2_2(mul2(pack2(fabsf(a.x), fabsf(a.y)), both(-LOG2E)));
+  const float2 n = unpack2(add2(e, both(2.f)));
+  const f32x2 w = mul2(e, pack2(rcp(n.x), rcp(n.y))), q = mul2(w, w);
+  f32x2 r = fma2(q, both(0.2817838788032532f), both(0.2796059250831604f));
+  r = fma2(q, r, both(0.4002491235733032f));
+  r = fma2(q, r, both(0.6666631698608398f));
+  r = fma2(q, r, both(2.0f));
+  return fma2(w, r, pack2(fmaxf(a.x, 0.f), fmaxf(a.y, 0.f)));
+}
+// Two neighbouring token values in shared memory.
+__device__ __forceinline__ f32x2 load_pair(const __nv_bfloat16* p) {
+  const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
+  return pack2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+}
+__device__ __forceinline__ f32x2 load_pair(const float* p) { return *reinterpret_cast<const f32x2*>(p); }
+// 16 bytes into shared memory without a register; zeros where `on` is false (the address is then not read).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// CV consecutive values of type T in one register image (CV = 2: one 4- or 8-byte load).
+template <typename T, int CV>
+struct Raw {
+  T v[CV];
+};
+template <>
+struct __align__(4) Raw<__nv_bfloat16, 2> {
+  __nv_bfloat16 v[2];
+};
+template <>
+struct __align__(8) Raw<float, 2> {
+  float v[2];
+};
+template <typename T, int CV>
+__device__ __forceinline__ Raw<T, CV> load_raw(const T* p) {
+  return *reinterpret_cast<const Raw<T, CV>*>(p);
+}
+template <typename T, int CV>
+__device__ __forceinline__ void store_raw(T* p, const float (&f)[CV]) {
+  Raw<T, CV> r;
+#pragma unroll
+  for (int i = 0; i < CV; ++i) store_as(&r.v[i], f[i]);
+  *reinterpret_cast<Raw<T, CV>*>(p) = r;
+}
+
+// Four consecutive states of B or C at one token: one load where rows allow, else one by one, zeros past N.
+template <typename T>
+struct Quad {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ Quad<T> load_quad(const T* p, int n, int N, bool vec) {
+  Quad<T> q;
+  if (vec) {
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(&q) = *reinterpret_cast<const float4*>(p + n);
+    else
+      *reinterpret_cast<uint2*>(&q) = *reinterpret_cast<const uint2*>(p + n);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      store_as(&q.v[i], 0.f);
+      if (n + i < N) q.v[i] = p[n + i];
+    }
+  }
+  return q;
+}
+template <typename T>
+__device__ __forceinline__ float4 quad_f32(const Quad<T>& q, bool on) {
+  return on ? make_float4(to_f32(q.v[0]), to_f32(q.v[1]), to_f32(q.v[2]), to_f32(q.v[3])) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 // v[i], i < NV, held by LANES lanes (stride STRIDE in lane index): sums over the lanes, spread so that lane l keeps
@@ -87,6 +202,8 @@ inline int scan_dblocks(int64_t D, int64_t G, int64_t N) {
 }
 
 int scan_check(const gdn_scan_args* a, bool step);
+bool scan_pairs(const ScanP& p, int es, bool bwd);
+bool scan_rows16(const ScanP& p, int es);
 ScanP scan_params(const gdn_scan_args* a);
 // Local pass over every segment (forward, or reversed for the adjoint) and the combination of the segments: fills
 // p.carry with the state that enters each segment, from p.h0 (p.dh_out).

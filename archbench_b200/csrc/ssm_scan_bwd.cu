@@ -12,7 +12,7 @@
 namespace gdn {
 namespace ssm {
 
-constexpr int CK = GDN_SCAN_CKPT;
+constexpr int CK = 16;  // tokens per tile (a multiple of GDN_SCAN_CKPT)
 
 template <typename T, int NL>
 __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
@@ -52,10 +52,24 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
   const T* Bp = static_cast<const T*>(p.Bm) + b * p.sB_b + grp * p.sB_g;
   const T* Cp = static_cast<const T*>(p.Cm) + b * p.sC_b + grp * p.sC_g;
   T *dxp = static_cast<T*>(p.dx), *ddtp = static_cast<T*>(p.ddt), *dzp = static_cast<T*>(p.dz);
-  const int nck = (p.T + CK - 1) / CK;
+  const int nck = (p.T + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT;
   float sumD = 0.f, sumB = 0.f;
 
   for (int t0 = tbeg + (tend - tbeg - 1) / CK * CK; t0 >= tbeg; t0 -= CK) {
+    if (t0 >= len) {  // nothing here: zero gradients, the adjoint passes through
+      for (int r = ct0; r < CK && t0 + r < tend; r += NL) {
+        const int64_t at = ((int64_t)b * p.T + t0 + r) * p.D + d;
+        if (!cok) continue;
+        store_as(dxp + at, 0.f);
+        store_as(ddtp + at, 0.f);
+        if (zp) store_as(dzp + at, 0.f);
+      }
+      for (int i = tid; i < CK * 2 * NP; i += SCAN_THREADS) {
+        const int t = t0 + i / (2 * NP), w = i % (2 * NP), n = w % NP;
+        if (n < p.N && t < tend) p.pBC[(((((int64_t)dblk * p.B + b) * p.T + t) * p.G + grp) * 2 + w / NP) * p.N + n] = 0.f;
+      }
+      continue;
+    }
     float xr[PER], sr[PER], zr[PER], dyr[PER], sg[PER];
     __syncthreads();
 #pragma unroll
@@ -86,7 +100,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
     float h[SPL], hp[CK][SPL];
 #pragma unroll
     for (int i = 0; i < SPL; ++i)
-      h[i] = live && n0 + i < p.N ? p.ckpt[(((int64_t)b * nck + t0 / CK) * p.D + d0 + hc) * p.N + n0 + i] : 0.f;
+      h[i] = live && n0 + i < p.N ? p.ckpt[(((int64_t)b * nck + t0 / GDN_SCAN_CKPT) * p.D + d0 + hc) * p.N + n0 + i] : 0.f;
     __syncthreads();
     // the tile's states, and C.h for the gate's gradient
 #pragma unroll
@@ -195,6 +209,341 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
   }
 }
 
+// The same for rows that 16-byte copies can take.  A lane holds four states of two channels, a warp 64 / NL channels, a
+// block four warps; tiles of 8 tokens (one checkpoint), last first, with one barrier each: a thread rebuilds the states of
+// tile k (decays and states stay in registers, so each exponential is formed once), walks the adjoint back, stages tile
+// k - 1 (earlier tokens) and finishes tile k + 1.
+template <typename T, int NL>
+struct BwdTiled {
+  static constexpr int TT = 8, CH = 256 / NL, NP = NL * SPL, ES = (int)sizeof(T), RING = 4, WARPS = 4;
+  static constexpr int ROW = CH * ES, BROW = NP * ES;
+  static constexpr int RAW = TT * (4 * ROW + 2 * BROW);  // x, dt, z, dy, B, C of a tile
+  static constexpr int S_OFF = RING * RAW, S_BYTES = TT * CH * 12;      // (s, u) of channel pairs, then dc
+  static constexpr int P_OFF = S_OFF + 2 * S_BYTES, P_BYTES = TT * SCAN_THREADS * 24;  // (g.B, ds) parts, then C.h parts
+  static constexpr int BC_OFF = P_OFF + 2 * P_BYTES, BC_BYTES = 2 * TT * NP * 4;
+  static constexpr int R_OFF = BC_OFF + 2 * BC_BYTES, R_BYTES = WARPS * TT * 2 * NP * 4;  // dB, dC of each warp
+  static constexpr int SMEM = R_OFF + 2 * R_BYTES;
+  static constexpr int XCH = ROW / 16, BCH = BROW / 16;
+  static constexpr int CHUNKS = TT * (4 * XCH + 2 * BCH), COPIES = (CHUNKS + SCAN_THREADS - 1) / SCAN_THREADS;
+};
+
+template <typename T, int NL>
+__global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const ScanP p) {
+  using K = BwdTiled<T, NL>;
+  constexpr int TT = K::TT, CH = K::CH, NP = K::NP;
+  static_assert(TT == GDN_SCAN_CKPT, "one checkpoint per tile");
+  constexpr int TSTEP = SCAN_THREADS / (CH / 2), PER = TT / TSTEP > 0 ? TT / TSTEP : 1;
+  constexpr int QUADS = 2 * TT * NL;                    // four-state groups of B and C
+  constexpr int QI = (QUADS + SCAN_THREADS - 1) / SCAN_THREADS;
+  constexpr int SHIFT4 = NL == 2 ? 2 : NL == 4 ? 1 : 0, SHIFT2 = NL == 2 ? 3 : NL == 4 ? 2 : NL == 8 ? 1 : 0;
+  constexpr float LN2 = 0.69314718055994530942f;
+  extern __shared__ __align__(16) char smem[];
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
+  const int seg = blockIdx.y, b = blockIdx.z;
+  const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
+  const int len = row_tokens(p.lengths, b, p.T);
+  const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T), lim = min(tend, len);
+  const int ntile = lim > tbeg ? (lim - tbeg + TT - 1) / TT : 0;
+  const int64_t row = (int64_t)b * p.nseg + seg;
+
+  const char* src[K::COPIES];
+  int64_t step[K::COPIES];
+  int tok[K::COPIES];
+  constexpr int NONE = 1 << 29;
+#pragma unroll
+  for (int i = 0; i < K::COPIES; ++i) {
+    int c = tid + i * SCAN_THREADS;
+    tok[i] = NONE;
+    src[i] = static_cast<const char*>(p.x);
+    step[i] = 0;
+    const void* base;
+    int64_t sb, st, off;
+    int r, j, bytes;
+    if (c < 4 * TT * K::XCH) {
+      const int which = c / (TT * K::XCH);
+      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = d0;
+      base = which == 0 ? p.x : which == 1 ? p.dt : which == 2 ? p.z : p.dy;
+      sb = which == 0 ? p.sx_b : which == 1 ? p.sdt_b : which == 2 ? p.sz_b : p.sdy_b;
+      st = which == 0 ? p.sx_t : which == 1 ? p.sdt_t : which == 2 ? p.sz_t : p.sdy_t;
+    } else {
+      c -= 4 * TT * K::XCH;
+      const int which = c / (TT * K::BCH);
+      r = c / K::BCH % TT; j = c % K::BCH; bytes = which < 2 ? p.N * K::ES : 0;
+      base = which ? p.Cm : p.Bm;
+      sb = which ? p.sC_b : p.sB_b;
+      st = which ? p.sC_t : p.sB_t;
+      off = grp * (which ? p.sC_g : p.sB_g);
+    }
+    if (base && j * 16 < bytes) {
+      tok[i] = r;
+      src[i] = static_cast<const char*>(base) + (b * sb + ((int64_t)tbeg + (ntile - 1) * TT + r) * st + off) * K::ES + j * 16;
+      step[i] = -st * TT * K::ES;
+    }
+  }
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  // Step k works on tile ntile - 1 - k.
+  auto fetch = [&](int k) {
+    if (k < ntile) {
+#pragma unroll
+      for (int i = 0; i < K::COPIES; ++i) {
+        if (K::CHUNKS % SCAN_THREADS == 0 || tid + i * SCAN_THREADS < K::CHUNKS)
+          copy16(ring + (k & (K::RING - 1)) * K::RAW + (tid + i * SCAN_THREADS) * 16, src[i], tbeg + (ntile - 1 - k) * TT + tok[i] < lim);
+        src[i] += step[i];
+      }
+    }
+    copies_commit();
+  };
+
+  // per-state role: channels hc, hc + 1 of the block
+  const int hc = tid / NL * 2, n0 = tid % NL * SPL;
+  const bool live = hc < nch && n0 < p.N;
+  f32x2 G[2][2], A2[2][2], dA[2][2];
+  const int64_t own = (int64_t)(d0 + hc) * p.N + n0;  // of channel hc; channel hc + 1 is N further
+  const float* from = p.nseg > 1 ? p.carry + row * p.D * p.N : p.dh_out ? p.dh_out + (int64_t)b * p.D * p.N : nullptr;
+  auto load4 = [&](const float* q, int c, f32x2 (&v)[2]) {
+    const ulonglong2 r = q && live ? *reinterpret_cast<const ulonglong2*>(q + own + c * p.N) : make_ulonglong2(0, 0);
+    v[0] = r.x;
+    v[1] = r.y;
+  };
+  auto store4 = [&](float* q, int c, const f32x2 (&v)[2]) {
+    if (live) *reinterpret_cast<ulonglong2*>(q + own + c * p.N) = make_ulonglong2(v[0], v[1]);
+  };
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    load4(from, c, G[c]);
+    load4(p.A, c, A2[c]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      A2[c][i] = mul2(A2[c][i], both(LOG2E));
+      dA[c][i] = both(0.f);
+    }
+  }
+  const int nck = (p.T + TT - 1) / TT;
+  auto checkpoint = [&](int k, int c, f32x2 (&v)[2]) {
+    load4(p.ckpt + ((int64_t)b * nck + tbeg / TT + ntile - 1 - k) * p.D * p.N, c, v);
+  };
+
+  // per-token role: channels cc, cc + 1, tokens ct0, ct0 + TSTEP, ...
+  const int pair = tid % (CH / 2), cc = pair * 2, ct0 = tid / (CH / 2);
+  const bool cok = cc < nch && ct0 < TT;
+  const int d = d0 + (cc < nch ? cc : 0);
+  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], p.dt_bias[d + 1]) : both(0.f);
+  const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], p.Dskip[d + 1]) : both(0.f);
+  T *dxp = static_cast<T*>(p.dx), *ddtp = static_cast<T*>(p.ddt), *dzp = static_cast<T*>(p.dz);
+  f32x2 sumD = both(0.f), sumB = both(0.f);
+
+  auto raw_pair = [&](int k, int which, int r) {
+    return load_pair(reinterpret_cast<const T*>(smem + (k & (K::RING - 1)) * K::RAW + (which * TT + r) * K::ROW + cc * K::ES));
+  };
+  auto stage = [&](int k, int i) {
+    const int r = ct0 + i * TSTEP;
+    if (TSTEP > TT && r >= TT) return;
+    f32x2 s = add2(raw_pair(k, 1, r), bias);
+    s = p.softplus ? softplus2(s) : s;
+    const f32x2 z = raw_pair(k, 2, r), dy = raw_pair(k, 3, r);
+    const f32x2 dc = p.z ? mul2(dy, mul2(z, sigmoid2(z))) : dy;
+    const float2 uv = unpack2(mul2(s, raw_pair(k, 0, r))), sv = unpack2(s);
+    const bool on = tbeg + (ntile - 1 - k) * TT + r < lim;
+    char* o = smem + K::S_OFF + (k & 1) * K::S_BYTES;
+    reinterpret_cast<float4*>(o)[r * (CH / 2) + pair] = on ? make_float4(sv.x, uv.x, sv.y, uv.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+    reinterpret_cast<f32x2*>(o + TT * CH * 8)[r * (CH / 2) + pair] = dc;  // 0 past the tokens: dy was filled with zeros
+  };
+  auto stage_bc = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+      const int q = tid + i * SCAN_THREADS;
+      if (QUADS % SCAN_THREADS && q >= QUADS) break;
+      const T* raw = reinterpret_cast<const T*>(smem + (k & (K::RING - 1)) * K::RAW + 4 * TT * K::ROW) + q * 4;
+      reinterpret_cast<ulonglong2*>(smem + K::BC_OFF + (k & 1) * K::BC_BYTES)[q] = make_ulonglong2(load_pair(raw), load_pair(raw + 2));
+    }
+  };
+  auto finish = [&](int k, int i) {
+    const int r = ct0 + i * TSTEP, t = tbeg + (ntile - 1 - k) * TT + r;
+    if (TSTEP > TT && r >= TT) return;
+    const char* parts = smem + K::P_OFF + (k & 1) * K::P_BYTES;
+    const ulonglong2* q4 = reinterpret_cast<const ulonglong2*>(parts) + r * SCAN_THREADS + pair * NL;
+    const f32x2* q2 = reinterpret_cast<const f32x2*>(parts + TT * SCAN_THREADS * 16) + r * SCAN_THREADS + pair * NL;
+    f32x2 gB = both(0.f), ds = both(0.f), core = both(0.f);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {  // each pair starts elsewhere, so that neighbours read different banks
+      const ulonglong2 v = q4[(j + (pair >> SHIFT4)) & (NL - 1)];
+      gB = add2(gB, v.x);
+      ds = add2(ds, v.y);
+      core = add2(core, q2[(j + (pair >> SHIFT2)) & (NL - 1)]);
+    }
+    const char* so = smem + K::S_OFF + (k & 1) * K::S_BYTES;
+    const float4 su = reinterpret_cast<const float4*>(so)[r * (CH / 2) + pair];
+    const f32x2 dc = reinterpret_cast<const f32x2*>(so + TT * CH * 8)[r * (CH / 2) + pair];
+    const f32x2 x = raw_pair(k, 0, r), z = raw_pair(k, 2, r), dy = raw_pair(k, 3, r);
+    const f32x2 v = add2(raw_pair(k, 1, r), bias);
+    const bool on = t < lim;
+    f32x2 ddt = fma2(ds, both(LN2), mul2(gB, x));
+    ddt = p.softplus ? mul2(ddt, sigmoid2(v)) : ddt;
+    ddt = on ? ddt : both(0.f);
+    const f32x2 dx = fma2(pack2(su.x, su.z), gB, mul2(skip, dc));
+    const f32x2 g = sigmoid2(z), dsilu = mul2(g, fma2(z, fma2(g, both(-1.f), both(1.f)), both(1.f)));
+    const f32x2 dz = mul2(mul2(dy, fma2(skip, x, core)), dsilu);
+    sumD = fma2(dc, x, sumD);
+    sumB = add2(sumB, ddt);
+    if (cok && t < tend) {
+      const int64_t at = ((int64_t)b * p.T + t) * p.D + d;
+      auto put = [&](T* q, f32x2 w) {
+        const float2 e = unpack2(w);
+        const float o[2] = {e.x, e.y};
+        store_raw<T, 2>(q + at, o);
+      };
+      put(dxp, dx);
+      put(ddtp, ddt);
+      if (p.z) put(dzp, dz);
+    }
+  };
+  auto finish_bc = [&](int k) {  // the four warps' dB and dC of tile k
+    const float* red = reinterpret_cast<const float*>(smem + K::R_OFF + (k & 1) * K::R_BYTES);
+    constexpr int N2 = TT * 2 * NP;
+#pragma unroll
+    for (int i = tid; i < N2; i += SCAN_THREADS) {
+      const int r = i / (2 * NP), w = i % (2 * NP), n = w % NP, t = tbeg + (ntile - 1 - k) * TT + r;
+      const float a = (red[i] + red[N2 + i]) + (red[2 * N2 + i] + red[3 * N2 + i]);
+      if (n < p.N && t < tend) p.pBC[(((((int64_t)dblk * p.B + b) * p.T + t) * p.G + grp) * 2 + w / NP) * p.N + n] = a;
+    }
+  };
+
+  fetch(0);
+  fetch(1);
+  f32x2 h0[2][2];
+  if (ntile > 0) {
+    checkpoint(0, 0, h0[0]);
+    checkpoint(0, 1, h0[1]);
+    copies_wait<1>();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) stage(0, i);
+    stage_bc(0);
+  }
+#pragma unroll 1
+  for (int k = 0; k < ntile; ++k) {
+    copies_wait<0>();
+    __syncthreads();
+    fetch(k + 2);
+    f32x2 h[TT + 1][2][2], a[TT][2][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      h[0][c][0] = h0[c][0];
+      h[0][c][1] = h0[c][1];
+      if (k + 1 < ntile) checkpoint(k + 1, c, h0[c]);
+    }
+    const char* sS = smem + K::S_OFF + (k & 1) * K::S_BYTES;
+    const float4* su_p = reinterpret_cast<const float4*>(sS) + hc / 2;
+    const f32x2* dc_p = reinterpret_cast<const f32x2*>(sS + TT * CH * 8) + hc / 2;
+    const float* sB = reinterpret_cast<const float*>(smem + K::BC_OFF + (k & 1) * K::BC_BYTES) + n0;
+    // the tile's states
+#pragma unroll
+    for (int r = 0; r < TT; ++r) {
+      const float4 su = su_p[r * (CH / 2)];
+      const float4 bv = *reinterpret_cast<const float4*>(sB + r * NP);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float s = c ? su.z : su.x, u = c ? su.w : su.y;
+        const float2 a0 = unpack2(A2[c][0]), a1 = unpack2(A2[c][1]);
+        a[r][c][0] = pack2(ex2(s * a0.x), ex2(s * a0.y));
+        a[r][c][1] = pack2(ex2(s * a1.x), ex2(s * a1.y));
+        h[r + 1][c][0] = fma2(a[r][c][0], h[r][c][0], pack2(u * bv.x, u * bv.y));
+        h[r + 1][c][1] = fma2(a[r][c][1], h[r][c][1], pack2(u * bv.z, u * bv.w));
+      }
+    }
+    // finish the previous step's tile and stage the next one; items of one thread are its own in both
+    if (k > 0) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) finish(k - 1, i);
+      finish_bc(k - 1);
+    }
+    if (k + 1 < ntile) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) stage(k + 1, i);
+      stage_bc(k + 1);
+    }
+    // the adjoint
+    ulonglong2* p4 = reinterpret_cast<ulonglong2*>(smem + K::P_OFF + (k & 1) * K::P_BYTES) + tid;
+    f32x2* p2 = reinterpret_cast<f32x2*>(smem + K::P_OFF + (k & 1) * K::P_BYTES + TT * SCAN_THREADS * 16) + tid;
+    float* red = reinterpret_cast<float*>(smem + K::R_OFF + (k & 1) * K::R_BYTES) + warp * TT * 2 * NP;
+#pragma unroll
+    for (int r = TT - 1; r >= 0; --r) {
+      const float4 su = su_p[r * (CH / 2)];
+      const float2 dc = unpack2(dc_p[r * (CH / 2)]);
+      const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(sB + r * NP);
+      const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sB + (TT + r) * NP);
+      f32x2 dB[2], dC[2];
+      float gb[2], ds[2], core[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const f32x2 dcd = both(c ? dc.y : dc.x), sd = both(c ? su.z : su.x), ud = both(c ? su.w : su.y);
+        const f32x2 g0 = fma2(cv.x, dcd, G[c][0]), g1 = fma2(cv.y, dcd, G[c][1]);
+        gb[c] = sum2(fma2(g1, bv.y, mul2(g0, bv.x)));
+        core[c] = sum2(fma2(cv.y, h[r + 1][c][1], mul2(cv.x, h[r + 1][c][0])));
+        dB[0] = c ? fma2(g0, ud, dB[0]) : mul2(g0, ud);
+        dB[1] = c ? fma2(g1, ud, dB[1]) : mul2(g1, ud);
+        dC[0] = c ? fma2(h[r + 1][c][0], dcd, dC[0]) : mul2(h[r + 1][c][0], dcd);
+        dC[1] = c ? fma2(h[r + 1][c][1], dcd, dC[1]) : mul2(h[r + 1][c][1], dcd);
+        G[c][0] = mul2(a[r][c][0], g0);
+        G[c][1] = mul2(a[r][c][1], g1);
+        const f32x2 f0 = mul2(G[c][0], h[r][c][0]), f1 = mul2(G[c][1], h[r][c][1]);
+        ds[c] = sum2(fma2(f1, A2[c][1], mul2(f0, A2[c][0])));
+        dA[c][0] = fma2(f0, sd, dA[c][0]);
+        dA[c][1] = fma2(f1, sd, dA[c][1]);
+      }
+      p4[r * SCAN_THREADS] = make_ulonglong2(pack2(gb[0], gb[1]), pack2(ds[0], ds[1]));
+      p2[r * SCAN_THREADS] = pack2(core[0], core[1]);
+      const float2 b0 = unpack2(dB[0]), b1 = unpack2(dB[1]), c0 = unpack2(dC[0]), c1 = unpack2(dC[1]);
+      float v[8] = {b0.x, b0.y, b1.x, b1.y, c0.x, c0.y, c1.x, c1.y};
+      const int f = spread_sum<8, 32 / NL, NL>(v, lane);
+      constexpr int LEFT = 8 * NL / 32 > 1 ? 8 * NL / 32 : 1;
+#pragma unroll
+      for (int i = 0; i < LEFT; ++i) red[r * 2 * NP + (f + i) / SPL * NP + n0 + (f + i) % SPL] = v[i];
+    }
+  }
+  __syncthreads();
+  if (ntile > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) finish(ntile - 1, i);
+    finish_bc(ntile - 1);
+  }
+  // past the row's tokens
+  const float zero[2] = {0.f, 0.f};
+  for (int t = tbeg + ntile * TT + ct0; t < tend; t += TSTEP) {
+    if (!cok) break;
+    const int64_t at = ((int64_t)b * p.T + t) * p.D + d;
+    store_raw<T, 2>(dxp + at, zero);
+    store_raw<T, 2>(ddtp + at, zero);
+    if (p.z) store_raw<T, 2>(dzp + at, zero);
+  }
+  for (int i = tid; i < (tend - tbeg - ntile * TT) * 2 * p.N; i += SCAN_THREADS) {
+    const int64_t t = tbeg + ntile * TT + i / (2 * p.N);
+    p.pBC[((((int64_t)dblk * p.B + b) * p.T + t) * p.G + grp) * 2 * p.N + i % (2 * p.N)] = 0.f;
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    store4(p.pA + row * p.D * p.N, c, dA[c]);
+    if (p.dh0 && seg == 0) store4(p.dh0 + (int64_t)b * p.D * p.N, c, G[c]);
+  }
+  // dD and ddt_bias over the threads of a channel pair
+  __syncthreads();
+  ulonglong2* sums = reinterpret_cast<ulonglong2*>(smem);
+  sums[ct0 * (CH / 2) + pair] = make_ulonglong2(sumD, sumB);
+  __syncthreads();
+  if (tid < nch / 2) {
+    f32x2 e = both(0.f), f = both(0.f);
+#pragma unroll
+    for (int i = 0; i < (TSTEP < TT ? TSTEP : TT); ++i) {
+      const ulonglong2 v = sums[i * (CH / 2) + tid];
+      e = add2(e, v.x);
+      f = add2(f, v.y);
+    }
+    *reinterpret_cast<f32x2*>(p.pD + row * 2 * p.D + d0 + 2 * tid) = e;
+    *reinterpret_cast<f32x2*>(p.pD + (row * 2 + 1) * p.D + d0 + 2 * tid) = f;
+  }
+}
+
 // dB and dC: the channel blocks' partial sums, (dblocks, B T G, 2, N) -> two (B T G, N) tensors.
 template <typename T>
 __global__ void __launch_bounds__(256) scan_sum_bc_kernel(const float* part, int dblocks, int64_t rows, int N, T* dB, T* dC) {
@@ -243,15 +592,38 @@ BwdPlan bwd_plan(const ScanP& p) {
   return w;
 }
 
+template <typename T, int NL>
+int launch_bwd_tiled(const ScanP& p, cudaStream_t s) {
+  using K = BwdTiled<T, NL>;
+  static std::atomic<unsigned long long> opted{0};
+  auto k = scan_bwd_tiled_kernel<T, NL>;
+  if (!opt_in_smem(opted, {{(const void*)k, K::SMEM}})) return GDN_ERR_LAUNCH;
+  k<<<dim3(p.dblocks * p.G, p.nseg, p.B), SCAN_THREADS, K::SMEM, s>>>(p);
+  return launched();
+}
+
+// Two channels per lane in the tiled kernel: half the channel blocks.
+bool bwd_tiled(const ScanP& p, int es) {
+  const int v = 16 / es;
+  return scan_rows16(p, es) && aligned16(p.dy) && p.sdy_b % v == 0 && p.sdy_t % v == 0;
+}
+
 template <typename T>
-int launch_bwd(const ScanP& p, const gdn_scan_bwd_args* a, cudaStream_t s) {
+int launch_bwd(ScanP p, const gdn_scan_bwd_args* a, cudaStream_t s) {
   const int nl = scan_lanes(p.N);
+  const bool tiled = bwd_tiled(p, sizeof(T));
+  if (tiled) p.dblocks = (int)((p.D / p.G + 256 / nl - 1) / (256 / nl));
   const dim3 g(p.dblocks * p.G, p.nseg, p.B);
+  int st = GDN_OK;
+  if (tiled) {
+    st = nl == 2 ? launch_bwd_tiled<T, 2>(p, s) : nl == 4 ? launch_bwd_tiled<T, 4>(p, s) : nl == 8 ? launch_bwd_tiled<T, 8>(p, s) : launch_bwd_tiled<T, 16>(p, s);
+  } else {
   if (nl == 2) scan_bwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
   if (nl == 4) scan_bwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
   if (nl == 8) scan_bwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
   if (nl == 16) scan_bwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
-  int st = launched();
+  st = launched();
+  }
   if (st != GDN_OK) return st;
   const int64_t rows = (int64_t)p.B * p.T * p.G, n = rows * 2 * p.N;
   scan_sum_bc_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p.pBC, p.dblocks, rows, p.N, static_cast<T*>(a->dB), static_cast<T*>(a->dC));

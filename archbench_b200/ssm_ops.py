@@ -23,7 +23,7 @@ from torch.autograd.function import once_differentiable
 from .native import SYMBOLS, _check, _check_cuda, _DT, load_library
 
 ACT = {None: 0, "silu": 1, "gelu": 2}
-SCAN_CKPT = 16  # GDN_SCAN_CKPT
+SCAN_CKPT = 8  # GDN_SCAN_CKPT
 
 
 class ConvArgs(ctypes.Structure):
@@ -323,7 +323,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     x, dt, z (B, T, D); A (D, N), usually negative; B, C (B, T, N) or (B, T, G, N), group g serving D / G consecutive
     channels; D, dt_bias (D); initial_state (B, D, N) fp32 (zeros if None); lengths (B): tokens of each right-padded row
     (past them y is 0 and the state stays).  N <= 64.  Returns (y, final_state or None): y in x's dtype, the state fp32.
-    Training keeps one state per 16 tokens."""
+    Training keeps one state per 8 tokens."""
     if x.dim() != 3:
         raise ValueError(f"x must be (B, T, D), got {tuple(x.shape)}")
     x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)

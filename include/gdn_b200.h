@@ -479,7 +479,7 @@ int gdn_conv_bwd(const gdn_conv_bwd_args* args, void* stream);
  * `ckpt`, when not NULL, receives the state before every GDN_SCAN_CKPT-th token, (B, ceil(T / GDN_SCAN_CKPT),
  * D, N), which the backward needs.  1 <= N <= 64, D a multiple of G.
  */
-#define GDN_SCAN_CKPT 16
+#define GDN_SCAN_CKPT 8
 
 typedef struct gdn_scan_args {
   const void *x, *dt, *Bm, *Cm, *z; /* z may be NULL */

@@ -107,6 +107,16 @@ SCAN = [  # B, T, D, N, G, dtype, gate, skip, bias, softplus, state, lengths, pa
     (1, 300, 40, 16, 1, "f32", True, True, True, True, True, False, 0),   # split over time
     (2, 530, 24, 16, 2, "f32", True, True, True, True, True, True, 0),    # split, ragged
     (1, 1100, 16, 33, 1, "bf16", True, True, True, True, False, False, 0),
+    # rows that 16-byte copies take, each layout of lanes, tiles cut by lengths, ends and channel blocks
+    (3, 37, 144, 8, 1, "bf16", True, True, True, True, True, True, 0),
+    (2, 50, 260, 4, 1, "f32", True, True, True, True, True, True, 0),
+    (3, 41, 72, 16, 3, "bf16", False, False, True, True, True, True, 0),
+    (2, 33, 80, 16, 2, "f32", True, True, True, False, True, False, 0),
+    (2, 57, 48, 24, 1, "bf16", True, True, True, True, True, True, 0),
+    (2, 35, 40, 32, 1, "f32", True, True, False, True, True, True, 0),
+    (2, 43, 24, 64, 1, "bf16", True, True, True, True, True, True, 0),
+    (2, 29, 28, 48, 1, "f32", False, True, True, True, True, True, 0),
+    (1, 700, 32, 16, 1, "bf16", True, True, True, True, True, True, 0),
 ]
 
 
