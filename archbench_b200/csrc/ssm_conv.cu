@@ -4,9 +4,9 @@
 //   p_t = b + sum_{w<W} k_w x_{t-W+1+w},  y_t = silu(p_t)
 //   dp_t = dy_t silu'(p_t),  dx_t = sum_w k_w dp_{t+W-1-w},  dk_w = sum_{b,t} dp_t x_{t-W+1+w},  db = sum dp_t
 //
-// HBM-bound: x is read and y written once (backward: x, dy read, dx written).  A thread owns one 16-byte
-// vector of channels (or one channel where rows are not aligned) and a run of consecutive tokens, and keeps the
-// last W - 1 inputs in registers, so only the run's first W - 1 rows are read twice (from L2).
+// HBM-bound: x is read and y written once (backward: x, dy read, dx written).  A thread owns a vector
+// of channels (one channel where rows are not aligned) and a run of consecutive tokens, and keeps the last W - 1 inputs
+// in registers, so only the run's first W - 1 rows are read twice (from L2).
 #include "ssm_common.cuh"
 
 namespace {
@@ -14,7 +14,6 @@ namespace {
 using namespace gdn;
 using namespace gdn::ssm;
 
-constexpr int RUN = 16;      // tokens per thread
 constexpr int THREADS = 128;
 constexpr int MAXW = 4;
 
@@ -24,7 +23,7 @@ struct ConvP {
   float* part;  // backward: (parts, C, W + 1) sums of dk and db
   const int32_t* lengths;
   int64_t sx_b, sx_t, sy_b, sy_t, sdy_b, sdy_t;
-  int B, T, C, runs, act, w_dtype;
+  int B, T, C, run, runs, act, w_dtype;  // runs of `run` tokens
 };
 
 // x_t of VEC channels from c for any t >= -(W - 1): before the row's first token it comes from the state.
@@ -52,42 +51,95 @@ __device__ __forceinline__ void load_weights(const ConvP& p, int c, float (&k)[W
   }
 }
 
+template <typename T, int VEC>
+struct __align__(VEC * sizeof(T)) Vec {
+  T v[VEC];
+};
+
+// Channels in pairs for the packed fp32 instructions; a single channel leaves the second half unused.
+template <typename T, int VEC>
+__device__ __forceinline__ void to_pairs(const Vec<T, VEC>& r, f32x2 (&o)[(VEC + 1) / 2]) {
+  if constexpr (VEC == 1) {
+    o[0] = pack2(to_f32(r.v[0]), 0.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) o[i] = load_pair(&r.v[2 * i]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> from_pairs(const f32x2 (&o)[(VEC + 1) / 2]) {
+  Vec<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < (VEC + 1) / 2; ++i) {
+    const float2 e = unpack2(o[i]);
+    store_as(&r.v[2 * i], e.x);
+    if (2 * i + 1 < VEC) store_as(&r.v[2 * i + 1], e.y);
+  }
+  return r;
+}
+template <int VEC, int W>
+__device__ __forceinline__ void load_weight_pairs(const ConvP& p, int c, f32x2 (&k)[W][(VEC + 1) / 2], f32x2 (&bias)[(VEC + 1) / 2]) {
+  float kv[W][VEC], bv[VEC];
+  load_weights<VEC, W>(p, c, kv, bv);
+#pragma unroll
+  for (int i = 0; i < (VEC + 1) / 2; ++i) {
+    const int j = 2 * i + 1 < VEC ? 2 * i + 1 : 2 * i;
+    bias[i] = pack2(bv[2 * i], bv[j]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) k[w][i] = pack2(kv[w][2 * i], kv[w][j]);
+  }
+}
+
+// The loads of BATCH tokens go out together; 64 KB in flight per SM cover HBM's latency.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(THREADS) conv_fwd_kernel(ConvP p) {
+__global__ void __launch_bounds__(THREADS) conv_fwd_kernel(const ConvP p) {
+  constexpr int HP = (VEC + 1) / 2, BATCH = 8;
+  using V = Vec<T, VEC>;
   const int cvecs = p.C / VEC;
   const int64_t id = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   if (id >= (int64_t)p.B * p.runs * cvecs) return;
-  const int c = (int)(id % cvecs) * VEC;
-  const int run = (int)((id / cvecs) % p.runs), b = (int)(id / ((int64_t)cvecs * p.runs));
+  const int64_t br = id / cvecs;
+  const int c = (int)(id - br * cvecs) * VEC;
+  const int b = (int)(br / p.runs), run = (int)(br - (int64_t)b * p.runs);
   const int len = row_tokens(p.lengths, b, p.T);
-  const int t0 = run * RUN, t1 = min(t0 + RUN, p.T);
-  float k[W][VEC], bias[VEC], x[W][VEC];
-  load_weights<VEC, W>(p, c, k, bias);
-  T* y = static_cast<T*>(p.y) + b * p.sy_b + c;
-  if (t0 < len) {
+  const int t0 = run * p.run, t1 = min(t0 + p.run, p.T), te = min(t1, len);
+  const T* xp = static_cast<const T*>(p.x) + b * p.sx_b + c;
+  T* yp = static_cast<T*>(p.y) + b * p.sy_b + c;
+  f32x2 k[W][HP], bias[HP], x[W][HP];
+  load_weight_pairs<VEC, W>(p, c, k, bias);
+  if (t0 < te) {
 #pragma unroll
-    for (int w = 0; w < W - 1; ++w) load_token<T, VEC, W>(p, b, t0 - (W - 1) + w, c, x[w]);
+    for (int w = 0; w < W - 1; ++w) {
+      float v[VEC];
+      load_token<T, VEC, W>(p, b, t0 - (W - 1) + w, c, v);
+#pragma unroll
+      for (int i = 0; i < HP; ++i) x[w][i] = pack2(v[2 * i], v[2 * i + 1 < VEC ? 2 * i + 1 : 2 * i]);
+    }
   }
-#pragma unroll 8
-  for (int t = t0; t < t1; ++t) {
-    float o[VEC];
-    if (t < len) {
-      load_vec<VEC>(static_cast<const T*>(p.x) + b * p.sx_b + t * p.sx_t + c, x[W - 1]);
+  for (int t = t0; t < te; t += BATCH) {
+    V raw[BATCH];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        float a = bias[i];
+    for (int q = 0; q < BATCH; ++q) raw[q] = *reinterpret_cast<const V*>(xp + (int64_t)min(t + q, te - 1) * p.sx_t);
 #pragma unroll
-        for (int w = 0; w < W; ++w) a = fmaf(k[w][i], x[w][i], a);
-        o[i] = p.act ? silu(a) : a;
+    for (int q = 0; q < BATCH; ++q) {
+      f32x2 o[HP];
+      to_pairs<T, VEC>(raw[q], x[W - 1]);
+#pragma unroll
+      for (int i = 0; i < HP; ++i) {
+        f32x2 a = fma2(k[0][i], x[0][i], bias[i]);
+#pragma unroll
+        for (int w = 1; w < W; ++w) a = fma2(k[w][i], x[w][i], a);
+        o[i] = p.act ? mul2(a, sigmoid2(a)) : a;
 #pragma unroll
         for (int w = 0; w < W - 1; ++w) x[w][i] = x[w + 1][i];
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+      if (t + q < te) *reinterpret_cast<V*>(yp + (int64_t)(t + q) * p.sy_t) = from_pairs<T, VEC>(o);
     }
-    store_vec<VEC>(y + t * p.sy_t, o);
   }
+  f32x2 zero[HP];
+#pragma unroll
+  for (int i = 0; i < HP; ++i) zero[i] = both(0.f);
+  for (int t = max(t0, te); t < t1; ++t) *reinterpret_cast<V*>(yp + (int64_t)t * p.sy_t) = from_pairs<T, VEC>(zero);
   if (p.state_out && run == 0) {  // the last W - 1 inputs of the row
     T* so = static_cast<T*>(p.state_out) + ((int64_t)b * p.C + c) * (W - 1);
 #pragma unroll
@@ -128,108 +180,128 @@ __global__ void __launch_bounds__(THREADS) conv_step_kernel(ConvP p) {
   store_as(static_cast<T*>(p.y) + b * p.sy_b + c, p.act ? silu(a) : a);
 }
 
-// Backward.  A thread walks its run once more than W - 1 tokens past its end: dp_t is formed as soon as x_t is
-// there, and dx_{t-W+1} once the W gradients dp_{t-W+1..t} that reach it are.  dk and db take the run's own tokens
-// only.  Their sums go to `part`, one row per thread, and are added in order by conv_sum_kernel.
+// Backward.  A thread walks its run and W - 1 tokens past it: dp_t is formed as soon as x_t is there, and dx_{t-W+1}
+// once the W gradients dp_{t-W+1..t} that reach it are.  dk and db take the run's own tokens only; a thread's sums go to
+// `part`, one row per (row, run), and conv_sum_kernel adds the rows in order.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(THREADS) conv_bwd_kernel(ConvP p) {
+__global__ void __launch_bounds__(THREADS) conv_bwd_kernel(const ConvP p) {
+  constexpr int HP = (VEC + 1) / 2, BATCH = 4;
+  using V = Vec<T, VEC>;
   const int cvecs = p.C / VEC;
   const int64_t id = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   if (id >= (int64_t)p.B * p.runs * cvecs) return;
-  const int c = (int)(id % cvecs) * VEC;
-  const int run = (int)((id / cvecs) % p.runs), b = (int)(id / ((int64_t)cvecs * p.runs));
+  const int64_t br = id / cvecs;
+  const int c = (int)(id - br * cvecs) * VEC;
+  const int b = (int)(br / p.runs), run = (int)(br - (int64_t)b * p.runs);
   const int len = row_tokens(p.lengths, b, p.T);
-  const int t0 = run * RUN, t1 = min(t0 + RUN, p.T);
-  float k[W][VEC], bias[VEC], x[W][VEC], dp[W][VEC], dk[W][VEC], db[VEC];
-  load_weights<VEC, W>(p, c, k, bias);
+  const int t0 = run * p.run, t1 = min(t0 + p.run, p.T);
+  f32x2 k[W][HP], bias[HP], x[W][HP], dp[W][HP], dk[W][HP], db[HP];
+  load_weight_pairs<VEC, W>(p, c, k, bias);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    db[i] = 0.f;
+  for (int i = 0; i < HP; ++i) {
+    db[i] = both(0.f);
 #pragma unroll
-    for (int w = 0; w < W; ++w) dk[w][i] = dp[w][i] = 0.f;
+    for (int w = 0; w < W; ++w) x[w][i] = dk[w][i] = dp[w][i] = both(0.f);
   }
-  // dp[w] = dp_{t-W+1+w} once token t is in.  The thread of the first run also owns the W - 1 inputs of the state,
-  // which tokens 0 .. W - 2 reach: its window starts with dp_{<0} = 0.  Other runs' first dx waits for t0 + W - 1.
   if (t0 < len) {
 #pragma unroll
-    for (int w = 0; w < W - 1; ++w) load_token<T, VEC, W>(p, b, t0 - (W - 1) + w, c, x[w]);
+    for (int w = 0; w < W - 1; ++w) {
+      float v[VEC];
+      load_token<T, VEC, W>(p, b, t0 - (W - 1) + w, c, v);
+#pragma unroll
+      for (int i = 0; i < HP; ++i) x[w][i] = pack2(v[2 * i], v[2 * i + 1 < VEC ? 2 * i + 1 : 2 * i]);
+    }
   }
+  // dp[w] = dp_{t-W+1+w} once token t is in.  The first run also owns the W - 1 inputs of the state, which tokens
+  // 0 .. W - 2 reach; its window starts with dp_{<0} = 0.  Other runs' first dx waits for token t0 + W - 1.
+  const T* xp = static_cast<const T*>(p.x) + b * p.sx_b + c;
   const T* dyp = static_cast<const T*>(p.dy) + b * p.sdy_b + c;
   T* dxp = static_cast<T*>(p.dx) + (int64_t)b * p.T * p.C + c;
-#pragma unroll 4
-  for (int t = t0; t < t1 + W - 1; ++t) {
-    float d[VEC];
-    if (t < len) {
-      load_vec<VEC>(static_cast<const T*>(p.x) + b * p.sx_b + t * p.sx_t + c, x[W - 1]);
-      load_vec<VEC>(dyp + t * p.sdy_t, d);
-      const bool mine = t < t1;
+  for (int tb = t0; tb < t1 + W - 1; tb += BATCH) {
+    V rx[BATCH], rd[BATCH];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
+    for (int q = 0; q < BATCH; ++q) {  // places past the row's tokens read its last one; their values are dropped
+      const int64_t t = max(min(tb + q, len - 1), 0);
+      rx[q] = *reinterpret_cast<const V*>(xp + t * p.sx_t);
+      rd[q] = *reinterpret_cast<const V*>(dyp + t * p.sdy_t);
+    }
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int t = tb + q;
+      const bool on = t < len, mine = t < t1 && on;
+      f32x2 d[HP], o[HP];
+      to_pairs<T, VEC>(rx[q], x[W - 1]);
+      to_pairs<T, VEC>(rd[q], d);
+#pragma unroll
+      for (int i = 0; i < HP; ++i) {
         if (p.act) {
-          float a = bias[i];
+          f32x2 a = fma2(k[0][i], x[0][i], bias[i]);
 #pragma unroll
-          for (int w = 0; w < W; ++w) a = fmaf(k[w][i], x[w][i], a);
-          d[i] *= dsilu(a);
+          for (int w = 1; w < W; ++w) a = fma2(k[w][i], x[w][i], a);
+          const f32x2 g = sigmoid2(a);
+          d[i] = mul2(d[i], mul2(g, fma2(a, fma2(g, both(-1.f), both(1.f)), both(1.f))));
         }
-        if (mine) {
-          db[i] += d[i];
+        d[i] = on ? d[i] : both(0.f);
+        const f32x2 m = mine ? d[i] : both(0.f);
+        db[i] = add2(db[i], m);
 #pragma unroll
-          for (int w = 0; w < W; ++w) dk[w][i] = fmaf(d[i], x[w][i], dk[w][i]);
+        for (int w = 0; w < W; ++w) dk[w][i] = fma2(m, on ? x[w][i] : both(0.f), dk[w][i]);
+#pragma unroll
+        for (int w = 0; w < W - 1; ++w) {
+          dp[w][i] = dp[w + 1][i];
+          x[w][i] = x[w + 1][i];
         }
+        dp[W - 1][i] = d[i];
+        o[i] = mul2(k[W - 1][i], dp[0][i]);
+#pragma unroll
+        for (int w = 1; w < W; ++w) o[i] = fma2(k[W - 1 - w][i], dp[w][i], o[i]);
       }
-    } else {
+      const int u = t - (W - 1);  // the input that is complete now
+      if (u >= t1) continue;
+      if (p.dstate_out && u >= len - (W - 1) && u < len && (u >= t0 || t0 == 0)) {  // state_out holds input u too
+        const T* ds = static_cast<const T*>(p.dstate_out) + ((int64_t)b * p.C + c) * (W - 1) + (u - len + W - 1);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) d[i] = 0.f;
-    }
-    const int u = t - (W - 1);  // the input that is complete now
-    float o[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-      for (int w = 0; w < W - 1; ++w) {
-        dp[w][i] = dp[w + 1][i];
-        x[w][i] = x[w + 1][i];
+        for (int i = 0; i < HP; ++i)
+          o[i] = add2(o[i], pack2(to_f32(ds[2 * i * (W - 1)]), 2 * i + 1 < VEC ? to_f32(ds[(2 * i + 1) * (W - 1)]) : 0.f));
       }
-      dp[W - 1][i] = d[i];
-      float a = 0.f;
+      if (u >= t0) {
+        *reinterpret_cast<V*>(dxp + (int64_t)u * p.C) = from_pairs<T, VEC>(o);
+      } else if (t0 == 0 && p.dstate_in) {  // u in -(W - 1) .. -1
+        T* ds = static_cast<T*>(p.dstate_in) + ((int64_t)b * p.C + c) * (W - 1) + (u + W - 1);
+        const V r = from_pairs<T, VEC>(o);
 #pragma unroll
-      for (int w = 0; w < W; ++w) a = fmaf(k[W - 1 - w][i], dp[w][i], a);
-      o[i] = a;
-    }
-    if (p.dstate_out && u >= len - (W - 1) && u < len && (u >= t0 || t0 == 0)) {  // state_out holds input u too
-      const T* ds = static_cast<const T*>(p.dstate_out) + ((int64_t)b * p.C + c) * (W - 1) + (u - len + W - 1);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i] += to_f32(ds[i * (W - 1)]);
-    }
-    if (u >= t0) {
-      store_vec<VEC>(dxp + (int64_t)u * p.C, o);
-    } else if (t0 == 0 && p.dstate_in) {  // u in -(W - 1) .. -1
-      T* ds = static_cast<T*>(p.dstate_in) + ((int64_t)b * p.C + c) * (W - 1) + (u + W - 1);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) store_as(ds + i * (W - 1), o[i]);
+        for (int i = 0; i < VEC; ++i) ds[i * (W - 1)] = r.v[i];
+      }
     }
   }
-  // Sums over the block's threads of one channel vector would save partial rows; one row per (b, run) is simple.
-  float* part = p.part + ((int64_t)(b * p.runs + run) * p.C + c) * (W + 1);
+  // (W + 1) planes of C channels
+  float* part = p.part + br * p.C * (W + 1) + c;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
+  for (int w = 0; w <= W; ++w)
 #pragma unroll
-    for (int w = 0; w < W; ++w) part[i * (W + 1) + w] = dk[w][i];
-    part[i * (W + 1) + W] = db[i];
-  }
+    for (int i = 0; i < HP; ++i) {
+      const float2 e = unpack2(w < W ? dk[w < W ? w : 0][i] : db[i]);
+      part[(int64_t)w * p.C + 2 * i] = e.x;
+      if (2 * i + 1 < VEC) part[(int64_t)w * p.C + 2 * i + 1] = e.y;
+    }
 }
 
-// One warp per (channel, tap): its partial sums, lane-strided then across the lanes.
-__global__ void conv_sum_kernel(const float* part, int64_t rows, int C, int W, void* dw, void* db, int w_dtype) {
-  const int i = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int n = C * (W + 1);
-  if (i >= n) return;
+// Column sums of the partial rows: 32 neighbouring columns and 8 groups of rows per block, added in order.
+__global__ void __launch_bounds__(256) conv_sum_kernel(const float* part, int64_t rows, int C, int W, void* dw, void* db, int w_dtype) {
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x % 32, g = threadIdx.x / 32;
+  const int64_t n = (int64_t)C * (W + 1), i = (int64_t)blockIdx.x * 32 + lane;
   float a = 0.f;
-  for (int64_t r = lane; r < rows; r += 32) a += part[r * n + i];
+  if (i < n) {
+#pragma unroll 4
+    for (int64_t r = g; r < rows; r += 8) a += part[r * n + i];
+  }
+  s[g][lane] = a;
+  __syncthreads();
+  if (g || i >= n) return;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if (lane) return;
-  const int c = i / (W + 1), w = i % (W + 1);
+  for (int k = 1; k < 8; ++k) a += s[k][lane];
+  const int w = (int)(i / C), c = (int)(i % C);
   if (w < W)
     store_param(dw, (int64_t)c * W + w, w_dtype, a);
   else if (db)
@@ -248,22 +320,30 @@ int check(const gdn_conv_args* a, bool step) {
   return GDN_OK;
 }
 
+// Tokens per thread: as many as still leave about 2048 threads per SM (a run's first W - 1 inputs are read twice, and the
+// backward writes one row of sums per run), 16 to 64.
+int run_tokens(int64_t work) {
+  const int64_t n = work / (148 * 2048);
+  return n >= 64 ? 64 : n >= 32 ? 32 : 16;
+}
+
 ConvP params(const gdn_conv_args* a) {
   ConvP p = {};
   p.x = a->x; p.w = a->weight; p.bias = a->bias; p.state_in = a->state_in; p.state_out = a->state_out; p.y = a->y;
   p.lengths = a->lengths;
   p.sx_b = a->sx_b; p.sx_t = a->sx_t; p.sy_b = a->sy_b; p.sy_t = a->sy_t;
   p.B = (int)a->B; p.T = (int)a->T; p.C = (int)a->C; p.act = a->act; p.w_dtype = a->w_dtype;
-  p.runs = (p.T + RUN - 1) / RUN;
+  p.run = run_tokens(a->B * a->T * a->C / 4);
+  p.runs = (p.T + p.run - 1) / p.run;
   return p;
 }
 
-// 16-byte vectors of channels where every row starts on one.
+// Vectors of channels where every row starts on one.
 bool vectors(const ConvP& p, int es, bool bwd) {
-  const int v = 16 / es;
-  auto ok = [&](const void* q, int64_t sb, int64_t st) { return aligned16(q) && sb % v == 0 && st % v == 0; };
+  const int v = bwd ? 4 : 16 / es;  // the backward's windows and sums leave room for four channels per thread
+  auto ok = [&](const void* q, int64_t sb, int64_t st) { return (uintptr_t)q % (v * es) == 0 && sb % v == 0 && st % v == 0; };
   if (p.C % v || !ok(p.x, p.sx_b, p.sx_t)) return false;
-  return bwd ? ok(p.dy, p.sdy_b, p.sdy_t) && aligned16(p.dx) : ok(p.y, p.sy_b, p.sy_t);
+  return bwd ? ok(p.dy, p.sdy_b, p.sdy_t) && (uintptr_t)p.dx % (v * es) == 0 : ok(p.y, p.sy_b, p.sy_t);
 }
 
 int64_t blocks(int64_t n) { return (n + THREADS - 1) / THREADS; }
@@ -364,10 +444,10 @@ int gdn_conv_bwd(const gdn_conv_bwd_args* a, void* stream) {
   if (f->dtype == GDN_DTYPE_F32)
     st = vectors(p, 4, true) ? launch_bwd<float, 4>(p, f->width, s) : launch_bwd<float, 1>(p, f->width, s);
   else
-    st = vectors(p, 2, true) ? launch_bwd<__nv_bfloat16, 8>(p, f->width, s) : launch_bwd<__nv_bfloat16, 1>(p, f->width, s);
+    st = vectors(p, 2, true) ? launch_bwd<__nv_bfloat16, 4>(p, f->width, s) : launch_bwd<__nv_bfloat16, 1>(p, f->width, s);
   if (st != GDN_OK) return st;
-  const int n = p.C * (f->width + 1);
-  conv_sum_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, (int64_t)p.B * p.runs, p.C, f->width, a->dweight, a->dbias, f->w_dtype);
+  const int64_t n = (int64_t)p.C * (f->width + 1);
+  conv_sum_kernel<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(p.part, (int64_t)p.B * p.runs, p.C, f->width, a->dweight, a->dbias, f->w_dtype);
   return launched();
 }
 

@@ -35,65 +35,6 @@ struct ScanP {
   int dblocks;        // channel blocks per group
 };
 
-// Two fp32 values in one 64-bit register: Blackwell multiplies and adds both with one instruction.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
-  const float2 v = unpack2(x);
-  return pack2(ex2(v.x), ex2(v.y));
-}
-__device__ __forceinline__ float sum2(f32x2 v) {
-  const float2 e = unpack2(v);
-  return e.x + e.y;
-}
-
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
-// softplus and the sigmoid of two values (see ssm_common.cuh for the formulas).
-__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
-  const float2 e = unpack2(add2(exp2_2(mul2(x, both(-LOG2E))), both(1.f)));
-  return pack2(rcp(e.x), rcp(e.y));
-}
-__device__ __forceinline__ f32x2 softplus2(f32x2 v) {
-  const float2 a = unpack2(v);
-  const f32x2 e = exp2_2(mul2(pack2(fabsf(a.x), fabsf(a.y)), both(-LOG2E)));
-  const float2 n = unpack2(add2(e, both(2.f)));
-  const f32x2 w = mul2(e, pack2(rcp(n.x), rcp(n.y))), q = mul2(w, w);
-  f32x2 r = fma2(q, both(0.2817838788032532f), both(0.2796059250831604f));
-  r = fma2(q, r, both(0.4002491235733032f));
-  r = fma2(q, r, both(0.6666631698608398f));
-  r = fma2(q, r, both(2.0f));
-  return fma2(w, r, pack2(fmaxf(a.x, 0.f), fmaxf(a.y, 0.f)));
-}
-// Two neighbouring token values in shared memory.
-__device__ __forceinline__ f32x2 load_pair(const __nv_bfloat16* p) {
-  const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
-  return pack2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
-}
-__device__ __forceinline__ f32x2 load_pair(const float* p) { return *reinterpret_cast<const f32x2*>(p); }
 // 16 bytes into shared memory without a register; zeros where `on` is false (the address is then not read).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
