@@ -7,7 +7,7 @@
 //            dW = dp^T x     A = dp  (M, N)  along the output  B = x (M, K)  along the output
 //
 // A persistent block computes 128 x BN tiles: one warp issues the TMA loads of 64-deep k blocks into a ring of stages,
-// one warp issues the MMAs, four warps read finished accumulators from tensor memory and run the epilogue while the
+// one warp issues the MMAs, eight warps read finished accumulators from tensor memory and run the epilogue while the
 // MMAs of the next tile go on (two accumulators).  Operands that TMA cannot address (rows not 16-byte aligned) are
 // written to the same shared-memory layout by four more warps with plain loads.
 #include "gdn_tiles.cuh"
@@ -18,13 +18,16 @@ namespace gdn {
 namespace linear {
 
 constexpr int BM = 128, BK = 64;
+constexpr int EPI_WARPS = 8;                        // two per quarter of the tensor-memory lanes
 constexpr int LOAD_WARPS = 4;                       // plain loaders, present only when an operand needs them
-constexpr int BASE_THREADS = 192, LOAD_THREADS = 32 * LOAD_WARPS;
+constexpr int BASE_THREADS = 64 + 32 * EPI_WARPS, LOAD_THREADS = 32 * LOAD_WARPS;
+constexpr int OUT_BYTES = 32 * 128;                 // a warp's output box: 32 rows x 64 columns
 constexpr long long WAIT_CYCLES = 4000000000ll;     // ~2 s: a wait that runs this long gives up
 
 __device__ int g_status = 0;
 
 using bf16 = __nv_bfloat16;
+using namespace ssm;  // packed fp32 arithmetic, vector loads and stores
 
 struct Operand {  // a row-major matrix, `rows` rows of `cols` contiguous values
   const bf16* p;
@@ -52,20 +55,47 @@ template <int BN>
 struct Cfg {
   static constexpr int STAGE = (BM + BN) * BK * 2;
   static constexpr int STAGES = 196608 / STAGE;  // 4, 6, 8 for BN = 256, 128, 64
-  static constexpr int SMEM = STAGES * STAGE + 1024 /* alignment */ + 256 /* barriers */;
+  static constexpr int COLS = BN == 64 ? 64 : BN / 2;  // columns per epilogue warp (with 64, half of the warps rest)
+  static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * OUT_BYTES + 1024 /* alignment */ + 256 /* barriers */;
 };
 
-__device__ __forceinline__ float act_fwd(float p, int act) {
-  if (act == GDN_ACT_SILU) return ssm::silu(p);
-  if (act == GDN_ACT_GELU) return 0.5f * p * (1.f + erff(p * 0.70710678118654752440f));
+// Phi(x), the normal distribution, and e^(-x^2 / 2), for two values: Phi(-|x|) = erfc(|x| / sqrt 2) / 2 by the rational
+// approximation 7.1.26 of Abramowitz and Stegun (absolute error 1.5e-7 in erfc, no cancellation in the lower tail).
+__device__ __forceinline__ f32x2 normal2(f32x2 x, f32x2& bell) {
+  const float2 v = unpack2(x);
+  const f32x2 ax = pack2(fabsf(v.x), fabsf(v.y));
+  const float2 n = unpack2(fma2(ax, both(0.3275911f * 0.70710678f), both(1.f)));
+  const f32x2 t = pack2(ssm::rcp(n.x), ssm::rcp(n.y));
+  bell = exp2_2(mul2(mul2(x, x), both(-0.5f * ssm::LOG2E)));
+  f32x2 q = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  q = fma2(t, q, both(0.5f * 1.421413741f));
+  q = fma2(t, q, both(0.5f * -0.284496736f));
+  q = fma2(t, q, both(0.5f * 0.254829592f));
+  const f32x2 low = mul2(mul2(t, q), bell);
+  const float2 l = unpack2(low), u = unpack2(fma2(low, both(-1.f), both(1.f)));
+  return pack2(v.x < 0.f ? l.x : u.x, v.y < 0.f ? l.y : u.y);
+}
+__device__ __forceinline__ f32x2 act_fwd2(f32x2 p, int act) {
+  if (act == GDN_ACT_SILU) return mul2(p, sigmoid2(p));
+  if (act == GDN_ACT_GELU) {
+    f32x2 bell;
+    return mul2(p, normal2(p, bell));
+  }
   return p;
 }
-__device__ __forceinline__ float act_grad(float p, int act) {
-  if (act == GDN_ACT_SILU) return ssm::dsilu(p);
-  if (act == GDN_ACT_GELU)
-    return 0.5f * (1.f + erff(p * 0.70710678118654752440f)) + p * 0.39894228040143267794f * __expf(-0.5f * p * p);
-  return 1.f;
+__device__ __forceinline__ f32x2 act_grad2(f32x2 p, int act) {
+  if (act == GDN_ACT_SILU) {
+    const f32x2 g = sigmoid2(p);
+    return mul2(g, fma2(p, fma2(g, both(-1.f), both(1.f)), both(1.f)));
+  }
+  if (act == GDN_ACT_GELU) {
+    f32x2 bell;
+    const f32x2 phi = normal2(p, bell);
+    return fma2(mul2(p, bell), both(0.39894228040143267794f), phi);
+  }
+  return both(1.f);
 }
+__device__ __forceinline__ float act_fwd(float p, int act) { return unpack2(act_fwd2(both(p), act)).x; }
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
   asm volatile(
@@ -118,72 +148,62 @@ __device__ __forceinline__ uint64_t step_desc(uint32_t base, int s) {
   return MN ? ptx::sdesc_sw128(base + s * 2048, 8192, 1024) : ptx::sdesc_sw128(base + s * 32, 16, 1024);
 }
 
-// 32 consecutive columns of one row of the result.
-__device__ __forceinline__ void epilogue32(const GemmP& p, int64_t row, int64_t col, float (&v)[32]) {
-  const bool full = p.vec && col + 32 <= p.N;
+// 32 consecutive columns of one row of the result, straight to global memory: rows that vectors or TMA cannot take, and
+// the ragged last columns.
+__device__ __noinline__ void epilogue32(const GemmP& p, int64_t row, int64_t col, const float (&v)[32]) {
   const int n = (int)(p.N - col < 32 ? p.N - col : 32);
-  if (p.bias) {
-    if (full) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float e[8];
-        load_vec<8>(p.bias + col + i * 8, e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[i * 8 + k] += e[k];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < n) v[i] += to_f32(p.bias[col + i]);
-    }
+  for (int i = 0; i < 32; ++i) {
+    if (i >= n) break;
+    float o = v[i];
+    if (p.bias) o += to_f32(p.bias[col + i]);
+    if (p.pre) p.pre[row * p.N + col + i] = __float2bfloat16_rn(o);
+    o = act_fwd(o, p.act);
+    if (p.res) o += to_f32(p.res[row * p.ldr + col + i]);
+    p.y[row * p.ldy + col + i] = __float2bfloat16_rn(o);
   }
-  auto put = [&](bf16* q) {
-    if (full) {
+}
+
+// A warp's 32 rows x 64 columns, written to `box` in the 128-byte-swizzled layout and stored by TMA (which clips rows
+// and columns past the matrix).  The box is free again once the copy has read it.
+__device__ __forceinline__ void box_ready(int lane) {
+  if (lane == 0) ptx::bulk_wait_read0();
+  __syncwarp();
+}
+__device__ __forceinline__ void box_put(char* box, int lane, int col, const f32x2 (&v)[16]) {  // 32 columns from col (0, 32)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float e[8];
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = v[i * 8 + k];
-        ssm::store_vec<8>(q + i * 8, e);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < n) q[i] = __float2bfloat16_rn(v[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 e = unpack2(v[j * 4 + i]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-  };
-  if (p.pre) put(p.pre + row * p.N + col);
-  if (p.act != GDN_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], p.act);
+    *reinterpret_cast<uint4*>(box + lane * 128 + (((col / 8 + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (p.res) {
-    const bf16* r = p.res + row * p.ldr + col;
-    if (full) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float e[8];
-        load_vec<8>(r + i * 8, e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[i * 8 + k] += e[k];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < n) v[i] += to_f32(r[i]);
-    }
+}
+__device__ __forceinline__ void box_store(const CUtensorMap* map, const char* box, int lane, int64_t row, int64_t col) {
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(ptx::smem_u32(box)), "r"((int)col), "r"((int)row)
+                 : "memory");
+    ptx::bulk_commit();
   }
-  put(p.y + row * p.ldy + col);
 }
 
 template <int BN, bool AMN, bool BMN>
 __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const GemmP p) {
+    gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap my,
+                const __grid_constant__ CUtensorMap mpre, const GemmP p) {
   using C = Cfg<BN>;
   constexpr int ST = C::STAGES, A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
   extern __shared__ char raw_smem[];
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + ST * C::STAGE);
+  char* boxes = tiles + ST * C::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(boxes + EPI_WARPS * OUT_BYTES);
   uint64_t* empty = full + ST;
   uint64_t* tfull = empty + ST;
   uint64_t* tempty = tfull + 2;
@@ -199,7 +219,7 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(tfull + i, 1);
-      ptx::mbar_init(tempty + i, 4);
+      ptx::mbar_init(tempty + i, BN == 64 ? 4 : EPI_WARPS);
     }
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -259,42 +279,100 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
       ptx::mma_commit_elect(tfull + buf);
       if (!ok) ptx::mbar_wait_bounded(tfull + buf, (acc >> 1) & 1, WAIT_CYCLES / 8);  // no MMA left in flight
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + EPI_WARPS) {
     const int quarter = warp % 4;  // tensor-memory lanes this warp can read
+    const int c0 = (warp - 2) / 4 * C::COLS;  // its first column of a tile
+    char* box = boxes + (warp - 2) * OUT_BYTES;
     uint32_t acc = 0;
-    for (int it = blockIdx.x; it < items; it += gridDim.x, ++acc) {
+    for (int it = blockIdx.x; c0 < BN && it < items; it += gridDim.x, ++acc) {
       const int tile = it / p.splits, sp = it % p.splits;
-      const int64_t row = (int64_t)(tile % p.tiles_m) * BM + quarter * 32 + lane, n0 = (int64_t)(tile / p.tiles_m) * BN;
+      const int64_t row0 = (int64_t)(tile % p.tiles_m) * BM + quarter * 32, row = row0 + lane, n0 = (int64_t)(tile / p.tiles_m) * BN;
       const uint32_t buf = acc & 1;
+      const bool in = row < p.M;
+      uint4 res[8];  // the residual of 64 columns, on its way while the accumulator is waited for
+      auto load_res = [&](int64_t col) {
+        if (!p.res || !p.vec || p.splits > 1) return;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          res[j] = make_uint4(0, 0, 0, 0);
+          if (in && col + j * 8 < p.N) res[j] = *reinterpret_cast<const uint4*>(p.res + row * p.ldr + col + j * 8);
+        }
+      };
+      load_res(n0 + c0);
       if (!wait(tfull + buf, (acc >> 1) & 1)) break;
       ptx::tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        if (n0 + c >= p.N) break;
-        float v[32];
-        ptx::tmem_ld32(tmem + (uint32_t)(quarter * 32 << 16) + buf * BN + c, v);
-        ptx::tc_wait_ld();
-        if (row >= p.M) {
-          // padding of the tile
-        } else if (p.splits > 1) {
-          float* q = p.part + ((int64_t)sp * p.M + row) * p.N + n0 + c;
-          if (p.N % 4 == 0 && n0 + c + 32 <= p.N) {
+      for (int c = c0; c < c0 + C::COLS; c += 64) {
+        if (n0 + c >= p.N || row0 >= p.M) break;  // the warp's part lies outside
+        const uint32_t t = tmem + (uint32_t)(quarter * 32 << 16) + buf * BN + c;
+        if (p.splits > 1 || !p.vec) {
+#pragma unroll 1
+          for (int e = 0; e < 64; e += 32) {
+            float v[32];
+            ptx::tmem_ld32(t + e, v);
+            ptx::tc_wait_ld();
+            const int64_t col = n0 + c + e;
+            if (in && p.splits > 1) {
+              float* q = p.part + ((int64_t)sp * p.M + row) * p.N + col;
+              if (p.N % 4 == 0 && col + 32 <= p.N) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(q + i * 4) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
-          } else {
+                for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(q + i * 4) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
+              } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (n0 + c + i < p.N) q[i] = v[i];
+                for (int i = 0; i < 32; ++i)
+                  if (col + i < p.N) q[i] = v[i];
+              }
+            } else if (in && col < p.N) {
+              epilogue32(p, row, col, v);
+            }
+            __syncwarp();  // the next load is warp-wide
           }
-        } else {
-          epilogue32(p, row, n0 + c, v);
+          continue;
         }
-        __syncwarp();  // the next load is warp-wide
+        f32x2 v[2][16];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float a[32];
+          ptx::tmem_ld32(t + e * 32, a);
+          ptx::tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[e][i] = pack2(a[2 * i], a[2 * i + 1]);
+          if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int64_t col = n0 + c + e * 32 + j * 8;
+              const uint4 bv = col < p.N ? __ldg(reinterpret_cast<const uint4*>(p.bias + col)) : make_uint4(0, 0, 0, 0);
+              const bf16* q = reinterpret_cast<const bf16*>(&bv);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[e][j * 4 + i] = add2(v[e][j * 4 + i], load_pair(q + 2 * i));
+            }
+          }
+        }
+        if (p.pre) {
+          box_ready(lane);
+          box_put(box, lane, 0, v[0]);
+          box_put(box, lane, 32, v[1]);
+          box_store(&mpre, box, lane, row0, n0 + c);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[e][i] = act_fwd2(v[e][i], p.act);
+            if (p.res) v[e][i] = add2(v[e][i], load_pair(reinterpret_cast<const bf16*>(&res[e * 4 + i / 4]) + i % 4 * 2));
+          }
+        if (c + 64 < c0 + C::COLS) load_res(n0 + c + 64);
+        box_ready(lane);
+        box_put(box, lane, 0, v[0]);
+        box_put(box, lane, 32, v[1]);
+        box_store(&my, box, lane, row0, n0 + c);
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(tempty + buf);
     }
+    if (lane == 0) ptx::bulk_wait0();  // the stores have read the boxes and are done
+    __syncwarp();
   } else if (plain) {
     const int ltid = tid - BASE_THREADS;
     uint32_t n = 0;
@@ -404,47 +482,78 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmP p) {
 
 // dp = dy act'(pre), with rows padded to a multiple of 8 values (zeros) so that TMA can address them, and the column
 // sums of each block's DP_ROWS rows.
-constexpr int DP_ROWS = 128;
+constexpr int DP_ROWS = 64;
+template <bool VEC>
 __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, const bf16* pre, bf16* dp, int64_t ldp, int64_t M, int64_t N,
                                                  int act, float* colsum) {
-  // 32 lanes x 2 columns, 8 row groups
+  // 32 lanes x 8 columns, 8 row groups
   const int lane = threadIdx.x % 32, rg = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane * 2, r0 = (int64_t)blockIdx.y * DP_ROWS;
-  float s0 = 0.f, s1 = 0.f;
-  for (int64_t r = r0 + rg; r < min(r0 + DP_ROWS, M); r += 8) {
-    float d[2] = {0.f, 0.f};
+  const int64_t col = (int64_t)blockIdx.x * 256 + lane * 8, r0 = (int64_t)blockIdx.y * DP_ROWS;
+  f32x2 sum[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (col + i < N) {
-        d[i] = to_f32(dy[r * ldd + col + i]);
-        if (act != GDN_ACT_NONE) d[i] *= act_grad(to_f32(pre[r * N + col + i]), act);
-      }
-    if (dp && col < ldp) *reinterpret_cast<__nv_bfloat162*>(dp + r * ldp + col) = __floats2bfloat162_rn(d[0], d[1]);
-    s0 += d[0];
-    s1 += d[1];
+  for (int i = 0; i < 4; ++i) sum[i] = both(0.f);
+  auto load8 = [&](const bf16* row) {
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (VEC) {
+      if (col < N) raw = *reinterpret_cast<const uint4*>(row + col);
+    } else {
+      bf16* e = reinterpret_cast<bf16*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < N) e[i] = row[col + i];
+    }
+    return raw;
+  };
+#pragma unroll 4
+  for (int64_t r = r0 + rg; r < min(r0 + DP_ROWS, M); r += 8) {
+    const uint4 rd = load8(dy + r * ldd);
+    const uint4 rp = act != GDN_ACT_NONE ? load8(pre + r * N) : rd;
+    f32x2 d[4];
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      d[i] = load_pair(reinterpret_cast<const bf16*>(&rd) + 2 * i);
+      if (act != GDN_ACT_NONE) d[i] = mul2(d[i], act_grad2(load_pair(reinterpret_cast<const bf16*>(&rp) + 2 * i), act));
+      sum[i] = add2(sum[i], d[i]);
+      const float2 e = unpack2(d[i]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if (dp && col < ldp) *reinterpret_cast<uint4*>(dp + r * ldp + col) = make_uint4(w[0], w[1], w[2], w[3]);
   }
   if (!colsum) return;
-  __shared__ float2 part[8][32];
-  part[rg][lane] = make_float2(s0, s1);
-  __syncthreads();
-  if (rg) return;
+  __shared__ float part[8][256 + 8];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    s0 += part[i][lane].x;
-    s1 += part[i][lane].y;
+  for (int i = 0; i < 4; ++i) {
+    const float2 e = unpack2(sum[i]);
+    part[rg][lane * 8 + 2 * i] = e.x;
+    part[rg][lane * 8 + 2 * i + 1] = e.y;
   }
-  if (col < N) colsum[blockIdx.y * N + col] = s0;
-  if (col + 1 < N) colsum[blockIdx.y * N + col + 1] = s1;
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= N) return;
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a += part[i][threadIdx.x];
+  colsum[blockIdx.y * N + c] = a;
 }
 
+// Column sums of the partial rows, added in order: 32 columns x 8 groups of rows per block.
 __global__ void __launch_bounds__(256) colsum_kernel(const float* part, int64_t rows, int64_t N, bf16* out) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (i >= N) return;
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x % 32, g = threadIdx.x / 32;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
   float a = 0.f;
-  for (int64_t r = threadIdx.x % 32; r < rows; r += 32) a += part[r * N + i];
+  if (i < N) {
+#pragma unroll 4
+    for (int64_t r = g; r < rows; r += 8) a += part[r * N + i];
+  }
+  s[g][lane] = a;
+  __syncthreads();
+  if (g || i >= N) return;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if (threadIdx.x % 32 == 0) out[i] = __float2bfloat16_rn(a);
+  for (int k = 1; k < 8; ++k) a += s[k][lane];
+  out[i] = __float2bfloat16_rn(a);
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -485,6 +594,12 @@ bool make_map2(CUtensorMap* m, const Operand& o, int box_rows) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// (N, M) map of an output, boxes of 64 columns x 32 rows.
+bool make_out_map(CUtensorMap* m, bf16* p, int64_t ld, int64_t M, int64_t N) {
+  memset(m, 0, sizeof(*m));
+  return !p || make_map2(m, Operand{p, ld, M, N, 1}, 32);
+}
+
 struct Plan {
   int bn, splits;
   size_t part;  // bytes
@@ -518,12 +633,15 @@ int launch_gemm(const GemmP& p, cudaStream_t s) {
   static std::atomic<unsigned long long> opted{0};
   auto k = gemm_kernel<BN, AMN, BMN>;
   if (!opt_in_smem(opted, {{(const void*)k, Cfg<BN>::SMEM}})) return GDN_ERR_LAUNCH;
-  CUtensorMap ma, mb;
-  if (!make_map2(&ma, p.a, AMN ? BK : BM) || !make_map2(&mb, p.b, BMN ? BK : BN)) return GDN_ERR_LAUNCH;
+  CUtensorMap ma, mb, my, mpre;
+  const bool out = p.vec && p.splits == 1;
+  if (!make_map2(&ma, p.a, AMN ? BK : BM) || !make_map2(&mb, p.b, BMN ? BK : BN) || !make_out_map(&my, out ? p.y : nullptr, p.ldy, p.M, p.N) ||
+      !make_out_map(&mpre, out ? p.pre : nullptr, p.N, p.M, p.N))
+    return GDN_ERR_LAUNCH;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
   const int grid = (int)(items < sm_count() ? items : sm_count());
   const bool plain = !p.a.tma || !p.b.tma;
-  k<<<grid, BASE_THREADS + (plain ? LOAD_THREADS : 0), Cfg<BN>::SMEM, s>>>(ma, mb, p);
+  k<<<grid, BASE_THREADS + (plain ? LOAD_THREADS : 0), Cfg<BN>::SMEM, s>>>(ma, mb, my, mpre, p);
   return ssm::launched();
 }
 
@@ -538,7 +656,7 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
   p.splits = pl.splits;
   p.kblocks = (int)((p.K + BK - 1) / BK);
   p.part = static_cast<float*>(ws);
-  p.vec = rows16(p.y, p.ldy) && (!p.bias || ssm::aligned16(p.bias)) && (!p.res || rows16(p.res, p.ldr)) && (!p.pre || rows16(p.pre, p.N));
+  p.vec = rows16(p.y, p.ldy) && p.N % 8 == 0 && (!p.bias || ssm::aligned16(p.bias)) && (!p.res || rows16(p.res, p.ldr)) && (!p.pre || rows16(p.pre, p.N));
   int st = pl.bn == 256 ? launch_gemm<256, AMN, BMN>(p, s) : pl.bn == 128 ? launch_gemm<128, AMN, BMN>(p, s) : launch_gemm<64, AMN, BMN>(p, s);
   if (st != GDN_OK || p.splits == 1) return st;
   const int64_t g = (p.M * ((p.N + 3) / 4) + 255) / 256;
@@ -662,11 +780,15 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
   float* colsum = a->dbias ? reinterpret_cast<float*>(ws + w.dp) : nullptr;
   void* part = ws + w.dp + w.colsum;
   if (dp || colsum) {
-    const int64_t gx = ((dp ? w.ldp : a->N) + 63) / 64, gy = (a->M + DP_ROWS - 1) / DP_ROWS;
+    const int64_t gx = ((dp ? w.ldp : a->N) + 255) / 256, gy = (a->M + DP_ROWS - 1) / DP_ROWS;
     if (gy > 65535) return GDN_ERR_SHAPE;
-    dp_kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, s>>>(static_cast<const bf16*>(a->dy), a->sdy, static_cast<const bf16*>(a->pre), dp,
-                                                               w.ldp, a->M, a->N, a->act, colsum);
-    if (colsum) colsum_kernel<<<(unsigned)((a->N + 7) / 8), 256, 0, s>>>(colsum, gy, a->N, static_cast<bf16*>(a->dbias));
+    const dim3 g((unsigned)gx, (unsigned)gy);
+    const bf16 *dy = static_cast<const bf16*>(a->dy), *pre = static_cast<const bf16*>(a->pre);
+    if (a->N % 8 == 0 && rows16(dy, a->sdy) && (a->act == GDN_ACT_NONE || ssm::aligned16(pre)))
+      dp_kernel<true><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, colsum);
+    else
+      dp_kernel<false><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, colsum);
+    if (colsum) colsum_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, s>>>(colsum, gy, a->N, static_cast<bf16*>(a->dbias));
     st = ssm::launched();
     if (st != GDN_OK) return st;
   }
