@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   }
   // past the row's tokens
   const float zero[2] = {0.f, 0.f};
-  for (int t = tbeg + ntile * TT + ct0; t < tend; t += TSTEP) {
-    if (!cok) break;
+  for (int t = tbeg + ntile * TT + ct0; t < tend; t += TSTEP) {  // (all token rows of threads: cok has only a tile's)
+    if (cc >= nch) break;
     const int64_t at = ((int64_t)b * p.T + t) * p.D + d;
     store_raw<T, 2>(dxp + at, zero);
     store_raw<T, 2>(ddtp + at, zero);

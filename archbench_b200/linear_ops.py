@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .native import SYMBOLS, _check_cuda
-from .ssm_ops import _P, _SZ, _act, _p, _wants_grad, launch
+from .ssm_ops import _P, _SZ, Entry, _act, _p, _wants_grad, eager, launch
 
 
 class LinearArgs(ctypes.Structure):
@@ -36,14 +36,16 @@ SYMBOLS.update({
 })
 
 
+_linear_fwd = Entry("gdn_linear_fwd", LinearArgs, need="gdn_linear_workspace_bytes")
+
+
 def _forward(x, weight, bias, residual, act, want_pre):
     M, K = x.shape
     N = weight.shape[0]
-    y = torch.empty(M, N, device=x.device, dtype=x.dtype)
-    pre = torch.empty(M, N, device=x.device, dtype=x.dtype) if want_pre and act else None
-    a = LinearArgs(_p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(pre), x.stride(0), weight.stride(0),
-                   0 if residual is None else residual.stride(0), N, M, N, K, act, 0, None, 0)
-    launch("gdn_linear_fwd", a, x.device, need="gdn_linear_workspace_bytes")
+    y = torch.empty(M, N, device=x.device, dtype=torch.bfloat16)
+    pre = torch.empty(M, N, device=x.device, dtype=torch.bfloat16) if want_pre and act else None
+    _linear_fwd(x.get_device(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(pre), x.stride(0),
+                weight.stride(0), 0 if residual is None else residual.stride(0), N, M, N, K, act, 0)
     return y, pre
 
 
@@ -74,20 +76,23 @@ class _Linear(torch.autograd.Function):
         return dx, dw, db, dy if need[3] else None, None
 
 
-def _rows(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+def _rows(t: torch.Tensor, name: str, shape, index: int) -> torch.Tensor:
     """A bf16 tensor as rows with a unit last stride."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}, got {t.device}")
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+        t = t.reshape(-1, shape[-1])
+    return t if t.stride(-1) == 1 or shape[-1] == 1 else t.contiguous()
 
 
-@torch.compiler.disable
+_ACTS = (None, "silu", "gelu")
+
+
+@eager
 def linear(x, weight, bias=None, activation=None, residual=None):
     """y = act(x weight^T + bias) + residual, in one kernel where one tile pass serves it.
 
@@ -95,18 +100,19 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     (the exact, erf form).  fp32 accumulation and epilogue, one rounding at the end.  Differentiable in x, weight, bias
     and residual; with an activation, training keeps x weight^T + bias in bf16."""
     _check_cuda(x)
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or not weight.numel():
-        raise ValueError(f"x must be (..., K) and weight (N, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
-    act = _act(activation, (None, "silu", "gelu"))
-    lead, N = x.shape[:-1], weight.shape[0]
-    rows = _rows(x, "x", x.shape, x.device) if x.dim() > 1 else _rows(x[None], "x", (1, *x.shape), x.device)
-    w = _rows(weight, "weight", weight.shape, x.device)
+    shape, index = x.shape, x.get_device()
+    if len(shape) < 1 or weight.dim() != 2 or weight.shape[1] != shape[-1] or not weight.numel():
+        raise ValueError(f"x must be (..., K) and weight (N, K), got {tuple(shape)} and {tuple(weight.shape)}")
+    act = _act(activation, _ACTS)
+    lead, N = shape[:-1], weight.shape[0]
+    rows = _rows(x, "x", shape, index) if lead else _rows(x[None], "x", (1, *shape), index)
+    w = _rows(weight, "weight", weight.shape, index)
     if bias is not None:
-        if tuple(bias.shape) != (N,) or bias.dtype != torch.bfloat16 or bias.device != x.device:
+        if bias.shape != (N,) or bias.dtype is not torch.bfloat16 or bias.get_device() != index:
             raise ValueError(f"bias must be a bfloat16 ({N},) tensor on {x.device}")
         bias = bias.contiguous()
     if residual is not None:
-        residual = _rows(residual, "residual", (*lead, N), x.device) if lead else _rows(residual[None], "residual", (1, N), x.device)
+        residual = _rows(residual, "residual", (*lead, N), index) if lead else _rows(residual[None], "residual", (1, N), index)
     if _wants_grad(rows, w, bias, residual):
         y = _Linear.apply(rows, w, bias, residual, act)
     else:

@@ -15,6 +15,8 @@ states and sums are fp32.  Calls that need gradients run the backward kernels th
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from typing import Optional
 
 import torch
@@ -74,79 +76,135 @@ SYMBOLS.update({
 })
 
 
-def _p(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _p(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def launch(name: str, args, device: torch.device, need=None) -> None:
-    """Run a library entry point on ``device``'s current stream; ``need`` names the entry point that sizes the workspace
-    of ``args`` (or of its ``fwd`` member), taken from torch's allocator for the call."""
+def eager(fn):
+    """Run ``fn`` between compiled regions under ``torch.compile``; a plain call elsewhere (a bare
+    ``torch.compiler.disable`` costs each call 1.5 us)."""
+    disabled = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        return disabled(*args, **kwargs) if torch.compiler.is_compiling() else fn(*args, **kwargs)
+
+    return call
+
+
+class Entry:
+    """An entry point taking one argument block and a stream.  The block is packed to the layout of its ctypes mirror:
+    filling 30 fields of a ctypes structure takes 3 us, packing them a third of that."""
+
+    _CODES = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint64: "Q", ctypes.c_float: "f"}
+
+    def __init__(self, name: str, block, need: Optional[str] = None):
+        self.name, self.need, self.run, self.size = name, need, None, None
+        codes = "@" + "".join(self._CODES[t] for _, t in block._fields_)
+        self.pack = struct.Struct(codes).pack
+        assert struct.calcsize(codes) == ctypes.sizeof(block), block
+
+    def __call__(self, index: int, *values) -> None:
+        """Run on device ``index``'s current stream.  ``values`` are the block's fields; with ``need``, all but the last
+        two, the workspace, which is taken from torch's allocator for the call."""
+        if self.run is None:
+            lib = load_library()
+            at = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
+            call = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
+            self.size = self.need and call(at(self.need))
+            self.run = call(at(self.name))
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return self(index, *values)
+        ws = None
+        if self.need is not None:
+            n = ctypes.c_size_t(0)
+            status = self.size(self.pack(*values, 0, 0), ctypes.addressof(n))
+            if status:
+                _check(status)
+            if n.value:
+                ws = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", index))
+            values = (*values, _p(ws), n.value)
+        status = self.run(self.pack(*values), torch._C._cuda_getCurrentRawStream(index))
+        if status:
+            _check(status)
+
+
+def launch(name: str, args, device: torch.device, need: str) -> None:
+    """Run a library entry point on ``device``'s current stream with the workspace that ``need`` sizes; ``args`` (or its
+    ``fwd`` member) holds the workspace fields."""
     lib = load_library()
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return launch(name, args, device, need)
-    ws = None
-    if need is not None:
+    with torch.cuda.device(device):
         n = ctypes.c_size_t(0)
         _check(getattr(lib, need)(ctypes.byref(args), ctypes.byref(n)))
-        if n.value:
-            ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-            holder = args if hasattr(args, "workspace") else args.fwd
-            holder.workspace, holder.workspace_bytes = ws.data_ptr(), n.value
-    status = getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
-    if status:
-        _check(status)
+        ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+        holder = args if hasattr(args, "workspace") else args.fwd
+        holder.workspace, holder.workspace_bytes = ws.data_ptr(), n.value
+        _check(getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index)))
 
 
-def _token(t: torch.Tensor, name: str, shape, dtype, device) -> torch.Tensor:
-    if tuple(t.shape) != tuple(shape):
+def _token(t: torch.Tensor, name: str, shape, dtype, index: int) -> torch.Tensor:
+    """``t`` checked against a shape and a device, in ``dtype`` with a unit last stride."""
+    if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.dtype != dtype:
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}, got {t.device}")
+    if t.dtype is not dtype:
         t = t.to(dtype)
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or shape[-1] == 1 else t.contiguous()
 
 
-def _dense(t: Optional[torch.Tensor], name: str, shape, dtype, device) -> Optional[torch.Tensor]:
-    return None if t is None else _token(t, name, shape, dtype, device).contiguous()
+def _dense(t: Optional[torch.Tensor], name: str, shape, dtype, index: int) -> Optional[torch.Tensor]:
+    return None if t is None else _token(t, name, shape, dtype, index).contiguous()
 
 
-def _dtype_of(x: torch.Tensor, name: str):
+def _device_of(x: torch.Tensor, name: str) -> int:
     _check_cuda(x)
     if x.dtype not in _DT:
         raise ValueError(f"{name} must be float32 or bfloat16, got {x.dtype}")
-    return x.dtype
+    return x.get_device()
 
 
-def _lengths(lengths, B: int, device) -> Optional[torch.Tensor]:
+def _lengths(lengths, B: int, index: int) -> Optional[torch.Tensor]:
     if lengths is None:
         return None
-    if lengths.is_floating_point() or tuple(lengths.shape) != (B,) or lengths.device != device:
-        raise ValueError(f"lengths must be an integer tensor of shape ({B},) on {device}")
+    if lengths.is_floating_point() or tuple(lengths.shape) != (B,) or lengths.get_device() != index:
+        raise ValueError(f"lengths must be an integer tensor of shape ({B},) on cuda:{index}")
     return lengths.to(torch.int32).contiguous()
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---- causal convolution -----------------------------------------------------------------------
 
 
-def _conv_args(x, weight, bias, state, act, lengths, y=None, state_out=None) -> ConvArgs:
-    tok = x.dim() == 3
-    B, T, C = x.shape if tok else (x.shape[0], 1, x.shape[1])
-    st = lambda t: (t.stride(0), t.stride(1) if tok else 0) if t is not None else (0, 0)
-    return ConvArgs(_p(x), _p(weight), _p(bias), _p(state), _p(state_out), _p(y), _p(lengths), *st(x), *st(y), B, T, C,
-                    weight.shape[1], act, _DT[x.dtype], _DT[weight.dtype])
+_conv_fwd = Entry("gdn_conv_fwd", ConvArgs)
+_conv_step = Entry("gdn_conv_step", ConvArgs)
+
+
+def _conv_values(x, weight, bias, state, act, lengths, y=None, state_out=None):
+    """The fields of ConvArgs."""
+    sx, sy = x.stride(), y.stride() if y is not None else (0, 0)
+    if x.dim() == 3:
+        B, T, C = x.shape
+        tx, ty = sx[1], sy[1]
+    else:
+        (B, C), T, tx, ty = x.shape, 1, 0, 0
+    return (x.data_ptr(), weight.data_ptr(), _p(bias), _p(state), _p(state_out), _p(y), _p(lengths), sx[0], tx, sy[0], ty, B, T, C,
+            weight.shape[1], act, _DT[x.dtype], _DT[weight.dtype])
 
 
 def _conv_forward(x, weight, bias, state, act, want_state, lengths):
     B, T, C = x.shape
     y = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
     out = torch.empty(B, C, weight.shape[1] - 1, device=x.device, dtype=x.dtype) if want_state else None
-    launch("gdn_conv_fwd", _conv_args(x, weight, bias, state, act, lengths, y, out), x.device)
+    _conv_fwd(x.get_device(), *_conv_values(x, weight, bias, state, act, lengths, y, out))
     return y, out
 
 
@@ -168,19 +226,19 @@ class _Conv(torch.autograd.Function):
         if x.numel() == 0:
             dstate = None if state is None else torch.zeros_like(state) if dlast is None else dlast
             return torch.zeros_like(x), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate, None, None, None
-        dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.device)
+        dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.get_device())
         dlast = None if dlast is None else dlast.contiguous()
         dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
         dw = torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         ds = None if state is None else torch.empty_like(state)
-        a = ConvBwdArgs(_conv_args(x, weight, bias, state, ctx.act, lengths), _p(dy), dy.stride(0), dy.stride(1), _p(dlast), _p(dx),
+        a = ConvBwdArgs(ConvArgs(*_conv_values(x, weight, bias, state, ctx.act, lengths)), _p(dy), dy.stride(0), dy.stride(1), _p(dlast), _p(dx),
                         _p(ds), _p(dw), _p(db), None, 0)
         launch("gdn_conv_bwd", a, x.device, need="gdn_conv_bwd_workspace_bytes")
         return dx, dw, db, ds, None, None, None
 
 
-def _conv_params(weight, bias, C, device):
+def _conv_params(weight, bias, C, index):
     if weight.dim() == 3 and weight.shape[1] == 1:
         weight = weight[:, 0]  # nn.Conv1d's (C, 1, W)
     if weight.dim() != 2 or weight.shape[0] != C:
@@ -189,8 +247,8 @@ def _conv_params(weight, bias, C, device):
         raise ValueError(f"the convolution kernels serve widths 2 to 4, got {weight.shape[1]}")
     if weight.dtype not in _DT:
         raise ValueError(f"weight must be float32 or bfloat16, got {weight.dtype}")
-    weight = _dense(weight, "weight", weight.shape, weight.dtype, device)
-    return weight, _dense(bias, "bias", (C,), weight.dtype, device)
+    weight = _dense(weight, "weight", weight.shape, weight.dtype, index)
+    return weight, None if bias is None else _dense(bias, "bias", (C,), weight.dtype, index)
 
 
 def _act(activation, allowed):
@@ -199,55 +257,68 @@ def _act(activation, allowed):
     return ACT[activation]
 
 
-@torch.compiler.disable
+_CONV_ACTS = (None, "silu")
+
+
+@eager
 def causal_conv(x, weight, bias=None, activation=None, initial_state=None, output_final_state=False, lengths=None):
     """Depthwise causal convolution: y_t = act(bias + sum_w weight[:, w] x_{t-W+1+w}).
 
     x (B, T, C); weight (C, W) or (C, 1, W), W 2 to 4; bias (C); activation None or "silu"; initial_state (B, C, W - 1),
     the inputs before the first token (zeros if None); lengths (B): tokens of each right-padded row (y is 0 past them).
     Returns (y, final_state or None), final_state the last W - 1 inputs, in x's dtype."""
-    dt = _dtype_of(x, "x")
+    index = _device_of(x, "x")
     if x.dim() != 3:
         raise ValueError(f"x must be (B, T, C), got {tuple(x.shape)}")
     B, T, C = x.shape
-    act = _act(activation, (None, "silu"))
-    x = _token(x, "x", x.shape, dt, x.device)
-    weight, bias = _conv_params(weight, bias, C, x.device)
-    state = _dense(initial_state, "initial_state", (B, C, weight.shape[1] - 1), dt, x.device)
-    lengths = _lengths(lengths, B, x.device)
+    act = _act(activation, _CONV_ACTS)
+    x = _token(x, "x", x.shape, x.dtype, index)
+    weight, bias = _conv_params(weight, bias, C, index)
+    state = _dense(initial_state, "initial_state", (B, C, weight.shape[1] - 1), x.dtype, index)
+    lengths = _lengths(lengths, B, index)
     if _wants_grad(x, weight, bias, state):
         return _Conv.apply(x, weight, bias, state, act, bool(output_final_state), lengths)
     return _conv_forward(x, weight, bias, state, act, bool(output_final_state), lengths)
 
 
-@torch.compiler.disable
+@eager
 def causal_conv_step(x, weight, state, bias=None, activation=None):
     """One token of ``causal_conv``: x (B, C), state (B, C, W - 1) contiguous, in x's dtype, advanced in place.  No
     autograd."""
-    dt = _dtype_of(x, "x")
+    index, dt = _device_of(x, "x"), x.dtype
     if x.dim() != 2:
         raise ValueError(f"x must be (B, C), got {tuple(x.shape)}")
     B, C = x.shape
-    act = _act(activation, (None, "silu"))
-    x = _token(x, "x", x.shape, dt, x.device)
-    weight, bias = _conv_params(weight, bias, C, x.device)
-    if tuple(state.shape) != (B, C, weight.shape[1] - 1) or state.dtype != dt or not state.is_contiguous() or state.device != x.device:
-        raise ValueError(f"state must be a contiguous {(B, C, weight.shape[1] - 1)} {dt} tensor on {x.device}: it is updated in place")
+    act = _act(activation, _CONV_ACTS)
+    x = _token(x, "x", x.shape, dt, index)
+    weight, bias = _conv_params(weight, bias, C, index)
+    want = (B, C, weight.shape[1] - 1)
+    if state.shape != want or state.dtype is not dt or not state.is_contiguous() or state.get_device() != index:
+        raise ValueError(f"state must be a contiguous {want} {dt} tensor on {x.device}: it is updated in place")
     y = torch.empty(B, C, device=x.device, dtype=dt)
-    launch("gdn_conv_step", _conv_args(x, weight, bias, state, act, None, y), x.device)
+    _conv_step(index, *_conv_values(x, weight, bias, state, act, None, y))
     return y
 
 
 # ---- selective scan ---------------------------------------------------------------------------
 
 
-def _scan_args(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y=None, h_out=None, ckpt=None) -> ScanArgs:
-    tok = x.dim() == 3
-    st = lambda t: (t.stride(0), t.stride(1) if tok else 0) if t is not None else (0, 0)
-    st3 = lambda t: (t.stride(0), t.stride(1) if tok else 0, t.stride(-2))
-    return ScanArgs(_p(x), _p(dt), _p(Bm), _p(Cm), _p(z), _p(A), _p(D), _p(bias), _p(h0), _p(lengths), _p(y), _p(h_out), _p(ckpt),
-                    *st(x), *st(dt), *st3(Bm), *st3(Cm), *st(z), *st(y), x.shape[0], x.shape[1] if tok else 1, x.shape[-1],
-                    A.shape[1], Bm.shape[-2], _DT[x.dtype], int(softplus), None, 0)
+_scan_fwd = Entry("gdn_scan_fwd", ScanArgs, need="gdn_scan_workspace_bytes")
+_scan_step = Entry("gdn_scan_step", ScanArgs)
+
+
+def _scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y=None, h_out=None, ckpt=None):
+    """The fields of ScanArgs before the workspace."""
+    sx, sdt, sB, sC = x.stride(), dt.stride(), Bm.stride(), Cm.stride()
+    sz, sy = z.stride() if z is not None else (0, 0), y.stride() if y is not None else (0, 0)
+    if x.dim() == 3:
+        B, T, Dm = x.shape
+        strides = (sx[0], sx[1], sdt[0], sdt[1], *sB[:3], *sC[:3], sz[0], sz[1], sy[0], sy[1])
+    else:
+        (B, Dm), T = x.shape, 1
+        strides = (sx[0], 0, sdt[0], 0, sB[0], 0, sB[1], sC[0], 0, sC[1], sz[0], 0, sy[0], 0)
+    return (x.data_ptr(), dt.data_ptr(), Bm.data_ptr(), Cm.data_ptr(), _p(z), A.data_ptr(), _p(D), _p(bias), _p(h0), _p(lengths), _p(y),
+            _p(h_out), _p(ckpt), *strides, B, T, Dm, A.shape[1], Bm.shape[-2], _DT[x.dtype], softplus)
 
 
 def _scan_forward(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, want_state, train):
@@ -256,8 +327,7 @@ def _scan_forward(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, want_stat
     y = torch.empty(B, T, Dm, device=x.device, dtype=x.dtype)
     h = torch.empty(B, Dm, N, device=x.device, dtype=torch.float32) if want_state else None
     ckpt = torch.empty(B, (T + SCAN_CKPT - 1) // SCAN_CKPT, Dm, N, device=x.device, dtype=torch.float32) if train else None
-    launch("gdn_scan_fwd", _scan_args(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y, h, ckpt), x.device,
-           need="gdn_scan_workspace_bytes")
+    _scan_fwd(x.get_device(), *_scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y, h, ckpt))
     return y, h, ckpt
 
 
@@ -280,10 +350,10 @@ class _Scan(torch.autograd.Function):
         if x.numel() == 0:
             zero = [None if t is None else torch.zeros_like(t) for t in (x, dt, A, Bm, Cm, D, z, bias)]
             return (*zero, None if h0 is None else torch.zeros_like(h0) if dh is None else dh, None, None, None)
-        dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.device)
+        dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.get_device())
         dh = None if dh is None else dh.contiguous()
         dx, ddt, dA, dB, dC, dD, dz, db, dh0 = (new(t) for t in (x, dt, A, Bm, Cm, D, z, bias, h0))
-        a = ScanBwdArgs(_scan_args(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ctx.softplus, ckpt=ckpt), _p(dy), dy.stride(0), dy.stride(1),
+        a = ScanBwdArgs(ScanArgs(*_scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ctx.softplus, ckpt=ckpt)), _p(dy), dy.stride(0), dy.stride(1),
                         _p(dh), _p(dx), _p(ddt), _p(dB), _p(dC), _p(dz), _p(dA), _p(dD), _p(db), _p(dh0))
         launch("gdn_scan_bwd", a, x.device, need="gdn_scan_bwd_workspace_bytes")
         return dx, ddt, dA, dB, dC, dD, dz, db, dh0, None, None, None
@@ -291,28 +361,31 @@ class _Scan(torch.autograd.Function):
 
 def _scan_inputs(x, dt, A, B, C, D, z, dt_bias):
     """Checked inputs: token tensors in x's dtype with unit last strides, B and C (..., G, N), parameters fp32."""
-    ty, dev, tok, Dm = _dtype_of(x, "x"), x.device, x.shape[:-1], x.shape[-1]
+    index, ty, shape, nd = _device_of(x, "x"), x.dtype, x.shape, x.dim()
+    tok, Dm = shape[:-1], shape[-1]
     if A.dim() != 2 or A.shape[0] != Dm:
         raise ValueError(f"A must be ({Dm}, N), got {tuple(A.shape)}")
     N = A.shape[1]
     if not 1 <= N <= 64:
         raise ValueError(f"the scan kernels serve 1 to 64 states per channel, got {N}")
-    if B.dim() == x.dim():
+    if B.dim() == nd:
         B = B.unsqueeze(-2)
-    if C.dim() == x.dim():
+    if C.dim() == nd:
         C = C.unsqueeze(-2)
-    G = B.shape[-2] if B.dim() == x.dim() + 1 else 0
+    G = B.shape[-2] if B.dim() == nd + 1 else 0
     if G < 1 or Dm % G:
         raise ValueError(f"B must be {(*tok, N)} or {(*tok, 'G', N)} with G a divisor of {Dm}, got {tuple(B.shape)}")
-    x = _token(x, "x", x.shape, ty, dev)
-    dt = _token(dt, "dt", x.shape, ty, dev)
-    B, C = _token(B, "B", (*tok, G, N), ty, dev), _token(C, "C", (*tok, G, N), ty, dev)
-    z = None if z is None else _token(z, "z", x.shape, ty, dev)
-    A = _dense(A, "A", (Dm, N), torch.float32, dev)
-    return x, dt, A, B, C, _dense(D, "D", (Dm,), torch.float32, dev), z, _dense(dt_bias, "dt_bias", (Dm,), torch.float32, dev)
+    x = _token(x, "x", shape, ty, index)
+    dt = _token(dt, "dt", shape, ty, index)
+    states = (*tok, G, N)
+    B, C = _token(B, "B", states, ty, index), _token(C, "C", states, ty, index)
+    if z is not None:
+        z = _token(z, "z", shape, ty, index)
+    A = _dense(A, "A", A.shape, torch.float32, index)
+    return index, x, dt, A, B, C, _dense(D, "D", (Dm,), torch.float32, index), z, _dense(dt_bias, "dt_bias", (Dm,), torch.float32, index)
 
 
-@torch.compiler.disable
+@eager
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None, output_final_state=False,
                    lengths=None):
     """Selective state space scan over a block of tokens.
@@ -326,24 +399,24 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     Training keeps one state per 8 tokens."""
     if x.dim() != 3:
         raise ValueError(f"x must be (B, T, D), got {tuple(x.shape)}")
-    x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
-    h0 = _dense(initial_state, "initial_state", (x.shape[0], x.shape[2], A.shape[1]), torch.float32, x.device)
-    lengths = _lengths(lengths, x.shape[0], x.device)
+    index, x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
+    h0 = _dense(initial_state, "initial_state", (x.shape[0], x.shape[2], A.shape[1]), torch.float32, index)
+    lengths = _lengths(lengths, x.shape[0], index)
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
         return _Scan.apply(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus), bool(output_final_state))
     return _scan_forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus), bool(output_final_state), False)[:2]
 
 
-@torch.compiler.disable
+@eager
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False):
     """One token of ``selective_scan``: x, dt, z (B, D), B, C (B, N) or (B, G, N), state (B, D, N) fp32 contiguous,
     advanced in place.  No autograd."""
     if x.dim() != 2:
         raise ValueError(f"x must be (B, D), got {tuple(x.shape)}")
-    x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
+    index, x, dt, A, B, C, D, z, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
     want = (x.shape[0], x.shape[1], A.shape[1])
-    if tuple(state.shape) != want or state.dtype != torch.float32 or not state.is_contiguous() or state.device != x.device:
+    if state.shape != want or state.dtype is not torch.float32 or not state.is_contiguous() or state.get_device() != index:
         raise ValueError(f"state must be a contiguous {want} float32 tensor on {x.device}: it is updated in place")
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    launch("gdn_scan_step", _scan_args(x, dt, A, B, C, D, z, dt_bias, None, None, dt_softplus, y, state), x.device)
+    y = torch.empty(want[0], want[1], device=x.device, dtype=x.dtype)
+    _scan_step(index, *_scan_values(x, dt, A, B, C, D, z, dt_bias, None, None, bool(dt_softplus), y, state), 0, 0)
     return y

@@ -111,7 +111,8 @@ SCAN = [  # B, T, D, N, G, dtype, gate, skip, bias, softplus, state, lengths, pa
     (3, 37, 144, 8, 1, "bf16", True, True, True, True, True, True, 0),
     (2, 50, 260, 4, 1, "f32", True, True, True, True, True, True, 0),
     (3, 41, 72, 16, 3, "bf16", False, False, True, True, True, True, 0),
-    (2, 33, 80, 16, 2, "f32", True, True, True, False, True, False, 0),
+    (2, 33, 80, 16, 2, "f32", True, True, True, True, True, False, 0),
+    (2, 40, 48, 16, 1, "f32", True, True, False, False, True, True, 0),
     (2, 57, 48, 24, 1, "bf16", True, True, True, True, True, True, 0),
     (2, 35, 40, 32, 1, "f32", True, True, False, True, True, True, 0),
     (2, 43, 24, 64, 1, "bf16", True, True, True, True, True, True, 0),
