@@ -185,12 +185,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
 // What bounds it beside the exponentials is shared memory's 128 bytes a clock into registers (a broadcast saves nothing
 // there), so a lane's B and C serve two channels: (s, u) of both, B and C are 48 bytes for eight states; with one
 // channel per lane the recurrence alone cost 386 us at 8 x 4096 tokens, 2048 channels, 16 states.  A warp by itself needs
-// no barrier, and 16 channels per block balance the 148 SMs better than 32.  Raw tiles of 16 tokens come in by
+// no barrier, and 16 channels per block balance the 148 SMs better than 32.  Raw tiles of 8 tokens (16 take
+// 4 % off 7 warps per SM and cost up to half where shared memory then holds 8 instead of 12 or more) come in by
 // asynchronous copies; a thread runs the recurrence of tile k, forms the step sizes of tile k + 1 and finishes the
 // outputs of tile k - 1 in one straight piece of code, so that their latencies overlap.
 template <typename T, int NL, int SL>
 struct Tiled {
-  static constexpr int TT = 16, CH = 64 / NL, NP = NL * SL, ES = (int)sizeof(T), RING = 4;
+  static constexpr int TT = 8, CH = 64 / NL, NP = NL * SL, ES = (int)sizeof(T), RING = 4;
   static constexpr int ROW = CH * ES, BROW = NP * ES;           // bytes of a token's channels, states
   static constexpr int RAW = TT * (3 * ROW + 2 * BROW);         // x, dt, z, B, C of a tile
   static constexpr int S_OFF = RING * RAW, S_BYTES = TT * CH * 8;
@@ -547,6 +548,185 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanP p) {
   }
 }
 
+// The same for rows that 16-byte copies can take: scan_fwd_tiled_kernel without outputs.  Reversed, tiles and their tokens
+// run from the last to the first.
+template <typename T, int NL, int SL>
+struct CarryTiled {
+  static constexpr int TT = 8, CH = 64 / NL, NP = NL * SL, ES = (int)sizeof(T), RING = 4;
+  static constexpr int ROW = CH * ES, BROW = NP * ES;
+  static constexpr int RAW = TT * (3 * ROW + BROW);  // x, dt and B, or dy, dt, z and C
+  static constexpr int S_OFF = RING * RAW, S_BYTES = TT * CH * 8;
+  static constexpr int BC_OFF = S_OFF + 2 * S_BYTES, BC_BYTES = TT * NP * 4;
+  static constexpr int SMEM = BC_OFF + 2 * BC_BYTES;
+  static constexpr int XCH = ROW / 16, BCH = BROW / 16;
+  static constexpr int CHUNKS = TT * (3 * XCH + BCH), COPIES = (CHUNKS + 31) / 32;
+};
+
+template <typename T, int NL, int SL, bool REV>
+__global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
+  using K = CarryTiled<T, NL, SL>;
+  constexpr int TT = K::TT, CH = K::CH, NP = K::NP, PAIRS = SL / 2, PER = TT / NL, QUADS = TT * NP / 4;
+  constexpr int QI = (QUADS + 31) / 32;
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x;
+  const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
+  const int seg = blockIdx.y, b = blockIdx.z;
+  if (seg == (REV ? 0 : p.nseg - 1)) return;  // nothing enters from here
+  const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
+  const int len = row_tokens(p.lengths, b, p.T);
+  const int tbeg = seg * p.seg_len, lim = min(min(tbeg + p.seg_len, p.T), len);
+  const int ntile = lim > tbeg ? (lim - tbeg + TT - 1) / TT : 0;
+  auto tile = [&](int k) { return REV ? ntile - 1 - k : k; };
+
+  const char* src[K::COPIES];
+  int64_t step[K::COPIES];
+  int tok[K::COPIES];
+  constexpr int NONE = 1 << 29;
+#pragma unroll
+  for (int i = 0; i < K::COPIES; ++i) {
+    int c = lane + i * 32;
+    tok[i] = NONE;
+    src[i] = static_cast<const char*>(p.dt);
+    step[i] = 0;
+    const void* base;
+    int64_t sb, st, off;
+    int r, j, bytes;
+    if (c < 3 * TT * K::XCH) {
+      const int which = c / (TT * K::XCH);
+      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = d0;
+      base = which == 1 ? p.dt : which == 2 ? (REV ? p.z : nullptr) : REV ? p.dy : p.x;
+      sb = which == 1 ? p.sdt_b : which == 2 ? p.sz_b : REV ? p.sdy_b : p.sx_b;
+      st = which == 1 ? p.sdt_t : which == 2 ? p.sz_t : REV ? p.sdy_t : p.sx_t;
+    } else {
+      c -= 3 * TT * K::XCH;
+      r = c / K::BCH; j = c % K::BCH; bytes = r < TT ? p.N * K::ES : 0;
+      base = REV ? p.Cm : p.Bm;
+      sb = REV ? p.sC_b : p.sB_b;
+      st = REV ? p.sC_t : p.sB_t;
+      off = grp * (REV ? p.sC_g : p.sB_g);
+    }
+    if (base && j * 16 < bytes) {
+      tok[i] = r;
+      src[i] = static_cast<const char*>(base) + (b * sb + ((int64_t)tbeg + tile(0) * TT + r) * st + off) * K::ES + j * 16;
+      step[i] = (REV ? -st : st) * TT * K::ES;
+    }
+  }
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  auto fetch = [&](int k) {
+    if (k < ntile) {
+#pragma unroll
+      for (int i = 0; i < K::COPIES; ++i) {
+        if (K::CHUNKS % 32 == 0 || lane + i * 32 < K::CHUNKS)
+          copy16(ring + (k & (K::RING - 1)) * K::RAW + (lane + i * 32) * 16, src[i], tbeg + tile(k) * TT + tok[i] < lim);
+        src[i] += step[i];
+      }
+    }
+    copies_commit();
+  };
+  const int hc = lane / NL * 2, n0 = lane % NL * SL;
+  const bool live = hc < nch && n0 < p.N;
+  f32x2 h[2][PAIRS];
+  float A2[2][SL];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int i = 0; i < SL; ++i) A2[c][i] = live && n0 + i < p.N ? p.A[(int64_t)(d0 + hc + c) * p.N + n0 + i] * LOG2E : 0.f;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) h[c][i] = both(0.f);
+  }
+  const int cc = lane % (CH / 2) * 2, ct0 = lane / (CH / 2);
+  const int d = d0 + (cc < nch ? cc : 0);
+  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], p.dt_bias[d + 1]) : both(0.f);
+  f32x2 total = both(0.f);
+  auto stage = [&](int k, int i) {
+    const int r = ct0 + i * NL;
+    const char* raw = smem + (k & (K::RING - 1)) * K::RAW + r * K::ROW + cc * K::ES;
+    f32x2 s = add2(load_pair(reinterpret_cast<const T*>(raw + TT * K::ROW)), bias);
+    s = p.softplus ? softplus2(s) : s;
+    f32x2 u = load_pair(reinterpret_cast<const T*>(raw));
+    if (REV) {
+      const f32x2 z = load_pair(reinterpret_cast<const T*>(raw + 2 * TT * K::ROW));
+      u = p.z ? mul2(u, mul2(z, sigmoid2(z))) : u;
+    } else {
+      u = mul2(u, s);
+    }
+    const bool on = tbeg + tile(k) * TT + r < lim;
+    s = on ? s : both(0.f);
+    u = on ? u : both(0.f);
+    total = add2(total, s);
+    const float2 sv = unpack2(s), uv = unpack2(u);
+    return make_float4(sv.x, uv.x, sv.y, uv.y);
+  };
+  auto stage_all = [&](int k) {
+    float4 v[PER];
+    ulonglong2 q[QI];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = stage(k, i);
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+      if (QUADS % 32 && lane + i * 32 >= QUADS) break;
+      const T* raw = reinterpret_cast<const T*>(smem + (k & (K::RING - 1)) * K::RAW + 3 * TT * K::ROW) + (lane + i * 32) * 4;
+      q[i] = make_ulonglong2(load_pair(raw), load_pair(raw + 2));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      *(reinterpret_cast<float4*>(smem + K::S_OFF + (k & 1) * K::S_BYTES) + ((ct0 + i * NL) * CH + cc) / 2) = v[i];
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+      if (QUADS % 32 && lane + i * 32 >= QUADS) break;
+      reinterpret_cast<ulonglong2*>(smem + K::BC_OFF + (k & 1) * K::BC_BYTES)[lane + i * 32] = q[i];
+    }
+  };
+  fetch(0);
+  fetch(1);
+  if (ntile > 0) {
+    copies_wait<1>();
+    __syncwarp();
+    stage_all(0);
+  }
+#pragma unroll 1
+  for (int k = 0; k < ntile; ++k) {
+    copies_wait<0>();
+    __syncwarp();
+    fetch(k + 2);
+    const float4* sS = reinterpret_cast<const float4*>(smem + K::S_OFF + (k & 1) * K::S_BYTES) + hc / 2;
+    const float* sB = reinterpret_cast<const float*>(smem + K::BC_OFF + (k & 1) * K::BC_BYTES) + n0;
+#pragma unroll
+    for (int q = 0; q < TT; ++q) {  // only reads until the staging of the next tile
+      const int r = REV ? TT - 1 - q : q;
+      const float4 su = sS[r * (CH / 2)];
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 bv = *reinterpret_cast<const float2*>(sB + r * NP + 2 * i);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float s = c ? su.z : su.x, u = c ? su.w : su.y;
+          const f32x2 a = pack2(ex2(s * A2[c][2 * i]), ex2(s * A2[c][2 * i + 1])), w = pack2(u * bv.x, u * bv.y);
+          h[c][i] = REV ? mul2(a, add2(h[c][i], w)) : fma2(a, h[c][i], w);
+        }
+      }
+    }
+    if (k + 1 < ntile) stage_all(k + 1);
+  }
+  const int64_t row = (int64_t)b * p.nseg + seg;
+  if (live) {
+    float* to = p.carry + (row * p.D + d0) * p.N;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < PAIRS; i += 2)
+        if (n0 + 2 * i < p.N)
+          *reinterpret_cast<ulonglong2*>(to + (int64_t)(hc + c) * p.N + n0 + 2 * i) = make_ulonglong2(h[c][i], h[c][i + 1]);
+  }
+  float2 sum = unpack2(total);
+#pragma unroll
+  for (int o = CH / 2; o < 32; o *= 2) {
+    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+  }
+  if (ct0 == 0 && cc < nch) *reinterpret_cast<float2*>(p.ssum + row * p.D + d0 + cc) = sum;
+}
+
 // carry[seg] <- the state that enters segment seg.  One thread per (row, channel, state).
 template <bool REV>
 __global__ void __launch_bounds__(256) scan_combine_kernel(ScanP p) {
@@ -607,11 +787,15 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_step_kernel(ScanP p) {
   }
 }
 
-SegPlan scan_segments(int64_t B, int64_t T, int64_t blocks_per_row) {
-  constexpr int64_t FILL = 148 * 4, MIN_SEG = 128;
-  SegPlan one = {1, (int)T};
-  if (B * blocks_per_row >= FILL / 2 || T < 2 * MIN_SEG) return one;
-  int64_t n = (FILL * 2 + B * blocks_per_row - 1) / (B * blocks_per_row);
+// Time is split where the rows leave the SMs short of warps.  A split adds the local pass (0.6 of the scan's own work);
+// a warp alone on a scheduler runs at 0.11 of the rate of a full SM (16 warps), so splitting pays below about 5 warps
+// per SM, and then fills one wave (1 x 65536 tokens, 2048 channels: 128 warps unsplit, 18 segments).
+SegPlan scan_segments(int64_t B, int64_t T, int64_t warps_per_row) {
+  constexpr int64_t SMS = 148, MIN_SEG = 128;
+  const SegPlan one = {1, (int)T};
+  const int64_t warps = B * warps_per_row;
+  if (warps >= SMS * 5 || T < 2 * MIN_SEG) return one;
+  int64_t n = SMS * 16 / warps;
   if (n > T / MIN_SEG) n = T / MIN_SEG;
   if (n < 2) return one;
   const int64_t len = ((T + n - 1) / n + TT - 1) / TT * TT;
@@ -661,14 +845,15 @@ ScanP scan_params(const gdn_scan_args* a) {
   auto quad = [&](const void* q, int64_t sb, int64_t st, int64_t sg) { return (uintptr_t)q % (4 * es) == 0 && sb % 4 == 0 && st % 4 == 0 && sg % 4 == 0; };
   p.quads = a->N % 4 == 0 && a->N == scan_lanes(a->N) * SPL && quad(a->Bm, a->sB_b, a->sB_t, a->sB_g) && quad(a->Cm, a->sC_b, a->sC_t, a->sC_g);
   p.dblocks = scan_dblocks(a->D, a->G, a->N);
-  const SegPlan sp = scan_segments(a->B > 0 ? a->B : 1, a->T, (int64_t)p.dblocks * a->G);
+  const int64_t warp_channels = a->N <= 8 ? 32 : a->N <= 16 ? 16 : 8;  // of the kernels for aligned rows
+  const SegPlan sp = scan_segments(a->B > 0 ? a->B : 1, a->T, (a->D / a->G + warp_channels - 1) / warp_channels * a->G);
   p.nseg = sp.nseg;
   p.seg_len = sp.seg_len;
   return p;
 }
 
 template <typename T, bool REV>
-void launch_carry(const ScanP& p, int nl, cudaStream_t s) {
+void launch_carry_plain(const ScanP& p, int nl, cudaStream_t s) {
   const dim3 g(p.dblocks * p.G, p.nseg, p.B);
   if (nl == 2) scan_carry_kernel<T, 2, REV><<<g, SCAN_THREADS, 0, s>>>(p);
   if (nl == 4) scan_carry_kernel<T, 4, REV><<<g, SCAN_THREADS, 0, s>>>(p);
@@ -676,17 +861,41 @@ void launch_carry(const ScanP& p, int nl, cudaStream_t s) {
   if (nl == 16) scan_carry_kernel<T, 16, REV><<<g, SCAN_THREADS, 0, s>>>(p);
 }
 
+template <typename T, int NL, int SL, bool REV>
+int launch_carry_tiled(ScanP p, cudaStream_t s) {
+  using K = CarryTiled<T, NL, SL>;
+  static std::atomic<unsigned long long> opted{0};
+  auto k = scan_carry_tiled_kernel<T, NL, SL, REV>;
+  if (!opt_in_smem(opted, {{(const void*)k, K::SMEM}})) return GDN_ERR_LAUNCH;
+  p.dblocks = (p.D / p.G + K::CH - 1) / K::CH;
+  k<<<dim3(p.dblocks * p.G, p.nseg, p.B), 32, K::SMEM, s>>>(p);
+  return launched();
+}
+template <typename T, bool REV>
+int launch_carry(const ScanP& p, cudaStream_t s) {
+  const int v = 16 / (int)sizeof(T);
+  if (scan_rows16(p, sizeof(T)) && (!REV || (aligned16(p.dy) && p.sdy_b % v == 0 && p.sdy_t % v == 0)))
+    return p.N <= 8    ? launch_carry_tiled<T, 2, 4, REV>(p, s)
+           : p.N <= 16 ? launch_carry_tiled<T, 4, 4, REV>(p, s)
+           : p.N <= 32 ? launch_carry_tiled<T, 8, 4, REV>(p, s)
+                       : launch_carry_tiled<T, 8, 8, REV>(p, s);
+  launch_carry_plain<T, REV>(p, scan_lanes(p.N), s);
+  return launched();
+}
+
 int scan_launch_carry(const ScanP& p, int dtype, bool reverse, cudaStream_t s) {
-  const int nl = scan_lanes(p.N);
   const int64_t g = ((int64_t)p.B * p.D * p.N + 255) / 256;
   if (g > 0x7fffffff) return GDN_ERR_SHAPE;
-  if (reverse) {
-    dtype == GDN_DTYPE_F32 ? launch_carry<float, true>(p, nl, s) : launch_carry<__nv_bfloat16, true>(p, nl, s);
+  int st;
+  if (reverse)
+    st = dtype == GDN_DTYPE_F32 ? launch_carry<float, true>(p, s) : launch_carry<__nv_bfloat16, true>(p, s);
+  else
+    st = dtype == GDN_DTYPE_F32 ? launch_carry<float, false>(p, s) : launch_carry<__nv_bfloat16, false>(p, s);
+  if (st != GDN_OK) return st;
+  if (reverse)
     scan_combine_kernel<true><<<(unsigned)g, 256, 0, s>>>(p);
-  } else {
-    dtype == GDN_DTYPE_F32 ? launch_carry<float, false>(p, nl, s) : launch_carry<__nv_bfloat16, false>(p, nl, s);
+  else
     scan_combine_kernel<false><<<(unsigned)g, 256, 0, s>>>(p);
-  }
   return launched();
 }
 

@@ -125,11 +125,11 @@ __device__ __forceinline__ int spread_sum(float (&v)[NV], int lane) {
   return first;
 }
 
-// Segments: as many as fill the device when B x channel blocks do not, each of at least MIN_SEG tokens.
+// Segments of time, each at least MIN_SEG tokens.
 struct SegPlan {
   int nseg, seg_len;
 };
-SegPlan scan_segments(int64_t B, int64_t T, int64_t blocks_per_row);
+SegPlan scan_segments(int64_t B, int64_t T, int64_t warps_per_row);
 
 // Lanes per channel: 2, 4, 8 or 16 for N up to 8, 16, 32, 64.
 inline int scan_lanes(int64_t N) {

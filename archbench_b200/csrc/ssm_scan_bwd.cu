@@ -222,7 +222,8 @@ struct BwdTiled {
   static constexpr int P_OFF = S_OFF + 2 * S_BYTES, P_BYTES = TT * SCAN_THREADS * 24;  // (g.B, ds) parts, then C.h parts
   static constexpr int BC_OFF = P_OFF + 2 * P_BYTES, BC_BYTES = 2 * TT * NP * 4;
   static constexpr int R_OFF = BC_OFF + 2 * BC_BYTES, R_BYTES = WARPS * TT * 2 * NP * 4;  // dB, dC of each warp
-  static constexpr int SMEM = R_OFF + 2 * R_BYTES;
+  static constexpr int A_OFF = R_OFF + 2 * R_BYTES, A_BYTES = SCAN_THREADS * 32;  // each lane's dA
+  static constexpr int SMEM = A_OFF + A_BYTES;
   static constexpr int XCH = ROW / 16, BCH = BROW / 16;
   static constexpr int CHUNKS = TT * (4 * XCH + 2 * BCH), COPIES = (CHUNKS + SCAN_THREADS - 1) / SCAN_THREADS;
 };
@@ -298,7 +299,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   // per-state role: channels hc, hc + 1 of the block
   const int hc = tid / NL * 2, n0 = tid % NL * SPL;
   const bool live = hc < nch && n0 < p.N;
-  f32x2 G[2][2], A2[2][2], dA[2][2];
+  f32x2 G[2][2], A2[2][2];
+  // dA of the lane, two halves of four states; a tile's terms are summed first, which keeps both its rounding and the
+  // registers small
+  ulonglong2* dA_sum = reinterpret_cast<ulonglong2*>(smem + K::A_OFF) + tid;
   const int64_t own = (int64_t)(d0 + hc) * p.N + n0;  // of channel hc; channel hc + 1 is N further
   const float* from = p.nseg > 1 ? p.carry + row * p.D * p.N : p.dh_out ? p.dh_out + (int64_t)b * p.D * p.N : nullptr;
   auto load4 = [&](const float* q, int c, f32x2 (&v)[2]) {
@@ -314,10 +318,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
     load4(from, c, G[c]);
     load4(p.A, c, A2[c]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      A2[c][i] = mul2(A2[c][i], both(LOG2E));
-      dA[c][i] = both(0.f);
-    }
+    for (int i = 0; i < 2; ++i) A2[c][i] = mul2(A2[c][i], both(LOG2E));
+    dA_sum[c * SCAN_THREADS] = make_ulonglong2(0, 0);
   }
   const int nck = (p.T + TT - 1) / TT;
   auto checkpoint = [&](int k, int c, f32x2 (&v)[2]) {
@@ -464,15 +466,28 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
       stage_bc(k + 1);
     }
     // the adjoint
+    f32x2 dA[2][2];
     ulonglong2* p4 = reinterpret_cast<ulonglong2*>(smem + K::P_OFF + (k & 1) * K::P_BYTES) + tid;
     f32x2* p2 = reinterpret_cast<f32x2*>(smem + K::P_OFF + (k & 1) * K::P_BYTES + TT * SCAN_THREADS * 16) + tid;
     float* red = reinterpret_cast<float*>(smem + K::R_OFF + (k & 1) * K::R_BYTES) + warp * TT * 2 * NP;
+    // A token's reads are issued before the stores of the token ahead of it: shared memory keeps the order of both.
+    struct Token {
+      float4 su;
+      f32x2 dc;
+      ulonglong2 bv, cv;
+    };
+    auto token = [&](int r) {
+      return Token{su_p[r * (CH / 2)], dc_p[r * (CH / 2)], *reinterpret_cast<const ulonglong2*>(sB + r * NP),
+                   *reinterpret_cast<const ulonglong2*>(sB + (TT + r) * NP)};
+    };
+    Token nxt = token(TT - 1);
 #pragma unroll
     for (int r = TT - 1; r >= 0; --r) {
-      const float4 su = su_p[r * (CH / 2)];
-      const float2 dc = unpack2(dc_p[r * (CH / 2)]);
-      const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(sB + r * NP);
-      const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sB + (TT + r) * NP);
+      const Token cur = nxt;
+      if (r > 0) nxt = token(r - 1);
+      const float4 su = cur.su;
+      const float2 dc = unpack2(cur.dc);
+      const ulonglong2 bv = cur.bv, cv = cur.cv;
       f32x2 dB[2], dC[2];
       float gb[2], ds[2], core[2];
 #pragma unroll
@@ -489,8 +504,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
         G[c][1] = mul2(a[r][c][1], g1);
         const f32x2 f0 = mul2(G[c][0], h[r][c][0]), f1 = mul2(G[c][1], h[r][c][1]);
         ds[c] = sum2(fma2(f1, A2[c][1], mul2(f0, A2[c][0])));
-        dA[c][0] = fma2(f0, sd, dA[c][0]);
-        dA[c][1] = fma2(f1, sd, dA[c][1]);
+        dA[c][0] = r == TT - 1 ? mul2(f0, sd) : fma2(f0, sd, dA[c][0]);
+        dA[c][1] = r == TT - 1 ? mul2(f1, sd) : fma2(f1, sd, dA[c][1]);
       }
       p4[r * SCAN_THREADS] = make_ulonglong2(pack2(gb[0], gb[1]), pack2(ds[0], ds[1]));
       p2[r * SCAN_THREADS] = pack2(core[0], core[1]);
@@ -500,6 +515,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
       constexpr int LEFT = 8 * NL / 32 > 1 ? 8 * NL / 32 : 1;
 #pragma unroll
       for (int i = 0; i < LEFT; ++i) red[r * 2 * NP + (f + i) / SPL * NP + n0 + (f + i) % SPL] = v[i];
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const ulonglong2 v = dA_sum[c * SCAN_THREADS];
+      dA_sum[c * SCAN_THREADS] = make_ulonglong2(add2(v.x, dA[c][0]), add2(v.y, dA[c][1]));
     }
   }
   __syncthreads();
@@ -523,7 +543,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    store4(p.pA + row * p.D * p.N, c, dA[c]);
+    const ulonglong2 v = dA_sum[c * SCAN_THREADS];
+    const f32x2 dA[2] = {v.x, v.y};
+    store4(p.pA + row * p.D * p.N, c, dA);
     if (p.dh0 && seg == 0) store4(p.dh0 + (int64_t)b * p.D * p.N, c, G[c]);
   }
   // dD and ddt_bias over the threads of a channel pair
