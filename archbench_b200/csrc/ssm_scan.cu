@@ -15,8 +15,9 @@ constexpr int TT = 32;  // tokens per tile of the local pass; segments are whole
 // per-token role (CV channels of some tokens): raw values of the next tile are already in registers while this one is
 // computed, so no load is waited for.  In their per-state role the threads read (s, s, s x, s x) of their channel and
 // the B and C of their four states, and leave their part of C . h in shared memory; the per-token role adds the parts.
-template <typename T, int NL, int CV>
+template <typename T, int NL>
 __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p) {
+  constexpr int CV = 1;  // channels per thread and token
   constexpr int TT = NL == 2 ? 16 : 32;  // tokens per tile (shared memory)
   constexpr int CH = SCAN_THREADS / NL, NP = NL * SPL;
   constexpr int TSTEP = SCAN_THREADS * CV / CH, PER = TT / TSTEP;  // tokens covered at once, tokens per thread
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
   }
 }
 
-// The same pass for rows that 16-byte copies can take; one warp per block.  A lane holds SL states of two channels.
+// The same pass where N is a multiple of four (rows are 16-byte aligned, or were laid out so); one warp per block.  A lane holds SL states of two channels.
 // What bounds it beside the exponentials is shared memory's 128 bytes a clock into registers (a broadcast saves nothing
 // there), so a lane's B and C serve two channels: (s, u) of both, B and C are 48 bytes for eight states; with one
 // channel per lane the recurrence alone cost 386 us at 8 x 4096 tokens, 2048 channels, 16 states.  A warp by itself needs
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
     int r, j, bytes;
     if (c < 3 * TT * K::XCH) {
       const int which = c / (TT * K::XCH);
-      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = d0;
+      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = (int64_t)grp * p.xgs + dblk * CH;
       base = which == 0 ? p.x : which == 1 ? p.dt : p.z;
       sb = which == 0 ? p.sx_b : which == 1 ? p.sdt_b : p.sz_b;
       st = which == 0 ? p.sx_t : which == 1 ? p.sdt_t : p.sz_t;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
     float hv[SL];
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
-      const bool ok = live && n0 + i < p.N;
+      const bool ok = live && hc + c < nch && n0 + i < p.N;
       const int64_t at = (int64_t)(d0 + hc + c) * p.N + n0 + i;
       A2[c][i] = ok ? p.A[at] * LOG2E : 0.f;
       hv[i] = ok && from ? from[at] : 0.f;
@@ -293,15 +294,24 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int i = 0; i < PAIRS; i += 2)
-        if (n0 + 2 * i < p.N)
+        if (hc + c < nch && n0 + 2 * i < p.N)
           *reinterpret_cast<ulonglong2*>(to + (int64_t)(hc + c) * p.N + n0 + 2 * i) = make_ulonglong2(h[c][i], h[c][i + 1]);
   };
   // per-token role: channels cc, cc + 1, tokens ct0, ct0 + NL, ...
   const int cc = lane % (CH / 2) * 2, ct0 = lane / (CH / 2);
   const bool cok = cc < nch;
   const int d = d0 + (cok ? cc : 0);
-  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], p.dt_bias[d + 1]) : both(0.f);
-  const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], p.Dskip[d + 1]) : both(0.f);
+  const bool two = cc + 1 < nch;  // an odd group's last pair has one channel
+  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], two ? p.dt_bias[d + 1] : 0.f) : both(0.f);
+  const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], two ? p.Dskip[d + 1] : 0.f) : both(0.f);
+  auto put_pair = [&](T* q, const float (&v)[2]) {
+    if (p.pairs_out) {
+      store_raw<T, 2>(q, v);
+    } else {
+      store_as(q, v[0]);
+      if (two) store_as(q + 1, v[1]);
+    }
+  };
   T* yp = static_cast<T*>(p.y) + b * p.sy_b + d;
   const int nck = (p.T + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT;
 
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
     const f32x2 gate = p.z ? mul2(g.z, sigmoid2(g.z)) : both(1.f);
     const float2 v = unpack2(mul2(fma2(skip, g.x, g.core), gate));
     const float out[2] = {t < lim ? v.x : 0.f, t < lim ? v.y : 0.f};
-    if (cok && t >= tbeg && t < tend) store_raw<T, 2>(yp + t * p.sy_t, out);
+    if (cok && t >= tbeg && t < tend) put_pair(yp + t * p.sy_t, out);
   };
   struct Tokens {  // what GT tokens of the recurrence read
     float4 su[GT], b[GT][SL / 4];
@@ -460,7 +470,7 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
   // past the row's tokens
   const float zero[2] = {0.f, 0.f};
   if (cok)
-    for (int t = tbeg + ntile * TT + ct0; t < tend; t += NL) store_raw<T, 2>(yp + t * p.sy_t, zero);
+    for (int t = tbeg + ntile * TT + ct0; t < tend; t += NL) put_pair(yp + t * p.sy_t, zero);
   if (p.h_out && seg == p.nseg - 1) put_states(p.h_out + ((int64_t)b * p.D + d0) * p.N);
 }
 
@@ -548,7 +558,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanP p) {
   }
 }
 
-// The same for rows that 16-byte copies can take: scan_fwd_tiled_kernel without outputs.  Reversed, tiles and their tokens
+// The same where N is a multiple of four: scan_fwd_tiled_kernel without outputs.  Reversed, tiles and their tokens
 // run from the last to the first.
 template <typename T, int NL, int SL>
 struct CarryTiled {
@@ -593,7 +603,7 @@ __global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
     int r, j, bytes;
     if (c < 3 * TT * K::XCH) {
       const int which = c / (TT * K::XCH);
-      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = d0;
+      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = (int64_t)grp * p.xgs + dblk * CH;
       base = which == 1 ? p.dt : which == 2 ? (REV ? p.z : nullptr) : REV ? p.dy : p.x;
       sb = which == 1 ? p.sdt_b : which == 2 ? p.sz_b : REV ? p.sdy_b : p.sx_b;
       st = which == 1 ? p.sdt_t : which == 2 ? p.sz_t : REV ? p.sdy_t : p.sx_t;
@@ -630,13 +640,14 @@ __global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int i = 0; i < SL; ++i) A2[c][i] = live && n0 + i < p.N ? p.A[(int64_t)(d0 + hc + c) * p.N + n0 + i] * LOG2E : 0.f;
+    for (int i = 0; i < SL; ++i) A2[c][i] = live && hc + c < nch && n0 + i < p.N ? p.A[(int64_t)(d0 + hc + c) * p.N + n0 + i] * LOG2E : 0.f;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) h[c][i] = both(0.f);
   }
   const int cc = lane % (CH / 2) * 2, ct0 = lane / (CH / 2);
   const int d = d0 + (cc < nch ? cc : 0);
-  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], p.dt_bias[d + 1]) : both(0.f);
+  const bool two = cc + 1 < nch;  // an odd group's last pair has one channel
+  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], two ? p.dt_bias[d + 1] : 0.f) : both(0.f);
   f32x2 total = both(0.f);
   auto stage = [&](int k, int i) {
     const int r = ct0 + i * NL;
@@ -715,7 +726,7 @@ __global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int i = 0; i < PAIRS; i += 2)
-        if (n0 + 2 * i < p.N)
+        if (hc + c < nch && n0 + 2 * i < p.N)
           *reinterpret_cast<ulonglong2*>(to + (int64_t)(hc + c) * p.N + n0 + 2 * i) = make_ulonglong2(h[c][i], h[c][i + 1]);
   }
   float2 sum = unpack2(total);
@@ -724,7 +735,10 @@ __global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
     sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
     sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
   }
-  if (ct0 == 0 && cc < nch) *reinterpret_cast<float2*>(p.ssum + row * p.D + d0 + cc) = sum;
+  if (ct0 == 0 && cc < nch) {
+    p.ssum[row * p.D + d0 + cc] = sum.x;
+    if (two) p.ssum[row * p.D + d0 + cc + 1] = sum.y;
+  }
 }
 
 // carry[seg] <- the state that enters segment seg.  One thread per (row, channel, state).
@@ -739,50 +753,76 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(ScanP p) {
   const float* from = REV ? p.dh_out : p.h0;
   float H = from ? from[i] : 0.f;
   const int last = REV ? 0 : p.nseg - 1;  // its local end state was not formed
-#pragma unroll 4
-  for (int k = 0; k < p.nseg; ++k) {
-    const int seg = REV ? p.nseg - 1 - k : k;
-    float* c = p.carry + (b * p.nseg + seg) * dn + at;
-    if (seg != last) {
-      const float e = *c;
-      *c = H;
-      H = fmaf(ex2(A2 * p.ssum[(b * p.nseg + seg) * p.D + d]), H, e);
-    } else {
-      *c = H;
+  constexpr int BATCH = 8;  // segments whose values are read together
+  for (int k0 = 0; k0 < p.nseg; k0 += BATCH) {
+    float e[BATCH], a[BATCH];
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int seg = REV ? p.nseg - 1 - (k0 + q) : k0 + q;
+      const bool in = k0 + q < p.nseg && seg != last;
+      e[q] = in ? p.carry[(b * p.nseg + seg) * dn + at] : 0.f;
+      a[q] = in ? p.ssum[(b * p.nseg + seg) * p.D + d] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int seg = REV ? p.nseg - 1 - (k0 + q) : k0 + q;
+      if (k0 + q >= p.nseg) break;
+      p.carry[(b * p.nseg + seg) * dn + at] = H;
+      H = fmaf(ex2(A2 * a[q]), H, e[q]);
     }
   }
 }
 
-// One token per row: the state is read and written once, 16 bytes per lane where N allows.
-template <typename T, int NL>
-__global__ void __launch_bounds__(SCAN_THREADS) scan_step_kernel(ScanP p) {
-  const int64_t id = ((int64_t)blockIdx.x * SCAN_THREADS + threadIdx.x) / NL;
+// One token per row: the state is read and written once, 16 bytes per lane where N is a multiple of four.  HBM-bound.
+template <typename T, int NL, bool VEC>
+__global__ void __launch_bounds__(256) scan_step_kernel(const ScanP p) {
+  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / NL;
   const int n0 = (threadIdx.x % NL) * SPL, lane = threadIdx.x % 32;
-  const bool live = id < (int64_t)p.B * p.D;
+  const bool live = id < (int64_t)p.B * p.D && n0 < p.N;
   const int b = live ? (int)(id / p.D) : 0, d = live ? (int)(id % p.D) : 0;
-  const int grp = d / (p.D / p.G);
-  float x = to_f32(static_cast<const T*>(p.x)[b * p.sx_b + d]);
-  float s = to_f32(static_cast<const T*>(p.dt)[b * p.sdt_b + d]) + (p.dt_bias ? p.dt_bias[d] : 0.f);
-  if (p.softplus) s = softplus(s);
-  const T* Bp = static_cast<const T*>(p.Bm) + b * p.sB_b + grp * p.sB_g + n0;
-  const T* Cp = static_cast<const T*>(p.Cm) + b * p.sC_b + grp * p.sC_g + n0;
+  const int grp = p.G == 1 ? 0 : d / (p.D / p.G);
   float* hp = p.h_out + ((int64_t)b * p.D + d) * p.N + n0;
   const float* Ap = p.A + (int64_t)d * p.N + n0;
-  float y[1] = {0.f};
-  if (live) {
+  float h[SPL], A[SPL];
+  if (VEC) {
+    if (live) {
+      load_vec<4>(hp, h);
+      load_vec<4>(Ap, A);
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < SPL; ++i) {
-      if (n0 + i < p.N) {
-        const float h = fmaf(ex2(s * Ap[i] * LOG2E), hp[i], s * x * to_f32(Bp[i]));
-        hp[i] = h;
-        y[0] = fmaf(to_f32(Cp[i]), h, y[0]);
-      }
+      const bool in = live && n0 + i < p.N;
+      h[i] = in ? hp[i] : 0.f;
+      A[i] = in ? Ap[i] : 0.f;
+    }
+  }
+  const T* Bp = static_cast<const T*>(p.Bm) + b * p.sB_b + grp * p.sB_g;
+  const T* Cp = static_cast<const T*>(p.Cm) + b * p.sC_b + grp * p.sC_g;
+  float y[1] = {0.f}, x = 0.f, s = 0.f, z = 0.f;
+  if (live) {
+    const Quad<T> qb = load_quad(Bp, n0, p.N, VEC && p.quads), qc = load_quad(Cp, n0, p.N, VEC && p.quads);
+    x = to_f32(static_cast<const T*>(p.x)[b * p.sx_b + d]);
+    s = to_f32(static_cast<const T*>(p.dt)[b * p.sdt_b + d]) + (p.dt_bias ? p.dt_bias[d] : 0.f);
+    if (p.z) z = to_f32(static_cast<const T*>(p.z)[b * p.sz_b + d]);
+    if (p.softplus) s = softplus(s);
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+      h[i] = fmaf(ex2(s * (A[i] * LOG2E)), h[i], s * x * to_f32(qb.v[i]));
+      y[0] = fmaf(to_f32(qc.v[i]), h[i], y[0]);
+    }
+    if (VEC) {
+      *reinterpret_cast<float4*>(hp) = make_float4(h[0], h[1], h[2], h[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < SPL; ++i)
+        if (n0 + i < p.N) hp[i] = h[i];
     }
   }
   spread_sum<1, NL, 1>(y, lane);
   if (live && n0 == 0) {
     float o = y[0] + (p.Dskip ? p.Dskip[d] * x : 0.f);
-    if (p.z) o *= silu(to_f32(static_cast<const T*>(p.z)[b * p.sz_b + d]));
+    if (p.z) o *= silu(z);
     store_as(static_cast<T*>(p.y) + b * p.sy_b + d, o);
   }
 }
@@ -791,30 +831,100 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_step_kernel(ScanP p) {
 // a warp alone on a scheduler runs at 0.11 of the rate of a full SM (16 warps), so splitting pays below about 5 warps
 // per SM, and then fills one wave (1 x 65536 tokens, 2048 channels: 128 warps unsplit, 18 segments).
 SegPlan scan_segments(int64_t B, int64_t T, int64_t warps_per_row) {
-  constexpr int64_t SMS = 148, MIN_SEG = 128;
+  constexpr int64_t SMS = 148, MIN_SEG = 32;
   const SegPlan one = {1, (int)T};
   const int64_t warps = B * warps_per_row;
-  if (warps >= SMS * 5 || T < 2 * MIN_SEG) return one;
+  if (warps >= SMS * 5 || T < 4 * MIN_SEG) return one;
   int64_t n = SMS * 16 / warps;
+  while (n > 1 && n * n > 2 * T) --n;  // the combination walks the segments: sqrt(2 T) balances its steps and a segment's
   if (n > T / MIN_SEG) n = T / MIN_SEG;
   if (n < 2) return one;
   const int64_t len = ((T + n - 1) / n + TT - 1) / TT * TT;
   return {(int)((T + len - 1) / len), (int)len};
 }
 
-// Two channels per load and store: even group widths and rows aligned to a pair.
-bool scan_pairs(const ScanP& p, int es, bool bwd) {
-  auto ok = [&](const void* q, int64_t sb, int64_t st) { return (uintptr_t)q % (2 * es) == 0 && sb % 2 == 0 && st % 2 == 0; };
-  if ((p.D / p.G) % 2 || !ok(p.x, p.sx_b, p.sx_t) || !ok(p.dt, p.sdt_b, p.sdt_t) || (p.z && !ok(p.z, p.sz_b, p.sz_t))) return false;
-  return bwd ? ok(p.dy, p.sdy_b, p.sdy_t) : ok(p.y, p.sy_b, p.sy_t);
+namespace {
+bool rows16(const void* q, int v, int64_t a, int64_t b, int64_t c = 0) { return aligned16(q) && a % v == 0 && b % v == 0 && c % v == 0; }
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+}  // namespace
+
+AlignPlan scan_align_plan(const ScanP& p, int es, bool bwd) {
+  AlignPlan a = {};
+  a.tiled = p.N % 4 == 0 && aligned16(p.A) && aligned16(p.h_out) && aligned16(p.ckpt) && aligned16(p.dh_out) && aligned16(p.dh0);
+  if (!a.tiled) return a;
+  const int v = 16 / es, dpg = p.D / p.G;
+  const bool all = dpg % v != 0;  // groups would start off a 16-byte boundary
+  a.x = all || !rows16(p.x, v, p.sx_b, p.sx_t);
+  a.dt = all || !rows16(p.dt, v, p.sdt_b, p.sdt_t);
+  a.z = p.z && (all || !rows16(p.z, v, p.sz_b, p.sz_t));
+  a.dy = bwd && (all || !rows16(p.dy, v, p.sdy_b, p.sdy_t));
+  a.B = p.N % v != 0 || !rows16(p.Bm, v, p.sB_b, p.sB_t, p.sB_g);
+  a.C = p.N % v != 0 || !rows16(p.Cm, v, p.sC_b, p.sC_t, p.sC_g);
+  const size_t tok = (size_t)p.B * p.T * p.G * es;
+  a.xb = up256(tok * ((dpg + v - 1) / v * v));
+  a.bb = up256(tok * ((p.N + v - 1) / v * v));
+  a.total = a.xb * (a.x + a.dt + a.z + a.dy) + a.bb * (a.B + a.C);
+  return a;
 }
 
-// Rows of x, dt, z, B and C (and pairs of y) that 16-byte copies can take.
-bool scan_rows16(const ScanP& p, int es) {
-  const int v = 16 / es;
-  auto ok = [&](const void* q, int64_t sb, int64_t st) { return aligned16(q) && sb % v == 0 && st % v == 0; };
-  return (p.D / p.G) % v == 0 && p.N % v == 0 && ok(p.x, p.sx_b, p.sx_t) && ok(p.dt, p.sdt_b, p.sdt_t) && (!p.z || ok(p.z, p.sz_b, p.sz_t)) &&
-         ok(p.Bm, p.sB_b, p.sB_t) && p.sB_g % v == 0 && ok(p.Cm, p.sC_b, p.sC_t) && p.sC_g % v == 0;
+// dst (tokens, G, padded) <- src (b, t, G groups of `width` values), zeros in the padding; 16 bytes per thread.
+struct AlignP {
+  const void* src[6];
+  void* dst[6];
+  int64_t sb[6], st[6], sg[6];
+  int width[6];
+  int64_t tokens;
+  int T, G;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) scan_align_kernel(const AlignP p) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int k = blockIdx.y, w = p.width[k], chunks = (w + V - 1) / V;
+  const int64_t n = p.tokens * p.G * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / chunks, tok = row / p.G;
+    const int c = (int)(i - row * chunks) * V;
+    const T* src = static_cast<const T*>(p.src[k]) + tok / p.T * p.sb[k] + tok % p.T * p.st[k] + row % p.G * p.sg[k] + c;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (c + j < w) e[j] = src[j];
+    static_cast<uint4*>(p.dst[k])[i] = raw;
+  }
+}
+
+int scan_align(ScanP& p, const AlignPlan& a, int dtype, char* ws, cudaStream_t s) {
+  const int es = elem_size(dtype), v = 16 / es, dpg = p.D / p.G;
+  const int64_t dp = (dpg + v - 1) / v * v, np = (p.N + v - 1) / v * v;
+  p.tiled = 1;
+  p.xgs = dpg;
+  AlignP q = {};
+  int n = 0;
+  auto move = [&](bool on, const void*& ptr, int64_t& sb, int64_t& st, int64_t* sg, int64_t from_g, int width, int64_t padded, size_t bytes) {
+    if (!on) return;
+    q.src[n] = ptr; q.dst[n] = ws; q.sb[n] = sb; q.st[n] = st; q.sg[n] = from_g; q.width[n] = width;
+    ptr = ws; st = p.G * padded; sb = p.T * st;
+    if (sg) *sg = padded;
+    ws += bytes;
+    ++n;
+  };
+  move(a.x, p.x, p.sx_b, p.sx_t, nullptr, dpg, dpg, dp, a.xb);
+  move(a.dt, p.dt, p.sdt_b, p.sdt_t, nullptr, dpg, dpg, dp, a.xb);
+  move(a.z, p.z, p.sz_b, p.sz_t, nullptr, dpg, dpg, dp, a.xb);
+  move(a.dy, p.dy, p.sdy_b, p.sdy_t, nullptr, dpg, dpg, dp, a.xb);
+  move(a.B, p.Bm, p.sB_b, p.sB_t, &p.sB_g, p.sB_g, p.N, np, a.bb);
+  move(a.C, p.Cm, p.sC_b, p.sC_t, &p.sC_g, p.sC_g, p.N, np, a.bb);
+  if (!n) return GDN_OK;
+  if (dpg % v) p.xgs = (int)dp;
+  q.tokens = (int64_t)p.B * p.T; q.T = p.T; q.G = p.G;
+  const int64_t chunks = q.tokens * p.G * ((dpg > p.N ? dp : np) / v), g = (chunks + 255) / 256;
+  const dim3 grid((unsigned)(g < 148 * 16 ? g : 148 * 16), n);
+  if (dtype == GDN_DTYPE_F32)
+    scan_align_kernel<float><<<grid, 256, 0, s>>>(q);
+  else
+    scan_align_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(q);
+  return launched();
 }
 
 int scan_check(const gdn_scan_args* a, bool step) {
@@ -843,7 +953,7 @@ ScanP scan_params(const gdn_scan_args* a) {
   p.softplus = a->softplus != 0;
   const int es = elem_size(a->dtype);
   auto quad = [&](const void* q, int64_t sb, int64_t st, int64_t sg) { return (uintptr_t)q % (4 * es) == 0 && sb % 4 == 0 && st % 4 == 0 && sg % 4 == 0; };
-  p.quads = a->N % 4 == 0 && a->N == scan_lanes(a->N) * SPL && quad(a->Bm, a->sB_b, a->sB_t, a->sB_g) && quad(a->Cm, a->sC_b, a->sC_t, a->sC_g);
+  p.quads = a->N % 4 == 0 && quad(a->Bm, a->sB_b, a->sB_t, a->sB_g) && quad(a->Cm, a->sC_b, a->sC_t, a->sC_g);
   p.dblocks = scan_dblocks(a->D, a->G, a->N);
   const int64_t warp_channels = a->N <= 8 ? 32 : a->N <= 16 ? 16 : 8;  // of the kernels for aligned rows
   const SegPlan sp = scan_segments(a->B > 0 ? a->B : 1, a->T, (a->D / a->G + warp_channels - 1) / warp_channels * a->G);
@@ -873,8 +983,7 @@ int launch_carry_tiled(ScanP p, cudaStream_t s) {
 }
 template <typename T, bool REV>
 int launch_carry(const ScanP& p, cudaStream_t s) {
-  const int v = 16 / (int)sizeof(T);
-  if (scan_rows16(p, sizeof(T)) && (!REV || (aligned16(p.dy) && p.sdy_b % v == 0 && p.sdy_t % v == 0)))
+  if (p.tiled)
     return p.N <= 8    ? launch_carry_tiled<T, 2, 4, REV>(p, s)
            : p.N <= 16 ? launch_carry_tiled<T, 4, 4, REV>(p, s)
            : p.N <= 32 ? launch_carry_tiled<T, 8, 4, REV>(p, s)
@@ -914,24 +1023,31 @@ int launch_tiled(const ScanP& p, cudaStream_t s) {
   return p.N <= 8 ? launch_tiled<T, 2, 4>(p, s) : p.N <= 16 ? launch_tiled<T, 4, 4>(p, s) : p.N <= 32 ? launch_tiled<T, 8, 4>(p, s) : launch_tiled<T, 8, 8>(p, s);
 }
 
-template <typename T, int CV>
-void launch_fwd(const ScanP& p, int nl, cudaStream_t s) {
+template <typename T>
+int launch_plain(const ScanP& p, cudaStream_t s) {
   const dim3 g(p.dblocks * p.G, p.nseg, p.B);
-  if (nl == 2) scan_fwd_kernel<T, 2, CV><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 4) scan_fwd_kernel<T, 4, CV><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 8) scan_fwd_kernel<T, 8, CV><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 16) scan_fwd_kernel<T, 16, CV><<<g, SCAN_THREADS, 0, s>>>(p);
+  const int nl = scan_lanes(p.N);
+  if (nl == 2) scan_fwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 4) scan_fwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 8) scan_fwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 16) scan_fwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
+  return launched();
 }
 
-template <typename T>
+template <typename T, bool VEC>
 int launch_step(const ScanP& p, int nl, cudaStream_t s) {
-  const int64_t g = ((int64_t)p.B * p.D * nl + SCAN_THREADS - 1) / SCAN_THREADS;
+  const int64_t g = ((int64_t)p.B * p.D * nl + 255) / 256;
   if (g > 0x7fffffff) return GDN_ERR_SHAPE;
-  if (nl == 2) scan_step_kernel<T, 2><<<(unsigned)g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 4) scan_step_kernel<T, 4><<<(unsigned)g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 8) scan_step_kernel<T, 8><<<(unsigned)g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 16) scan_step_kernel<T, 16><<<(unsigned)g, SCAN_THREADS, 0, s>>>(p);
+  if (nl == 2) scan_step_kernel<T, 2, VEC><<<(unsigned)g, 256, 0, s>>>(p);
+  if (nl == 4) scan_step_kernel<T, 4, VEC><<<(unsigned)g, 256, 0, s>>>(p);
+  if (nl == 8) scan_step_kernel<T, 8, VEC><<<(unsigned)g, 256, 0, s>>>(p);
+  if (nl == 16) scan_step_kernel<T, 16, VEC><<<(unsigned)g, 256, 0, s>>>(p);
   return launched();
+}
+template <typename T>
+int launch_step(const ScanP& p, cudaStream_t s) {
+  const bool vec = p.N % 4 == 0 && aligned16(p.h_out) && aligned16(p.A);
+  return vec ? launch_step<T, true>(p, scan_lanes(p.N), s) : launch_step<T, false>(p, scan_lanes(p.N), s);
 }
 
 }  // namespace ssm
@@ -946,7 +1062,7 @@ int gdn_scan_workspace_bytes(const gdn_scan_args* a, size_t* bytes) {
   int st = scan_check(a, false);
   if (st != GDN_OK) return st;
   const ScanP p = scan_params(a);
-  *bytes = p.nseg > 1 ? (size_t)p.B * p.nseg * p.D * (p.N + 1) * sizeof(float) : 0;
+  *bytes = scan_align_plan(p, elem_size(a->dtype), false).total + (p.nseg > 1 ? (size_t)p.B * p.nseg * p.D * (p.N + 1) * sizeof(float) : 0);
   return GDN_OK;
 }
 
@@ -966,20 +1082,22 @@ int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
     const cudaError_t e = p.h0 ? cudaMemcpyAsync(p.h_out, p.h0, n, cudaMemcpyDeviceToDevice, s) : cudaMemsetAsync(p.h_out, 0, n, s);
     return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
   }
+  const int es = elem_size(a->dtype);
+  const AlignPlan al = scan_align_plan(p, es, false);
+  char* ws = static_cast<char*>(a->workspace);
+  if (al.tiled) {
+    st = scan_align(p, al, a->dtype, ws, s);
+    if (st != GDN_OK) return st;
+  }
   if (p.nseg > 1) {
-    p.carry = static_cast<float*>(a->workspace);
+    p.carry = reinterpret_cast<float*>(ws + al.total);
     p.ssum = p.carry + (int64_t)p.B * p.nseg * p.D * p.N;
     st = scan_launch_carry(p, a->dtype, false, s);
     if (st != GDN_OK) return st;
   }
-  const int nl = scan_lanes(p.N);
-  if (scan_rows16(p, elem_size(a->dtype)) && scan_pairs(p, elem_size(a->dtype), false))
-    return a->dtype == GDN_DTYPE_F32 ? launch_tiled<float>(p, s) : launch_tiled<__nv_bfloat16>(p, s);
-  if (scan_pairs(p, elem_size(a->dtype), false))
-    a->dtype == GDN_DTYPE_F32 ? launch_fwd<float, 2>(p, nl, s) : launch_fwd<__nv_bfloat16, 2>(p, nl, s);
-  else
-    a->dtype == GDN_DTYPE_F32 ? launch_fwd<float, 1>(p, nl, s) : launch_fwd<__nv_bfloat16, 1>(p, nl, s);
-  return launched();
+  if (!al.tiled) return a->dtype == GDN_DTYPE_F32 ? launch_plain<float>(p, s) : launch_plain<__nv_bfloat16>(p, s);
+  p.pairs_out = (p.D / p.G) % 2 == 0 && (uintptr_t)p.y % (2 * es) == 0 && p.sy_b % 2 == 0 && p.sy_t % 2 == 0;
+  return a->dtype == GDN_DTYPE_F32 ? launch_tiled<float>(p, s) : launch_tiled<__nv_bfloat16>(p, s);
 }
 
 int gdn_scan_step(const gdn_scan_args* a, void* stream) {
@@ -989,7 +1107,7 @@ int gdn_scan_step(const gdn_scan_args* a, void* stream) {
   if (!device_ok()) return GDN_ERR_DEVICE;
   const ScanP p = scan_params(a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a->dtype == GDN_DTYPE_F32 ? launch_step<float>(p, scan_lanes(p.N), s) : launch_step<__nv_bfloat16>(p, scan_lanes(p.N), s);
+  return a->dtype == GDN_DTYPE_F32 ? launch_step<float>(p, s) : launch_step<__nv_bfloat16>(p, s);
 }
 
 }  // extern "C"

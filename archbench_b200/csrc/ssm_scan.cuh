@@ -33,6 +33,9 @@ struct ScanP {
   int quads;  // rows of B and C can be loaded four states at a time
   int nseg, seg_len;  // segments of seg_len tokens (a multiple of GDN_SCAN_CKPT)
   int dblocks;        // channel blocks per group
+  int xgs;            // channels from one group to the next in x, dt, z and dy (padded copies have more than D / G)
+  int tiled;          // the kernels on asynchronous tiles serve it (scan_align_plan)
+  int pairs_out;      // rows of y (or dx, ddt, dz) take stores of channel pairs
 };
 
 // 16 bytes into shared memory without a register; zeros where `on` is false (the address is then not read).
@@ -78,7 +81,7 @@ struct Quad {
 template <typename T>
 __device__ __forceinline__ Quad<T> load_quad(const T* p, int n, int N, bool vec) {
   Quad<T> q;
-  if (vec) {
+  if (vec && n < N) {  // N is a multiple of four
     if constexpr (sizeof(T) == 4)
       *reinterpret_cast<float4*>(&q) = *reinterpret_cast<const float4*>(p + n);
     else
@@ -143,9 +146,18 @@ inline int scan_dblocks(int64_t D, int64_t G, int64_t N) {
 }
 
 int scan_check(const gdn_scan_args* a, bool step);
-bool scan_pairs(const ScanP& p, int es, bool bwd);
-bool scan_rows16(const ScanP& p, int es);
 ScanP scan_params(const gdn_scan_args* a);
+
+// Rows that 16-byte copies cannot take are first laid out again, padded, in the workspace: about 4 bytes moved per value
+// against the kernels' 30 to 100 us per million values.  Tensors that are aligned stay where they are.
+struct AlignPlan {
+  bool tiled;           // the kernels on asynchronous tiles serve it: N a multiple of four, states on 16-byte boundaries
+  bool x, dt, z, dy, B, C;
+  size_t xb, bb;        // bytes of one copied channel tensor, of one copied B or C
+  size_t total;
+};
+AlignPlan scan_align_plan(const ScanP& p, int es, bool bwd);
+int scan_align(ScanP& p, const AlignPlan& a, int dtype, char* ws, cudaStream_t s);
 // Local pass over every segment (forward, or reversed for the adjoint) and the combination of the segments: fills
 // p.carry with the state that enters each segment, from p.h0 (p.dh_out).
 int scan_launch_carry(const ScanP& p, int dtype, bool reverse, cudaStream_t s);

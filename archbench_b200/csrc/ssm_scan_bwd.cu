@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
   }
 }
 
-// The same for rows that 16-byte copies can take.  A lane holds four states of two channels, a warp 64 / NL channels, a
+// The same where N is a multiple of four (rows are 16-byte aligned, or were laid out so).  A lane holds four states of two channels, a warp 64 / NL channels, a
 // block four warps; tiles of 8 tokens (one checkpoint), last first, with one barrier each: a thread rebuilds the states of
 // tile k (decays and states stay in registers, so each exponential is formed once), walks the adjoint back, stages tile
 // k - 1 (earlier tokens) and finishes tile k + 1.
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
     int r, j, bytes;
     if (c < 4 * TT * K::XCH) {
       const int which = c / (TT * K::XCH);
-      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = d0;
+      r = c / K::XCH % TT; j = c % K::XCH; bytes = nch * K::ES; off = (int64_t)grp * p.xgs + dblk * CH;
       base = which == 0 ? p.x : which == 1 ? p.dt : which == 2 ? p.z : p.dy;
       sb = which == 0 ? p.sx_b : which == 1 ? p.sdt_b : which == 2 ? p.sz_b : p.sdy_b;
       st = which == 0 ? p.sx_t : which == 1 ? p.sdt_t : which == 2 ? p.sz_t : p.sdy_t;
@@ -306,12 +306,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   const int64_t own = (int64_t)(d0 + hc) * p.N + n0;  // of channel hc; channel hc + 1 is N further
   const float* from = p.nseg > 1 ? p.carry + row * p.D * p.N : p.dh_out ? p.dh_out + (int64_t)b * p.D * p.N : nullptr;
   auto load4 = [&](const float* q, int c, f32x2 (&v)[2]) {
-    const ulonglong2 r = q && live ? *reinterpret_cast<const ulonglong2*>(q + own + c * p.N) : make_ulonglong2(0, 0);
+    const ulonglong2 r = q && live && hc + c < nch ? *reinterpret_cast<const ulonglong2*>(q + own + c * p.N) : make_ulonglong2(0, 0);
     v[0] = r.x;
     v[1] = r.y;
   };
   auto store4 = [&](float* q, int c, const f32x2 (&v)[2]) {
-    if (live) *reinterpret_cast<ulonglong2*>(q + own + c * p.N) = make_ulonglong2(v[0], v[1]);
+    if (live && hc + c < nch) *reinterpret_cast<ulonglong2*>(q + own + c * p.N) = make_ulonglong2(v[0], v[1]);
   };
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -330,8 +330,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   const int pair = tid % (CH / 2), cc = pair * 2, ct0 = tid / (CH / 2);
   const bool cok = cc < nch && ct0 < TT;
   const int d = d0 + (cc < nch ? cc : 0);
-  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], p.dt_bias[d + 1]) : both(0.f);
-  const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], p.Dskip[d + 1]) : both(0.f);
+  const bool two = cc + 1 < nch;  // an odd group's last pair has one channel
+  const f32x2 bias = p.dt_bias ? pack2(p.dt_bias[d], two ? p.dt_bias[d + 1] : 0.f) : both(0.f);
+  const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], two ? p.Dskip[d + 1] : 0.f) : both(0.f);
+  auto put_pair = [&](T* q, const float (&v)[2]) {
+    if (p.pairs_out) {
+      store_raw<T, 2>(q, v);
+    } else {
+      store_as(q, v[0]);
+      if (two) store_as(q + 1, v[1]);
+    }
+  };
   T *dxp = static_cast<T*>(p.dx), *ddtp = static_cast<T*>(p.ddt), *dzp = static_cast<T*>(p.dz);
   f32x2 sumD = both(0.f), sumB = both(0.f);
 
@@ -393,7 +402,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
       auto put = [&](T* q, f32x2 w) {
         const float2 e = unpack2(w);
         const float o[2] = {e.x, e.y};
-        store_raw<T, 2>(q + at, o);
+        put_pair(q + at, o);
       };
       put(dxp, dx);
       put(ddtp, ddt);
@@ -533,9 +542,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   for (int t = tbeg + ntile * TT + ct0; t < tend; t += TSTEP) {  // (all token rows of threads: cok has only a tile's)
     if (cc >= nch) break;
     const int64_t at = ((int64_t)b * p.T + t) * p.D + d;
-    store_raw<T, 2>(dxp + at, zero);
-    store_raw<T, 2>(ddtp + at, zero);
-    if (p.z) store_raw<T, 2>(dzp + at, zero);
+    put_pair(dxp + at, zero);
+    put_pair(ddtp + at, zero);
+    if (p.z) put_pair(dzp + at, zero);
   }
   for (int i = tid; i < (tend - tbeg - ntile * TT) * 2 * p.N; i += SCAN_THREADS) {
     const int64_t t = tbeg + ntile * TT + i / (2 * p.N);
@@ -553,7 +562,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   ulonglong2* sums = reinterpret_cast<ulonglong2*>(smem);
   sums[ct0 * (CH / 2) + pair] = make_ulonglong2(sumD, sumB);
   __syncthreads();
-  if (tid < nch / 2) {
+  if (tid < (nch + 1) / 2) {
     f32x2 e = both(0.f), f = both(0.f);
 #pragma unroll
     for (int i = 0; i < (TSTEP < TT ? TSTEP : TT); ++i) {
@@ -561,8 +570,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
       e = add2(e, v.x);
       f = add2(f, v.y);
     }
-    *reinterpret_cast<f32x2*>(p.pD + row * 2 * p.D + d0 + 2 * tid) = e;
-    *reinterpret_cast<f32x2*>(p.pD + (row * 2 + 1) * p.D + d0 + 2 * tid) = f;
+    const float2 ev = unpack2(e), fv = unpack2(f);
+    float *pd = p.pD + row * 2 * p.D + d0 + 2 * tid, *pb = pd + p.D;
+    pd[0] = ev.x;
+    pb[0] = fv.x;
+    if (2 * tid + 1 < nch) {
+      pd[1] = ev.y;
+      pb[1] = fv.y;
+    }
   }
 }
 
@@ -598,20 +613,29 @@ __global__ void __launch_bounds__(256) scan_sum_params_kernel(ScanP p, float* dA
 }
 
 struct BwdPlan {
-  size_t carry, ssum, bc, a, d, total;  // floats
+  size_t carry, ssum, bc, a, d, total;  // floats; then the aligned copies
 };
 
 BwdPlan bwd_plan(const ScanP& p) {
   BwdPlan w = {};
+  auto up = [](size_t n) { return (n + 63) & ~(size_t)63; };  // every part on a 256-byte boundary
   if (p.nseg > 1) {
-    w.carry = (size_t)p.B * p.nseg * p.D * p.N;
-    w.ssum = (size_t)p.B * p.nseg * p.D;
+    w.carry = up((size_t)p.B * p.nseg * p.D * p.N);
+    w.ssum = up((size_t)p.B * p.nseg * p.D);
   }
-  w.bc = (size_t)p.dblocks * p.B * p.T * p.G * 2 * p.N;
-  w.a = (size_t)p.B * p.nseg * p.D * p.N;
-  w.d = (size_t)p.B * p.nseg * p.D * 2;
+  w.bc = up((size_t)p.dblocks * p.B * p.T * p.G * 2 * p.N);
+  w.a = up((size_t)p.B * p.nseg * p.D * p.N);
+  w.d = up((size_t)p.B * p.nseg * p.D * 2);
   w.total = w.carry + w.ssum + w.bc + w.a + w.d;
   return w;
+}
+
+ScanP bwd_params(const gdn_scan_bwd_args* a) {
+  ScanP p = scan_params(&a->fwd);
+  p.h_out = nullptr;
+  p.dy = a->dy; p.sdy_b = a->sdy_b; p.sdy_t = a->sdy_t;
+  p.dh_out = a->dh_out; p.dx = a->dx; p.ddt = a->ddt; p.dz = a->dz; p.dh0 = a->dh0;
+  return p;
 }
 
 template <typename T, int NL>
@@ -624,17 +648,12 @@ int launch_bwd_tiled(const ScanP& p, cudaStream_t s) {
   return launched();
 }
 
-// Two channels per lane in the tiled kernel: half the channel blocks.
-bool bwd_tiled(const ScanP& p, int es) {
-  const int v = 16 / es;
-  return scan_rows16(p, es) && aligned16(p.dy) && p.sdy_b % v == 0 && p.sdy_t % v == 0;
-}
-
 template <typename T>
 int launch_bwd(ScanP p, const gdn_scan_bwd_args* a, cudaStream_t s) {
   const int nl = scan_lanes(p.N);
-  const bool tiled = bwd_tiled(p, sizeof(T));
-  if (tiled) p.dblocks = (int)((p.D / p.G + 256 / nl - 1) / (256 / nl));
+  const bool tiled = p.tiled;
+  if (tiled) p.dblocks = (int)((p.D / p.G + 256 / nl - 1) / (256 / nl));  // two channels per lane: half the blocks
+  p.pairs_out = (p.D / p.G) % 2 == 0;                                    // dx, ddt and dz are contiguous
   const dim3 g(p.dblocks * p.G, p.nseg, p.B);
   int st = GDN_OK;
   if (tiled) {
@@ -665,7 +684,8 @@ int gdn_scan_bwd_workspace_bytes(const gdn_scan_bwd_args* a, size_t* bytes) {
   if (!a || !bytes) return GDN_ERR_NULL;
   int st = scan_check(&a->fwd, false);
   if (st != GDN_OK) return st;
-  *bytes = bwd_plan(scan_params(&a->fwd)).total * sizeof(float);
+  const ScanP p = bwd_params(a);
+  *bytes = bwd_plan(p).total * sizeof(float) + scan_align_plan(p, elem_size(a->fwd.dtype), true).total;
   return GDN_OK;
 }
 
@@ -680,9 +700,7 @@ int gdn_scan_bwd(const gdn_scan_bwd_args* a, void* stream) {
   if ((int64_t)f->B * f->T * f->G * 2 * f->N > (int64_t)0x7fffffff * 256) return GDN_ERR_SHAPE;
   if (!a->fwd.workspace || a->fwd.workspace_bytes < need) return GDN_ERR_WORKSPACE;
   if (!device_ok()) return GDN_ERR_DEVICE;
-  ScanP p = scan_params(f);
-  p.dy = a->dy; p.sdy_b = a->sdy_b; p.sdy_t = a->sdy_t;
-  p.dh_out = a->dh_out; p.dx = a->dx; p.ddt = a->ddt; p.dz = a->dz; p.dh0 = a->dh0;
+  ScanP p = bwd_params(a);
   const BwdPlan w = bwd_plan(p);
   float* ws = static_cast<float*>(f->workspace);
   p.carry = ws; ws += w.carry;
@@ -691,6 +709,11 @@ int gdn_scan_bwd(const gdn_scan_bwd_args* a, void* stream) {
   p.pA = ws; ws += w.a;
   p.pD = ws;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const AlignPlan al = scan_align_plan(p, elem_size(f->dtype), true);
+  if (al.tiled) {
+    st = scan_align(p, al, f->dtype, static_cast<char*>(f->workspace) + w.total * sizeof(float), s);
+    if (st != GDN_OK) return st;
+  }
   if (p.nseg > 1) {
     st = scan_launch_carry(p, f->dtype, true, s);
     if (st != GDN_OK) return st;

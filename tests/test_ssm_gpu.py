@@ -118,6 +118,12 @@ SCAN = [  # B, T, D, N, G, dtype, gate, skip, bias, softplus, state, lengths, pa
     (2, 43, 24, 64, 1, "bf16", True, True, True, True, True, True, 0),
     (2, 29, 28, 48, 1, "f32", False, True, True, True, True, True, 0),
     (1, 700, 32, 16, 1, "bf16", True, True, True, True, True, True, 0),
+    # odd widths and rows off their boundaries: laid out again first
+    (2, 45, 57, 16, 3, "bf16", True, True, True, True, True, True, 0),
+    (2, 300, 21, 4, 1, "bf16", True, True, True, True, True, True, 3),
+    (1, 200, 35, 24, 5, "f32", True, True, True, True, True, False, 1),
+    (2, 50, 67, 64, 1, "f32", False, True, True, True, True, True, 0),
+    (2, 40, 31, 8, 1, "f32", True, False, True, True, False, True, 2),
 ]
 
 
