@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .native import SYMBOLS, _check_cuda
-from .ssm_ops import _P, _SZ, Entry, _act, _p, _wants_grad, eager, launch
+from .ssm_ops import _P, _SZ, Entry, _act, _p, _wants_grad, eager
 
 
 class LinearArgs(ctypes.Structure):
@@ -37,6 +37,7 @@ SYMBOLS.update({
 
 
 _linear_fwd = Entry("gdn_linear_fwd", LinearArgs, need="gdn_linear_workspace_bytes")
+_linear_bwd = Entry("gdn_linear_bwd", LinearBwdArgs, need="gdn_linear_bwd_workspace_bytes")
 
 
 def _forward(x, weight, bias, residual, act, want_pre):
@@ -45,7 +46,7 @@ def _forward(x, weight, bias, residual, act, want_pre):
     y = torch.empty(M, N, device=x.device, dtype=torch.bfloat16)
     pre = torch.empty(M, N, device=x.device, dtype=torch.bfloat16) if want_pre and act else None
     _linear_fwd(x.get_device(), x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(pre), x.stride(0),
-                weight.stride(0), 0 if residual is None else residual.stride(0), N, M, N, K, act, 0)
+                weight.stride(0), 0 if residual is None else residual.stride(0), N, M, N, K, act, 0, 0, 0)
     return y, pre
 
 
@@ -70,9 +71,8 @@ class _Linear(torch.autograd.Function):
             dy = dy.contiguous()
         dx, dw, db = new(need[0], M, K), new(need[1], N, K), new(bias is not None and need[2], N)
         if dx is not None or dw is not None or db is not None:
-            a = LinearBwdArgs(_p(x), _p(weight), _p(pre), _p(dy), _p(dx), _p(dw), _p(db), x.stride(0), weight.stride(0), dy.stride(0),
-                              M, N, K, ctx.act, 0, None, 0)
-            launch("gdn_linear_bwd", a, x.device, need="gdn_linear_bwd_workspace_bytes")
+            _linear_bwd(x.get_device(), x.data_ptr(), weight.data_ptr(), _p(pre), dy.data_ptr(), _p(dx), _p(dw), _p(db), x.stride(0),
+                        weight.stride(0), dy.stride(0), M, N, K, ctx.act, 0, 0, 0)
         return dx, dw, db, dy if need[3] else None, None
 
 

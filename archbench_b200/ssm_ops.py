@@ -92,21 +92,25 @@ def eager(fn):
     return call
 
 
+def _layout(block) -> str:
+    """The struct codes of a ctypes structure's fields, nested ones in place."""
+    codes = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint64: "Q", ctypes.c_float: "f"}
+    return "".join(codes[t] if t in codes else _layout(t) for _, t in block._fields_)
+
+
 class Entry:
     """An entry point taking one argument block and a stream.  The block is packed to the layout of its ctypes mirror:
     filling 30 fields of a ctypes structure takes 3 us, packing them a third of that."""
 
-    _CODES = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint64: "Q", ctypes.c_float: "f"}
-
-    def __init__(self, name: str, block, need: Optional[str] = None):
-        self.name, self.need, self.run, self.size = name, need, None, None
-        codes = "@" + "".join(self._CODES[t] for _, t in block._fields_)
+    def __init__(self, name: str, block, need: Optional[str] = None, ws: int = -2):
+        self.name, self.need, self.ws, self.run, self.size = name, need, ws, None, None
+        codes = "@" + _layout(block)
         self.pack = struct.Struct(codes).pack
         assert struct.calcsize(codes) == ctypes.sizeof(block), block
 
     def __call__(self, index: int, *values) -> None:
-        """Run on device ``index``'s current stream.  ``values`` are the block's fields; with ``need``, all but the last
-        two, the workspace, which is taken from torch's allocator for the call."""
+        """Run on device ``index``'s current stream.  ``values`` are the block's fields; with ``need``, the entry point
+        that sizes the workspace, the two from place ``ws`` on are set to one taken from torch's allocator for the call."""
         if self.run is None:
             lib = load_library()
             at = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
@@ -116,31 +120,21 @@ class Entry:
         if torch.cuda.current_device() != index:
             with torch.cuda.device(index):
                 return self(index, *values)
-        ws = None
+        block = self.pack(*values)
         if self.need is not None:
             n = ctypes.c_size_t(0)
-            status = self.size(self.pack(*values, 0, 0), ctypes.addressof(n))
+            status = self.size(block, ctypes.addressof(n))
             if status:
                 _check(status)
             if n.value:
                 ws = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", index))
-            values = (*values, _p(ws), n.value)
-        status = self.run(self.pack(*values), torch._C._cuda_getCurrentRawStream(index))
+                values = list(values)
+                i = self.ws % len(values)
+                values[i], values[i + 1] = ws.data_ptr(), n.value
+                block = self.pack(*values)
+        status = self.run(block, torch._C._cuda_getCurrentRawStream(index))
         if status:
             _check(status)
-
-
-def launch(name: str, args, device: torch.device, need: str) -> None:
-    """Run a library entry point on ``device``'s current stream with the workspace that ``need`` sizes; ``args`` (or its
-    ``fwd`` member) holds the workspace fields."""
-    lib = load_library()
-    with torch.cuda.device(device):
-        n = ctypes.c_size_t(0)
-        _check(getattr(lib, need)(ctypes.byref(args), ctypes.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-        holder = args if hasattr(args, "workspace") else args.fwd
-        holder.workspace, holder.workspace_bytes = ws.data_ptr(), n.value
-        _check(getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def _token(t: torch.Tensor, name: str, shape, dtype, index: int) -> torch.Tensor:
@@ -186,6 +180,7 @@ def _wants_grad(*ts) -> bool:
 
 _conv_fwd = Entry("gdn_conv_fwd", ConvArgs)
 _conv_step = Entry("gdn_conv_step", ConvArgs)
+_conv_bwd = Entry("gdn_conv_bwd", ConvBwdArgs, need="gdn_conv_bwd_workspace_bytes")
 
 
 def _conv_values(x, weight, bias, state, act, lengths, y=None, state_out=None):
@@ -232,9 +227,8 @@ class _Conv(torch.autograd.Function):
         dw = torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         ds = None if state is None else torch.empty_like(state)
-        a = ConvBwdArgs(ConvArgs(*_conv_values(x, weight, bias, state, ctx.act, lengths)), _p(dy), dy.stride(0), dy.stride(1), _p(dlast), _p(dx),
-                        _p(ds), _p(dw), _p(db), None, 0)
-        launch("gdn_conv_bwd", a, x.device, need="gdn_conv_bwd_workspace_bytes")
+        _conv_bwd(x.get_device(), *_conv_values(x, weight, bias, state, ctx.act, lengths), dy.data_ptr(), dy.stride(0), dy.stride(1),
+                  _p(dlast), dx.data_ptr(), _p(ds), dw.data_ptr(), _p(db), 0, 0)
         return dx, dw, db, ds, None, None, None
 
 
@@ -305,6 +299,7 @@ def causal_conv_step(x, weight, state, bias=None, activation=None):
 
 _scan_fwd = Entry("gdn_scan_fwd", ScanArgs, need="gdn_scan_workspace_bytes")
 _scan_step = Entry("gdn_scan_step", ScanArgs)
+_scan_bwd = Entry("gdn_scan_bwd", ScanBwdArgs, need="gdn_scan_bwd_workspace_bytes", ws=len(ScanArgs._fields_) - 2)
 
 
 def _scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y=None, h_out=None, ckpt=None):
@@ -327,7 +322,7 @@ def _scan_forward(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, want_stat
     y = torch.empty(B, T, Dm, device=x.device, dtype=x.dtype)
     h = torch.empty(B, Dm, N, device=x.device, dtype=torch.float32) if want_state else None
     ckpt = torch.empty(B, (T + SCAN_CKPT - 1) // SCAN_CKPT, Dm, N, device=x.device, dtype=torch.float32) if train else None
-    _scan_fwd(x.get_device(), *_scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y, h, ckpt))
+    _scan_fwd(x.get_device(), *_scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, softplus, y, h, ckpt), 0, 0)
     return y, h, ckpt
 
 
@@ -346,16 +341,16 @@ class _Scan(torch.autograd.Function):
         x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ckpt = ctx.saved_tensors
         if dy is None and dh is None:
             return (None,) * 12
-        new = lambda t: None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+        new = lambda t: None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype)  # contiguous
         if x.numel() == 0:
             zero = [None if t is None else torch.zeros_like(t) for t in (x, dt, A, Bm, Cm, D, z, bias)]
             return (*zero, None if h0 is None else torch.zeros_like(h0) if dh is None else dh, None, None, None)
         dy = torch.zeros_like(x) if dy is None else _token(dy, "dy", x.shape, x.dtype, x.get_device())
         dh = None if dh is None else dh.contiguous()
         dx, ddt, dA, dB, dC, dD, dz, db, dh0 = (new(t) for t in (x, dt, A, Bm, Cm, D, z, bias, h0))
-        a = ScanBwdArgs(ScanArgs(*_scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ctx.softplus, ckpt=ckpt)), _p(dy), dy.stride(0), dy.stride(1),
-                        _p(dh), _p(dx), _p(ddt), _p(dB), _p(dC), _p(dz), _p(dA), _p(dD), _p(db), _p(dh0))
-        launch("gdn_scan_bwd", a, x.device, need="gdn_scan_bwd_workspace_bytes")
+        _scan_bwd(x.get_device(), *_scan_values(x, dt, A, Bm, Cm, D, z, bias, h0, lengths, ctx.softplus, ckpt=ckpt), 0, 0, dy.data_ptr(),
+                  dy.stride(0), dy.stride(1), _p(dh), dx.data_ptr(), ddt.data_ptr(), dB.data_ptr(), dC.data_ptr(), _p(dz), dA.data_ptr(),
+                  _p(dD), _p(db), _p(dh0))
         return dx, ddt, dA, dB, dC, dD, dz, db, dh0, None, None, None
 
 
