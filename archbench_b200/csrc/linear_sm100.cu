@@ -8,8 +8,8 @@
 //
 // A persistent block computes 128 x BN tiles: one warp issues the TMA loads of 64-deep k blocks into a ring of stages,
 // one warp issues the MMAs, eight warps read finished accumulators from tensor memory and run the epilogue while the
-// MMAs of the next tile go on (two accumulators).  Operands that TMA cannot address (rows not 16-byte aligned) are
-// written to the same shared-memory layout by four more warps with plain loads.
+// MMAs of the next tile go on (two accumulators).  Operands that TMA cannot address (rows not 16-byte aligned) are laid
+// out again first, padded, in the workspace.
 #include "gdn_tiles.cuh"
 #include "sm100_ptx.cuh"
 #include "ssm_common.cuh"
@@ -19,8 +19,7 @@ namespace linear {
 
 constexpr int BM = 128, BK = 64;
 constexpr int EPI_WARPS = 8;                        // two per quarter of the tensor-memory lanes
-constexpr int LOAD_WARPS = 4;                       // plain loaders, present only when an operand needs them
-constexpr int BASE_THREADS = 64 + 32 * EPI_WARPS, LOAD_THREADS = 32 * LOAD_WARPS;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int OUT_BYTES = 32 * 128;                 // a warp's output box: 32 rows x 64 columns
 constexpr long long WAIT_CYCLES = 4000000000ll;     // ~2 s: a wait that runs this long gives up
 
@@ -33,7 +32,7 @@ struct Operand {  // a row-major matrix, `rows` rows of `cols` contiguous values
   const bf16* p;
   int64_t ld;
   int64_t rows, cols;
-  int tma;  // addressed by its tensor map, else by plain loads
+  int tma;  // rows start on 16-byte boundaries: a tensor map can address it
 };
 
 struct GemmP {
@@ -105,23 +104,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// A box of `nrow` rows x 64 values starting at (row, col), zero outside, into the 128-byte-swizzled tile at `dst`:
-// 16-byte chunk j of row r sits at chunk j ^ (r % 8).  64 x 8 chunks by 128 threads.
-__device__ __forceinline__ void load_box(char* dst, const Operand& o, int64_t row, int64_t col, int nrow, int tid) {
-  for (int i = tid; i < nrow * 8; i += LOAD_THREADS) {
-    const int r = i / 8, j = i % 8;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    bf16* e = reinterpret_cast<bf16*>(&raw);
-    if (row + r < o.rows) {
-      const bf16* p = o.p + (row + r) * o.ld + col + j * 8;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (col + j * 8 + k < o.cols) e[k] = p[k];
-    }
-    *reinterpret_cast<uint4*>(dst + r * 128 + ((j ^ (r & 7)) << 4)) = raw;
-  }
-}
-
 // One operand's part of a stage: ROWS output indices x 64 k.  k-contiguous: one box of ROWS rows; else ROWS / 64 boxes
 // of 64 k rows.
 template <int ROWS, bool MN>
@@ -133,35 +115,10 @@ __device__ __forceinline__ void stage_tma(char* dst, const CUtensorMap* map, uin
     for (int i = 0; i < ROWS / 64; ++i) tma_load_2d(dst + i * 8192, map, bar, idx0 + i * 64, k0);
   }
 }
-template <int ROWS, bool MN>
-__device__ __forceinline__ void stage_plain(char* dst, const Operand& o, int64_t idx0, int64_t k0, int tid) {
-  if (!MN) {
-    load_box(dst, o, idx0, k0, ROWS, tid);
-  } else {
-    for (int i = 0; i < ROWS / 64; ++i) load_box(dst + i * 8192, o, k0, idx0 + i * 64, 64, tid);
-  }
-}
-
 // Operand descriptor of k step s (16 deep) in a stage part at shared address `base`.
 template <bool MN>
 __device__ __forceinline__ uint64_t step_desc(uint32_t base, int s) {
   return MN ? ptx::sdesc_sw128(base + s * 2048, 8192, 1024) : ptx::sdesc_sw128(base + s * 32, 16, 1024);
-}
-
-// 32 consecutive columns of one row of the result, straight to global memory: rows that vectors or TMA cannot take, and
-// the ragged last columns.
-__device__ __noinline__ void epilogue32(const GemmP& p, int64_t row, int64_t col, const float (&v)[32]) {
-  const int n = (int)(p.N - col < 32 ? p.N - col : 32);
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (i >= n) break;
-    float o = v[i];
-    if (p.bias) o += to_f32(p.bias[col + i]);
-    if (p.pre) p.pre[row * p.N + col + i] = __float2bfloat16_rn(o);
-    o = act_fwd(o, p.act);
-    if (p.res) o += to_f32(p.res[row * p.ldr + col + i]);
-    p.y[row * p.ldy + col + i] = __float2bfloat16_rn(o);
-  }
 }
 
 // A warp's 32 rows x 64 columns, written to `box` in the 128-byte-swizzled layout and stored by TMA (which clips rows
@@ -194,8 +151,36 @@ __device__ __forceinline__ void box_store(const CUtensorMap* map, const char* bo
   }
 }
 
+// The same box from and to rows that no vector takes: a row at a time, the lanes along its columns.
+__device__ __forceinline__ bf16* box_at(char* box, int row, int col) {
+  return reinterpret_cast<bf16*>(box + row * 128 + (((col >> 3) ^ (row & 7)) << 4)) + (col & 7);
+}
+__device__ __noinline__ void box_copy_out(char* box, int lane, bf16* p, int64_t ld, int64_t row0, int64_t col0, int64_t M, int64_t N) {
+  __syncwarp();
+  const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
+  const bool a = col0 + lane < N, b = col0 + 32 + lane < N;
+  bf16* q = p + row0 * ld + col0 + lane;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r, q += ld) {
+    if (a) q[0] = *box_at(box, r, lane);
+    if (b) q[32] = *box_at(box, r, lane + 32);
+  }
+  __syncwarp();
+}
+__device__ __noinline__ void box_copy_in(char* box, int lane, const bf16* p, int64_t ld, int64_t row0, int64_t col0, int64_t M, int64_t N) {
+  const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
+  const bool a = col0 + lane < N, b = col0 + 32 + lane < N;
+  const bf16* q = p + row0 * ld + col0 + lane;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r, q += ld) {
+    *box_at(box, r, lane) = a ? q[0] : __float2bfloat16_rn(0.f);
+    *box_at(box, r, lane + 32) = b ? q[32] : __float2bfloat16_rn(0.f);
+  }
+  __syncwarp();
+}
+
 template <int BN, bool AMN, bool BMN>
-__global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap my,
                 const __grid_constant__ CUtensorMap mpre, const GemmP p) {
   using C = Cfg<BN>;
@@ -211,10 +196,9 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const bool plain = !p.a.tma || !p.b.tma;
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
-      ptx::mbar_init(full + i, 1 + (plain ? LOAD_WARPS : 0));
+      ptx::mbar_init(full + i, 1);
       ptx::mbar_init(empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -237,7 +221,6 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t bytes = (p.a.tma ? A_BYTES : 0) + (p.b.tma ? B_BYTES : 0);
       uint32_t n = 0;  // k blocks issued
       bool ok = true;
       for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
@@ -248,9 +231,9 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
           const int s = n % ST;
           if (!wait(empty + s, ((n / ST) & 1) ^ 1)) { ok = false; break; }
           char* st = tiles + s * C::STAGE;
-          ptx::mbar_arrive_expect_tx(full + s, bytes);
-          if (p.a.tma) stage_tma<BM, AMN>(st, &ma, full + s, m0, kb * BK);
-          if (p.b.tma) stage_tma<BN, BMN>(st + A_BYTES, &mb, full + s, n0, kb * BK);
+          ptx::mbar_arrive_expect_tx(full + s, A_BYTES + B_BYTES);
+          stage_tma<BM, AMN>(st, &ma, full + s, m0, kb * BK);
+          stage_tma<BN, BMN>(st + A_BYTES, &mb, full + s, n0, kb * BK);
         }
       }
       if (!ok)  // leave no copy in flight: each outstanding stage's own barrier, with a limit
@@ -279,7 +262,7 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
       ptx::mma_commit_elect(tfull + buf);
       if (!ok) ptx::mbar_wait_bounded(tfull + buf, (acc >> 1) & 1, WAIT_CYCLES / 8);  // no MMA left in flight
     }
-  } else if (warp < 2 + EPI_WARPS) {
+  } else {
     const int quarter = warp % 4;  // tensor-memory lanes this warp can read
     const int c0 = (warp - 2) / 4 * C::COLS;  // its first column of a tile
     char* box = boxes + (warp - 2) * OUT_BYTES;
@@ -291,12 +274,28 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
       const bool in = row < p.M;
       uint4 res[8];  // the residual of 64 columns, on its way while the accumulator is waited for
       auto load_res = [&](int64_t col) {
-        if (!p.res || !p.vec || p.splits > 1) return;
+        if (!p.res || p.splits > 1 || row0 >= p.M) return;
+        if (!p.vec) {
+          box_copy_in(box, lane, p.res, p.ldr, row0, col, p.M, p.N);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) res[j] = *reinterpret_cast<const uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
+          __syncwarp();
+          return;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           res[j] = make_uint4(0, 0, 0, 0);
           if (in && col + j * 8 < p.N) res[j] = *reinterpret_cast<const uint4*>(p.res + row * p.ldr + col + j * 8);
         }
+      };
+      auto put = [&](const CUtensorMap* map, bf16* to, int64_t ld, int64_t col, const f32x2 (&v)[2][16]) {
+        if (p.vec) box_ready(lane);
+        box_put(box, lane, 0, v[0]);
+        box_put(box, lane, 32, v[1]);
+        if (p.vec)
+          box_store(map, box, lane, row0, col);
+        else
+          box_copy_out(box, lane, to, ld, row0, col, p.M, p.N);
       };
       load_res(n0 + c0);
       if (!wait(tfull + buf, (acc >> 1) & 1)) break;
@@ -305,25 +304,21 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
       for (int c = c0; c < c0 + C::COLS; c += 64) {
         if (n0 + c >= p.N || row0 >= p.M) break;  // the warp's part lies outside
         const uint32_t t = tmem + (uint32_t)(quarter * 32 << 16) + buf * BN + c;
-        if (p.splits > 1 || !p.vec) {
+        if (p.splits > 1) {
 #pragma unroll 1
           for (int e = 0; e < 64; e += 32) {
             float v[32];
             ptx::tmem_ld32(t + e, v);
             ptx::tc_wait_ld();
             const int64_t col = n0 + c + e;
-            if (in && p.splits > 1) {
-              float* q = p.part + ((int64_t)sp * p.M + row) * p.N + col;
-              if (p.N % 4 == 0 && col + 32 <= p.N) {
+            float* q = p.part + ((int64_t)sp * p.M + row) * p.N + col;
+            if (in && p.N % 4 == 0 && col + 32 <= p.N) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(q + i * 4) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
-              } else {
+              for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(q + i * 4) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
+            } else if (in) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (col + i < p.N) q[i] = v[i];
-              }
-            } else if (in && col < p.N) {
-              epilogue32(p, row, col, v);
+              for (int i = 0; i < 32; ++i)
+                if (col + i < p.N) q[i] = v[i];
             }
             __syncwarp();  // the next load is warp-wide
           }
@@ -332,28 +327,28 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
         f32x2 v[2][16];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          const int64_t col0 = n0 + c + e * 32;
           float a[32];
           ptx::tmem_ld32(t + e * 32, a);
           ptx::tc_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[e][i] = pack2(a[2 * i], a[2 * i + 1]);
-          if (p.bias) {
+          if (p.bias && p.vec) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int64_t col = n0 + c + e * 32 + j * 8;
-              const uint4 bv = col < p.N ? __ldg(reinterpret_cast<const uint4*>(p.bias + col)) : make_uint4(0, 0, 0, 0);
+              const uint4 bv = col0 + j * 8 < p.N ? __ldg(reinterpret_cast<const uint4*>(p.bias + col0 + j * 8)) : make_uint4(0, 0, 0, 0);
               const bf16* q = reinterpret_cast<const bf16*>(&bv);
 #pragma unroll
               for (int i = 0; i < 4; ++i) v[e][j * 4 + i] = add2(v[e][j * 4 + i], load_pair(q + 2 * i));
             }
+          } else if (p.bias) {
+            const float bl = col0 + lane < p.N ? to_f32(p.bias[col0 + lane]) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              v[e][i] = add2(v[e][i], pack2(__shfl_sync(0xffffffffu, bl, 2 * i), __shfl_sync(0xffffffffu, bl, 2 * i + 1)));
           }
         }
-        if (p.pre) {
-          box_ready(lane);
-          box_put(box, lane, 0, v[0]);
-          box_put(box, lane, 32, v[1]);
-          box_store(&mpre, box, lane, row0, n0 + c);
-        }
+        if (p.pre) put(&mpre, p.pre, p.N, n0 + c, v);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -361,11 +356,8 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
             v[e][i] = act_fwd2(v[e][i], p.act);
             if (p.res) v[e][i] = add2(v[e][i], load_pair(reinterpret_cast<const bf16*>(&res[e * 4 + i / 4]) + i % 4 * 2));
           }
+        put(&my, p.y, p.ldy, n0 + c, v);
         if (c + 64 < c0 + C::COLS) load_res(n0 + c + 64);
-        box_ready(lane);
-        box_put(box, lane, 0, v[0]);
-        box_put(box, lane, 32, v[1]);
-        box_store(&my, box, lane, row0, n0 + c);
       }
       ptx::tc_fence_before();
       __syncwarp();
@@ -373,25 +365,6 @@ __global__ void __launch_bounds__(BASE_THREADS + LOAD_THREADS, 1)
     }
     if (lane == 0) ptx::bulk_wait0();  // the stores have read the boxes and are done
     __syncwarp();
-  } else if (plain) {
-    const int ltid = tid - BASE_THREADS;
-    uint32_t n = 0;
-    bool ok = true;
-    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
-      const int tile = it / p.splits, sp = it % p.splits;
-      const int64_t m0 = (int64_t)(tile % p.tiles_m) * BM, n0 = (int64_t)(tile / p.tiles_m) * BN;
-      const int kb1 = min((sp + 1) * per, p.kblocks);
-      for (int kb = sp * per; kb < kb1; ++kb, ++n) {
-        const int s = n % ST;
-        if (!wait(empty + s, ((n / ST) & 1) ^ 1)) { ok = false; break; }
-        char* st = tiles + s * C::STAGE;
-        if (!p.a.tma) stage_plain<BM, AMN>(st, p.a, m0, (int64_t)kb * BK, ltid);
-        if (!p.b.tma) stage_plain<BN, BMN>(st + A_BYTES, p.b, n0, (int64_t)kb * BK, ltid);
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(full + s);
-      }
-    }
   }
   __syncthreads();
   if (tid == 0 && *abort_flag) atomicExch(&g_status, GDN_ERR_TIMEOUT);
@@ -580,10 +553,6 @@ Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols) {
 
 // (cols, rows) map with boxes of 64 columns x box_rows rows, 128-byte swizzle, zeros outside.
 bool make_map2(CUtensorMap* m, const Operand& o, int box_rows) {
-  if (!o.tma) {
-    memset(m, 0, sizeof(*m));
-    return true;
-  }
   auto fn = tiles::encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
@@ -600,32 +569,39 @@ bool make_out_map(CUtensorMap* m, bf16* p, int64_t ld, int64_t M, int64_t N) {
   return !p || make_map2(m, Operand{p, ld, M, N, 1}, 32);
 }
 
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
 struct Plan {
   int bn, splits;
   size_t part;  // bytes
 };
 
-// Tile width and splits of the contraction: the widest tile that still gives every SM one, else 64-wide tiles with the
-// contraction split until they do (at least 4 k blocks each).
+// Tile width and splits of the contraction by a model of the time in SM clocks: waves of tiles, a k block taking 540, 300
+// or 200 clocks with 256, 128 or 64 columns (the tensor pipe's 512 clocks, then the operands' way out of shared memory)
+// and a tile 2500 to start and drain; splits add their sums' way through memory (2 x 4 bytes at 3400 bytes a clock) and a
+// launch.  16384 x 1024 x 2816 runs 256-wide (98 us; 105 us 128-wide), 1024 x 2816 x 16384 in two waves of split tiles.
 Plan plan(int64_t M, int64_t N, int64_t K) {
-  const int sms = sm_count();
-  const int64_t tm = (M + BM - 1) / BM;
-  Plan r = {64, 1, 0};
-  for (int bn : {256, 128})
-    if (tm * ((N + bn - 1) / bn) >= sms) {
-      r.bn = bn;
-      return r;
+  const int64_t sms = sm_count(), tm = (M + BM - 1) / BM, kb = (K + BK - 1) / BK;
+  Plan best = {64, 1, 0};
+  double least = 1e300;
+  const struct {
+    int bn, clocks;
+  } widths[] = {{256, 540}, {128, 300}, {64, 200}};
+  for (const auto& w : widths) {
+    const int64_t tiles = tm * ((N + w.bn - 1) / w.bn);
+    for (int64_t s = 1; s <= 16; ++s) {
+      if (s > 1 && (kb / s < 4 || tiles >= 4 * sms)) break;
+      const int64_t per = (kb + s - 1) / s, splits = (kb + per - 1) / per, waves = (tiles * splits + sms - 1) / sms;
+      const double t = (double)waves * (double)(per * w.clocks + 2500) + (splits > 1 ? (double)splits * (double)(M * N) * 8 / 3400 + 6000 : 0);
+      if (t < least) {
+        least = t;
+        best.bn = w.bn;
+        best.splits = (int)splits;
+      }
     }
-  const int64_t t = tm * ((N + 63) / 64), kb = (K + BK - 1) / BK;
-  int64_t s = t < sms ? sms / t : 1;
-  if (s > kb / 4) s = kb / 4;
-  if (s > 16) s = 16;
-  if (s > 1) {
-    const int64_t per = (kb + s - 1) / s;
-    r.splits = (int)((kb + per - 1) / per);
-    r.part = (size_t)r.splits * M * N * sizeof(float);
   }
-  return r;
+  if (best.splits > 1) best.part = up256((size_t)best.splits * M * N * sizeof(float));
+  return best;
 }
 
 template <int BN, bool AMN, bool BMN>
@@ -640,8 +616,36 @@ int launch_gemm(const GemmP& p, cudaStream_t s) {
     return GDN_ERR_LAUNCH;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
   const int grid = (int)(items < sm_count() ? items : sm_count());
-  const bool plain = !p.a.tma || !p.b.tma;
-  k<<<grid, BASE_THREADS + (plain ? LOAD_THREADS : 0), Cfg<BN>::SMEM, s>>>(ma, mb, my, mpre, p);
+  k<<<grid, THREADS, Cfg<BN>::SMEM, s>>>(ma, mb, my, mpre, p);
+  return ssm::launched();
+}
+
+// Bytes of an operand's aligned copy, 0 where it needs none, and the copy itself (which then stands for it).
+size_t align_bytes(const Operand& o) { return o.tma ? 0 : up256((size_t)o.rows * ((o.cols + 7) / 8 * 8) * 2); }
+
+__global__ void __launch_bounds__(256) align_kernel(const bf16* src, int64_t ld, bf16* dst, int64_t rows, int64_t cols) {
+  const int64_t chunks = (cols + 7) / 8, n = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+    const bf16* s = src + r * ld + c;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    bf16* e = reinterpret_cast<bf16*>(&raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) e[j] = s[j];
+    reinterpret_cast<uint4*>(dst)[i] = raw;
+  }
+}
+
+int align_operand(Operand& o, char*& ws, cudaStream_t s) {
+  if (o.tma) return GDN_OK;
+  const size_t bytes = align_bytes(o);
+  const int64_t ld = (o.cols + 7) / 8 * 8, g = (o.rows * (ld / 8) + 255) / 256;
+  align_kernel<<<(unsigned)(g < 148 * 16 ? g : 148 * 16), 256, 0, s>>>(o.p, o.ld, reinterpret_cast<bf16*>(ws), o.rows, o.cols);
+  o.p = reinterpret_cast<const bf16*>(ws);
+  o.ld = ld;
+  o.tma = 1;
+  ws += bytes;
   return ssm::launched();
 }
 
@@ -687,24 +691,25 @@ int check_sizes(int64_t M, int64_t N, int64_t K, int act) {
 
 struct BwdPlan {
   int64_t ldp;       // row length of dp, 0 when dy itself serves
-  size_t dp, colsum, part, total;
+  size_t dp, colsum, x, w, part, total;  // bytes; x and w: their aligned copies
 };
 
 BwdPlan bwd_plan(const gdn_linear_bwd_args* a) {
   BwdPlan w = {};
   const bool copy = a->act != GDN_ACT_NONE || !rows16(a->dy, a->sdy);
-  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   if (copy) {
     w.ldp = (a->N + 7) / 8 * 8;
-    w.dp = up((size_t)a->M * w.ldp * 2);
+    w.dp = up256((size_t)a->M * w.ldp * 2);
   }
-  if (a->dbias) w.colsum = up((size_t)((a->M + DP_ROWS - 1) / DP_ROWS) * a->N * 4);
+  if (a->dweight) w.x = align_bytes(operand(a->x, a->sx, a->M, a->K));
+  if (a->dx) w.w = align_bytes(operand(a->weight, a->sw, a->N, a->K));
+  if (a->dbias) w.colsum = up256((size_t)((a->M + DP_ROWS - 1) / DP_ROWS) * a->N * 4);
   if (a->dx) w.part = plan(a->M, a->K, a->N).part;
   if (a->dweight) {
     const size_t q = plan(a->N, a->K, a->M).part;
     if (q > w.part) w.part = q;
   }
-  w.total = w.dp + w.colsum + w.part;
+  w.total = w.dp + w.colsum + w.x + w.w + w.part;
   return w;
 }
 
@@ -731,7 +736,9 @@ int gdn_linear_workspace_bytes(const gdn_linear_args* a, size_t* bytes) {
   if (!a || !bytes) return GDN_ERR_NULL;
   const int st = check_sizes(a->M, a->N, a->K, a->act);
   if (st != GDN_OK) return st;
-  *bytes = a->M <= FEW_ROWS ? 0 : plan(a->M, a->N, a->K).part;
+  *bytes = a->M <= FEW_ROWS ? 0
+                            : plan(a->M, a->N, a->K).part + align_bytes(operand(a->x, a->sx, a->M, a->K)) +
+                                  align_bytes(operand(a->weight, a->sw, a->N, a->K));
   return GDN_OK;
 }
 
@@ -753,7 +760,10 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
   p.act = a->act;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.M <= FEW_ROWS) return launch_few(p, s);
-  return gemm<false, false>(p, a->workspace, s);
+  char* ws = static_cast<char*>(a->workspace);
+  st = align_operand(p.a, ws, s);
+  if (st == GDN_OK) st = align_operand(p.b, ws, s);
+  return st == GDN_OK ? gemm<false, false>(p, ws, s) : st;
 }
 
 int gdn_linear_bwd_workspace_bytes(const gdn_linear_bwd_args* a, size_t* bytes) {
@@ -778,7 +788,8 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
   char* ws = static_cast<char*>(a->workspace);
   bf16* dp = w.ldp ? reinterpret_cast<bf16*>(ws) : nullptr;
   float* colsum = a->dbias ? reinterpret_cast<float*>(ws + w.dp) : nullptr;
-  void* part = ws + w.dp + w.colsum;
+  char* copies = ws + w.dp + w.colsum;
+  void* part = copies + w.x + w.w;
   if (dp || colsum) {
     const int64_t gx = ((dp ? w.ldp : a->N) + 255) / 256, gy = (a->M + DP_ROWS - 1) / DP_ROWS;
     if (gy > 65535) return GDN_ERR_SHAPE;
@@ -800,7 +811,8 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
     p.b = operand(a->weight, a->sw, a->N, a->K);
     p.M = a->M; p.N = a->K; p.K = a->N;
     p.y = static_cast<bf16*>(a->dx); p.ldy = a->K;
-    st = gemm<false, true>(p, part, s);
+    st = align_operand(p.b, copies, s);
+    if (st == GDN_OK) st = gemm<false, true>(p, part, s);
     if (st != GDN_OK) return st;
   }
   if (a->dweight) {  // (N, K) = dp^T (N, M) x (M, K)
@@ -808,7 +820,8 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
     p.b = operand(a->x, a->sx, a->M, a->K);
     p.M = a->N; p.N = a->K; p.K = a->M;
     p.y = static_cast<bf16*>(a->dweight); p.ldy = a->K;
-    st = gemm<true, true>(p, part, s);
+    st = align_operand(p.b, copies, s);
+    if (st == GDN_OK) st = gemm<true, true>(p, part, s);
   }
   return st;
 }
