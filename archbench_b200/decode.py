@@ -68,8 +68,8 @@ class GraphDecoder:
     ``token`` (B,) holds the current token; each ``step()`` runs the model on it, leaves the step's
     last-position logits in ``logits`` and the greedy next token in ``token``, and advances every
     cache by one token.  The caches are switched to static (in-place updates), so the captured
-    kernels read and write the same state buffers on every replay.  Capturing does not advance the
-    caches: the warm-up call that precedes the capture runs on saved copies, which are put back."""
+    kernels read and write the same state buffers on every replay.  Capturing advances neither the
+    caches nor the token: what the warm-up call that precedes the capture changes is put back."""
 
     def __init__(self, model: nn.Module, caches: List[GDNCache], token: torch.Tensor):
         self.model = model
@@ -82,6 +82,7 @@ class GraphDecoder:
         with torch.cuda.stream(side):  # warm-up: cuBLAS handles, library state, allocator pool
             self._run()
         torch.cuda.current_stream().wait_stream(side)
+        self.token.copy_(token)  # the warm-up call advanced it too
         for c, (st, conv, seen) in zip(caches, saved):
             c.state.copy_(st)
             for k, v in conv.items():
