@@ -48,6 +48,7 @@ struct GemmP {
   int64_t ldr;
   int act, vec;
   float* part;  // splits > 1: (splits, M, N) sums
+  int part_tma; // N a multiple of four: TMA stores them
 };
 
 template <int BN>
@@ -146,6 +147,17 @@ __device__ __forceinline__ void box_store(const CUtensorMap* map, const char* bo
   if (lane == 0) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
                  "r"(ptx::smem_u32(box)), "r"((int)col), "r"((int)row)
+                 : "memory");
+    ptx::bulk_commit();
+  }
+}
+
+__device__ __forceinline__ void box_store3(const CUtensorMap* map, const char* box, int lane, int64_t row, int64_t col, int split) {
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(ptx::smem_u32(box)), "r"((int)col), "r"((int)row), "r"(split)
                  : "memory");
     ptx::bulk_commit();
   }
@@ -304,18 +316,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int c = c0; c < c0 + C::COLS; c += 64) {
         if (n0 + c >= p.N || row0 >= p.M) break;  // the warp's part lies outside
         const uint32_t t = tmem + (uint32_t)(quarter * 32 << 16) + buf * BN + c;
-        if (p.splits > 1) {
+        if (p.splits > 1) {  // 32 x 32 sums at a time, staged and stored like the outputs
 #pragma unroll 1
           for (int e = 0; e < 64; e += 32) {
             float v[32];
             ptx::tmem_ld32(t + e, v);
             ptx::tc_wait_ld();
             const int64_t col = n0 + c + e;
-            float* q = p.part + ((int64_t)sp * p.M + row) * p.N + col;
-            if (in && p.N % 4 == 0 && col + 32 <= p.N) {
+            if (p.part_tma) {
+              box_ready(lane);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(q + i * 4) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[j * 4], v[j * 4 + 1], v[j * 4 + 2], v[j * 4 + 3]);
+              box_store3(&my, box, lane, row0, col, sp);
             } else if (in) {
+              float* q = p.part + ((int64_t)sp * p.M + row) * p.N + col;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (col + i < p.N) q[i] = v[i];
@@ -371,22 +386,50 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 1) ptx::tmem_dealloc(tmem, 2 * BN);
 }
 
-// The splits' sums, in order, and the epilogue; 4 columns per thread.
+// The splits' sums, in order, and the epilogue; 4 columns per thread (VEC: as vectors).
+template <bool VEC>
 __global__ void __launch_bounds__(256) split_epilogue_kernel(const GemmP p) {
   const int64_t cols = (p.N + 3) / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= p.M * cols) return;
-  const int64_t row = i / cols, col = i % cols * 4;
+  const int64_t row = i / cols, col = (i - row * cols) * 4;
+  if constexpr (VEC) {
+    const float4* q = reinterpret_cast<const float4*>(p.part + row * p.N + col);
+    float4 v = *q;
+#pragma unroll 4
+    for (int s = 1; s < p.splits; ++s) {
+      const float4 w = q[(int64_t)s * p.M * p.N / 4];
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
+    f32x2 o[2] = {pack2(v.x, v.y), pack2(v.z, v.w)};
+    auto put = [&](bf16* to) {
+      const float2 a = unpack2(o[0]), b = unpack2(o[1]);
+      const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(b.x, b.y)};
+      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(h);
+    };
+    auto add = [&](const bf16* from) {
+      const uint2 r = *reinterpret_cast<const uint2*>(from);
+      o[0] = add2(o[0], load_pair(reinterpret_cast<const bf16*>(&r)));
+      o[1] = add2(o[1], load_pair(reinterpret_cast<const bf16*>(&r) + 2));
+    };
+    if (p.bias) add(p.bias + col);
+    if (p.pre) put(p.pre + row * p.N + col);
+    o[0] = act_fwd2(o[0], p.act);
+    o[1] = act_fwd2(o[1], p.act);
+    if (p.res) add(p.res + row * p.ldr + col);
+    put(p.y + row * p.ldy + col);
+  } else {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (col + k >= p.N) break;
-    float v = 0.f;
-    for (int s = 0; s < p.splits; ++s) v += p.part[((int64_t)s * p.M + row) * p.N + col + k];
-    if (p.bias) v += to_f32(p.bias[col + k]);
-    if (p.pre) p.pre[row * p.N + col + k] = __float2bfloat16_rn(v);
-    v = act_fwd(v, p.act);
-    if (p.res) v += to_f32(p.res[row * p.ldr + col + k]);
-    p.y[row * p.ldy + col + k] = __float2bfloat16_rn(v);
+    for (int k = 0; k < 4; ++k) {
+      if (col + k >= p.N) break;
+      float v = 0.f;
+      for (int s = 0; s < p.splits; ++s) v += p.part[((int64_t)s * p.M + row) * p.N + col + k];
+      if (p.bias) v += to_f32(p.bias[col + k]);
+      if (p.pre) p.pre[row * p.N + col + k] = __float2bfloat16_rn(v);
+      v = act_fwd(v, p.act);
+      if (p.res) v += to_f32(p.res[row * p.ldr + col + k]);
+      p.y[row * p.ldy + col + k] = __float2bfloat16_rn(v);
+    }
   }
 }
 
@@ -571,6 +614,18 @@ bool make_out_map(CUtensorMap* m, bf16* p, int64_t ld, int64_t M, int64_t N) {
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// (N, M, splits) map of the splits' sums, boxes of 32 x 32 fp32.
+bool make_part_map(CUtensorMap* m, float* p, int64_t M, int64_t N, int64_t splits) {
+  auto fn = tiles::encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)splits};
+  cuuint64_t strides[2] = {(cuuint64_t)N * 4, (cuuint64_t)(M * N) * 4};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct Plan {
   int bn, splits;
   size_t part;  // bytes
@@ -614,6 +669,7 @@ int launch_gemm(const GemmP& p, cudaStream_t s) {
   if (!make_map2(&ma, p.a, AMN ? BK : BM) || !make_map2(&mb, p.b, BMN ? BK : BN) || !make_out_map(&my, out ? p.y : nullptr, p.ldy, p.M, p.N) ||
       !make_out_map(&mpre, out ? p.pre : nullptr, p.N, p.M, p.N))
     return GDN_ERR_LAUNCH;
+  if (p.part_tma && !make_part_map(&my, p.part, p.M, p.N, p.splits)) return GDN_ERR_LAUNCH;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
   const int grid = (int)(items < sm_count() ? items : sm_count());
   k<<<grid, THREADS, Cfg<BN>::SMEM, s>>>(ma, mb, my, mpre, p);
@@ -660,12 +716,13 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
   p.splits = pl.splits;
   p.kblocks = (int)((p.K + BK - 1) / BK);
   p.part = static_cast<float*>(ws);
+  p.part_tma = p.splits > 1 && p.N % 4 == 0;
   p.vec = rows16(p.y, p.ldy) && p.N % 8 == 0 && (!p.bias || ssm::aligned16(p.bias)) && (!p.res || rows16(p.res, p.ldr)) && (!p.pre || rows16(p.pre, p.N));
   int st = pl.bn == 256 ? launch_gemm<256, AMN, BMN>(p, s) : pl.bn == 128 ? launch_gemm<128, AMN, BMN>(p, s) : launch_gemm<64, AMN, BMN>(p, s);
   if (st != GDN_OK || p.splits == 1) return st;
   const int64_t g = (p.M * ((p.N + 3) / 4) + 255) / 256;
   if (g > 0x7fffffff) return GDN_ERR_SHAPE;
-  split_epilogue_kernel<<<(unsigned)g, 256, 0, s>>>(p);
+  p.vec ? split_epilogue_kernel<true><<<(unsigned)g, 256, 0, s>>>(p) : split_epilogue_kernel<false><<<(unsigned)g, 256, 0, s>>>(p);
   return ssm::launched();
 }
 

@@ -23,25 +23,26 @@ import torch
 import torch.nn as nn
 
 from .layers import GatedDeltaNet, GDNCache, NStepGDN
+from .ssm_layer import SelectiveSSM
 
 
 def _stateful_layers(model: nn.Module) -> List[nn.Module]:
-    layers = [m for m in model.modules() if isinstance(m, (NStepGDN, GatedDeltaNet))]
+    layers = [m for m in model.modules() if isinstance(m, (NStepGDN, GatedDeltaNet, SelectiveSSM))]
     for name, m in model.named_modules():
         if name.split(".")[-1] == "mixer" and not any(l is m or any(l is c for c in m.modules()) for l in layers):
             raise ValueError(f"{name} ({type(m).__name__}) keeps no recurrent state across calls; "
-                             "cached decoding needs every mixer to be a B200 gdn/nsgdn layer")
+                             "cached decoding needs every mixer to be a B200 gdn/nsgdn/ssm layer")
     if getattr(model, "smear_gate", None) is not None:
         raise ValueError("the embedding smear mixes each token with the previous one's embedding, "
                          "which a one-token call does not see; cached decoding needs smear off")
     if not layers:
-        raise ValueError("model has no B200 gdn/nsgdn layers")
+        raise ValueError("model has no B200 gdn/nsgdn/ssm layers")
     return layers
 
 
 @contextlib.contextmanager
 def bind_caches(model: nn.Module) -> Iterator[List[GDNCache]]:
-    """Bind a fresh ``GDNCache`` to every gdn/nsgdn layer of ``model`` (yielded in module order);
+    """Bind a fresh ``GDNCache`` to every gdn/nsgdn/ssm layer of ``model`` (yielded in module order);
     the bindings are removed on exit."""
     layers = _stateful_layers(model)
     if any(l.bound_cache is not None for l in layers):

@@ -9,7 +9,8 @@ restates the part of it configuration 4 uses, with the same module names and mat
     mlp: SwiGLU, hidden = round_up(2/3 * mlp_ratio * d_model, 64)      (model.py:18-33)
 
 archbench's optional extras (per-layer residual scalars, the mid-depth backout, embedding norm)
-are available as keywords; the embedding smear is not, since cached decoding cannot serve it
+are available as keywords, and so is ``mlp="silu"`` or ``"gelu"`` (a biased two-matrix MLP whose
+bias, activation and residual run in the products' epilogues); the embedding smear is not, since cached decoding cannot serve it
 (``decode.bind_caches``).  Configuration 4: 24 ``gdn`` blocks, d_model 1024, 8 heads of
 head_dim 128 with expand_v 1, short convolutions of width 4, output gate, RMSNorm, SwiGLU hidden
 2816 (mlp_ratio 4.125), vocabulary 50304, bf16 weights ~ N(0, 0.02) (``config4_lm``).
@@ -22,6 +23,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .registry import build_mixer
+from .ssm_layer import FusedMLP
 
 
 class MLP(nn.Module):
@@ -37,25 +39,28 @@ class MLP(nn.Module):
 
 
 class Block(nn.Module):
-    def __init__(self, arch: str, d_model: int, layer_idx: int, n_layer: int, mlp_ratio: float, norm_eps: float, layer: dict):
+    def __init__(self, arch: str, d_model: int, layer_idx: int, n_layer: int, mlp_ratio: float, norm_eps: float, layer: dict,
+                 mlp: str = "swiglu"):
         super().__init__()
         self.norm1 = nn.RMSNorm(d_model, eps=norm_eps)
         self.mixer = build_mixer(arch, d_model, layer_idx, n_layer, **layer)
         self.norm2 = nn.RMSNorm(d_model, eps=norm_eps)
-        self.mlp = MLP(d_model, mlp_ratio)
+        self.mlp = MLP(d_model, mlp_ratio) if mlp == "swiglu" else FusedMLP(d_model, mlp_ratio, mlp)
 
     def forward(self, x):
-        x = x + self.mixer(self.norm1(x))
-        return x + self.mlp(self.norm2(x))
+        for part, norm in ((self.mixer, self.norm1), (self.mlp, self.norm2)):
+            # parts whose last projection adds the residual itself take it along
+            x = part(norm(x), residual=x) if getattr(part, "fuses_residual", False) else x + part(norm(x))
+        return x
 
 
 class LM(nn.Module):
     def __init__(self, arch="gdn", d_model=1024, n_layer=24, vocab_size=50304, mlp_ratio=4.125, norm_eps=1e-5,
-                 layer=None, resid_scalars=False, backout=False, embed_norm=False, init_std=0.02):
+                 layer=None, resid_scalars=False, backout=False, embed_norm=False, init_std=0.02, mlp="swiglu"):
         super().__init__()
         self.n_layer, self.embed_norm = n_layer, embed_norm
         self.embed = nn.Embedding(vocab_size, d_model)
-        self.blocks = nn.ModuleList(Block(arch, d_model, i, n_layer, mlp_ratio, norm_eps, dict(layer or {}))
+        self.blocks = nn.ModuleList(Block(arch, d_model, i, n_layer, mlp_ratio, norm_eps, dict(layer or {}), mlp)
                                     for i in range(n_layer))
         self.norm = nn.RMSNorm(d_model, eps=norm_eps)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)

@@ -2,7 +2,7 @@
 archbench/layers/__init__.py:1-26) or builds them standalone.
 
     import archbench_b200.registry as r
-    r.install()          # archbench's build_mixer("gdn" | "nsgdn", ...) now builds the B200 layers
+    r.install()          # archbench's build_mixer("gdn" | "nsgdn" | "ssm", ...) now builds the B200 layers
 
 Builders keep archbench's signature ``builder(d_model, layer_idx, n_layer, **layer_kwargs)`` so
 ``Block.__init__`` (archbench/model.py:40) and the configs' ``model.layer`` keys work unchanged.
@@ -17,6 +17,7 @@ import inspect
 import torch.nn as nn
 
 from .layers import GatedDeltaNet, NStepGDN
+from .ssm_layer import SelectiveSSM
 
 
 class MixerWrapper(nn.Module):
@@ -51,7 +52,12 @@ def build_gdn(d_model: int, layer_idx: int, n_layer: int, **kwargs) -> nn.Module
     return wrapper(GatedDeltaNet(**kwargs))
 
 
-BUILDERS = {"gdn": build_gdn, "nsgdn": build_nsgdn}
+def build_ssm(d_model: int, layer_idx: int, n_layer: int, **kwargs) -> nn.Module:
+    """This package's selective-state-space mixer (no archbench counterpart under this name)."""
+    return SelectiveSSM(d_model, layer_idx=layer_idx, **kwargs)
+
+
+BUILDERS = {"gdn": build_gdn, "nsgdn": build_nsgdn, "ssm": build_ssm}
 
 
 def build_mixer(name: str, d_model: int, layer_idx: int, n_layer: int, **kwargs) -> nn.Module:
@@ -61,7 +67,7 @@ def build_mixer(name: str, d_model: int, layer_idx: int, n_layer: int, **kwargs)
 
 
 def install() -> None:
-    """Point archbench's registry entries ``gdn`` and ``nsgdn`` at the B200 layers."""
+    """Point archbench's registry entries ``gdn`` and ``nsgdn`` at the B200 layers and add ``ssm``."""
     from archbench import layers as L
 
     for name, fn in BUILDERS.items():
