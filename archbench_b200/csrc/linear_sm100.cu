@@ -51,10 +51,14 @@ struct GemmP {
   int part_tma; // N a multiple of four: TMA stores them
 };
 
-template <int BN>
+// PAIR: two CTAs of a cluster work on one 256 x BN tile, each with half of A's rows, half of B's and half of the
+// accumulator's rows; one of them issues the MMAs of both.  Half the operand bytes per multiplication come from L2 and
+// shared memory.
+template <int BN, bool PAIR>
 struct Cfg {
-  static constexpr int STAGE = (BM + BN) * BK * 2;
-  static constexpr int STAGES = 196608 / STAGE;  // 4, 6, 8 for BN = 256, 128, 64
+  static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B that a CTA holds
+  static constexpr int STAGE = (BM + BROWS) * BK * 2;
+  static constexpr int STAGES = 196608 / STAGE;  // 4, 6, 8 for BN = 256 (6 in pairs), 128, 64
   static constexpr int COLS = BN == 64 ? 64 : BN / 2;  // columns per epilogue warp (with 64, half of the warps rest)
   static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * OUT_BYTES + 1024 /* alignment */ + 256 /* barriers */;
 };
@@ -105,17 +109,52 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+// The pair's forms: a load into this CTA's memory that reports to a barrier of the pair's first CTA, the MMA over both
+// CTAs' operands and accumulators, and the arrival on the same barrier of both.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          ptx::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair_elect(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair_elect(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+          ptx::smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
 // One operand's part of a stage: ROWS output indices x 64 k.  k-contiguous: one box of ROWS rows; else ROWS / 64 boxes
 // of 64 k rows.
-template <int ROWS, bool MN>
-__device__ __forceinline__ void stage_tma(char* dst, const CUtensorMap* map, uint64_t* bar, int idx0, int k0) {
+template <int ROWS, bool MN, bool PAIR>
+__device__ __forceinline__ void stage_tma(char* dst, const CUtensorMap* map, uint64_t* bar, uint32_t pair_bar, int idx0, int k0) {
+  auto load = [&](char* to, int c0, int c1) {
+    if (PAIR)
+      tma_load_2d_pair(to, map, pair_bar, c0, c1);
+    else
+      tma_load_2d(to, map, bar, c0, c1);
+  };
   if (!MN) {
-    tma_load_2d(dst, map, bar, k0, idx0);
+    load(dst, k0, idx0);
   } else {
 #pragma unroll
-    for (int i = 0; i < ROWS / 64; ++i) tma_load_2d(dst + i * 8192, map, bar, idx0 + i * 64, k0);
+    for (int i = 0; i < ROWS / 64; ++i) load(dst + i * 8192, idx0 + i * 64, k0);
   }
 }
+
 // Operand descriptor of k step s (16 deep) in a stage part at shared address `base`.
 template <bool MN>
 __device__ __forceinline__ uint64_t step_desc(uint32_t base, int s) {
@@ -191,12 +230,12 @@ __device__ __noinline__ void box_copy_in(char* box, int lane, const bf16* p, int
   __syncwarp();
 }
 
-template <int BN, bool AMN, bool BMN>
+template <int BN, bool AMN, bool BMN, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap my,
-                const __grid_constant__ CUtensorMap mpre, const GemmP p) {
-  using C = Cfg<BN>;
-  constexpr int ST = C::STAGES, A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+                const __grid_constant__ CUtensorMap mpre, const __grid_constant__ CUtensorMap mres, const GemmP p) {
+  using C = Cfg<BN, PAIR>;
+  constexpr int ST = C::STAGES, A_BYTES = BM * BK * 2, B_BYTES = C::BROWS * BK * 2, CTAS = PAIR ? 2 : 1;
   extern __shared__ char raw_smem[];
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
   char* boxes = tiles + ST * C::STAGE;
@@ -204,7 +243,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* empty = full + ST;
   uint64_t* tfull = empty + ST;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* rfull = tempty + 2;  // per epilogue warp: its residual box is in
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + EPI_WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -215,18 +255,28 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(tfull + i, 1);
-      ptx::mbar_init(tempty + i, BN == 64 ? 4 : EPI_WARPS);
+      ptx::mbar_init(tempty + i, BN == 64 ? 4 : EPI_WARPS * CTAS);
     }
+    for (int i = 0; i < EPI_WARPS; ++i) ptx::mbar_init(rfull + i, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
   if (warp == 1) {
-    ptx::tmem_alloc(tmem_slot, 2 * BN);
-    ptx::tmem_relinquish();
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      ptx::tmem_alloc(tmem_slot, 2 * BN);
+      ptx::tmem_relinquish();
+    }
   }
   __syncthreads();
+  if (PAIR) ptx::cluster_sync();  // both CTAs' barriers are ready
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // A CTA, or a pair of them, takes every `units`-th item; row and column offsets of its half of the operands.
+  const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0;
+  const int unit = blockIdx.x / CTAS, units = gridDim.x / CTAS, half = rank * BM;
   const int items = p.tiles_m * p.tiles_n * p.splits;
   const int per = (p.kblocks + p.splits - 1) / p.splits;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return ptx::mbar_wait_abortable(bar, parity, WAIT_CYCLES, abort_flag); };
@@ -235,31 +285,36 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       uint32_t n = 0;  // k blocks issued
       bool ok = true;
-      for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
+      for (int it = unit; ok && it < items; it += units) {
         const int tile = it / p.splits, sp = it % p.splits;
-        const int m0 = tile % p.tiles_m * BM, n0 = tile / p.tiles_m * BN;
+        const int m0 = tile % p.tiles_m * (BM * CTAS) + half, n0 = tile / p.tiles_m * BN + (PAIR ? half : 0);
         const int kb1 = min((sp + 1) * per, p.kblocks);
         for (int kb = sp * per; kb < kb1; ++kb, ++n) {
           const int s = n % ST;
           if (!wait(empty + s, ((n / ST) & 1) ^ 1)) { ok = false; break; }
           char* st = tiles + s * C::STAGE;
-          ptx::mbar_arrive_expect_tx(full + s, A_BYTES + B_BYTES);
-          stage_tma<BM, AMN>(st, &ma, full + s, m0, kb * BK);
-          stage_tma<BN, BMN>(st + A_BYTES, &mb, full + s, n0, kb * BK);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full + s, (A_BYTES + B_BYTES) * CTAS);
+          const uint32_t pair_bar = PAIR ? ptx::mapa_shared(ptx::smem_u32(full + s), 0) : 0;
+          stage_tma<BM, AMN, PAIR>(st, &ma, full + s, pair_bar, m0, kb * BK);
+          stage_tma<C::BROWS, BMN, PAIR>(st + A_BYTES, &mb, full + s, pair_bar, n0, kb * BK);
         }
       }
-      if (!ok)  // leave no copy in flight: each outstanding stage's own barrier, with a limit
+      if (ok && PAIR)  // the MMAs' arrivals on this CTA's barriers come from the other one: all of them, before it can leave
+        for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i) wait(empty + i % ST, (i / ST) & 1);
+      if (!ok && rank == 0)  // leave no copy in flight: each outstanding stage's barrier, with a limit
         for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i) ptx::mbar_wait_bounded(full + i % ST, (i / ST) & 1, WAIT_CYCLES / 8);
     }
-  } else if (warp == 1) {
-    constexpr uint32_t idesc = ptx::idesc_bf16_f32(BM, BN, AMN, BMN);
+  } else if (warp == 1 && rank == 0) {
+    constexpr uint32_t idesc = ptx::idesc_bf16_f32(BM * CTAS, BN, AMN, BMN);
     uint32_t n = 0, acc = 0;
     bool ok = true;
-    for (int it = blockIdx.x; ok && it < items; it += gridDim.x, ++acc) {
+    for (int it = unit; ok && it < items; it += units, ++acc) {
       const int sp = it % p.splits;
       const int kb0 = sp * per, kb1 = min((sp + 1) * per, p.kblocks);
       const uint32_t buf = acc & 1;
-      if (!wait(tempty + buf, ((acc >> 1) & 1) ^ 1)) break;
+      if (PAIR ? !ptx::mbar_wait_abortable_cluster(tempty + buf, ((acc >> 1) & 1) ^ 1, WAIT_CYCLES, abort_flag)
+               : !wait(tempty + buf, ((acc >> 1) & 1) ^ 1))
+        break;
       ptx::tc_fence_after();
       for (int kb = kb0; kb < kb1; ++kb, ++n) {
         const int s = n % ST;
@@ -267,38 +322,49 @@ __global__ void __launch_bounds__(THREADS, 1)
         ptx::tc_fence_after();
         const uint32_t a = ptx::smem_u32(tiles + s * C::STAGE), b = a + A_BYTES;
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          ptx::mma_f16_ss_elect(tmem + buf * BN, step_desc<AMN>(a, k), step_desc<BMN>(b, k), idesc, kb > kb0 || k > 0);
-        ptx::mma_commit_elect(empty + s);
+        for (int k = 0; k < BK / 16; ++k) {
+          if (PAIR)
+            mma_pair_elect(tmem + buf * BN, step_desc<AMN>(a, k), step_desc<BMN>(b, k), idesc, kb > kb0 || k > 0);
+          else
+            ptx::mma_f16_ss_elect(tmem + buf * BN, step_desc<AMN>(a, k), step_desc<BMN>(b, k), idesc, kb > kb0 || k > 0);
+        }
+        PAIR ? commit_pair_elect(empty + s) : ptx::mma_commit_elect(empty + s);
       }
-      ptx::mma_commit_elect(tfull + buf);
+      PAIR ? commit_pair_elect(tfull + buf) : ptx::mma_commit_elect(tfull + buf);
       if (!ok) ptx::mbar_wait_bounded(tfull + buf, (acc >> 1) & 1, WAIT_CYCLES / 8);  // no MMA left in flight
     }
-  } else {
+  } else if (warp >= 2) {
     const int quarter = warp % 4;  // tensor-memory lanes this warp can read
     const int c0 = (warp - 2) / 4 * C::COLS;  // its first column of a tile
     char* box = boxes + (warp - 2) * OUT_BYTES;
-    uint32_t acc = 0;
-    for (int it = blockIdx.x; c0 < BN && it < items; it += gridDim.x, ++acc) {
+    uint32_t acc = 0, fetched = 0;
+    for (int it = unit; c0 < BN && it < items; it += units, ++acc) {
       const int tile = it / p.splits, sp = it % p.splits;
-      const int64_t row0 = (int64_t)(tile % p.tiles_m) * BM + quarter * 32, row = row0 + lane, n0 = (int64_t)(tile / p.tiles_m) * BN;
+      const int64_t row0 = (int64_t)(tile % p.tiles_m) * (BM * CTAS) + half + quarter * 32, row = row0 + lane, n0 = (int64_t)(tile / p.tiles_m) * BN;
       const uint32_t buf = acc & 1;
       const bool in = row < p.M;
-      uint4 res[8];  // the residual of 64 columns, on its way while the accumulator is waited for
-      auto load_res = [&](int64_t col) {
-        if (!p.res || p.splits > 1 || row0 >= p.M) return;
-        if (!p.vec) {
+      // The residual of 64 columns: fetched into the box while the accumulator is waited for, taken into registers before
+      // the box carries an output.
+      uint4 res[8];
+      auto fetch_res = [&](int64_t col) {
+        if (!p.res || !p.vec || p.splits > 1 || row0 >= p.M || col >= p.N) return;
+        if (lane == 0) {
+          ptx::bulk_wait_read0();
+          ptx::mbar_arrive_expect_tx(rfull + warp - 2, OUT_BYTES);
+          tma_load_2d(box, &mres, rfull + warp - 2, (int)col, (int)row0);
+        }
+      };
+      auto take_res = [&](int64_t col) {
+        if (!p.res) return true;
+        if (p.vec) {
+          if (!wait(rfull + warp - 2, fetched++ & 1)) return false;
+        } else {
           box_copy_in(box, lane, p.res, p.ldr, row0, col, p.M, p.N);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) res[j] = *reinterpret_cast<const uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
-          __syncwarp();
-          return;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          res[j] = make_uint4(0, 0, 0, 0);
-          if (in && col + j * 8 < p.N) res[j] = *reinterpret_cast<const uint4*>(p.res + row * p.ldr + col + j * 8);
-        }
+        for (int j = 0; j < 8; ++j) res[j] = *reinterpret_cast<const uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
+        __syncwarp();
+        return true;
       };
       auto put = [&](const CUtensorMap* map, bf16* to, int64_t ld, int64_t col, const f32x2 (&v)[2][16]) {
         if (p.vec) box_ready(lane);
@@ -309,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         else
           box_copy_out(box, lane, to, ld, row0, col, p.M, p.N);
       };
-      load_res(n0 + c0);
+      fetch_res(n0 + c0);
       if (!wait(tfull + buf, (acc >> 1) & 1)) break;
       ptx::tc_fence_after();
 #pragma unroll 1
@@ -363,6 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               v[e][i] = add2(v[e][i], pack2(__shfl_sync(0xffffffffu, bl, 2 * i), __shfl_sync(0xffffffffu, bl, 2 * i + 1)));
           }
         }
+        if (!__all_sync(0xffffffffu, take_res(n0 + c))) break;
         if (p.pre) put(&mpre, p.pre, p.N, n0 + c, v);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -372,18 +439,30 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (p.res) v[e][i] = add2(v[e][i], load_pair(reinterpret_cast<const bf16*>(&res[e * 4 + i / 4]) + i % 4 * 2));
           }
         put(&my, p.y, p.ldy, n0 + c, v);
-        if (c + 64 < c0 + C::COLS) load_res(n0 + c + 64);
+        if (c + 64 < c0 + C::COLS) fetch_res(n0 + c + 64);
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(tempty + buf);
+      if (lane == 0) {
+        if (PAIR)
+          ptx::mbar_arrive_remote(ptx::mapa_shared(ptx::smem_u32(tempty + buf), 0));
+        else
+          ptx::mbar_arrive(tempty + buf);
+      }
     }
+    if (*abort_flag && p.res && p.vec && lane == 0)  // a residual box may still be on its way
+      ptx::mbar_wait_bounded(rfull + warp - 2, fetched & 1, WAIT_CYCLES / 8);
     if (lane == 0) ptx::bulk_wait0();  // the stores have read the boxes and are done
     __syncwarp();
   }
   __syncthreads();
   if (tid == 0 && *abort_flag) atomicExch(&g_status, GDN_ERR_TIMEOUT);
-  if (warp == 1) ptx::tmem_dealloc(tmem, 2 * BN);
+  if (PAIR) {
+    ptx::cluster_sync();  // neither CTA leaves while the other may still reach its barriers or accumulators
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+  } else if (warp == 1) {
+    ptx::tmem_dealloc(tmem, 2 * BN);
+  }
 }
 
 // The splits' sums, in order, and the epilogue; 4 columns per thread (VEC: as vectors).
@@ -626,32 +705,66 @@ bool make_part_map(CUtensorMap* m, float* p, int64_t M, int64_t N, int64_t split
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// CTA pairs that run at once (the same for every pair kernel: one CTA per SM), 0 where the device cannot say.
+int pair_count() {
+  static std::atomic<int> cached[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  const int c = cached[dev].load(std::memory_order_relaxed);
+  if (c) return c - 1;
+  using C = Cfg<256, true>;
+  static std::atomic<unsigned long long> opted{0};
+  auto k = gemm_kernel<256, false, false, true>;
+  int n = 0;
+  if (opt_in_smem(opted, {{(const void*)k, C::SMEM}})) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+  }
+  cached[dev].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 struct Plan {
-  int bn, splits;
-  size_t part;  // bytes
+  int bn, splits, pairs;  // pairs: CTA pairs on 256 x 256 tiles
+  size_t part;            // bytes
 };
 
-// Tile width and splits of the contraction by a model of the time in SM clocks: waves of tiles, a k block taking 540, 300
-// or 200 clocks with 256, 128 or 64 columns (the tensor pipe's 512 clocks, then the operands' way out of shared memory)
-// and a tile 2500 to start and drain; splits add their sums' way through memory (2 x 4 bytes at 3400 bytes a clock) and a
-// launch.  16384 x 1024 x 2816 runs 256-wide (98 us; 105 us 128-wide), 1024 x 2816 x 16384 in two waves of split tiles.
+// Tile shape and splits of the contraction by a model of the time in SM clocks: waves of tiles, a k block taking 540, 300
+// or 200 clocks with 256, 128 or 64 columns (the tensor pipe's 512 clocks, then the operands' way out of shared memory; a
+// pair's 256 x 256 tile PAIR_CLOCKS) and a tile 2500 to start and drain; splits add their sums' way through memory (2 x 4
+// bytes at 3400 bytes a clock) and a launch.
+constexpr int PAIR_CLOCKS = 530;
+
 Plan plan(int64_t M, int64_t N, int64_t K) {
-  const int64_t sms = sm_count(), tm = (M + BM - 1) / BM, kb = (K + BK - 1) / BK;
-  Plan best = {64, 1, 0};
+  const int64_t sms = sm_count(), pairs = pair_count(), kb = (K + BK - 1) / BK;
+  Plan best = {64, 1, 0, 0};
   double least = 1e300;
   const struct {
-    int bn, clocks;
-  } widths[] = {{256, 540}, {128, 300}, {64, 200}};
-  for (const auto& w : widths) {
-    const int64_t tiles = tm * ((N + w.bn - 1) / w.bn);
+    int bm, bn, clocks;
+    int64_t units;
+  } shapes[] = {{256, 256, PAIR_CLOCKS, pairs}, {128, 256, 540, sms}, {128, 128, 300, sms}, {128, 64, 200, sms}};
+  for (const auto& w : shapes) {
+    if (w.units < 1) continue;
+    const int64_t tiles = (M + w.bm - 1) / w.bm * ((N + w.bn - 1) / w.bn);
     for (int64_t s = 1; s <= 16; ++s) {
-      if (s > 1 && (kb / s < 4 || tiles >= 4 * sms)) break;
-      const int64_t per = (kb + s - 1) / s, splits = (kb + per - 1) / per, waves = (tiles * splits + sms - 1) / sms;
+      if (s > 1 && (kb / s < 4 || tiles >= 4 * w.units)) break;
+      const int64_t per = (kb + s - 1) / s, splits = (kb + per - 1) / per, waves = (tiles * splits + w.units - 1) / w.units;
       const double t = (double)waves * (double)(per * w.clocks + 2500) + (splits > 1 ? (double)splits * (double)(M * N) * 8 / 3400 + 6000 : 0);
       if (t < least) {
         least = t;
-        best.bn = w.bn;
-        best.splits = (int)splits;
+        best = {w.bn, (int)splits, w.bm == 256 ? (int)pairs : 0, 0};
       }
     }
   }
@@ -659,21 +772,32 @@ Plan plan(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-template <int BN, bool AMN, bool BMN>
-int launch_gemm(const GemmP& p, cudaStream_t s) {
+template <int BN, bool AMN, bool BMN, bool PAIR>
+int launch_gemm(const GemmP& p, int pairs, cudaStream_t s) {
+  using C = Cfg<BN, PAIR>;
   static std::atomic<unsigned long long> opted{0};
-  auto k = gemm_kernel<BN, AMN, BMN>;
-  if (!opt_in_smem(opted, {{(const void*)k, Cfg<BN>::SMEM}})) return GDN_ERR_LAUNCH;
-  CUtensorMap ma, mb, my, mpre;
+  auto k = gemm_kernel<BN, AMN, BMN, PAIR>;
+  if (!opt_in_smem(opted, {{(const void*)k, C::SMEM}})) return GDN_ERR_LAUNCH;
+  CUtensorMap ma, mb, my, mpre, mres;
   const bool out = p.vec && p.splits == 1;
-  if (!make_map2(&ma, p.a, AMN ? BK : BM) || !make_map2(&mb, p.b, BMN ? BK : BN) || !make_out_map(&my, out ? p.y : nullptr, p.ldy, p.M, p.N) ||
-      !make_out_map(&mpre, out ? p.pre : nullptr, p.N, p.M, p.N))
+  if (!make_map2(&ma, p.a, AMN ? BK : BM) || !make_map2(&mb, p.b, BMN ? BK : C::BROWS) || !make_out_map(&my, out ? p.y : nullptr, p.ldy, p.M, p.N) ||
+      !make_out_map(&mpre, out ? p.pre : nullptr, p.N, p.M, p.N) || !make_out_map(&mres, out ? const_cast<bf16*>(p.res) : nullptr, p.ldr, p.M, p.N))
     return GDN_ERR_LAUNCH;
   if (p.part_tma && !make_part_map(&my, p.part, p.M, p.N, p.splits)) return GDN_ERR_LAUNCH;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  const int grid = (int)(items < sm_count() ? items : sm_count());
-  k<<<grid, THREADS, Cfg<BN>::SMEM, s>>>(ma, mb, my, mpre, p);
-  return ssm::launched();
+  const int64_t units = PAIR ? pairs : sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((items < units ? items : units) * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 2;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, ma, mb, my, mpre, mres, p) == cudaSuccess ? ssm::launched() : GDN_ERR_LAUNCH;
 }
 
 // Bytes of an operand's aligned copy, 0 where it needs none, and the copy itself (which then stands for it).
@@ -709,7 +833,8 @@ int align_operand(Operand& o, char*& ws, cudaStream_t s) {
 template <bool AMN, bool BMN>
 int gemm(GemmP p, void* ws, cudaStream_t s) {
   const Plan pl = plan(p.M, p.N, p.K);
-  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + pl.bn - 1) / pl.bn;
+  const int bm = pl.pairs ? 2 * BM : BM;
+  const int64_t tm = (p.M + bm - 1) / bm, tn = (p.N + pl.bn - 1) / pl.bn;
   if (tm * tn * pl.splits > 0x7fffffff) return GDN_ERR_SHAPE;
   p.tiles_m = (int)tm;
   p.tiles_n = (int)tn;
@@ -718,7 +843,10 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
   p.part = static_cast<float*>(ws);
   p.part_tma = p.splits > 1 && p.N % 4 == 0;
   p.vec = rows16(p.y, p.ldy) && p.N % 8 == 0 && (!p.bias || ssm::aligned16(p.bias)) && (!p.res || rows16(p.res, p.ldr)) && (!p.pre || rows16(p.pre, p.N));
-  int st = pl.bn == 256 ? launch_gemm<256, AMN, BMN>(p, s) : pl.bn == 128 ? launch_gemm<128, AMN, BMN>(p, s) : launch_gemm<64, AMN, BMN>(p, s);
+  const int st = pl.pairs      ? launch_gemm<256, AMN, BMN, true>(p, pl.pairs, s)
+                 : pl.bn == 256 ? launch_gemm<256, AMN, BMN, false>(p, 0, s)
+                 : pl.bn == 128 ? launch_gemm<128, AMN, BMN, false>(p, 0, s)
+                                : launch_gemm<64, AMN, BMN, false>(p, 0, s);
   if (st != GDN_OK || p.splits == 1) return st;
   const int64_t g = (p.M * ((p.N + 3) / 4) + 255) / 256;
   if (g > 0x7fffffff) return GDN_ERR_SHAPE;

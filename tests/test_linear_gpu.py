@@ -26,6 +26,8 @@ CASES = [  # M, N, K, bias, act, residual, odd rows (views that start off a 16-b
     (2500, 1024, 72, True, "gelu", True, False),   # 128-wide tiles
     (5000, 1024, 136, True, None, True, False),    # 256-wide tiles
     (4777, 1032, 200, False, "silu", True, True),
+    (2300, 2048, 320, True, "silu", True, False),  # pairs of CTAs on 256 x 256 tiles
+    (9500, 2304, 72, False, "gelu", True, False),
 ]
 
 
@@ -71,6 +73,24 @@ def test_linear_forward_and_backward(case):
     sizes = dict(x=max(1.0, (N / K) ** 0.5), weight=M ** 0.5, bias=M ** 0.5, residual=1.0)
     for k, a, b in zip(names, got, want):
         close(a, b, sizes[k], "d" + k, r if k != "residual" else 0)
+
+
+@pytest.mark.parametrize("M,N,K,odd", [(2305, 2056, 1100, False), (2200, 2047, 333, True), (9728, 2304, 200, False), (512, 4096, 5000, False)])
+def test_linear_large_tiles(M, N, K, odd):
+    """Pairs of CTAs, split contractions and ragged edges of both, with no activation between: each value differs from the
+    64-bit one by its own rounding, at most 2^-9 of it, and by fp32 sums' errors (5000 terms: 2^-12 of their rms at most),
+    so the difference's 2-norm is within 2^-9 + 2^-12."""
+    g = torch.Generator("cuda").manual_seed(M + N)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    x, w, b, r, dy = off(rnd(M, K), odd), off(rnd(N, K), odd), rnd(N), off(rnd(M, N), odd), rnd(M, N)
+    ref = [t.double().requires_grad_() for t in (x, w, b, r)]
+    own = [t.detach().requires_grad_() for t in (x, w, b, r)]
+    y0, y = R.linear(ref[0], ref[1], ref[2], None, ref[3]), ops.linear(own[0], own[1], own[2], None, own[3])
+    got, want = [y, *torch.autograd.grad(y, own, dy)], [y0, *torch.autograd.grad(y0, ref, dy.double())]
+    for n, a, e in zip("y dx dw db dr".split(), got, want):
+        rel = ((a.double() - e).norm() / e.norm()).item()
+        assert rel <= 2.0 ** -9 + 2.0 ** -12, (n, rel)
+    assert ops.device_status() == 0
 
 
 def test_linear_shapes_and_partial_gradients():
