@@ -49,6 +49,11 @@ struct GemmP {
   int act, vec;
   float* part;  // splits > 1: (splits, M, N) sums
   int part_tma; // N a multiple of four: TMA stores them
+  // Tiles run along the shorter side first: a wave then reads few rows of the longer operand, once, and the shorter
+  // operand stays in L2.
+  int n_first;
+  __device__ int tile_m(int t) const { return n_first ? t / tiles_n : t % tiles_m; }
+  __device__ int tile_n(int t) const { return n_first ? t % tiles_n : t / tiles_m; }
 };
 
 // PAIR: two CTAs of a cluster work on one 256 x BN tile, each with half of A's rows, half of B's and half of the
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       for (int it = unit; ok && it < items; it += units) {
         const int tile = it / p.splits, sp = it % p.splits;
-        const int m0 = tile % p.tiles_m * (BM * CTAS) + half, n0 = tile / p.tiles_m * BN + (PAIR ? half : 0);
+        const int m0 = p.tile_m(tile) * (BM * CTAS) + half, n0 = p.tile_n(tile) * BN + (PAIR ? half : 0);
         const int kb1 = min((sp + 1) * per, p.kblocks);
         for (int kb = sp * per; kb < kb1; ++kb, ++n) {
           const int s = n % ST;
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t acc = 0, fetched = 0;
     for (int it = unit; c0 < BN && it < items; it += units, ++acc) {
       const int tile = it / p.splits, sp = it % p.splits;
-      const int64_t row0 = (int64_t)(tile % p.tiles_m) * (BM * CTAS) + half + quarter * 32, row = row0 + lane, n0 = (int64_t)(tile / p.tiles_m) * BN;
+      const int64_t row0 = (int64_t)p.tile_m(tile) * (BM * CTAS) + half + quarter * 32, row = row0 + lane, n0 = (int64_t)p.tile_n(tile) * BN;
       const uint32_t buf = acc & 1;
       const bool in = row < p.M;
       // The residual of 64 columns: fetched into the box while the accumulator is waited for, taken into registers before
@@ -838,6 +843,7 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
   if (tm * tn * pl.splits > 0x7fffffff) return GDN_ERR_SHAPE;
   p.tiles_m = (int)tm;
   p.tiles_n = (int)tn;
+  p.n_first = tn <= tm;
   p.splits = pl.splits;
   p.kblocks = (int)((p.K + BK - 1) / BK);
   p.part = static_cast<float*>(ws);
