@@ -809,24 +809,26 @@ int launch_gemm(const GemmP& p, int pairs, cudaStream_t s) {
 size_t align_bytes(const Operand& o) { return o.tma ? 0 : up256((size_t)o.rows * ((o.cols + 7) / 8 * 8) * 2); }
 
 __global__ void __launch_bounds__(256) align_kernel(const bf16* src, int64_t ld, bf16* dst, int64_t rows, int64_t cols) {
-  const int64_t chunks = (cols + 7) / 8, n = rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+  // rows by blockIdx.y, 16 bytes per thread
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (c >= cols) return;
     const bf16* s = src + r * ld + c;
     uint4 raw = make_uint4(0, 0, 0, 0);
     bf16* e = reinterpret_cast<bf16*>(&raw);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (c + j < cols) e[j] = s[j];
-    reinterpret_cast<uint4*>(dst)[i] = raw;
+    *reinterpret_cast<uint4*>(dst + r * ((cols + 7) / 8 * 8) + c) = raw;
   }
 }
 
 int align_operand(Operand& o, char*& ws, cudaStream_t s) {
   if (o.tma) return GDN_OK;
   const size_t bytes = align_bytes(o);
-  const int64_t ld = (o.cols + 7) / 8 * 8, g = (o.rows * (ld / 8) + 255) / 256;
-  align_kernel<<<(unsigned)(g < 148 * 16 ? g : 148 * 16), 256, 0, s>>>(o.p, o.ld, reinterpret_cast<bf16*>(ws), o.rows, o.cols);
+  const int64_t ld = (o.cols + 7) / 8 * 8;
+  const dim3 g((unsigned)((ld / 8 + 255) / 256), (unsigned)(o.rows < 65535 ? o.rows : 65535));
+  align_kernel<<<g, 256, 0, s>>>(o.p, o.ld, reinterpret_cast<bf16*>(ws), o.rows, o.cols);
   o.p = reinterpret_cast<const bf16*>(ws);
   o.ld = ld;
   o.tma = 1;

@@ -124,7 +124,7 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 __device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
-// softplus and the sigmoid of two values (see ssm_common.cuh for the formulas).
+// softplus and the sigmoid of two values (see above for the formulas).
 __device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
   const float2 e = unpack2(add2(exp2_2(mul2(x, both(-LOG2E))), both(1.f)));
   return pack2(rcp(e.x), rcp(e.y));

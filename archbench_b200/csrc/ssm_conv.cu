@@ -90,9 +90,12 @@ __device__ __forceinline__ void load_weight_pairs(const ConvP& p, int c, f32x2 (
   }
 }
 
-// The loads of BATCH tokens go out together; 64 KB in flight per SM cover HBM's latency.
+// The loads of BATCH tokens go out together.  Four channels per thread keep 32 warps on an SM: 68 us at 8 x 4096 x 2048
+// (bf16, width 4) against 74 us with eight channels, and loads a batch ahead, in registers, cost more warps than they hide
+// (82 us).  The sigmoids' two operations per value on their pipe
+// (30 us) and the packed arithmetic (20 us) overlap HBM's 41 us in part.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(THREADS) conv_fwd_kernel(const ConvP p) {
+__global__ void __launch_bounds__(THREADS, 8) conv_fwd_kernel(const ConvP p) {
   constexpr int HP = (VEC + 1) / 2, BATCH = 8;
   using V = Vec<T, VEC>;
   const int cvecs = p.C / VEC;
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(THREADS) conv_step_kernel(ConvP p) {
 // once the W gradients dp_{t-W+1..t} that reach it are.  dk and db take the run's own tokens only; a thread's sums go to
 // `part`, one row per (row, run), and conv_sum_kernel adds the rows in order.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(THREADS) conv_bwd_kernel(const ConvP p) {
+__global__ void __launch_bounds__(THREADS, 4) conv_bwd_kernel(const ConvP p) {
   constexpr int HP = (VEC + 1) / 2, BATCH = 4;
   using V = Vec<T, VEC>;
   const int cvecs = p.C / VEC;
@@ -320,10 +323,10 @@ int check(const gdn_conv_args* a, bool step) {
   return GDN_OK;
 }
 
-// Tokens per thread: as many as still leave about 2048 threads per SM (a run's first W - 1 inputs are read twice, and the
-// backward writes one row of sums per run), 16 to 64.
+// Tokens per thread, 16 to 64: as many as still leave about 768 threads of four channels per SM (a run's first W - 1
+// inputs are read twice, and the backward writes one row of sums per run).
 int run_tokens(int64_t work) {
-  const int64_t n = work / (148 * 2048);
+  const int64_t n = work / (148 * 768);
   return n >= 64 ? 64 : n >= 32 ? 32 : 16;
 }
 
@@ -340,7 +343,7 @@ ConvP params(const gdn_conv_args* a) {
 
 // Vectors of channels where every row starts on one.
 bool vectors(const ConvP& p, int es, bool bwd) {
-  const int v = bwd ? 4 : 16 / es;  // the backward's windows and sums leave room for four channels per thread
+  const int v = 4;
   auto ok = [&](const void* q, int64_t sb, int64_t st) { return (uintptr_t)q % (v * es) == 0 && sb % v == 0 && st % v == 0; };
   if (p.C % v || !ok(p.x, p.sx_b, p.sx_t)) return false;
   return bwd ? ok(p.dy, p.sdy_b, p.sdy_t) && (uintptr_t)p.dx % (v * es) == 0 : ok(p.y, p.sy_b, p.sy_t);
@@ -403,7 +406,7 @@ int gdn_conv_fwd(const gdn_conv_args* a, void* stream) {
   }
   if (a->dtype == GDN_DTYPE_F32)
     return vectors(p, 4, false) ? launch_fwd<float, 4>(p, a->width, s) : launch_fwd<float, 1>(p, a->width, s);
-  return vectors(p, 2, false) ? launch_fwd<__nv_bfloat16, 8>(p, a->width, s) : launch_fwd<__nv_bfloat16, 1>(p, a->width, s);
+  return vectors(p, 2, false) ? launch_fwd<__nv_bfloat16, 4>(p, a->width, s) : launch_fwd<__nv_bfloat16, 1>(p, a->width, s);
 }
 
 int gdn_conv_step(const gdn_conv_args* a, void* stream) {

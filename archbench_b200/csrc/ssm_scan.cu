@@ -776,10 +776,10 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(ScanP p) {
 // One token per row: the state is read and written once, 16 bytes per lane where N is a multiple of four.  HBM-bound.
 template <typename T, int NL, bool VEC>
 __global__ void __launch_bounds__(256) scan_step_kernel(const ScanP p) {
-  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / NL;
+  const int at = (blockIdx.x * 256 + threadIdx.x) / NL;  // a channel of row b
   const int n0 = (threadIdx.x % NL) * SPL, lane = threadIdx.x % 32;
-  const bool live = id < (int64_t)p.B * p.D && n0 < p.N;
-  const int b = live ? (int)(id / p.D) : 0, d = live ? (int)(id % p.D) : 0;
+  const bool live = at < p.D && n0 < p.N;
+  const int b = blockIdx.y, d = live ? at : 0;
   const int grp = p.G == 1 ? 0 : d / (p.D / p.G);
   float* hp = p.h_out + ((int64_t)b * p.D + d) * p.N + n0;
   const float* Ap = p.A + (int64_t)d * p.N + n0;
@@ -876,15 +876,15 @@ struct AlignP {
   int64_t tokens;
   int T, G;
 };
-template <typename T>
+template <typename T, typename I>  // I: 32-bit indices where they reach (divisions by 64-bit ones cost more than the copy)
 __global__ void __launch_bounds__(256) scan_align_kernel(const AlignP p) {
   constexpr int V = 16 / (int)sizeof(T);
   const int k = blockIdx.y, w = p.width[k], chunks = (w + V - 1) / V;
-  const int64_t n = p.tokens * p.G * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / chunks, tok = row / p.G;
+  const I n = (I)(p.tokens * p.G * chunks), T_ = (I)p.T, G = (I)p.G;
+  for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < n; i += (I)gridDim.x * 256) {
+    const I row = i / chunks, tok = row / G, b = tok / T_;
     const int c = (int)(i - row * chunks) * V;
-    const T* src = static_cast<const T*>(p.src[k]) + tok / p.T * p.sb[k] + tok % p.T * p.st[k] + row % p.G * p.sg[k] + c;
+    const T* src = static_cast<const T*>(p.src[k]) + b * p.sb[k] + (tok - b * T_) * p.st[k] + (row - tok * G) * p.sg[k] + c;
     uint4 raw = make_uint4(0, 0, 0, 0);
     T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
@@ -920,10 +920,11 @@ int scan_align(ScanP& p, const AlignPlan& a, int dtype, char* ws, cudaStream_t s
   q.tokens = (int64_t)p.B * p.T; q.T = p.T; q.G = p.G;
   const int64_t chunks = q.tokens * p.G * ((dpg > p.N ? dp : np) / v), g = (chunks + 255) / 256;
   const dim3 grid((unsigned)(g < 148 * 16 ? g : 148 * 16), n);
+  const bool wide = chunks > (1ll << 31);
   if (dtype == GDN_DTYPE_F32)
-    scan_align_kernel<float><<<grid, 256, 0, s>>>(q);
+    wide ? scan_align_kernel<float, uint64_t><<<grid, 256, 0, s>>>(q) : scan_align_kernel<float, uint32_t><<<grid, 256, 0, s>>>(q);
   else
-    scan_align_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(q);
+    wide ? scan_align_kernel<__nv_bfloat16, uint64_t><<<grid, 256, 0, s>>>(q) : scan_align_kernel<__nv_bfloat16, uint32_t><<<grid, 256, 0, s>>>(q);
   return launched();
 }
 
@@ -1036,12 +1037,11 @@ int launch_plain(const ScanP& p, cudaStream_t s) {
 
 template <typename T, bool VEC>
 int launch_step(const ScanP& p, int nl, cudaStream_t s) {
-  const int64_t g = ((int64_t)p.B * p.D * nl + 255) / 256;
-  if (g > 0x7fffffff) return GDN_ERR_SHAPE;
-  if (nl == 2) scan_step_kernel<T, 2, VEC><<<(unsigned)g, 256, 0, s>>>(p);
-  if (nl == 4) scan_step_kernel<T, 4, VEC><<<(unsigned)g, 256, 0, s>>>(p);
-  if (nl == 8) scan_step_kernel<T, 8, VEC><<<(unsigned)g, 256, 0, s>>>(p);
-  if (nl == 16) scan_step_kernel<T, 16, VEC><<<(unsigned)g, 256, 0, s>>>(p);
+  const dim3 g((unsigned)(((int64_t)p.D * nl + 255) / 256), p.B);
+  if (nl == 2) scan_step_kernel<T, 2, VEC><<<g, 256, 0, s>>>(p);
+  if (nl == 4) scan_step_kernel<T, 4, VEC><<<g, 256, 0, s>>>(p);
+  if (nl == 8) scan_step_kernel<T, 8, VEC><<<g, 256, 0, s>>>(p);
+  if (nl == 16) scan_step_kernel<T, 16, VEC><<<g, 256, 0, s>>>(p);
   return launched();
 }
 template <typename T>
