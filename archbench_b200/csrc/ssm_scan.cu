@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
         const ulonglong2 su = *reinterpret_cast<const ulonglong2*>(&sS[r][hc]);
         const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sB[r][n0]);
         const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sC[r][n0]);
-        h[0] = fma2(exp2_2(mul2(su.x, A2[0])), h[0], mul2(su.y, bv.x));
-        h[1] = fma2(exp2_2(mul2(su.x, A2[1])), h[1], mul2(su.y, bv.y));
+        h[0] = fma2(exp2_2(fma2(su.x, A2[0], both(EX2_MEAN))), h[0], mul2(su.y, bv.x));
+        h[1] = fma2(exp2_2(fma2(su.x, A2[1], both(EX2_MEAN))), h[1], mul2(su.y, bv.y));
         sY[r][tid] = sum2(fma2(cv.y, h[1], mul2(cv.x, h[0])));
       }
     }
@@ -439,10 +439,10 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
         for (int i = 0; i < PAIRS; i += 2) {
           const float4 bv = cur.b[q][i / 2];
           const ulonglong2 cv = cur.c[q][i / 2];
-          h[0][i] = fma2(pack2(ex2(su.x * A2[0][2 * i]), ex2(su.x * A2[0][2 * i + 1])), h[0][i], pack2(su.y * bv.x, su.y * bv.y));
-          h[1][i] = fma2(pack2(ex2(su.z * A2[1][2 * i]), ex2(su.z * A2[1][2 * i + 1])), h[1][i], pack2(su.w * bv.x, su.w * bv.y));
-          h[0][i + 1] = fma2(pack2(ex2(su.x * A2[0][2 * i + 2]), ex2(su.x * A2[0][2 * i + 3])), h[0][i + 1], pack2(su.y * bv.z, su.y * bv.w));
-          h[1][i + 1] = fma2(pack2(ex2(su.z * A2[1][2 * i + 2]), ex2(su.z * A2[1][2 * i + 3])), h[1][i + 1], pack2(su.w * bv.z, su.w * bv.w));
+          h[0][i] = fma2(pack2(decay(su.x, A2[0][2 * i]), decay(su.x, A2[0][2 * i + 1])), h[0][i], pack2(su.y * bv.x, su.y * bv.y));
+          h[1][i] = fma2(pack2(decay(su.z, A2[1][2 * i]), decay(su.z, A2[1][2 * i + 1])), h[1][i], pack2(su.w * bv.x, su.w * bv.y));
+          h[0][i + 1] = fma2(pack2(decay(su.x, A2[0][2 * i + 2]), decay(su.x, A2[0][2 * i + 3])), h[0][i + 1], pack2(su.y * bv.z, su.y * bv.w));
+          h[1][i + 1] = fma2(pack2(decay(su.z, A2[1][2 * i + 2]), decay(su.z, A2[1][2 * i + 3])), h[1][i + 1], pack2(su.w * bv.z, su.w * bv.w));
           y0 = fma2(cv.y, h[0][i + 1], i ? fma2(cv.x, h[0][i], y0) : mul2(cv.x, h[0][i]));
           y1 = fma2(cv.y, h[1][i + 1], i ? fma2(cv.x, h[1][i], y1) : mul2(cv.x, h[1][i]));
         }
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanP p) {
       const float bb[4] = {bv.x, bv.y, bv.z, bv.w};
 #pragma unroll
       for (int i = 0; i < SPL; ++i) {
-        const float a = ex2(ss.x * A2[i]);
+        const float a = decay(ss.x, A2[i]);
         h[i] = REV ? a * fmaf(bb[i], ss.y, h[i]) : fmaf(a, h[i], ss.y * bb[i]);
       }
     }
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float s = c ? su.z : su.x, u = c ? su.w : su.y;
-          const f32x2 a = pack2(ex2(s * A2[c][2 * i]), ex2(s * A2[c][2 * i + 1])), w = pack2(u * bv.x, u * bv.y);
+          const f32x2 a = pack2(decay(s, A2[c][2 * i]), decay(s, A2[c][2 * i + 1])), w = pack2(u * bv.x, u * bv.y);
           h[c][i] = REV ? mul2(a, add2(h[c][i], w)) : fma2(a, h[c][i], w);
         }
       }
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(ScanP p) {
       const int seg = REV ? p.nseg - 1 - (k0 + q) : k0 + q;
       if (k0 + q >= p.nseg) break;
       p.carry[(b * p.nseg + seg) * dn + at] = H;
-      H = fmaf(ex2(A2 * a[q]), H, e[q]);
+      H = fmaf(decay(a[q], A2), H, e[q]);
     }
   }
 }
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanP p) {
     if (p.softplus) s = softplus(s);
 #pragma unroll
     for (int i = 0; i < SPL; ++i) {
-      h[i] = fmaf(ex2(s * (A[i] * LOG2E)), h[i], s * x * to_f32(qb.v[i]));
+      h[i] = fmaf(decay(s, A[i] * LOG2E), h[i], s * x * to_f32(qb.v[i]));
       y[0] = fmaf(to_f32(qc.v[i]), h[i], y[0]);
     }
     if (VEC) {

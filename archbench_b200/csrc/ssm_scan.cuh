@@ -100,6 +100,12 @@ __device__ __forceinline__ float4 quad_f32(const Quad<T>& q, bool on) {
   return on ? make_float4(to_f32(q.v[0]), to_f32(q.v[1]), to_f32(q.v[2]), to_f32(q.v[3])) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
+// exp(s A) with A2 = A log2 e.  The instruction's mean error is -1 to -2.5 parts in 10^8 for exponents from -1e-3 to -1;
+// over the hundreds of tokens that slow states remember it adds up (dA came out 1.1e-6 low), so it is taken out of the
+// exponent, at no cost.  2^EX2_MEAN itself is exactly 1: a step of size 0 still leaves the state alone.
+constexpr float EX2_MEAN = 2.2e-8f;
+__device__ __forceinline__ float decay(float s, float A2) { return ex2(fmaf(s, A2, EX2_MEAN)); }
+
 // v[i], i < NV, held by LANES lanes (stride STRIDE in lane index): sums over the lanes, spread so that lane l keeps
 // the sums i = l * NV / LANES ..; with fewer values than lanes, every lane keeps one (equal on LANES / NV of them).
 // On return v[0 .. max(NV / LANES, 1)) hold them and `first` is the index of v[0].

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
 #pragma unroll
         for (int i = 0; i < SPL; ++i) {
           hp[r][i] = h[i];
-          h[i] = fmaf(ex2(ss.x * (A[i] * LOG2E)), h[i], ss.y * bb[i]);
+          h[i] = fmaf(decay(ss.x, A[i] * LOG2E), h[i], ss.y * bb[i]);
           acc[j] = fmaf(cq[i], h[i], acc[j]);
         }
       }
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
         gb[j] = ga[j] = 0.f;
 #pragma unroll
         for (int i = 0; i < SPL; ++i) {
-          const float a = ex2(ss.x * (A[i] * LOG2E));
+          const float a = decay(ss.x, A[i] * LOG2E);
           const float g = fmaf(cq[i], dc, G[i]);
           gb[j] = fmaf(g, bb[i], gb[j]);
           v[i] = g * ss.y;
@@ -457,8 +457,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
       for (int c = 0; c < 2; ++c) {
         const float s = c ? su.z : su.x, u = c ? su.w : su.y;
         const float2 a0 = unpack2(A2[c][0]), a1 = unpack2(A2[c][1]);
-        a[r][c][0] = pack2(ex2(s * a0.x), ex2(s * a0.y));
-        a[r][c][1] = pack2(ex2(s * a1.x), ex2(s * a1.y));
+        a[r][c][0] = pack2(decay(s, a0.x), decay(s, a0.y));
+        a[r][c][1] = pack2(decay(s, a1.x), decay(s, a1.y));
         h[r + 1][c][0] = fma2(a[r][c][0], h[r][c][0], pack2(u * bv.x, u * bv.y));
         h[r + 1][c][1] = fma2(a[r][c][1], h[r][c][1], pack2(u * bv.z, u * bv.w));
       }
