@@ -146,6 +146,24 @@ __device__ __forceinline__ f32x2 load_pair(const __nv_bfloat16* p) {
   return pack2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
 }
 __device__ __forceinline__ f32x2 load_pair(const float* p) { return *reinterpret_cast<const f32x2*>(p); }
+// 16 bytes into shared memory without a register; zeros where `on` is false (the address is then not read).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+// 4, 8 or 16 bytes, always copied.
+template <int BYTES>
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const void* src) {
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES < 4 ? 4 : BYTES) : "memory");
+}
+
 // Tokens of row b.
 __device__ __forceinline__ int row_tokens(const int32_t* lengths, int b, int T) {
   return lengths ? min(max(lengths[b], 0), T) : T;

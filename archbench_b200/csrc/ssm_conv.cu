@@ -90,14 +90,39 @@ __device__ __forceinline__ void load_weight_pairs(const ConvP& p, int c, f32x2 (
   }
 }
 
-// The loads of BATCH tokens go out together.  Four channels per thread keep 32 warps on an SM: 68 us at 8 x 4096 x 2048
-// (bf16, width 4) against 74 us with eight channels, and loads a batch ahead, in registers, cost more warps than they hide
-// (82 us).  The sigmoids' two operations per value on their pipe
-// (30 us) and the packed arithmetic (20 us) overlap HBM's 41 us in part.
+// A thread's own queue of its coming tokens, GROUPS groups of TOK tokens, filled by asynchronous copies: values on their
+// way take no registers (queued in registers they cost more warps than they hide).  Only the thread itself reads its
+// places, so no barrier is needed; a group is refilled one iteration after it was used.  Values of less than 4 bytes,
+// which no such copy takes, are loaded a group at a time instead.
+template <typename V, int STREAMS, int TOK, int GROUPS>
+struct Queue {
+  static constexpr bool ASYNC = sizeof(V) >= 4;
+  static constexpr int BYTES = ASYNC ? GROUPS * TOK * STREAMS * THREADS * (int)sizeof(V) : 16;
+  V* at;  // this thread's first place
+  __device__ explicit Queue(char* smem) : at(reinterpret_cast<V*>(smem) + threadIdx.x) {}
+  __device__ V* place(int g, int q, int stream) const { return at + ((g * TOK + q) * STREAMS + stream) * THREADS; }
+  // Into place g: token q of a stream is at address src(q, stream).
+  template <typename F>
+  __device__ void fill(int g, F src) const {
+#pragma unroll
+    for (int q = 0; q < TOK; ++q)
+#pragma unroll
+      for (int s = 0; s < STREAMS; ++s)
+        copy_bytes<(int)sizeof(V)>(static_cast<uint32_t>(__cvta_generic_to_shared(place(g, q, s))), src(q, s));
+    copies_commit();
+  }
+};
+
+// Four channels per thread keep 32 warps on an SM.  At 8 x 4096 x 2048 (bf16, width 4) 60.5 us; 67 us with batches of eight
+// loads in registers and no queue.  A batch is a multiple of W - 1 tokens, so that the window turns by renaming registers:
+// with four tokens of width 4 it is 64 us.  HBM's share is 41 us, the sigmoids' two operations per value on their pipe 30 us
+// and the packed arithmetic 20 us; they overlap in part.
 template <typename T, int VEC, int W>
 __global__ void __launch_bounds__(THREADS, 8) conv_fwd_kernel(const ConvP p) {
-  constexpr int HP = (VEC + 1) / 2, BATCH = 8;
+  constexpr int HP = (VEC + 1) / 2, BATCH = W == 4 ? 3 : 4, GROUPS = 3;
   using V = Vec<T, VEC>;
+  using Q = Queue<V, 1, BATCH, GROUPS>;
+  __shared__ __align__(16) char smem[Q::BYTES];
   const int cvecs = p.C / VEC;
   const int64_t id = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   if (id >= (int64_t)p.B * p.runs * cvecs) return;
@@ -119,10 +144,24 @@ __global__ void __launch_bounds__(THREADS, 8) conv_fwd_kernel(const ConvP p) {
       for (int i = 0; i < HP; ++i) x[w][i] = pack2(v[2 * i], v[2 * i + 1 < VEC ? 2 * i + 1 : 2 * i]);
     }
   }
-  for (int t = t0; t < te; t += BATCH) {
-    V raw[BATCH];
+  const Q queue(smem);
+  auto src = [&](int t) { return xp + (int64_t)min(t, te - 1) * p.sx_t; };  // past the run's end the last token again
+  auto fill = [&](int g, int t) { queue.fill(g, [&](int q, int) { return src(t + q); }); };
+  if (Q::ASYNC && t0 < te) {
 #pragma unroll
-    for (int q = 0; q < BATCH; ++q) raw[q] = *reinterpret_cast<const V*>(xp + (int64_t)min(t + q, te - 1) * p.sx_t);
+    for (int g = 0; g < GROUPS - 1; ++g) fill(g, t0 + g * BATCH);
+  }
+  for (int t = t0, g = 0; t < te; t += BATCH, g = g + 1 == GROUPS ? 0 : g + 1) {
+    V raw[BATCH];
+    if (Q::ASYNC) {
+      copies_wait<GROUPS - 2>();
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) raw[q] = *queue.place(g, q, 0);
+      fill(g == 0 ? GROUPS - 1 : g - 1, t + (GROUPS - 1) * BATCH);
+    } else {
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) raw[q] = *reinterpret_cast<const V*>(src(t + q));
+    }
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
       f32x2 o[HP];
@@ -185,11 +224,14 @@ __global__ void __launch_bounds__(THREADS) conv_step_kernel(ConvP p) {
 
 // Backward.  A thread walks its run and W - 1 tokens past it: dp_t is formed as soon as x_t is there, and dx_{t-W+1}
 // once the W gradients dp_{t-W+1..t} that reach it are.  dk and db take the run's own tokens only; a thread's sums go to
-// `part`, one row per (row, run), and conv_sum_kernel adds the rows in order.
+// `part`, one row per (row, run), and conv_sum_kernel adds the rows in order.  At 8 x 2048 x 2048 (bf16, width 4) 72 us, 82 us
+// without the queue; HBM's share is 31 us.
 template <typename T, int VEC, int W>
 __global__ void __launch_bounds__(THREADS, 4) conv_bwd_kernel(const ConvP p) {
-  constexpr int HP = (VEC + 1) / 2, BATCH = 4;
+  constexpr int HP = (VEC + 1) / 2, BATCH = sizeof(Vec<T, VEC>) == 16 ? 2 : 4, GROUPS = 2;
   using V = Vec<T, VEC>;
+  using Q = Queue<V, 2, BATCH, GROUPS>;
+  __shared__ __align__(16) char smem[Q::BYTES];
   const int cvecs = p.C / VEC;
   const int64_t id = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   if (id >= (int64_t)p.B * p.runs * cvecs) return;
@@ -220,13 +262,32 @@ __global__ void __launch_bounds__(THREADS, 4) conv_bwd_kernel(const ConvP p) {
   const T* xp = static_cast<const T*>(p.x) + b * p.sx_b + c;
   const T* dyp = static_cast<const T*>(p.dy) + b * p.sdy_b + c;
   T* dxp = static_cast<T*>(p.dx) + (int64_t)b * p.T * p.C + c;
-  for (int tb = t0; tb < t1 + W - 1; tb += BATCH) {
-    V rx[BATCH], rd[BATCH];
+  const Q queue(smem);
+  auto src = [&](int t, int stream) {  // places past the row's tokens read its last one; their values are dropped
+    const int64_t u = max(min(t, len - 1), 0);
+    return stream ? dyp + u * p.sdy_t : xp + u * p.sx_t;
+  };
+  auto fill = [&](int g, int t) { queue.fill(g, [&](int q, int s) { return src(t + q, s); }); };
+  if (Q::ASYNC) {
 #pragma unroll
-    for (int q = 0; q < BATCH; ++q) {  // places past the row's tokens read its last one; their values are dropped
-      const int64_t t = max(min(tb + q, len - 1), 0);
-      rx[q] = *reinterpret_cast<const V*>(xp + t * p.sx_t);
-      rd[q] = *reinterpret_cast<const V*>(dyp + t * p.sdy_t);
+    for (int g = 0; g < GROUPS - 1; ++g) fill(g, t0 + g * BATCH);
+  }
+  for (int tb = t0, g = 0; tb < t1 + W - 1; tb += BATCH, g = g + 1 == GROUPS ? 0 : g + 1) {
+    V rx[BATCH], rd[BATCH];
+    if (Q::ASYNC) {
+      copies_wait<GROUPS - 2>();
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
+        rx[q] = *queue.place(g, q, 0);
+        rd[q] = *queue.place(g, q, 1);
+      }
+      fill(g == 0 ? GROUPS - 1 : g - 1, tb + (GROUPS - 1) * BATCH);
+    } else {
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
+        rx[q] = *reinterpret_cast<const V*>(src(tb + q, 0));
+        rd[q] = *reinterpret_cast<const V*>(src(tb + q, 1));
+      }
     }
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {

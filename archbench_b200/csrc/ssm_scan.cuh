@@ -38,16 +38,6 @@ struct ScanP {
   int pairs_out;      // rows of y (or dx, ddt, dz) take stores of channel pairs
 };
 
-// 16 bytes into shared memory without a register; zeros where `on` is false (the address is then not read).
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
 // CV consecutive values of type T in one register image (CV = 2: one 4- or 8-byte load).
 template <typename T, int CV>
 struct Raw {
