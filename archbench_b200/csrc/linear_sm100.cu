@@ -211,26 +211,47 @@ __device__ __forceinline__ void box_store3(const CUtensorMap* map, const char* b
 __device__ __forceinline__ bf16* box_at(char* box, int row, int col) {
   return reinterpret_cast<bf16*>(box + row * 128 + (((col >> 3) ^ (row & 7)) << 4)) + (col & 7);
 }
+// ROWS at a time: the reads of a batch go out before its writes, which the compiler must keep in order.
 __device__ __noinline__ void box_copy_out(char* box, int lane, bf16* p, int64_t ld, int64_t row0, int64_t col0, int64_t M, int64_t N) {
+  constexpr int ROWS = 8;
   __syncwarp();
   const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
   const bool a = col0 + lane < N, b = col0 + 32 + lane < N;
   bf16* q = p + row0 * ld + col0 + lane;
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r, q += ld) {
-    if (a) q[0] = *box_at(box, r, lane);
-    if (b) q[32] = *box_at(box, r, lane + 32);
+#pragma unroll 1
+  for (int r = 0; r < rows; r += ROWS, q += ROWS * ld) {
+    bf16 v[ROWS][2];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      v[i][0] = *box_at(box, r + i, lane);
+      v[i][1] = *box_at(box, r + i, lane + 32);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (a && r + i < rows) q[i * ld] = v[i][0];
+      if (b && r + i < rows) q[i * ld + 32] = v[i][1];
+    }
   }
   __syncwarp();
 }
 __device__ __noinline__ void box_copy_in(char* box, int lane, const bf16* p, int64_t ld, int64_t row0, int64_t col0, int64_t M, int64_t N) {
+  constexpr int ROWS = 16;
   const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
   const bool a = col0 + lane < N, b = col0 + 32 + lane < N;
   const bf16* q = p + row0 * ld + col0 + lane;
-#pragma unroll 8
-  for (int r = 0; r < rows; ++r, q += ld) {
-    *box_at(box, r, lane) = a ? q[0] : __float2bfloat16_rn(0.f);
-    *box_at(box, r, lane + 32) = b ? q[32] : __float2bfloat16_rn(0.f);
+#pragma unroll 1
+  for (int r = 0; r < rows; r += ROWS, q += ROWS * ld) {
+    bf16 v[ROWS][2];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      v[i][0] = a && r + i < rows ? q[i * ld] : __float2bfloat16_rn(0.f);
+      v[i][1] = b && r + i < rows ? q[i * ld + 32] : __float2bfloat16_rn(0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      *box_at(box, r + i, lane) = v[i][0];
+      *box_at(box, r + i, lane + 32) = v[i][1];
+    }
   }
   __syncwarp();
 }
@@ -352,8 +373,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       // the box carries an output.
       uint4 res[8];
       auto fetch_res = [&](int64_t col) {
-        if (!p.res || !p.vec || p.splits > 1 || row0 >= p.M || col >= p.N) return;
-        if (lane == 0) {
+        if (!p.res || p.splits > 1 || row0 >= p.M || col >= p.N) return;
+        if (!p.vec) {
+          box_copy_in(box, lane, p.res, p.ldr, row0, col, p.M, p.N);
+        } else if (lane == 0) {
           ptx::bulk_wait_read0();
           ptx::mbar_arrive_expect_tx(rfull + warp - 2, OUT_BYTES);
           tma_load_2d(box, &mres, rfull + warp - 2, (int)col, (int)row0);
@@ -361,11 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto take_res = [&](int64_t col) {
         if (!p.res) return true;
-        if (p.vec) {
-          if (!wait(rfull + warp - 2, fetched++ & 1)) return false;
-        } else {
-          box_copy_in(box, lane, p.res, p.ldr, row0, col, p.M, p.N);
-        }
+        if (p.vec && !wait(rfull + warp - 2, fetched++ & 1)) return false;
 #pragma unroll
         for (int j = 0; j < 8; ++j) res[j] = *reinterpret_cast<const uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
         __syncwarp();
