@@ -224,8 +224,8 @@ __global__ void __launch_bounds__(THREADS) conv_step_kernel(ConvP p) {
 
 // Backward.  A thread walks its run and W - 1 tokens past it: dp_t is formed as soon as x_t is there, and dx_{t-W+1}
 // once the W gradients dp_{t-W+1..t} that reach it are.  dk and db take the run's own tokens only; a thread's sums go to
-// `part`, one row per (row, run), and conv_sum_kernel adds the rows in order.  At 8 x 2048 x 2048 (bf16, width 4) 72 us, 82 us
-// without the queue; HBM's share is 31 us.
+// `part`, one row per (row, run), and conv_sum_kernel adds the rows in order.  At 8 x 2048 x 2048 (bf16, width 4) 69 us, and
+// 4 us for the sums; without the queue the kernel took 10 us more.  HBM's share is 31 us.
 template <typename T, int VEC, int W>
 __global__ void __launch_bounds__(THREADS, 4) conv_bwd_kernel(const ConvP p) {
   constexpr int HP = (VEC + 1) / 2, BATCH = sizeof(Vec<T, VEC>) == 16 ? 2 : 4, GROUPS = 2;
@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(256) conv_sum_kernel(const float* part, int64_
 int check(const gdn_conv_args* a, bool step) {
   if (!a) return GDN_ERR_NULL;
   if (a->B < 0 || a->T < 0 || a->C < 1 || a->B > (1 << 30) || a->T > (1 << 30) || a->C > (1 << 24)) return GDN_ERR_SHAPE;
+  if ((double)a->B * (double)a->T * (double)a->C > (double)(1ll << 46)) return GDN_ERR_SHAPE;  // products stay in 64 bits
   if (a->width < 2 || a->width > MAXW) return GDN_ERR_UNSUPPORTED;
   if (a->act != GDN_ACT_NONE && a->act != GDN_ACT_SILU) return GDN_ERR_UNSUPPORTED;
   if (!elem_size(a->dtype) || !elem_size(a->w_dtype)) return GDN_ERR_DTYPE;
@@ -384,20 +385,30 @@ int check(const gdn_conv_args* a, bool step) {
   return GDN_OK;
 }
 
-// Tokens per thread, 16 to 64: as many as still leave about 768 threads of four channels per SM (a run's first W - 1
-// inputs are read twice, and the backward writes one row of sums per run).
-int run_tokens(int64_t work) {
-  const int64_t n = work / (148 * 768);
+// Tokens per thread in the forward, 16 to 64: as many as still leave about 768 threads of four channels per SM (a run's
+// first W - 1 inputs are read twice).  Whole waves, as below, are level here (60.5 and 59.8 us).
+int fwd_run(int64_t B, int64_t T, int64_t C) {
+  const int64_t n = B * T * C / 4 / (148 * 768);
   return n >= 64 ? 64 : n >= 32 ? 32 : 16;
 }
 
-ConvP params(const gdn_conv_args* a) {
+// In the backward, at least 16 and at most 128 in the fewest whole waves of the 512 threads an SM holds: a run also costs a
+// row of sums (8 x 2048 x 2048: one wave of 114 tokens 74 us, 1.7 waves of 64 tokens 83 us, sums included).
+int bwd_run(int64_t B, int64_t T, int64_t C) {
+  const int64_t at_once = 148 * 512, row = (B * C + 3) / 4;  // threads of one run per row
+  if (row < 1 || T < 1) return 16;
+  const int64_t waves = ((T + 127) / 128 * row + at_once - 1) / at_once, runs = waves * at_once / row;
+  const int64_t n = (T + runs - 1) / runs;
+  return n < 16 ? 16 : (int)n;
+}
+
+ConvP params(const gdn_conv_args* a, bool bwd) {
   ConvP p = {};
   p.x = a->x; p.w = a->weight; p.bias = a->bias; p.state_in = a->state_in; p.state_out = a->state_out; p.y = a->y;
   p.lengths = a->lengths;
   p.sx_b = a->sx_b; p.sx_t = a->sx_t; p.sy_b = a->sy_b; p.sy_t = a->sy_t;
   p.B = (int)a->B; p.T = (int)a->T; p.C = (int)a->C; p.act = a->act; p.w_dtype = a->w_dtype;
-  p.run = run_tokens(a->B * a->T * a->C / 4);
+  p.run = bwd ? bwd_run(a->B, a->T, a->C) : fwd_run(a->B, a->T, a->C);
   p.runs = (p.T + p.run - 1) / p.run;
   return p;
 }
@@ -453,7 +464,7 @@ int gdn_conv_fwd(const gdn_conv_args* a, void* stream) {
   if (a->T > 0 && (!a->x || !a->y)) return GDN_ERR_NULL;
   if (!device_ok()) return GDN_ERR_DEVICE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const ConvP p = params(a);
+  const ConvP p = params(a, false);
   if (p.T == 0) {
     if (!a->state_out) return GDN_OK;
     const int64_t n = (int64_t)p.B * p.C * (a->width - 1), g = (n + 255) / 256;
@@ -475,7 +486,7 @@ int gdn_conv_step(const gdn_conv_args* a, void* stream) {
   if (st != GDN_OK) return st;
   if (a->B == 0) return GDN_OK;
   if (!device_ok()) return GDN_ERR_DEVICE;
-  ConvP p = params(a);
+  ConvP p = params(a, false);
   p.state_out = const_cast<void*>(a->state_in);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return a->dtype == GDN_DTYPE_F32 ? launch_step<float>(p, a->width, s) : launch_step<__nv_bfloat16>(p, a->width, s);
@@ -485,7 +496,7 @@ int gdn_conv_bwd_workspace_bytes(const gdn_conv_bwd_args* a, size_t* bytes) {
   if (!a || !bytes) return GDN_ERR_NULL;
   int st = check(&a->fwd, false);
   if (st != GDN_OK) return st;
-  const ConvP p = params(&a->fwd);
+  const ConvP p = params(&a->fwd, true);
   *bytes = (size_t)p.B * p.runs * p.C * (a->fwd.width + 1) * sizeof(float);
   return GDN_OK;
 }
@@ -500,7 +511,7 @@ int gdn_conv_bwd(const gdn_conv_bwd_args* a, void* stream) {
   if (a->sdy_b < 0 || a->sdy_t < 0) return GDN_ERR_SHAPE;
   if (a->workspace_bytes < need) return GDN_ERR_WORKSPACE;
   if (!device_ok()) return GDN_ERR_DEVICE;
-  ConvP p = params(f);
+  ConvP p = params(f, true);
   p.dy = a->dy; p.dx = a->dx; p.dstate_out = a->dstate_out; p.dstate_in = a->dstate_in;
   p.sdy_b = a->sdy_b; p.sdy_t = a->sdy_t;
   p.part = static_cast<float*>(a->workspace);
