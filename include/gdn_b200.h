@@ -426,7 +426,7 @@ int gdn_abi_version(void);
  * x_{t < 0} comes from state_in (zeros when NULL): (B, C, width - 1), oldest first.  state_out gets the
  * last width - 1 inputs.  With `lengths`, row b has min(max(lengths[b], 0), T) tokens: y is 0 past them and
  * state_out ends at the last of them.  x and y have a unit channel stride; weight (C, width), bias (C) and the
- * states are contiguous.  Any alignment; 16-byte aligned rows with C a multiple of the 16-byte vector are faster.
+ * states are contiguous.  Any alignment; rows that start on four values, with C a multiple of four, are faster.
  */
 typedef enum { GDN_ACT_NONE = 0, GDN_ACT_SILU = 1, GDN_ACT_GELU = 2 } gdn_act;
 
