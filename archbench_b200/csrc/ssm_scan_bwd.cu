@@ -7,6 +7,8 @@
 // The states are rebuilt from the forward's checkpoints, 16 tokens at a time, in registers; the adjoint then walks the
 // tile backwards.  dB and dC are summed over a block's channels (lanes, then warps) and over the blocks by a second
 // kernel, in a fixed order.
+#include <algorithm>
+
 #include "ssm_scan.cuh"
 
 namespace gdn {
@@ -630,8 +632,43 @@ BwdPlan bwd_plan(const ScanP& p) {
   return w;
 }
 
+// Blocks of the tiled backward that run at once: two per SM by their registers, one where shared memory allows no more.
+int64_t tiled_at_once(int es, int nl) {
+  auto smem = [&](auto v) {
+    using T = decltype(v);
+    return nl == 2 ? BwdTiled<T, 2>::SMEM : nl == 4 ? BwdTiled<T, 4>::SMEM : nl == 8 ? BwdTiled<T, 8>::SMEM : BwdTiled<T, 16>::SMEM;
+  };
+  return (es == 4 ? smem(float()) : smem(__nv_bfloat16())) > 113 * 1024 ? 148 : 2 * 148;
+}
+
+// The backward's own segments of time: the blocks' whole waves decide.  In tokens of a block's work, a segment costs 16 more
+// to start and end, the local pass 0.28 of everything and its launches 30.  With 2048 tokens, 2048 channels and 16 states, split
+// and not: 4 rows 454 and 593 us, 6 rows 661 and 752 us, 7 rows 770 and 754 us; by the forward's segments 4 rows took 498 us.
+SegPlan bwd_segments(const ScanP& p, int es) {
+  const int nl = scan_lanes(p.N);
+  const int64_t row = ((p.D / p.G + 256 / nl - 1) / (256 / nl)) * p.G, nb = std::max<int64_t>(p.B, 1) * row, slots = tiled_at_once(es, nl);
+  SegPlan best = {1, p.T};
+  int64_t least = 100 * ((nb + slots - 1) / slots) * (p.T + 16);
+  for (int64_t k = 1; k <= 4; ++k) {
+    const int64_t n = std::min<int64_t>(k * slots / nb, p.T / 32);
+    if (n < 2 || n * n > 2 * (int64_t)p.T) continue;
+    const int64_t len = ((p.T + n - 1) / n + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT * GDN_SCAN_CKPT, segs = (p.T + len - 1) / len;
+    const int64_t cost = 100 * ((nb * segs + slots - 1) / slots) * (len + 16) + 28 * p.T * nb / slots + 3000;
+    if (segs > 1 && cost < least) {
+      least = cost;
+      best = {(int)segs, (int)len};
+    }
+  }
+  return best;
+}
+
 ScanP bwd_params(const gdn_scan_bwd_args* a) {
   ScanP p = scan_params(&a->fwd);
+  if (p.N % 4 == 0) {
+    const SegPlan sp = bwd_segments(p, elem_size(a->fwd.dtype));
+    p.nseg = sp.nseg;
+    p.seg_len = sp.seg_len;
+  }
   p.h_out = nullptr;
   p.dy = a->dy; p.sdy_b = a->sdy_b; p.sdy_t = a->sdy_t;
   p.dh_out = a->dh_out; p.dx = a->dx; p.ddt = a->ddt; p.dz = a->dz; p.dh0 = a->dh0;
@@ -659,11 +696,11 @@ int launch_bwd(ScanP p, const gdn_scan_bwd_args* a, cudaStream_t s) {
   if (tiled) {
     st = nl == 2 ? launch_bwd_tiled<T, 2>(p, s) : nl == 4 ? launch_bwd_tiled<T, 4>(p, s) : nl == 8 ? launch_bwd_tiled<T, 8>(p, s) : launch_bwd_tiled<T, 16>(p, s);
   } else {
-  if (nl == 2) scan_bwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 4) scan_bwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 8) scan_bwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
-  if (nl == 16) scan_bwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
-  st = launched();
+    if (nl == 2) scan_bwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
+    if (nl == 4) scan_bwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
+    if (nl == 8) scan_bwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
+    if (nl == 16) scan_bwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
+    st = launched();
   }
   if (st != GDN_OK) return st;
   const int64_t rows = (int64_t)p.B * p.T * p.G, n = rows * 2 * p.N;
