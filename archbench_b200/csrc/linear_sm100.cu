@@ -854,31 +854,70 @@ int launch_gemm(const GemmP& p, int pairs, cudaStream_t s) {
 // Bytes of an operand's aligned copy, 0 where it needs none, and the copy itself (which then stands for it).
 size_t align_bytes(const Operand& o) { return o.tma ? 0 : up256((size_t)o.rows * ((o.cols + 7) / 8 * 8) * 2); }
 
-__global__ void __launch_bounds__(256) align_kernel(const bf16* src, int64_t ld, bf16* dst, int64_t rows, int64_t cols) {
-  // rows by blockIdx.y, 16 bytes per thread
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (c >= cols) return;
-    const bf16* s = src + r * ld + c;
-    uint4 raw = make_uint4(0, 0, 0, 0);
+struct Copies {
+  struct {
+    const bf16* src;
+    int64_t ld;
+    bf16* dst;
+    int64_t rows, cols;
+  } o[2];
+};
+
+// The operands' 16-byte pieces one after the other, one per thread; inside a row words of 4 bytes are read, shifted by one
+// value where the row starts between two of them.  INDEX: an unsigned type that holds the number of pieces.
+template <typename INDEX>
+__global__ void __launch_bounds__(256) align_kernel(const Copies q) {
+  INDEX i = (INDEX)blockIdx.x * 256 + threadIdx.x;
+  const INDEX first = (INDEX)(q.o[0].rows * ((q.o[0].cols + 7) / 8));
+  const bool other = i >= first;
+  if (other) i -= first;
+  const bf16* src = other ? q.o[1].src : q.o[0].src;
+  bf16* dst = other ? q.o[1].dst : q.o[0].dst;
+  const int64_t ld = other ? q.o[1].ld : q.o[0].ld, rows = other ? q.o[1].rows : q.o[0].rows, cols = other ? q.o[1].cols : q.o[0].cols;
+  const INDEX pieces = (INDEX)((cols + 7) / 8);
+  if (rows == 0 || i >= (INDEX)rows * pieces) return;
+  const INDEX r = i / pieces;
+  const int64_t c = (int64_t)(i - r * pieces) * 8;
+  const bf16* s = src + (int64_t)r * ld + c;
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  const bool odd = (uintptr_t)s & 2;
+  if (!odd && c + 8 <= cols) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(s);
+    raw = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if (odd && c > 0 && c + 9 <= cols) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(s - 1);
+    const uint32_t v[5] = {w[0], w[1], w[2], w[3], w[4]};
+    raw = make_uint4(__funnelshift_r(v[0], v[1], 16), __funnelshift_r(v[1], v[2], 16), __funnelshift_r(v[2], v[3], 16), __funnelshift_r(v[3], v[4], 16));
+  } else {
     bf16* e = reinterpret_cast<bf16*>(&raw);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (c + j < cols) e[j] = s[j];
-    *reinterpret_cast<uint4*>(dst + r * ((cols + 7) / 8 * 8) + c) = raw;
   }
+  reinterpret_cast<uint4*>(dst)[i] = raw;
 }
 
-int align_operand(Operand& o, char*& ws, cudaStream_t s) {
-  if (o.tma) return GDN_OK;
-  const size_t bytes = align_bytes(o);
-  const int64_t ld = (o.cols + 7) / 8 * 8;
-  const dim3 g((unsigned)((ld / 8 + 255) / 256), (unsigned)(o.rows < 65535 ? o.rows : 65535));
-  align_kernel<<<g, 256, 0, s>>>(o.p, o.ld, reinterpret_cast<bf16*>(ws), o.rows, o.cols);
-  o.p = reinterpret_cast<const bf16*>(ws);
-  o.ld = ld;
-  o.tma = 1;
-  ws += bytes;
+// Those of the operands (second may be NULL) that TMA cannot address, laid out again in one launch.
+int align_operands(Operand* first, Operand* second, char*& ws, cudaStream_t s) {
+  Copies q = {};
+  int n = 0;
+  int64_t pieces = 0;
+  for (Operand* o : {first, second}) {
+    if (!o || o->tma) continue;
+    q.o[n++] = {o->p, o->ld, reinterpret_cast<bf16*>(ws), o->rows, o->cols};
+    pieces += o->rows * ((o->cols + 7) / 8);
+    ws += align_bytes(*o);
+    o->p = q.o[n - 1].dst;
+    o->ld = (o->cols + 7) / 8 * 8;
+    o->tma = 1;
+  }
+  if (!n) return GDN_OK;
+  const int64_t g = (pieces + 255) / 256;
+  if (g > 0x7fffffff) return GDN_ERR_SHAPE;
+  if (pieces + 256 <= 0xffffffffll)
+    align_kernel<uint32_t><<<(unsigned)g, 256, 0, s>>>(q);
+  else
+    align_kernel<uint64_t><<<(unsigned)g, 256, 0, s>>>(q);
   return ssm::launched();
 }
 
@@ -1000,8 +1039,7 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.M <= FEW_ROWS) return launch_few(p, s);
   char* ws = static_cast<char*>(a->workspace);
-  st = align_operand(p.a, ws, s);
-  if (st == GDN_OK) st = align_operand(p.b, ws, s);
+  st = align_operands(&p.a, &p.b, ws, s);
   return st == GDN_OK ? gemm<false, false>(p, ws, s) : st;
 }
 
@@ -1050,7 +1088,7 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
     p.b = operand(a->weight, a->sw, a->N, a->K);
     p.M = a->M; p.N = a->K; p.K = a->N;
     p.y = static_cast<bf16*>(a->dx); p.ldy = a->K;
-    st = align_operand(p.b, copies, s);
+    st = align_operands(&p.b, nullptr, copies, s);
     if (st == GDN_OK) st = gemm<false, true>(p, part, s);
     if (st != GDN_OK) return st;
   }
@@ -1059,7 +1097,7 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
     p.b = operand(a->x, a->sx, a->M, a->K);
     p.M = a->N; p.N = a->K; p.K = a->M;
     p.y = static_cast<bf16*>(a->dweight); p.ldy = a->K;
-    st = align_operand(p.b, copies, s);
+    st = align_operands(&p.b, nullptr, copies, s);
     if (st == GDN_OK) st = gemm<true, true>(p, part, s);
   }
   return st;
