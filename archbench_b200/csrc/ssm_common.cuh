@@ -30,21 +30,6 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 inline int launched() { return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH; }
 
-// Store N consecutive values, as one 16-byte vector where they fill one.
-template <int N, typename T>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[N]) {
-  if constexpr (sizeof(T) * N == 16) {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < N; ++i) store_as(e + i, v[i]);
-    *reinterpret_cast<uint4*>(p) = raw;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) store_as(p + i, v[i]);
-  }
-}
-
 // A parameter stored as fp32 or bf16.
 __device__ __forceinline__ float load_param(const void* p, int64_t i, int dtype) {
   return dtype == GDN_DTYPE_F32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
@@ -146,6 +131,7 @@ __device__ __forceinline__ f32x2 load_pair(const __nv_bfloat16* p) {
   return pack2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
 }
 __device__ __forceinline__ f32x2 load_pair(const float* p) { return *reinterpret_cast<const f32x2*>(p); }
+
 // 16 bytes into shared memory without a register; zeros where `on` is false (the address is then not read).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");

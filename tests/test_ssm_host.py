@@ -85,6 +85,13 @@ def test_offsets_past_32_bits_are_sized():
     assert lib().gdn_scan_bwd_workspace_bytes(ctypes.byref(b), ctypes.byref(n)) == 0 and n.value > 2 ** 33
 
 
+def test_convolution_sizes_past_64_bits_are_refused():
+    assert lib().gdn_conv_fwd(ctypes.byref(conv(B=1 << 20, T=1 << 20, C=1 << 20)), None) == -2
+    n = ctypes.c_size_t(0)
+    b = S.ConvBwdArgs(fwd=conv(B=1 << 20, T=1 << 20, C=1 << 20))
+    assert lib().gdn_conv_bwd_workspace_bytes(ctypes.byref(b), ctypes.byref(n)) == -2
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 3, 8)
     with pytest.raises(ValueError, match="CUDA"):
