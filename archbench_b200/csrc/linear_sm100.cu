@@ -42,11 +42,11 @@ struct GemmP {
   // epilogue (splits == 1)
   bf16* y;
   int64_t ldy;
-  bf16* pre;  // (M, N) contiguous, or NULL
+  bf16* pre;  // (M, N) contiguous, or NULL: x W^T + b, or with `slope` act'(x W^T + b) in fp16
   const bf16* bias;
   const bf16* res;
   int64_t ldr;
-  int act, vec;
+  int act, vec, slope;
   float* part;  // splits > 1: (splits, M, N) sums
   int part_tma; // N a multiple of four: TMA stores them
   // Tiles run along the shorter side first: a wave then reads few rows of the longer operand, once, and the shorter
@@ -92,19 +92,49 @@ __device__ __forceinline__ f32x2 act_fwd2(f32x2 p, int act) {
   }
   return p;
 }
-__device__ __forceinline__ f32x2 act_grad2(f32x2 p, int act) {
+// act(p), and act'(p) in `slope`.
+__device__ __forceinline__ f32x2 act_both2(f32x2 p, int act, f32x2& slope) {
+  slope = both(1.f);
   if (act == GDN_ACT_SILU) {
     const f32x2 g = sigmoid2(p);
-    return mul2(g, fma2(p, fma2(g, both(-1.f), both(1.f)), both(1.f)));
+    slope = mul2(g, fma2(p, fma2(g, both(-1.f), both(1.f)), both(1.f)));
+    return mul2(p, g);
   }
   if (act == GDN_ACT_GELU) {
     f32x2 bell;
     const f32x2 phi = normal2(p, bell);
-    return fma2(mul2(p, bell), both(0.39894228040143267794f), phi);
+    slope = fma2(mul2(p, bell), both(0.39894228040143267794f), phi);
+    return mul2(p, phi);
   }
-  return both(1.f);
+  return p;
 }
-__device__ __forceinline__ float act_fwd(float p, int act) { return unpack2(act_fwd2(both(p), act)).x; }
+__device__ __forceinline__ f32x2 act_grad2(f32x2 p, int act) {
+  f32x2 slope;
+  act_both2(p, act, slope);
+  return slope;
+}
+// What the backward needs of the activation is kept as act'(p) in fp16: a slope within [-0.2, 1.2] loses 2^-12 of itself, an
+// eighth of what dp then loses on its way into the bf16 matrix product.  p itself in bf16 lost 2^-9 of p, which near the
+// slope's zero (p = -1.28 for SiLU, -0.75 for GELU) is many times the slope.  The bytes are the same.
+__device__ __forceinline__ uint32_t slope_bits(f32x2 v) {
+  const float2 e = unpack2(v);
+  const __half2 h = __floats2half2_rn(e.x, e.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ f32x2 slope_pair(uint32_t bits) {
+  const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&bits));
+  return pack2(e.x, e.y);
+}
+// One value: the activation of v, with what the backward reads of it put at `pre` first.
+__device__ __forceinline__ float act_one(float v, int act, bf16* pre, int slope) {
+  f32x2 d;
+  const float y = unpack2(act_both2(both(v), act, d)).x;
+  if (pre && slope)
+    *reinterpret_cast<__half*>(pre) = __float2half_rn(unpack2(d).x);
+  else if (pre)
+    *pre = __float2bfloat16_rn(v);
+  return y;
+}
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
   asm volatile(
@@ -390,14 +420,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         return true;
       };
-      auto put = [&](const CUtensorMap* map, bf16* to, int64_t ld, int64_t col, const f32x2 (&v)[2][16]) {
-        if (p.vec) box_ready(lane);
-        box_put(box, lane, 0, v[0]);
-        box_put(box, lane, 32, v[1]);
+      auto send = [&](const CUtensorMap* map, bf16* to, int64_t ld, int64_t col) {  // the box's 64 columns
         if (p.vec)
           box_store(map, box, lane, row0, col);
         else
           box_copy_out(box, lane, to, ld, row0, col, p.M, p.N);
+      };
+      auto put = [&](const CUtensorMap* map, bf16* to, int64_t ld, int64_t col, const f32x2 (&v)[2][16]) {
+        if (p.vec) box_ready(lane);
+        box_put(box, lane, 0, v[0]);
+        box_put(box, lane, 32, v[1]);
+        send(map, to, ld, col);
       };
       fetch_res(n0 + c0);
       if (!wait(tfull + buf, (acc >> 1) & 1)) break;
@@ -459,15 +492,36 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         if (!__all_sync(0xffffffffu, take_res(n0 + c))) break;
-        if (p.pre) put(&mpre, p.pre, p.N, n0 + c, v);
         auto apply = [&](int act) {  // a loop per activation: choosing it per value cost 30 us of 183 at 32768 x 2816 x 1024
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[e][i] = act_fwd2(v[e][i], act);
         };
-        if (p.act == GDN_ACT_SILU) apply(GDN_ACT_SILU);
-        if (p.act == GDN_ACT_GELU) apply(GDN_ACT_GELU);
+        auto apply_with_slope = [&](int act) {  // the slopes go to the box as they are formed
+          if (p.vec) box_ready(lane);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f32x2& q = v[j / 4][j % 4 * 4 + i];
+              f32x2 d;
+              q = act_both2(q, act, d);
+              w[i] = slope_bits(d);
+            }
+            *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          send(&mpre, p.pre, p.N, n0 + c);
+        };
+        if (p.pre && !p.slope) put(&mpre, p.pre, p.N, n0 + c, v);
+        if (p.pre && p.slope) {
+          if (p.act == GDN_ACT_SILU) apply_with_slope(GDN_ACT_SILU);
+          if (p.act == GDN_ACT_GELU) apply_with_slope(GDN_ACT_GELU);
+        } else {
+          if (p.act == GDN_ACT_SILU) apply(GDN_ACT_SILU);
+          if (p.act == GDN_ACT_GELU) apply(GDN_ACT_GELU);
+        }
         if (p.res) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -528,9 +582,11 @@ __global__ void __launch_bounds__(256) split_epilogue_kernel(const GemmP p) {
       o[1] = add2(o[1], load_pair(reinterpret_cast<const bf16*>(&r) + 2));
     };
     if (p.bias) add(p.bias + col);
-    if (p.pre) put(p.pre + row * p.N + col);
-    o[0] = act_fwd2(o[0], p.act);
-    o[1] = act_fwd2(o[1], p.act);
+    if (p.pre && !p.slope) put(p.pre + row * p.N + col);
+    f32x2 d[2];
+    o[0] = act_both2(o[0], p.act, d[0]);
+    o[1] = act_both2(o[1], p.act, d[1]);
+    if (p.pre && p.slope) *reinterpret_cast<uint2*>(p.pre + row * p.N + col) = make_uint2(slope_bits(d[0]), slope_bits(d[1]));
     if (p.res) add(p.res + row * p.ldr + col);
     put(p.y + row * p.ldy + col);
   } else {
@@ -540,8 +596,7 @@ __global__ void __launch_bounds__(256) split_epilogue_kernel(const GemmP p) {
       float v = 0.f;
       for (int s = 0; s < p.splits; ++s) v += p.part[((int64_t)s * p.M + row) * p.N + col + k];
       if (p.bias) v += to_f32(p.bias[col + k]);
-      if (p.pre) p.pre[row * p.N + col + k] = __float2bfloat16_rn(v);
-      v = act_fwd(v, p.act);
+      v = act_one(v, p.act, p.pre ? p.pre + row * p.N + col + k : nullptr, p.slope);
       if (p.res) v += to_f32(p.res[row * p.ldr + col + k]);
       p.y[row * p.ldy + col + k] = __float2bfloat16_rn(v);
     }
@@ -604,21 +659,20 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmP p) {
 #pragma unroll
     for (int w = 0; w < 8; ++w) v += sums[w][row][i % 8];
     if (p.bias) v += to_f32(p.bias[col]);
-    if (p.pre) p.pre[row * p.N + col] = __float2bfloat16_rn(v);
-    v = act_fwd(v, p.act);
+    v = act_one(v, p.act, p.pre ? p.pre + row * p.N + col : nullptr, p.slope);
     if (p.res) v += to_f32(p.res[row * p.ldr + col]);
     p.y[row * p.ldy + col] = __float2bfloat16_rn(v);
   }
 }
 
-// dp = dy act'(pre), with rows padded to a multiple of 8 values (zeros) so that TMA can address them, and the column
+// dp = dy act'(pre) (`slope`: pre holds act' itself, in fp16), with rows padded to a multiple of 8 values (zeros) so that TMA can address them, and the column
 // sums of each block's DP_ROWS rows.
 // A thread's loads of DP_BATCH rows go out together (16384 x 1024 with GELU: 21 us, 30 us where each row's store stood
 // before the next row's loads).
 constexpr int DP_ROWS = 64, DP_BATCH = 2;
 template <bool VEC>
 __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, const bf16* pre, bf16* dp, int64_t ldp, int64_t M, int64_t N,
-                                                 int act, float* colsum) {
+                                                 int act, int slope, float* colsum) {
   // 32 lanes x 8 columns, 8 row groups
   const int lane = threadIdx.x % 32, rg = threadIdx.x / 32;
   const int64_t col = (int64_t)blockIdx.x * 256 + lane * 8, r0 = (int64_t)blockIdx.y * DP_ROWS;
@@ -638,7 +692,7 @@ __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, co
     return raw;
   };
   const int64_t r1 = min(r0 + DP_ROWS, M);
-  auto walk = [&](int act) {
+  auto walk = [&](int act, bool slope) {
     for (int64_t r = r0 + rg; r < r1; r += 8 * DP_BATCH) {
       uint4 rd[DP_BATCH], rp[DP_BATCH];
 #pragma unroll
@@ -654,7 +708,8 @@ __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, co
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           f32x2 d = load_pair(reinterpret_cast<const bf16*>(&rd[q]) + 2 * i);
-          if (act != GDN_ACT_NONE) d = mul2(d, act_grad2(load_pair(reinterpret_cast<const bf16*>(&rp[q]) + 2 * i), act));
+          const uint32_t kept = reinterpret_cast<const uint32_t*>(&rp[q])[i];
+          if (act != GDN_ACT_NONE) d = mul2(d, slope ? slope_pair(kept) : act_grad2(load_pair(reinterpret_cast<const bf16*>(&kept)), act));
           sum[i] = add2(sum[i], d);
           const float2 e = unpack2(d);
           const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
@@ -664,9 +719,10 @@ __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, co
       }
     }
   };
-  if (act == GDN_ACT_NONE) walk(GDN_ACT_NONE);
-  if (act == GDN_ACT_SILU) walk(GDN_ACT_SILU);
-  if (act == GDN_ACT_GELU) walk(GDN_ACT_GELU);
+  if (act == GDN_ACT_NONE) walk(GDN_ACT_NONE, false);
+  else if (slope) walk(GDN_ACT_SILU, true);  // the same for every activation
+  else if (act == GDN_ACT_SILU) walk(GDN_ACT_SILU, false);
+  else walk(GDN_ACT_GELU, false);
   if (!colsum) return;
   __shared__ float part[8][256 + 8];
 #pragma unroll
@@ -961,9 +1017,10 @@ int launch_few(const GemmP& p, cudaStream_t s) {
   return ssm::launched();
 }
 
-int check_sizes(int64_t M, int64_t N, int64_t K, int act) {
+int check_sizes(int64_t M, int64_t N, int64_t K, int act, int keep) {
   if (M < 0 || N < 1 || K < 1 || M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return GDN_ERR_SHAPE;
   if (act != GDN_ACT_NONE && act != GDN_ACT_SILU && act != GDN_ACT_GELU) return GDN_ERR_UNSUPPORTED;
+  if (keep != GDN_LINEAR_KEEP_PRE && keep != GDN_LINEAR_KEEP_SLOPE) return GDN_ERR_UNSUPPORTED;
   return GDN_OK;
 }
 
@@ -1012,7 +1069,7 @@ extern "C" {
 
 int gdn_linear_workspace_bytes(const gdn_linear_args* a, size_t* bytes) {
   if (!a || !bytes) return GDN_ERR_NULL;
-  const int st = check_sizes(a->M, a->N, a->K, a->act);
+  const int st = check_sizes(a->M, a->N, a->K, a->act, a->keep);
   if (st != GDN_OK) return st;
   *bytes = a->M <= FEW_ROWS ? 0
                             : plan(a->M, a->N, a->K).part + align_bytes(operand(a->x, a->sx, a->M, a->K)) +
@@ -1036,6 +1093,7 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
   p.y = static_cast<bf16*>(a->y); p.ldy = a->sy; p.pre = static_cast<bf16*>(a->pre);
   p.bias = static_cast<const bf16*>(a->bias); p.res = static_cast<const bf16*>(a->residual); p.ldr = a->sr;
   p.act = a->act;
+  p.slope = a->keep == GDN_LINEAR_KEEP_SLOPE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.M <= FEW_ROWS) return launch_few(p, s);
   char* ws = static_cast<char*>(a->workspace);
@@ -1045,7 +1103,7 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
 
 int gdn_linear_bwd_workspace_bytes(const gdn_linear_bwd_args* a, size_t* bytes) {
   if (!a || !bytes) return GDN_ERR_NULL;
-  const int st = check_sizes(a->M, a->N, a->K, a->act);
+  const int st = check_sizes(a->M, a->N, a->K, a->act, a->keep);
   if (st != GDN_OK) return st;
   *bytes = bwd_plan(a).total;
   return GDN_OK;
@@ -1073,9 +1131,9 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
     const dim3 g((unsigned)gx, (unsigned)gy);
     const bf16 *dy = static_cast<const bf16*>(a->dy), *pre = static_cast<const bf16*>(a->pre);
     if (a->N % 8 == 0 && rows16(dy, a->sdy) && (a->act == GDN_ACT_NONE || ssm::aligned16(pre)))
-      dp_kernel<true><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, colsum);
+      dp_kernel<true><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, a->keep, colsum);
     else
-      dp_kernel<false><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, colsum);
+      dp_kernel<false><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, a->keep, colsum);
     if (colsum) colsum_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, s>>>(colsum, gy, a->N, static_cast<bf16*>(a->dbias));
     st = ssm::launched();
     if (st != GDN_OK) return st;

@@ -387,11 +387,11 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const Tensor y = at::empty({M, N}, x.options());
   Tensor pre;
-  if (want_pre && act) pre = at::empty({M, N}, x.options());
+  if (want_pre && act) pre = at::empty({M, N}, x.options().dtype(at::kHalf));  // act'(x W^T + b)
   gdn_linear_args a = {};
   a.x = ptr(x); a.weight = ptr(w); a.bias = ptr(bias); a.residual = ptr(res); a.y = ptr(y); a.pre = ptr(pre);
   a.sx = x.stride(0); a.sw = w.stride(0); a.sr = res.defined() ? res.stride(0) : 0; a.sy = N;
-  a.M = M; a.N = N; a.K = K; a.act = act;
+  a.M = M; a.N = N; a.K = K; a.act = act; a.keep = GDN_LINEAR_KEEP_SLOPE;
   size_t need = 0;
   check(gdn_linear_workspace_bytes(&a, &need));
   const Tensor ws = workspace(need, x);
@@ -433,7 +433,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     a.x = ptr(x); a.weight = ptr(w); a.pre = ptr(pre); a.dy = ptr(dy);
     a.dx = ptr(out[0]); a.dweight = ptr(out[1]); a.dbias = ptr(out[2]);
     a.sx = x.stride(0); a.sw = w.stride(0); a.sdy = dy.stride(0);
-    a.M = M; a.N = N; a.K = K; a.act = (int)ctx->saved_data["act"].toInt();
+    a.M = M; a.N = N; a.K = K; a.act = (int)ctx->saved_data["act"].toInt(); a.keep = GDN_LINEAR_KEEP_SLOPE;
     size_t need = 0;
     check(gdn_linear_bwd_workspace_bytes(&a, &need));
     const Tensor ws = workspace(need, x);

@@ -15,7 +15,7 @@ class LinearArgs(ctypes.Structure):
 
     _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "residual", "y", "pre")] + \
                [(n, ctypes.c_int64) for n in ("sx", "sw", "sr", "sy", "M", "N", "K")] + \
-               [("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+               [("act", ctypes.c_int32), ("keep", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
 class LinearBwdArgs(ctypes.Structure):
@@ -23,7 +23,7 @@ class LinearBwdArgs(ctypes.Structure):
 
     _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "pre", "dy", "dx", "dweight", "dbias")] + \
                [(n, ctypes.c_int64) for n in ("sx", "sw", "sdy", "M", "N", "K")] + \
-               [("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+               [("act", ctypes.c_int32), ("keep", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
 SYMBOLS.update({
@@ -40,5 +40,5 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 
     x (..., K), weight (N, K), bias (N), residual (..., N), all bf16 with any strides; activation None, "silu" or "gelu"
     (the erf form).  fp32 accumulation and epilogue, one rounding at the end.  Differentiable in x, weight, bias and
-    residual; with an activation, training keeps x weight^T + bias in bf16."""
+    residual; with an activation, training keeps its slope at x weight^T + bias in fp16."""
     return (ssm_ops._EXT or ssm_ops.extension()).linear(x, weight, bias, activation, residual)

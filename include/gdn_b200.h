@@ -520,15 +520,19 @@ int gdn_scan_bwd(const gdn_scan_bwd_args* args, void* stream);
 
 /*
  * y = act(x weight^T + bias) + residual; x (M, K), weight (N, K), y and residual (M, N), bias (N), all bf16 with
- * unit last strides and fp32 accumulation, one rounding at the end.  `pre`, when not NULL, receives
- * x weight^T + bias (the backward's input; contiguous).  Any strides and alignment; 16-byte aligned rows are faster.
+ * unit last strides and fp32 accumulation, one rounding at the end.  `pre`, when not NULL, receives what the backward
+ * reads (contiguous, 2 bytes a value): with keep GDN_LINEAR_KEEP_PRE x weight^T + bias in bf16, with
+ * GDN_LINEAR_KEEP_SLOPE act'(x weight^T + bias) in fp16, which keeps an activation's gradient to 2^-12 of itself.  Any
+ * strides and alignment; 16-byte aligned rows are faster.
  */
+typedef enum { GDN_LINEAR_KEEP_PRE = 0, GDN_LINEAR_KEEP_SLOPE = 1 } gdn_linear_keep;
+
 typedef struct gdn_linear_args {
   const void *x, *weight, *bias, *residual; /* bias, residual may be NULL */
   void *y, *pre;                            /* pre may be NULL */
   int64_t sx, sw, sr, sy;                   /* row strides in elements */
   int64_t M, N, K;
-  int32_t act, reserved;
+  int32_t act, keep;
   void* workspace; /* gdn_linear_workspace_bytes */
   uint64_t workspace_bytes;
 } gdn_linear_args;
@@ -536,14 +540,14 @@ typedef struct gdn_linear_args {
 int gdn_linear_workspace_bytes(const gdn_linear_args* args, size_t* bytes);
 int gdn_linear_fwd(const gdn_linear_args* args, void* stream);
 
-/* Backward: dp = dy act'(pre); dx = dp weight, dweight = dp^T x, dbias = sum_m dp.  dx, dweight, dbias are
+/* Backward: dp = dy act'(x weight^T + bias), from `pre`; dx = dp weight, dweight = dp^T x, dbias = sum_m dp.  dx, dweight, dbias are
  * contiguous bf16 and may be NULL. */
 typedef struct gdn_linear_bwd_args {
   const void *x, *weight, *pre, *dy; /* pre may be NULL without an activation */
   void *dx, *dweight, *dbias;
   int64_t sx, sw, sdy;
   int64_t M, N, K;
-  int32_t act, reserved;
+  int32_t act, keep; /* as in the forward that wrote `pre` */
   void* workspace; /* gdn_linear_bwd_workspace_bytes */
   uint64_t workspace_bytes;
 } gdn_linear_bwd_args;
