@@ -1085,6 +1085,7 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
   if (!a->x || !a->weight || !a->y) return GDN_ERR_NULL;
   if (a->sx < 0 || a->sw < 0 || a->sr < 0 || a->sy < 0) return GDN_ERR_SHAPE;
   if (need && (!a->workspace || a->workspace_bytes < need)) return GDN_ERR_WORKSPACE;
+  if (need && !ssm::aligned16(a->workspace)) return GDN_ERR_ALIGN;
   if (!ssm::device_ok()) return GDN_ERR_DEVICE;
   GemmP p = {};
   p.a = operand(a->x, a->sx, a->M, a->K);
@@ -1117,6 +1118,7 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
   if (!a->dy || (a->act != GDN_ACT_NONE && !a->pre) || (a->dx && !a->weight) || (a->dweight && !a->x)) return GDN_ERR_NULL;
   if (a->sx < 0 || a->sw < 0 || a->sdy < 0) return GDN_ERR_SHAPE;
   if (need && (!a->workspace || a->workspace_bytes < need)) return GDN_ERR_WORKSPACE;
+  if (need && !ssm::aligned16(a->workspace)) return GDN_ERR_ALIGN;
   if (!ssm::device_ok()) return GDN_ERR_DEVICE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const BwdPlan w = bwd_plan(a);

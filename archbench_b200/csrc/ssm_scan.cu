@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
       if (p.ckpt && live) {
         float* c = p.ckpt + (((int64_t)b * nck + (t0 + r0) / GDN_SCAN_CKPT) * p.D + d0 + hc) * p.N + n0;
         const float2 lo = unpack2(h[0]), hi = unpack2(h[1]);
-        if (p.N % 4 == 0) {
+        if (p.ckpt_quads) {
           if (n0 < p.N) *reinterpret_cast<float4*>(c) = make_float4(lo.x, lo.y, hi.x, hi.y);
         } else {
           const float hv[SPL] = {lo.x, lo.y, hi.x, hi.y};
@@ -972,6 +972,7 @@ ScanP scan_params(const gdn_scan_args* a) {
   const int es = elem_size(a->dtype);
   auto quad = [&](const void* q, int64_t sb, int64_t st, int64_t sg) { return (uintptr_t)q % (4 * es) == 0 && sb % 4 == 0 && st % 4 == 0 && sg % 4 == 0; };
   p.quads = a->N % 4 == 0 && quad(a->Bm, a->sB_b, a->sB_t, a->sB_g) && quad(a->Cm, a->sC_b, a->sC_t, a->sC_g);
+  p.ckpt_quads = a->N % 4 == 0 && aligned16(a->ckpt);
   p.dblocks = scan_dblocks(a->D, a->G, a->N);
   const int64_t warp_channels = a->N <= 8 ? 32 : a->N <= 16 ? 16 : 8;  // of the kernels for aligned rows
   const SegPlan sp = scan_segments(a->B > 0 ? a->B : 1, a->T, (a->D / a->G + warp_channels - 1) / warp_channels * a->G);
@@ -1092,6 +1093,7 @@ int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
   if (a->B == 0) return GDN_OK;
   if (a->T > 0 && !a->y) return GDN_ERR_NULL;
   if (need && (!a->workspace || a->workspace_bytes < need)) return GDN_ERR_WORKSPACE;
+  if (need && !aligned16(a->workspace)) return GDN_ERR_ALIGN;
   if (!device_ok()) return GDN_ERR_DEVICE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ScanP p = scan_params(a);

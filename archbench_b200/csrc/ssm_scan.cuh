@@ -31,6 +31,7 @@ struct ScanP {
   int B, T, D, N, G;
   int softplus;
   int quads;  // rows of B and C can be loaded four states at a time
+  int ckpt_quads;  // and rows of ckpt stored so
   int nseg, seg_len;  // segments of seg_len tokens (a multiple of GDN_SCAN_CKPT)
   int dblocks;        // channel blocks per group
   int xgs;            // channels from one group to the next in x, dt, z and dy (padded copies have more than D / G)

@@ -690,7 +690,8 @@ int launch_bwd(ScanP p, const gdn_scan_bwd_args* a, cudaStream_t s) {
   const int nl = scan_lanes(p.N);
   const bool tiled = p.tiled;
   if (tiled) p.dblocks = (int)((p.D / p.G + 256 / nl - 1) / (256 / nl));  // two channels per lane: half the blocks
-  p.pairs_out = (p.D / p.G) % 2 == 0;                                    // dx, ddt and dz are contiguous
+  auto pair = [](const void* q) { return (uintptr_t)q % (2 * sizeof(T)) == 0; };
+  p.pairs_out = (p.D / p.G) % 2 == 0 && pair(p.dx) && pair(p.ddt) && pair(p.dz);  // their rows are contiguous
   const dim3 g(p.dblocks * p.G, p.nseg, p.B);
   int st = GDN_OK;
   if (tiled) {
@@ -736,6 +737,7 @@ int gdn_scan_bwd(const gdn_scan_bwd_args* a, void* stream) {
   if (a->sdy_b < 0 || a->sdy_t < 0) return GDN_ERR_SHAPE;
   if ((int64_t)f->B * f->T * f->G * 2 * f->N > (int64_t)0x7fffffff * 256) return GDN_ERR_SHAPE;
   if (!a->fwd.workspace || a->fwd.workspace_bytes < need) return GDN_ERR_WORKSPACE;
+  if (!aligned16(a->fwd.workspace)) return GDN_ERR_ALIGN;
   if (!device_ok()) return GDN_ERR_DEVICE;
   ScanP p = bwd_params(a);
   const BwdPlan w = bwd_plan(p);

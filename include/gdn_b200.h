@@ -420,6 +420,9 @@ int gdn_abi_version(void);
 
 /* ---- selective state space mixer: short convolution, scan, single tokens -------------------- */
 
+/* In this section and the next, pointers stand on their elements' boundaries and need no other alignment, except that the
+ * scan's and the matrix product's `workspace` starts on a 16-byte boundary (GDN_ERR_ALIGN). */
+
 /*
  * Depthwise causal convolution, channels last, with an optional bias and SiLU:
  *     p_t = bias + sum_{w < width} weight[:, w] x_{t - width + 1 + w},   y_t = act(p_t)
