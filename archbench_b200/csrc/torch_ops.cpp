@@ -88,6 +88,12 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// A kernel wrote `t` in place: a graph that keeps the old values refuses its backward.  (Tensors of inference mode are in no
+// graph and have no counter.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int activation_code(const std::optional<std::string>& a, bool gelu) {
   if (!a) return GDN_ACT_NONE;
   if (*a == "silu") return GDN_ACT_SILU;
@@ -217,6 +223,7 @@ Tensor causal_conv_step(const Tensor& x0, const Tensor& weight, const Tensor& st
   gdn_conv_args a = conv_block(x, w, bias, state, act, Tensor());
   a.y = ptr(y); a.sy_b = y.stride(0);
   check(gdn_conv_step(&a, stream_of(x)));
+  written(state);
   return y;
 }
 
@@ -377,6 +384,7 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& A, c
   gdn_scan_args a = scan_block(s);
   a.y = ptr(y); a.sy_b = y.stride(0); a.h_out = ptr_as<float>(state);
   check(gdn_scan_step(&a, stream_of(x)));
+  written(state);
   return y;
 }
 
