@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <functional>
 #include <optional>
 #include <string>
 
@@ -92,6 +93,25 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
 // graph and have no counter.)
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The one-token forms have no gradient.  Where one would be wanted their output says so in its backward, as a node on
+// `source`; `run` makes the output.
+struct OneTokenNode : torch::autograd::Function<OneTokenNode> {
+  static Tensor forward(AutogradContext*, const Tensor&, const std::function<Tensor()>& run) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return run();
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    C10_THROW_ERROR(Error, "the one-token forms are not differentiable: call the prompt's form on one token");
+  }
+};
+template <typename F>
+Tensor one_token(std::initializer_list<Tensor> inputs, const Tensor& state, const F& run) {
+  VALUE(!wants_grad({state}), "state is updated in place and must not require a gradient: detach it");
+  for (const Tensor& t : inputs)
+    if (wants_grad({t})) return OneTokenNode::apply(t, std::function<Tensor()>(run));
+  return run();
 }
 
 int activation_code(const std::optional<std::string>& a, bool gelu) {
@@ -218,13 +238,15 @@ Tensor causal_conv_step(const Tensor& x0, const Tensor& weight, const Tensor& st
   const int64_t st[] = {B, C, w.size(1) - 1};
   VALUE(state.sizes() == at::IntArrayRef(st) && state.scalar_type() == x.scalar_type() && state.is_contiguous() && state.device() == x.device(),
         "state must be a contiguous ", at::IntArrayRef(st), " ", x.scalar_type(), " tensor on ", x.device(), ": it is updated in place");
-  const c10::cuda::OptionalCUDAGuard guard(x.device());
-  const Tensor y = at::empty({B, C}, x.options());
-  gdn_conv_args a = conv_block(x, w, bias, state, act, Tensor());
-  a.y = ptr(y); a.sy_b = y.stride(0);
-  check(gdn_conv_step(&a, stream_of(x)));
-  written(state);
-  return y;
+  return one_token({x, w, bias}, state, [&, &w = w, &bias = bias] {
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const Tensor y = at::empty({B, C}, x.options());
+    gdn_conv_args a = conv_block(x, w, bias, state, act, Tensor());
+    a.y = ptr(y); a.sy_b = y.stride(0);
+    check(gdn_conv_step(&a, stream_of(x)));
+    written(state);
+    return y;
+  });
 }
 
 // ---- selective scan ---------------------------------------------------------------------------
@@ -379,13 +401,15 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& A, c
   const int64_t st[] = {x.size(0), x.size(1), s.A.size(1)};
   VALUE(state.sizes() == at::IntArrayRef(st) && state.scalar_type() == at::kFloat && state.is_contiguous() && state.device() == x.device(),
         "state must be a contiguous ", at::IntArrayRef(st), " float32 tensor on ", x.device(), ": it is updated in place");
-  const c10::cuda::OptionalCUDAGuard guard(x.device());
-  const Tensor y = at::empty(x.sizes(), x.options());
-  gdn_scan_args a = scan_block(s);
-  a.y = ptr(y); a.sy_b = y.stride(0); a.h_out = ptr_as<float>(state);
-  check(gdn_scan_step(&a, stream_of(x)));
-  written(state);
-  return y;
+  return one_token({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias}, state, [&] {
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const Tensor y = at::empty(x.sizes(), x.options());
+    gdn_scan_args a = scan_block(s);
+    a.y = ptr(y); a.sy_b = y.stride(0); a.h_out = ptr_as<float>(state);
+    check(gdn_scan_step(&a, stream_of(x)));
+    written(state);
+    return y;
+  });
 }
 
 // ---- linear -----------------------------------------------------------------------------------

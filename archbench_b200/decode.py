@@ -72,6 +72,7 @@ class GraphDecoder:
     kernels read and write the same state buffers on every replay.  Capturing advances neither the
     caches nor the token: what the warm-up call that precedes the capture changes is put back."""
 
+    @torch.no_grad()
     def __init__(self, model: nn.Module, caches: List[GDNCache], token: torch.Tensor):
         self.model = model
         self.token = token.clone()
@@ -96,6 +97,7 @@ class GraphDecoder:
             c.seen = seen
         self.caches = caches
 
+    @torch.no_grad()
     def _run(self) -> torch.Tensor:
         logits = _logits(self.model(self.token[:, None]))[:, -1]
         self.token.copy_(logits.argmax(-1))

@@ -6,8 +6,8 @@
 It is the diagonal counterpart of the gated-DeltaNet mixers (registry name ``ssm``, ``LM(arch="ssm")``): the same call
 ``forward(x)`` and the same ``GDNCache`` for prompts and single tokens, so ``decode.greedy_decode`` and its CUDA graph
 serve it.  Four projections run as ``ops.linear`` (the output projection with the block's residual in its epilogue), the
-convolution as ``ops.causal_conv`` and the recurrence as ``ops.selective_scan``, each with its backward; one token takes
-``ops.causal_conv_step`` and ``ops.selective_scan_step``, which advance the cache in place.  bf16 activations use the
+convolution as ``ops.causal_conv`` and the recurrence as ``ops.selective_scan``, each with its backward; one token without
+gradients takes ``ops.causal_conv_step`` and ``ops.selective_scan_step``, which advance the cache in place.  bf16 activations use the
 package's matrix product; fp32 ones take ``torch.nn.functional.linear``."""
 
 from __future__ import annotations
@@ -84,7 +84,9 @@ class SelectiveSSM(nn.Module):
         A, D, dt_bias = self._parameters_f32(_training(x, self))
         conv_w = self.conv1d.weight.to(x.dtype)
         conv_b = None if self.conv1d.bias is None else self.conv1d.bias.to(x.dtype)
-        one = cache is not None and cache.state is not None and T == 1
+        # the one-token forms have no gradient; where one is wanted one token takes the prompt's
+        one = cache is not None and cache.state is not None and T == 1 and (
+            cache.static or not (_training(x, self) or torch.is_grad_enabled() and cache.state.requires_grad))
         u, z = _linear(x, self.in_proj.weight, self.in_proj.bias).chunk(2, -1)
         if one:
             u = ops.causal_conv_step(u[:, 0], conv_w, cache.conv["x"], conv_b, "silu")[:, None]

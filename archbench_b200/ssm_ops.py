@@ -114,7 +114,7 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, outpu
 @eager
 def causal_conv_step(x, weight, state, bias=None, activation=None):
     """One token of ``causal_conv``: x (B, C), state (B, C, W - 1) contiguous, in x's dtype, advanced in place.  No
-    autograd."""
+    gradient: a backward through its output raises, and a state that requires one is refused."""
     return (_EXT or extension()).causal_conv_step(x, weight, state, bias, activation)
 
 
@@ -136,5 +136,5 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
 @eager
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False):
     """One token of ``selective_scan``: x, dt, z (B, D), B, C (B, N) or (B, G, N), state (B, D, N) fp32 contiguous,
-    advanced in place.  No autograd."""
+    advanced in place.  No gradient, as for ``causal_conv_step``."""
     return (_EXT or extension()).selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
