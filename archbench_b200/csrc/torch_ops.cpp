@@ -83,6 +83,9 @@ Tensor row_lengths(const Opt& lengths, int64_t B, int64_t device) {
 }
 
 bool wants_grad(std::initializer_list<Tensor> ts) {
+  for (const Tensor& t : ts)  // the kernels would drop a tangent
+    if (t.defined() && C10_UNLIKELY(t._fw_grad(/*level=*/0).defined()))
+      C10_THROW_ERROR(NotImplementedError, "the kernels have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor& t : ts)
     if (t.defined() && t.requires_grad()) return true;

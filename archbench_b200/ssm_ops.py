@@ -9,7 +9,8 @@ causal convolution, the selective scan and their one-token forms.
   selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False) -> y  (state in place)
 
 All are reachable as ``archbench_b200.ops.<name>``.  CUDA tensors only, bf16 or fp32 token tensors with any strides;
-states and sums are fp32.  Calls that need gradients run the backward kernels through autograd (first order).  Under
+states and sums are fp32.  Calls that need gradients run the backward kernels through autograd (first order;
+forward-mode tangents are refused).  Under
 ``torch.compile`` the calls run eagerly between compiled regions.
 
 The calls themselves -- checks, allocation, autograd nodes -- are compiled (``csrc/torch_ops.cpp``, the extension module
