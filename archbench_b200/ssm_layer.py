@@ -24,10 +24,13 @@ from .layers import GDNCache, _put, _training
 
 
 def _linear(x, weight, bias=None, activation=None, residual=None):
-    """``ops.linear`` in bf16; the same formula from torch's functions for fp32 activations."""
+    """``ops.linear`` in bf16; the same formula from torch's functions for fp32 activations.  A residual of another type
+    than the activations (the fp32 stream of a model under autocast) is added outside the product and keeps its type."""
     weight, bias = weight.to(x.dtype), None if bias is None else bias.to(x.dtype)
     if x.dtype == torch.bfloat16:
-        return ops.linear(x, weight, bias, activation, None if residual is None else residual.to(x.dtype))
+        fused = residual is None or residual.dtype == x.dtype
+        y = ops.linear(x, weight, bias, activation, residual if fused else None)
+        return y if fused else y + residual
     y = F.linear(x, weight, bias)
     y = y if activation is None else F.silu(y) if activation == "silu" else F.gelu(y)
     return y if residual is None else y + residual
@@ -43,7 +46,7 @@ class SelectiveSSM(nn.Module):
     64), ``conv_size`` taps (2 to 4), step sizes through a projection of rank ``dt_rank`` (d_model / 16 rounded up by
     default) that start log-uniform in [dt_min, dt_max]."""
 
-    fuses_residual = True  # forward takes the block's residual and adds it in the output projection
+    fuses_residual = True  # forward takes the block's residual and adds it, in the output projection if the types agree
 
     def __init__(self, d_model: int, layer_idx: int = 0, expand: float = 2.0, state_size: int = 16, conv_size: int = 4,
                  dt_rank: Optional[int] = None, dt_min: float = 1e-3, dt_max: float = 1e-1, bias: bool = False, conv_bias: bool = True):
