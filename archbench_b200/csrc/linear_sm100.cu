@@ -672,10 +672,11 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmP p) {
 constexpr int DP_ROWS = 64, DP_BATCH = 2;
 template <bool VEC>
 __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, const bf16* pre, bf16* dp, int64_t ldp, int64_t M, int64_t N,
-                                                 int act, int slope, float* colsum) {
-  // 32 lanes x 8 columns, 8 row groups
+                                                 int act, int slope, uint32_t col_blocks, float* colsum) {
+  // 32 lanes x 8 columns, 8 row groups; the blocks of one group of DP_ROWS rows follow one another
   const int lane = threadIdx.x % 32, rg = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * 256 + lane * 8, r0 = (int64_t)blockIdx.y * DP_ROWS;
+  const uint32_t gr = blockIdx.x / col_blocks;
+  const int64_t c0 = (int64_t)(blockIdx.x - gr * col_blocks) * 256, col = c0 + lane * 8, r0 = (int64_t)gr * DP_ROWS;
   f32x2 sum[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) sum[i] = both(0.f);
@@ -732,12 +733,12 @@ __global__ void __launch_bounds__(256) dp_kernel(const bf16* dy, int64_t ldd, co
     part[rg][lane * 8 + 2 * i + 1] = e.y;
   }
   __syncthreads();
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t c = c0 + threadIdx.x;
   if (c >= N) return;
   float a = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) a += part[i][threadIdx.x];
-  colsum[blockIdx.y * N + c] = a;
+  colsum[gr * N + c] = a;
 }
 
 // Column sums of the partial rows, added in order: 32 columns x 8 groups of rows per block.
@@ -1129,13 +1130,13 @@ int gdn_linear_bwd(const gdn_linear_bwd_args* a, void* stream) {
   void* part = copies + w.x + w.w;
   if (dp || colsum) {
     const int64_t gx = ((dp ? w.ldp : a->N) + 255) / 256, gy = (a->M + DP_ROWS - 1) / DP_ROWS;
-    if (gy > 65535) return GDN_ERR_SHAPE;
-    const dim3 g((unsigned)gx, (unsigned)gy);
+    if (gx * gy > 0x7fffffff) return GDN_ERR_SHAPE;  // 2^45 values of dy: past any memory
+    const unsigned g = (unsigned)(gx * gy);
     const bf16 *dy = static_cast<const bf16*>(a->dy), *pre = static_cast<const bf16*>(a->pre);
     if (a->N % 8 == 0 && rows16(dy, a->sdy) && (a->act == GDN_ACT_NONE || ssm::aligned16(pre)))
-      dp_kernel<true><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, a->keep, colsum);
+      dp_kernel<true><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, a->keep, (uint32_t)gx, colsum);
     else
-      dp_kernel<false><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, a->keep, colsum);
+      dp_kernel<false><<<g, 256, 0, s>>>(dy, a->sdy, pre, dp, w.ldp, a->M, a->N, a->act, a->keep, (uint32_t)gx, colsum);
     if (colsum) colsum_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, s>>>(colsum, gy, a->N, static_cast<bf16*>(a->dbias));
     st = ssm::launched();
     if (st != GDN_OK) return st;
