@@ -29,6 +29,7 @@ struct ScanP {
   float *pD;     // backward: (B * nseg, 2, D) partial sums of dDskip and ddt_bias
   int64_t sx_b, sx_t, sdt_b, sdt_t, sB_b, sB_t, sB_g, sC_b, sC_t, sC_g, sz_b, sz_t, sy_b, sy_t, sdy_b, sdy_t;
   int B, T, D, N, G;
+  int b0;  // the launch's first row
   int softplus;
   int quads;  // rows of B and C can be loaded four states at a time
   int ckpt_quads;  // and rows of ckpt stored so
@@ -123,6 +124,13 @@ __device__ __forceinline__ int spread_sum(float (&v)[NV], int lane) {
     }
   }
   return first;
+}
+
+// Rows are the last dimension of a grid, which ends at 65535: launch(rows) with p.b0 set, as often as it takes.
+template <typename F>
+void for_grid_rows(ScanP& p, F launch) {
+  constexpr int MOST = 65535;
+  for (p.b0 = 0; p.b0 < p.B; p.b0 += MOST) launch((unsigned)(p.B - p.b0 < MOST ? p.B - p.b0 : MOST));
 }
 
 // Segments of time, each at least MIN_SEG tokens.

@@ -34,3 +34,41 @@ def test_linear_backward_of_many_rows(act):
     assert torch.equal(y[-65:], y[at[-65:]]) and torch.equal(dx[-65:], dx[at[-65:]])
     for got, want in ((dx[:1024], x0), (dw, w0), (db, b0)):
         assert ((got.double() - want).norm() <= 2.0 ** -6 * want.norm()).item(), ((got.double() - want).norm() / want.norm()).item()
+
+
+def test_scan_of_many_rows():
+    """More rows than a grid's last dimension: forward, gradients, ragged lengths and the one-token form."""
+    B, T, D, N = 65535 + 70, 2, 4, 4
+    g = torch.Generator("cuda").manual_seed(2)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    v = [rnd(B, T, D), rnd(B, T, D), -torch.rand(D, N, generator=g, device="cuda") - 0.1, rnd(B, T, 1, N), rnd(B, T, 1, N), rnd(D), rnd(B, T, D), rnd(D),
+         rnd(B, D, N)]
+    n = torch.randint(0, T + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    dy, dh = rnd(B, T, D), rnd(B, D, N)
+
+    def own(ts):
+        x, dt, A, Bm, C, Dk, z, bias, h = ts
+        return ops.selective_scan(x, dt, A, Bm, C, D=Dk, z=z, dt_bias=bias, dt_softplus=True, initial_state=h, output_final_state=True, lengths=n)
+
+    def ref(ts):
+        x, dt, A, Bm, C, Dk, z, bias, h = ts
+        return R.scan(x, dt, A, Bm, C, Dk, z, bias, True, h, n)
+
+    a = [t.clone().requires_grad_() for t in v]
+    b = [t.double().cpu().requires_grad_() for t in v]
+    oa, ob = own(a), ref(b)
+    with torch.no_grad():
+        for p, q in zip(own(v), oa):
+            assert torch.equal(p, q)
+    for p, q in zip(oa, ob):
+        R.close(p, q, "out", accumulated=128 + N)
+    ga, gb = torch.autograd.grad(oa, a, [dy, dh]), torch.autograd.grad(ob, b, [dy.double().cpu(), dh.double().cpu()])
+    for i, (p, q) in enumerate(zip(ga, gb)):
+        R.close(p, q, str(i), accumulated=256 + (B * T if i in (2, 5, 7) else D if i in (3, 4) else 0))
+    h = v[8].clone()
+    y = ops.selective_scan_step(v[0][:, 0], v[1][:, 0], v[2], v[3][:, 0], v[4][:, 0], h, D=v[5], z=v[6][:, 0], dt_bias=v[7], dt_softplus=True)
+    cut = [t[:, :1] if t.dim() >= 3 and t.shape[1] == T and i != 8 else t for i, t in enumerate(v)]
+    c = lambda t: t.double().cpu()
+    y0, h0 = R.scan(*(c(t) for t in cut[:5]), c(v[5]), c(cut[6]), c(v[7]), True, c(v[8]))
+    R.close(y, y0[:, 0], "step", accumulated=128)
+    R.close(h, h0, "step state", accumulated=128)
