@@ -41,9 +41,10 @@ std::string message(const P&... parts) {
     if (C10_UNLIKELY(!(cond))) C10_THROW_ERROR(ValueError, message(__VA_ARGS__)); \
   } while (0)
 
-// A library status as archbench_b200.native.GdnError.
+// A library status: sizes that no kernel serves as a ValueError, the rest as archbench_b200.native.GdnError.
 void check(int status) {
   if (status == GDN_OK) return;
+  if (status == GDN_ERR_SHAPE || status == GDN_ERR_UNSUPPORTED) C10_THROW_ERROR(ValueError, message("sizes out of range: ", gdn_status_string(status)));
   py::gil_scoped_acquire gil;  // an autograd thread may be here without it
   py::module_::import("archbench_b200.native").attr("_check")(status);
 }

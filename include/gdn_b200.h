@@ -421,7 +421,9 @@ int gdn_abi_version(void);
 /* ---- selective state space mixer: short convolution, scan, single tokens -------------------- */
 
 /* In this section and the next, pointers stand on their elements' boundaries and need no other alignment, except that the
- * scan's and the matrix product's `workspace` starts on a 16-byte boundary (GDN_ERR_ALIGN). */
+ * scan's and the matrix product's `workspace` starts on a 16-byte boundary (GDN_ERR_ALIGN).  Sizes (GDN_ERR_SHAPE past
+ * them): B up to 2^30; T up to 2^30 for the convolution, 2^29 for the scan; C and D up to 2^24, B T C and B T D up to
+ * 2^46; M, N and K of the matrix product up to 2^30; strides not negative. */
 
 /*
  * Depthwise causal convolution, channels last, with an optional bias and SiLU:

@@ -72,3 +72,16 @@ def test_scan_of_many_rows():
     y0, h0 = R.scan(*(c(t) for t in cut[:5]), c(v[5]), c(cut[6]), c(v[7]), True, c(v[8]))
     R.close(y, y0[:, 0], "step", accumulated=128)
     R.close(h, h0, "step state", accumulated=128)
+
+
+def test_unserved_sizes_raise_value_errors():
+    """Refused before anything is launched or allocated at that size: broadcast views."""
+    x = torch.zeros(1, 1, 1, device="cuda")
+    A, w = -torch.ones(2 ** 24 + 1, 1, device="cuda"), torch.zeros(2 ** 24 + 1, 2, device="cuda")
+    z = x.expand(1, 1, 2 ** 24 + 1)
+    with pytest.raises(ValueError):
+        ops.selective_scan(z, z, A, x, x)
+    with pytest.raises(ValueError):
+        ops.causal_conv(z, w)
+    with pytest.raises(ValueError):
+        ops.selective_scan_step(z[0], z[0], A, x[0], x[0], torch.zeros(1, 2 ** 24 + 1, 1, device="cuda"))
