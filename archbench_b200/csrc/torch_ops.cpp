@@ -76,11 +76,15 @@ Tensor dense(const Tensor& t, const char* name, at::IntArrayRef shape, at::Scala
   return t.defined() ? token(t, name, shape, dtype, device).contiguous() : t;
 }
 
-Tensor row_lengths(const Opt& lengths, int64_t B, int64_t device) {
+// Token counts as int32; the kernels take min(max(n, 0), T).  Wider types are brought into range first: their low 32 bits alone
+// may be any count.
+Tensor row_lengths(const Opt& lengths, int64_t B, int64_t T, int64_t device) {
   if (!lengths) return Tensor();
-  VALUE(!lengths->is_floating_point() && lengths->dim() == 1 && lengths->size(0) == B && lengths->is_cuda() && lengths->get_device() == device,
+  VALUE(!lengths->is_floating_point() && !lengths->is_complex() && lengths->dim() == 1 && lengths->size(0) == B && lengths->is_cuda() && lengths->get_device() == device,
         "lengths must be an integer tensor of shape (", B, ",) on cuda:", device);
-  return lengths->to(at::kInt).contiguous();
+  Tensor n = *lengths;
+  if (n.element_size() > 4 || n.scalar_type() == at::kUInt32) n = n.to(at::kLong).clamp(0, T);
+  return n.to(at::kInt).contiguous();
 }
 
 bool wants_grad(std::initializer_list<Tensor> ts) {
@@ -220,7 +224,7 @@ std::pair<Tensor, Opt> causal_conv(const Tensor& x0, const Tensor& weight, const
   const Tensor x = token(x0, "x", x0.sizes(), x0.scalar_type(), device);
   const auto [w, bias] = conv_params(weight, bias0, C, device);
   const int64_t st[] = {B, C, w.size(1) - 1};
-  const Tensor state = dense(get(initial_state), "initial_state", st, x.scalar_type(), device), lengths = row_lengths(lengths0, B, device);
+  const Tensor state = dense(get(initial_state), "initial_state", st, x.scalar_type(), device), lengths = row_lengths(lengths0, B, x.size(1), device);
   Tensor y, last;
   if (wants_grad({x, w, bias, state})) {
     const variable_list r = ConvNode::apply(x, w, opt(bias), opt(state), opt(lengths), (int64_t)act, output_final_state);
@@ -383,7 +387,7 @@ std::pair<Tensor, Opt> selective_scan(const Tensor& x, const Tensor& dt, const T
   ScanIn s = scan_inputs(x, dt, A, B, C, D, z, dt_bias, dt_softplus);
   const int64_t st[] = {x.size(0), x.size(2), s.A.size(1)};
   s.h0 = dense(get(initial_state), "initial_state", st, at::kFloat, x.get_device());
-  s.lengths = row_lengths(lengths, x.size(0), x.get_device());
+  s.lengths = row_lengths(lengths, x.size(0), x.size(1), x.get_device());
   Tensor y, h;
   if (wants_grad({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.h0})) {
     const variable_list r = ScanNode::apply(s.x, s.dt, s.A, s.B, s.C, opt(s.D), opt(s.z), opt(s.bias), opt(s.h0), opt(s.lengths),

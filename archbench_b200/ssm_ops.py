@@ -128,8 +128,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
         y_t = (C_t . h_t + D x_t) silu(z_t)
 
     x, dt, z (B, T, D); A (D, N), usually negative; B, C (B, T, N) or (B, T, G, N), group g serving D / G consecutive
-    channels; D, dt_bias (D); initial_state (B, D, N) fp32 (zeros if None); lengths (B): tokens of each right-padded row
-    (past them y is 0 and the state stays).  N <= 64.  Returns (y, final_state or None): y in x's dtype, the state fp32.
+    channels; D, dt_bias (D); initial_state (B, D, N) fp32 (zeros if None); lengths (B): tokens of each right-padded row, int32
+    for no conversion (past them y is 0 and the state stays).  N <= 64.  Returns (y, final_state or None): y in x's dtype, the state fp32.
     Training keeps one state per 8 tokens."""
     return (_EXT or extension()).selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, lengths)
 
