@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(ScanP p) {
       const int seg = REV ? p.nseg - 1 - (k0 + q) : k0 + q;
       if (k0 + q >= p.nseg) break;
       p.carry[(b * p.nseg + seg) * dn + at] = H;
-      H = fmaf(decay(a[q], A2), H, e[q]);
+      H = H == 0.f ? e[q] : fmaf(decay(a[q], A2), H, e[q]);  // zero times a growth past fp32 is zero
     }
   }
 }
