@@ -36,6 +36,24 @@ def _linear(x, weight, bias=None, activation=None, residual=None):
     return y if residual is None else y + residual
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _plain(m: nn.Module) -> bool:
+    """True for an ``nn.Linear`` that is its weight and bias and nothing else.  A replacement (an adapter, a quantised
+    layer), a parametrised layer or one with hooks runs through its own call."""
+    return type(m) is nn.Linear and "forward" not in m.__dict__ and not any(getattr(m, h) for h in _HOOKS)
+
+
+def _project(m: nn.Module, x, activation=None, residual=None):
+    """activation(m(x)) + residual, in one product where ``m`` is a plain ``nn.Linear``."""
+    if _plain(m):
+        return _linear(x, m.weight, m.bias, activation, residual)
+    y = m(x)
+    y = y if activation is None else F.silu(y) if activation == "silu" else F.gelu(y)
+    return y if residual is None else y + residual
+
+
 def _activations(x: torch.Tensor) -> torch.Tensor:
     """``x`` in the dtype of an enclosing autocast region."""
     return x.to(torch.get_autocast_dtype("cuda")) if torch.is_autocast_enabled("cuda") else x
@@ -73,11 +91,13 @@ class SelectiveSSM(nn.Module):
     bound_cache: Optional[GDNCache] = None  # used when called without a cache (decode.bind_caches)
 
     def _parameters_f32(self, train: bool):
-        """A, D and the step bias in fp32; kept between calls while the parameters are unchanged, except in training."""
+        """A, D and the step bias (None where ``dt_proj`` adds it itself) in fp32; kept between calls while the parameters are
+        unchanged, except in training."""
+        bias = self.dt_proj.bias if _plain(self.dt_proj) else None
         if train:
-            return -torch.exp(self.A_log.float()), self.D.float(), self.dt_proj.bias.float()
+            return -torch.exp(self.A_log.float()), self.D.float(), None if bias is None else bias.float()
         return (ops._cached(self.A_log, "neg_exp", lambda t: -torch.exp(t.float())), ops._cached(self.D, "f32", lambda t: t.float()),
-                ops._cached(self.dt_proj.bias, "f32", lambda t: t.float()))
+                None if bias is None else ops._cached(bias, "f32", lambda t: t.float()))
 
     def forward(self, x: torch.Tensor, cache: Optional[GDNCache] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if cache is None:
@@ -90,15 +110,16 @@ class SelectiveSSM(nn.Module):
         # the one-token forms have no gradient; where one is wanted one token takes the prompt's
         one = cache is not None and cache.state is not None and T == 1 and (
             cache.static or not (_training(x, self) or torch.is_grad_enabled() and cache.state.requires_grad))
-        u, z = _linear(x, self.in_proj.weight, self.in_proj.bias).chunk(2, -1)
+        u, z = _project(self.in_proj, x).chunk(2, -1)
         if one:
             u = ops.causal_conv_step(u[:, 0], conv_w, cache.conv["x"], conv_b, "silu")[:, None]
         else:
             u, last = ops.causal_conv(u, conv_w, conv_b, "silu", None if cache is None else cache.conv.get("x"), cache is not None)
             if cache is not None:
                 _put(cache, "x", last)
-        r, B, C = _linear(u, self.x_proj.weight).split([R, N, N], -1)
-        dt = _linear(r, self.dt_proj.weight)
+        r, B, C = _project(self.x_proj, u).split([R, N, N], -1)
+        # a plain projection's bias is added to the step sizes inside the scan, in fp32
+        dt = _linear(r, self.dt_proj.weight) if dt_bias is not None else self.dt_proj(r)
         if one:
             y = ops.selective_scan_step(u[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], cache.state, D=D, z=z[:, 0], dt_bias=dt_bias,
                                         dt_softplus=True)[:, None]
@@ -109,7 +130,7 @@ class SelectiveSSM(nn.Module):
                 cache.state = state
         if cache is not None:
             cache.seen += T
-        return _linear(y, self.out_proj.weight, self.out_proj.bias, residual=residual)
+        return _project(self.out_proj, y, residual=residual)
 
 
 class FusedMLP(nn.Module):
@@ -128,5 +149,4 @@ class FusedMLP(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         x = _activations(x)
-        h = _linear(x, self.up.weight, self.up.bias, self.activation)
-        return _linear(h, self.down.weight, self.down.bias, residual=residual)
+        return _project(self.down, _project(self.up, x, self.activation), residual=residual)
