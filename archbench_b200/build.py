@@ -6,13 +6,16 @@
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` and the objects link into
 ``archbench_b200/libgdn_b200.so`` (static CUDA runtime, C ABI of ``include/gdn_b200.h``).  ``csrc/torch_ops.cpp``, the
 operators as functions of torch tensors, compiles with the host compiler to the extension module
-``archbench_b200/_torch_ops.so``, which links against that library beside it.
+``archbench_b200/_torch_ops.so``, which links against that library beside it.  Where the host compiler, ``Python.h`` or torch
+is missing, the library is built without it.
 """
 
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
+import shlex
 import shutil
 import subprocess
 import sys
@@ -59,10 +62,29 @@ def _compile(src, force, verbose):
     return obj, r.stderr if verbose else ""
 
 
+def _cxx():
+    return shlex.split(os.environ.get("CXX", "g++"))
+
+
+def _torch_ops_lack():
+    """What the torch extension needs and this machine lacks, or None.  The library itself needs nvcc alone."""
+    if shutil.which(_cxx()[0]) is None:
+        return f"no host compiler {_cxx()[0]}"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "no Python.h"
+    if importlib.util.find_spec("torch") is None:
+        return "no torch"
+    return None
+
+
+def _torch_ops_sources():
+    return [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(INCLUDE, "gdn_b200.h")]
+
+
 def _compile_torch_ops(force):
     """The object of the torch extension (30 s with torch's headers)."""
-    src, obj = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(OBJ, "torch_ops.o")
-    deps = [src, os.path.join(INCLUDE, "gdn_b200.h")]
+    deps = _torch_ops_sources()
+    src, obj = deps[0], os.path.join(OBJ, "torch_ops.o")
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     import torch
@@ -70,7 +92,7 @@ def _compile_torch_ops(force):
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
     dirs = [inc, os.path.join(inc, "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-c", src, "-o", obj, "-DTORCH_EXTENSION_NAME=_torch_ops",
+    cmd = [*_cxx(), "-O2", "-std=c++17", "-fPIC", "-c", src, "-o", obj, "-DTORCH_EXTENSION_NAME=_torch_ops",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE]
     for d in dirs:
         cmd += ["-isystem", d]
@@ -87,7 +109,7 @@ def _link_torch_ops(obj, force):
 
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = TORCH_OPS + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj, "-L" + lib, "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
+    cmd = [*_cxx(), "-shared", "-o", tmp, obj, "-L" + lib, "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
            "-L" + PKG, "-l:libgdn_b200.so", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
@@ -99,9 +121,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs)) + 1) as ex:
-        torch_obj = ex.submit(_compile_torch_ops, force)
+        lack = _torch_ops_lack()
+        torch_obj = None if lack else ex.submit(_compile_torch_ops, force)
         results = list(ex.map(lambda s: _compile(s, force, verbose), srcs))
-        torch_obj = torch_obj.result()
     objs = [o for o, _ in results]
     for _, log in results:
         if log:
@@ -113,7 +135,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
-    _link_torch_ops(torch_obj, force)
+    if lack:
+        if os.path.exists(TORCH_OPS) and os.path.getmtime(TORCH_OPS) < max(os.path.getmtime(d) for d in _torch_ops_sources()):
+            os.remove(TORCH_OPS)  # none rather than one of other sources: the operators that need it then name it
+        print(f"{os.path.basename(TORCH_OPS)} not built: {lack}", file=sys.stderr)
+    else:
+        _link_torch_ops(torch_obj.result(), force)  # a failure here leaves the library built
     return LIB
 
 
