@@ -13,6 +13,7 @@ is missing, the library is built without it.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
 import importlib.util
 import os
 import shlex
@@ -81,11 +82,18 @@ def _torch_ops_sources():
     return [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(INCLUDE, "gdn_b200.h")]
 
 
+def _torch_ops_built_for():
+    """What the extension's binary interface hangs on beside its sources."""
+    return f"torch {importlib.metadata.version('torch')}, python {sys.version}, {' '.join(_cxx())}\n"
+
+
 def _compile_torch_ops(force):
     """The object of the torch extension (30 s with torch's headers)."""
     deps = _torch_ops_sources()
     src, obj = deps[0], os.path.join(OBJ, "torch_ops.o")
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
+    built_for = os.path.join(OBJ, "torch_ops.txt")
+    same = os.path.exists(built_for) and open(built_for).read() == _torch_ops_built_for()
+    if not force and same and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     import torch
 
@@ -99,6 +107,8 @@ def _compile_torch_ops(force):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on {src}:\n{r.stdout}\n{r.stderr}")
+    with open(built_for, "w") as f:
+        f.write(_torch_ops_built_for())
     return obj
 
 

@@ -1,8 +1,10 @@
 """The build of the native library and of the torch extension beside it, on a small stand-in for the sources."""
 
 import ctypes
+import importlib.metadata
 import os
 import shutil
+import sys
 
 import pytest
 
@@ -54,3 +56,21 @@ def test_both_are_built(tree):
     first = os.path.getmtime(B.TORCH_OPS)
     B.build()
     assert os.path.getmtime(B.TORCH_OPS) == first
+
+
+@pytest.mark.parametrize("what", ["torch", "python", "compiler"])
+def test_extension_is_built_again_for_another_torch_python_or_compiler(tree, monkeypatch, what):
+    B.build()
+    first = os.stat(B.TORCH_OPS).st_mtime_ns
+    if what == "torch":
+        version = importlib.metadata.version
+        monkeypatch.setattr(importlib.metadata, "version", lambda name: "0.0" if name == "torch" else version(name))
+    elif what == "python":
+        monkeypatch.setattr(sys, "version", "another")
+    else:
+        monkeypatch.setenv("CXX", shutil.which("g++") + " -g0")
+    B.build()
+    again = os.stat(B.TORCH_OPS).st_mtime_ns
+    assert again > first
+    B.build()
+    assert os.stat(B.TORCH_OPS).st_mtime_ns == again
