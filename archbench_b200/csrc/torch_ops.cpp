@@ -166,6 +166,28 @@ std::pair<Tensor, Tensor> conv_forward(const Tensor& x, const Tensor& w, const T
   return {y, last};
 }
 
+// Gradients of x, the weight, the bias and the initial state, in the order and form of the forward's arguments; dy or dlast
+// may be absent.
+variable_list conv_backward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& state, const Tensor& lengths, int act,
+                            Tensor dy, Tensor dlast) {
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  if (x.numel() == 0)
+    return {zeros_like_dense(x), zeros_like_dense(w), zeros_like_dense(bias), !state.defined() ? Tensor() : dlast.defined() ? dlast : zeros_like_dense(state)};
+  dy = dy.defined() ? token(dy, "dy", x.sizes(), x.scalar_type(), x.get_device()) : at::zeros(x.sizes(), x.options());
+  if (dlast.defined()) dlast = dlast.contiguous();
+  variable_list out = {empty_like_dense(x), empty_like_dense(w), empty_like_dense(bias), empty_like_dense(state)};
+  gdn_conv_bwd_args a = {};
+  a.fwd = conv_block(x, w, bias, state, act, lengths);
+  a.dy = ptr(dy); a.sdy_b = dy.stride(0); a.sdy_t = dy.stride(1);
+  a.dstate_out = ptr(dlast); a.dx = ptr(out[0]); a.dweight = ptr(out[1]); a.dbias = ptr(out[2]); a.dstate_in = ptr(out[3]);
+  size_t need = 0;
+  check(gdn_conv_bwd_workspace_bytes(&a, &need));
+  const Tensor ws = workspace(need, x);
+  a.workspace = ptr(ws); a.workspace_bytes = need;
+  check(gdn_conv_bwd(&a, stream_of(x)));
+  return out;
+}
+
 struct ConvNode : torch::autograd::Function<ConvNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& bias0, const Opt& state0, const Opt& lengths0,
                                int64_t act, bool want) {
@@ -180,28 +202,10 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     first_order();
     const auto s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &bias = s[2], &state = s[3], &lengths = s[4];
-    Tensor dy = g[0], dlast = g.size() > 1 ? g[1] : Tensor();
-    variable_list out(7);
-    if (!dy.defined() && !dlast.defined()) return out;
-    const c10::cuda::OptionalCUDAGuard guard(x.device());
-    if (x.numel() == 0) {
-      out[0] = zeros_like_dense(x); out[1] = zeros_like_dense(w); out[2] = zeros_like_dense(bias);
-      out[3] = !state.defined() ? Tensor() : dlast.defined() ? dlast : zeros_like_dense(state);
-      return out;
-    }
-    dy = dy.defined() ? token(dy, "dy", x.sizes(), x.scalar_type(), x.get_device()) : at::zeros(x.sizes(), x.options());
-    if (dlast.defined()) dlast = dlast.contiguous();
-    out[0] = empty_like_dense(x); out[1] = empty_like_dense(w); out[2] = empty_like_dense(bias); out[3] = empty_like_dense(state);
-    gdn_conv_bwd_args a = {};
-    a.fwd = conv_block(x, w, bias, state, (int)ctx->saved_data["act"].toInt(), lengths);
-    a.dy = ptr(dy); a.sdy_b = dy.stride(0); a.sdy_t = dy.stride(1);
-    a.dstate_out = ptr(dlast); a.dx = ptr(out[0]); a.dweight = ptr(out[1]); a.dbias = ptr(out[2]); a.dstate_in = ptr(out[3]);
-    size_t need = 0;
-    check(gdn_conv_bwd_workspace_bytes(&a, &need));
-    const Tensor ws = workspace(need, x);
-    a.workspace = ptr(ws); a.workspace_bytes = need;
-    check(gdn_conv_bwd(&a, stream_of(x)));
+    const Tensor dy = g[0], dlast = g.size() > 1 ? g[1] : Tensor();
+    if (!dy.defined() && !dlast.defined()) return variable_list(7);
+    variable_list out = conv_backward(s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["act"].toInt(), dy, dlast);
+    out.resize(7);
     return out;
   }
 };
@@ -307,6 +311,34 @@ ScanOut scan_forward(const ScanIn& s, bool want, bool train) {
   return o;
 }
 
+// Gradients of x, dt, A, B, C, D, z, the bias and the initial state, as for the convolution.
+variable_list scan_backward(const ScanIn& s, const Tensor& ckpt, Tensor dy, Tensor dh) {
+  const Tensor& x = s.x;
+  const Tensor in[] = {s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.h0};
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  variable_list out(9);
+  if (x.numel() == 0) {
+    for (int i = 0; i < 8; ++i) out[i] = zeros_like_dense(in[i]);
+    out[8] = !s.h0.defined() ? Tensor() : dh.defined() ? dh : zeros_like_dense(s.h0);
+    return out;
+  }
+  dy = dy.defined() ? token(dy, "dy", x.sizes(), x.scalar_type(), x.get_device()) : at::zeros(x.sizes(), x.options());
+  if (dh.defined()) dh = dh.contiguous();
+  for (int i = 0; i < 9; ++i) out[i] = empty_like_dense(in[i]);
+  gdn_scan_bwd_args a = {};
+  a.fwd = scan_block(s);
+  a.fwd.ckpt = ptr_as<float>(ckpt);
+  a.dy = ptr(dy); a.sdy_b = dy.stride(0); a.sdy_t = dy.stride(1); a.dh_out = ptr_as<float>(dh);
+  a.dx = ptr(out[0]); a.ddt = ptr(out[1]); a.dA = ptr_as<float>(out[2]); a.dB = ptr(out[3]); a.dC = ptr(out[4]);
+  a.dDskip = ptr_as<float>(out[5]); a.dz = ptr(out[6]); a.ddt_bias = ptr_as<float>(out[7]); a.dh0 = ptr_as<float>(out[8]);
+  size_t need = 0;
+  check(gdn_scan_bwd_workspace_bytes(&a, &need));
+  const Tensor ws = workspace(need, x);
+  a.fwd.workspace = ptr(ws); a.fwd.workspace_bytes = need;
+  check(gdn_scan_bwd(&a, stream_of(x)));
+  return out;
+}
+
 struct ScanNode : torch::autograd::Function<ScanNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                                const Opt& D0, const Opt& z0, const Opt& bias0, const Opt& h00, const Opt& lengths0, bool softplus, bool want) {
@@ -321,31 +353,10 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     first_order();
     const auto v = ctx->get_saved_variables();
-    const ScanIn s = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], ctx->saved_data["softplus"].toBool()};
-    Tensor dy = g[0], dh = g.size() > 1 ? g[1] : Tensor();
-    variable_list out(12);
-    if (!dy.defined() && !dh.defined()) return out;
-    const Tensor& x = s.x;
-    const c10::cuda::OptionalCUDAGuard guard(x.device());
-    if (x.numel() == 0) {
-      for (int i = 0; i < 8; ++i) out[i] = zeros_like_dense(v[i]);
-      out[8] = !s.h0.defined() ? Tensor() : dh.defined() ? dh : zeros_like_dense(s.h0);
-      return out;
-    }
-    dy = dy.defined() ? token(dy, "dy", x.sizes(), x.scalar_type(), x.get_device()) : at::zeros(x.sizes(), x.options());
-    if (dh.defined()) dh = dh.contiguous();
-    for (int i = 0; i < 9; ++i) out[i] = empty_like_dense(v[i]);
-    gdn_scan_bwd_args a = {};
-    a.fwd = scan_block(s);
-    a.fwd.ckpt = ptr_as<float>(v[10]);
-    a.dy = ptr(dy); a.sdy_b = dy.stride(0); a.sdy_t = dy.stride(1); a.dh_out = ptr_as<float>(dh);
-    a.dx = ptr(out[0]); a.ddt = ptr(out[1]); a.dA = ptr_as<float>(out[2]); a.dB = ptr(out[3]); a.dC = ptr(out[4]);
-    a.dDskip = ptr_as<float>(out[5]); a.dz = ptr(out[6]); a.ddt_bias = ptr_as<float>(out[7]); a.dh0 = ptr_as<float>(out[8]);
-    size_t need = 0;
-    check(gdn_scan_bwd_workspace_bytes(&a, &need));
-    const Tensor ws = workspace(need, x);
-    a.fwd.workspace = ptr(ws); a.fwd.workspace_bytes = need;
-    check(gdn_scan_bwd(&a, stream_of(x)));
+    const Tensor dy = g[0], dh = g.size() > 1 ? g[1] : Tensor();
+    if (!dy.defined() && !dh.defined()) return variable_list(12);
+    variable_list out = scan_backward({v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], ctx->saved_data["softplus"].toBool()}, v[10], dy, dh);
+    out.resize(12);
     return out;
   }
 };
@@ -380,14 +391,20 @@ ScanIn scan_inputs(const Tensor& x, const Tensor& dt, const Tensor& A, Tensor B,
   return s;
 }
 
+ScanIn scan_block_inputs(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Opt& D, const Opt& z,
+                         const Opt& dt_bias, bool softplus, const Opt& h0, const Opt& lengths) {
+  VALUE(x.dim() == 3, "x must be (B, T, D), got ", x.sizes());
+  ScanIn s = scan_inputs(x, dt, A, B, C, D, z, dt_bias, softplus);
+  const int64_t st[] = {x.size(0), x.size(2), s.A.size(1)};
+  s.h0 = dense(get(h0), "initial_state", st, at::kFloat, x.get_device());
+  s.lengths = row_lengths(lengths, x.size(0), x.size(1), x.get_device());
+  return s;
+}
+
 std::pair<Tensor, Opt> selective_scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Opt& D,
                                       const Opt& z, const Opt& dt_bias, bool dt_softplus, const Opt& initial_state, bool output_final_state,
                                       const Opt& lengths) {
-  VALUE(x.dim() == 3, "x must be (B, T, D), got ", x.sizes());
-  ScanIn s = scan_inputs(x, dt, A, B, C, D, z, dt_bias, dt_softplus);
-  const int64_t st[] = {x.size(0), x.size(2), s.A.size(1)};
-  s.h0 = dense(get(initial_state), "initial_state", st, at::kFloat, x.get_device());
-  s.lengths = row_lengths(lengths, x.size(0), x.size(1), x.get_device());
+  const ScanIn s = scan_block_inputs(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, lengths);
   Tensor y, h;
   if (wants_grad({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.h0})) {
     const variable_list r = ScanNode::apply(s.x, s.dt, s.A, s.B, s.C, opt(s.D), opt(s.z), opt(s.bias), opt(s.h0), opt(s.lengths),
@@ -440,6 +457,32 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
   return {y, pre};
 }
 
+// Gradients of x, the weight and the bias, those whose bit is set in `needs`.
+variable_list linear_backward(const Tensor& x, const Tensor& w, const Tensor& pre, Tensor dy, int act, int64_t needs) {
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  variable_list out(3);
+  auto make = [&](int i, at::IntArrayRef shape) {
+    if (needs >> i & 1) out[i] = M ? at::empty(shape, x.options()) : at::zeros(shape, x.options());
+  };
+  make(0, {M, K});
+  make(1, {N, K});
+  make(2, {N});
+  if (M == 0 || !(needs & 7)) return out;
+  if (dy.stride(-1) != 1) dy = dy.contiguous();
+  gdn_linear_bwd_args a = {};
+  a.x = ptr(x); a.weight = ptr(w); a.pre = ptr(pre); a.dy = ptr(dy);
+  a.dx = ptr(out[0]); a.dweight = ptr(out[1]); a.dbias = ptr(out[2]);
+  a.sx = x.stride(0); a.sw = w.stride(0); a.sdy = dy.stride(0);
+  a.M = M; a.N = N; a.K = K; a.act = act; a.keep = GDN_LINEAR_KEEP_SLOPE;
+  size_t need = 0;
+  check(gdn_linear_bwd_workspace_bytes(&a, &need));
+  const Tensor ws = workspace(need, x);
+  a.workspace = ptr(ws); a.workspace_bytes = need;
+  check(gdn_linear_bwd(&a, stream_of(x)));
+  return out;
+}
+
 struct LinearNode : torch::autograd::Function<LinearNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& bias0, const Opt& res0, int64_t act) {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -454,31 +497,13 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     first_order();
     const auto s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &pre = s[2];
-    Tensor dy = g[0];
+    const Tensor dy = g[0];
     variable_list out(5);
     if (!dy.defined()) return out;
-    const int64_t needs = ctx->saved_data["needs"].toInt(), M = x.size(0), K = x.size(1), N = w.size(0);
-    const c10::cuda::OptionalCUDAGuard guard(x.device());
-    auto make = [&](int i, at::IntArrayRef shape) {
-      if (needs >> i & 1) out[i] = M ? at::empty(shape, x.options()) : at::zeros(shape, x.options());
-    };
-    make(0, {M, K});
-    make(1, {N, K});
-    make(2, {N});
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    const variable_list made = linear_backward(s[0], s[1], s[2], dy, (int)ctx->saved_data["act"].toInt(), needs);
+    std::copy(made.begin(), made.end(), out.begin());
     if (needs & 8) out[3] = dy;
-    if (M == 0 || !(needs & 7)) return out;
-    if (dy.stride(-1) != 1) dy = dy.contiguous();
-    gdn_linear_bwd_args a = {};
-    a.x = ptr(x); a.weight = ptr(w); a.pre = ptr(pre); a.dy = ptr(dy);
-    a.dx = ptr(out[0]); a.dweight = ptr(out[1]); a.dbias = ptr(out[2]);
-    a.sx = x.stride(0); a.sw = w.stride(0); a.sdy = dy.stride(0);
-    a.M = M; a.N = N; a.K = K; a.act = (int)ctx->saved_data["act"].toInt(); a.keep = GDN_LINEAR_KEEP_SLOPE;
-    size_t need = 0;
-    check(gdn_linear_bwd_workspace_bytes(&a, &need));
-    const Tensor ws = workspace(need, x);
-    a.workspace = ptr(ws); a.workspace_bytes = need;
-    check(gdn_linear_bwd(&a, stream_of(x)));
     return out;
   }
 };
@@ -492,30 +517,92 @@ Tensor rows(const Tensor& t, const char* name, at::IntArrayRef shape, int64_t de
   return r.stride(-1) == 1 || shape.back() == 1 ? r : r.contiguous();
 }
 
-Tensor linear(const Tensor& x0, const Tensor& weight, const Opt& bias0, const std::optional<std::string>& activation, const Opt& residual0) {
+struct LinearIn {
+  Tensor x, w, bias, residual;
+};
+
+// x as (M, K) rows, the weight, the bias and the residual as (M, N) rows, checked.
+LinearIn linear_inputs(const Tensor& x0, const Tensor& weight, const Opt& bias0, const Opt& residual0) {
   VALUE(x0.is_cuda(), "archbench_b200 ops run on CUDA tensors only (no CPU path)");
   VALUE(x0.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x0.size(-1) && weight.numel() > 0, "x must be (..., K) and weight (N, K), got ",
         x0.sizes(), " and ", weight.sizes());
-  const int act = activation_code(activation, true);
   const int64_t device = x0.get_device(), N = weight.size(0), K = weight.size(1);
   c10::SmallVector<int64_t, 5> shape(x0.sizes().begin(), x0.sizes().end());
-  Tensor x, residual, bias = get(bias0);
+  LinearIn in;
   if (x0.numel() || x0.dim() == 2)
-    x = rows(x0, "x", shape, device);
+    in.x = rows(x0, "x", shape, device);
   else  // reshape cannot infer a row count of an empty tensor
-    x = rows(x0.reshape({0, K}), "x", {0, K}, device);
-  const Tensor w = rows(weight, "weight", weight.sizes(), device);
+    in.x = rows(x0.reshape({0, K}), "x", {0, K}, device);
+  in.w = rows(weight, "weight", weight.sizes(), device);
   shape.back() = N;
-  if (bias.defined()) {
+  in.bias = get(bias0);
+  if (in.bias.defined()) {
     const int64_t one[] = {N};
-    VALUE(bias.sizes() == at::IntArrayRef(one) && bias.scalar_type() == at::kBFloat16 && bias.is_cuda() && bias.get_device() == device,
+    VALUE(in.bias.sizes() == at::IntArrayRef(one) && in.bias.scalar_type() == at::kBFloat16 && in.bias.is_cuda() && in.bias.get_device() == device,
           "bias must be a bfloat16 (", N, ",) tensor on cuda:", device);
-    bias = bias.contiguous();
+    in.bias = in.bias.contiguous();
   }
-  if (residual0) residual = x.size(0) ? rows(*residual0, "residual", shape, device) : Tensor();
+  if (residual0) in.residual = in.x.size(0) ? rows(*residual0, "residual", shape, device) : Tensor();
+  return in;
+}
+
+Tensor linear(const Tensor& x0, const Tensor& weight, const Opt& bias0, const std::optional<std::string>& activation, const Opt& residual0) {
+  const LinearIn in = linear_inputs(x0, weight, bias0, residual0);
+  const auto& [x, w, bias, residual] = in;
+  const int act = activation_code(activation, true);
   Tensor y = wants_grad({x, w, bias, residual}) ? LinearNode::apply(x, w, opt(bias), opt(residual), (int64_t)act)
                                                 : linear_forward(x, w, bias, residual, act, false).first;
-  return x0.dim() == 2 ? y : y.reshape(shape);
+  if (x0.dim() == 2) return y;
+  c10::SmallVector<int64_t, 5> shape(x0.sizes().begin(), x0.sizes().end());
+  shape.back() = w.size(0);
+  return y.reshape(shape);
+}
+
+// ---- the same in parts, for the registered forms (traced_ops.py) -----------------------------
+
+std::vector<Opt> causal_conv_backward(const Tensor& x0, const Tensor& weight, const Opt& bias0, const std::optional<std::string>& activation,
+                                      const Opt& state0, const Opt& lengths0, const Opt& dy, const Opt& dlast) {
+  dtype_code(x0, "x");
+  VALUE(x0.dim() == 3, "x must be (B, T, C), got ", x0.sizes());
+  const int64_t device = x0.get_device(), B = x0.size(0), C = x0.size(2);
+  const Tensor x = token(x0, "x", x0.sizes(), x0.scalar_type(), device);
+  const auto [w, bias] = conv_params(weight, bias0, C, device);
+  const int64_t st[] = {B, C, w.size(1) - 1};
+  const Tensor state = dense(get(state0), "initial_state", st, x.scalar_type(), device);
+  const variable_list g = conv_backward(x, w, bias, state, row_lengths(lengths0, B, x.size(1), device), activation_code(activation, false), get(dy), get(dlast));
+  return {opt(g[0]), opt(g[1]), opt(g[2]), opt(g[3])};
+}
+
+// y, the final state and the states that the backward reads.
+std::vector<Opt> selective_scan_forward(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Opt& D,
+                                        const Opt& z, const Opt& dt_bias, bool softplus, const Opt& h0, bool want, const Opt& lengths, bool train) {
+  const ScanOut o = scan_forward(scan_block_inputs(x, dt, A, B, C, D, z, dt_bias, softplus, h0, lengths), want, train);
+  return {opt(o.y), opt(o.h), opt(o.ckpt)};
+}
+
+std::vector<Opt> selective_scan_backward(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Opt& D,
+                                         const Opt& z, const Opt& dt_bias, bool softplus, const Opt& h0, const Opt& lengths, const Tensor& ckpt,
+                                         const Opt& dy, const Opt& dh) {
+  std::vector<Opt> out;
+  for (const Tensor& g : scan_backward(scan_block_inputs(x, dt, A, B, C, D, z, dt_bias, softplus, h0, lengths), ckpt, get(dy), get(dh)))
+    out.push_back(opt(g));
+  return out;
+}
+
+// y (M, N) and what the backward reads of the activation, for x (M, K).
+std::vector<Opt> linear_forward_parts(const Tensor& x, const Tensor& weight, const Opt& bias, const std::optional<std::string>& activation,
+                                      const Opt& residual, bool train) {
+  const LinearIn in = linear_inputs(x, weight, bias, residual);
+  const auto [y, pre] = linear_forward(in.x, in.w, in.bias, in.residual, activation_code(activation, true), train);
+  return {opt(y), opt(pre)};
+}
+
+std::vector<Opt> linear_backward_parts(const Tensor& x, const Tensor& weight, const Opt& pre, const Tensor& dy,
+                                       const std::optional<std::string>& activation, int64_t needs) {
+  const LinearIn in = linear_inputs(x, weight, std::nullopt, std::nullopt);
+  const int64_t shape[] = {in.x.size(0), in.w.size(0)};
+  const variable_list g = linear_backward(in.x, in.w, get(pre), rows(dy, "dy", shape, x.get_device()), activation_code(activation, true), needs);
+  return {opt(g[0]), opt(g[1]), opt(g[2])};
 }
 
 }  // namespace
@@ -526,4 +613,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("selective_scan", &selective_scan);
   m.def("selective_scan_step", &selective_scan_step);
   m.def("linear", &linear);
+  m.def("causal_conv_backward", &causal_conv_backward);
+  m.def("selective_scan_forward", &selective_scan_forward);
+  m.def("selective_scan_backward", &selective_scan_backward);
+  m.def("linear_forward", &linear_forward_parts);
+  m.def("linear_backward", &linear_backward_parts);
 }

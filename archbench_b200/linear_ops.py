@@ -7,7 +7,7 @@ import ctypes
 
 from . import ssm_ops
 from .native import SYMBOLS
-from .ssm_ops import _P, _SZ, eager
+from .ssm_ops import _P, _SZ, traceable
 
 
 class LinearArgs(ctypes.Structure):
@@ -34,7 +34,7 @@ SYMBOLS.update({
 })
 
 
-@eager
+@traceable
 def linear(x, weight, bias=None, activation=None, residual=None):
     """y = act(x weight^T + bias) + residual, in one kernel where one tile pass serves it.
 

@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .layers import GDNCache, _put, _training
+from .ssm_ops import tracing
 
 
 def _linear(x, weight, bias=None, activation=None, residual=None):
@@ -92,9 +93,9 @@ class SelectiveSSM(nn.Module):
 
     def _parameters_f32(self, train: bool):
         """A, D and the step bias (None where ``dt_proj`` adds it itself) in fp32; kept between calls while the parameters are
-        unchanged, except in training."""
+        unchanged, except in training and where the call is traced."""
         bias = self.dt_proj.bias if _plain(self.dt_proj) else None
-        if train:
+        if train or tracing():
             return -torch.exp(self.A_log.float()), self.D.float(), None if bias is None else bias.float()
         return (ops._cached(self.A_log, "neg_exp", lambda t: -torch.exp(t.float())), ops._cached(self.D, "f32", lambda t: t.float()),
                 None if bias is None else ops._cached(bias, "f32", lambda t: t.float()))

@@ -11,7 +11,7 @@ causal convolution, the selective scan and their one-token forms.
 All are reachable as ``archbench_b200.ops.<name>``.  CUDA tensors only, bf16 or fp32 token tensors with any strides;
 states and sums are fp32.  Calls that need gradients run the backward kernels through autograd (first order;
 forward-mode tangents are refused).  Under
-``torch.compile`` the calls run eagerly between compiled regions.
+``torch.compile``, ``torch.export`` and ``torch.jit.trace`` they are registered operators (``traced_ops``).
 
 The calls themselves -- checks, allocation, autograd nodes -- are compiled (``csrc/torch_ops.cpp``, the extension module
 ``_torch_ops``); the ctypes structures here mirror the C ABI's argument blocks for callers that drive it directly."""
@@ -90,19 +90,24 @@ def extension():
     return _EXT
 
 
-def eager(fn):
-    """Run ``fn`` between compiled regions under ``torch.compile``; a plain call elsewhere (a bare
-    ``torch.compiler.disable`` costs each call 1.5 us)."""
-    disabled = torch.compiler.disable(fn)
+def tracing() -> bool:
+    """Under ``torch.compile``, ``torch.export`` or ``torch.jit.trace``."""
+    return torch.compiler.is_compiling() or torch.jit.is_tracing()
+
+
+def traceable(fn):
+    """``fn`` itself in plain calls, its namesake among the registered operators (``traced_ops``) where a call is traced."""
 
     @functools.wraps(fn)
     def call(*args, **kwargs):
-        return disabled(*args, **kwargs) if torch.compiler.is_compiling() else fn(*args, **kwargs)
+        if tracing():
+            return getattr(traced_ops, fn.__name__)(*args, **kwargs)
+        return fn(*args, **kwargs)
 
     return call
 
 
-@eager
+@traceable
 def causal_conv(x, weight, bias=None, activation=None, initial_state=None, output_final_state=False, lengths=None):
     """Depthwise causal convolution: y_t = act(bias + sum_w weight[:, w] x_{t-W+1+w}).
 
@@ -112,14 +117,14 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, outpu
     return (_EXT or extension()).causal_conv(x, weight, bias, activation, initial_state, output_final_state, lengths)
 
 
-@eager
+@traceable
 def causal_conv_step(x, weight, state, bias=None, activation=None):
     """One token of ``causal_conv``: x (B, C), state (B, C, W - 1) contiguous, in x's dtype, advanced in place.  No
     gradient: a backward through its output raises, and a state that requires one is refused."""
     return (_EXT or extension()).causal_conv_step(x, weight, state, bias, activation)
 
 
-@eager
+@traceable
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None, output_final_state=False,
                    lengths=None):
     """Selective state space scan over a block of tokens.
@@ -134,8 +139,11 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     return (_EXT or extension()).selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, lengths)
 
 
-@eager
+@traceable
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False):
     """One token of ``selective_scan``: x, dt, z (B, D), B, C (B, N) or (B, G, N), state (B, D, N) fp32 contiguous,
     advanced in place.  No gradient, as for ``causal_conv_step``."""
     return (_EXT or extension()).selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
+
+
+from . import traced_ops  # noqa: E402  (which calls this module's extension)
