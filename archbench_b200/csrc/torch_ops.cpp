@@ -526,13 +526,10 @@ LinearIn linear_inputs(const Tensor& x0, const Tensor& weight, const Opt& bias0,
   VALUE(x0.is_cuda(), "archbench_b200 ops run on CUDA tensors only (no CPU path)");
   VALUE(x0.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x0.size(-1) && weight.numel() > 0, "x must be (..., K) and weight (N, K), got ",
         x0.sizes(), " and ", weight.sizes());
-  const int64_t device = x0.get_device(), N = weight.size(0), K = weight.size(1);
+  const int64_t device = x0.get_device(), N = weight.size(0);
   c10::SmallVector<int64_t, 5> shape(x0.sizes().begin(), x0.sizes().end());
   LinearIn in;
-  if (x0.numel() || x0.dim() == 2)
-    in.x = rows(x0, "x", shape, device);
-  else  // reshape cannot infer a row count of an empty tensor
-    in.x = rows(x0.reshape({0, K}), "x", {0, K}, device);
+  in.x = rows(x0, "x", shape, device);
   in.w = rows(weight, "weight", weight.sizes(), device);
   shape.back() = N;
   in.bias = get(bias0);
@@ -542,7 +539,7 @@ LinearIn linear_inputs(const Tensor& x0, const Tensor& weight, const Opt& bias0,
           "bias must be a bfloat16 (", N, ",) tensor on cuda:", device);
     in.bias = in.bias.contiguous();
   }
-  if (residual0) in.residual = in.x.size(0) ? rows(*residual0, "residual", shape, device) : Tensor();
+  if (residual0) in.residual = rows(*residual0, "residual", shape, device);
   return in;
 }
 
