@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(256) split_epilogue_kernel(const GemmP p) {
   }
 }
 
-// Few rows (M <= 16 MT): the weight is streamed once, straight into MMA fragments.  A block owns 8 columns of y and its
+// Few rows (M <= 16 MT; use_few): the weight is streamed once, straight into MMA fragments.  A block owns 8 columns of y and its
 // 8 warps share the contraction; lane (g, q) reads 8 consecutive k of weight row g and of x rows g, g + 8 and the
 // fragments take them in that order -- the contraction runs over the same permuted k on both sides.  The warps' sums
 // are added in order in shared memory.
@@ -1004,11 +1004,29 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
   return ssm::launched();
 }
 
-constexpr int64_t FEW_ROWS = 64;
+// Vector loads of the few-rows kernel.
+bool few_vec(const Operand& a, const Operand& b) { return a.tma && b.tma && a.cols % 8 == 0; }
+
+// Where the few-rows kernel is the faster one.  It needs one launch and no tiles, but each of its warps walks an eighth of the
+// contraction (12.5 us for 4096 values at 16 rows) and every 8 columns read all of x again.  Few rows / tiles in us, device
+// time, weights out of HBM (N x K, aligned):
+//   16 rows: 1024 x 1024 3.1 / 7.2, 1024 x 2816 9.6 / 9.7, 1024 x 3584 11.4 / 10.1, 256 x 8192 22.5 / 10.1,
+//            12288 x 2048 15.5 / 19.1, 16384 x 1024 12.9 / 12.2, 32768 x 1024 21.0 / 18.1
+//   32 rows: 2048 x 2048 9.8 / 11.1, 4096 x 2048 10.1 / 11.1, 6144 x 1024 10.9 / 9.2, 1024 x 2560 12.1 / 8.8
+//   64 rows: 1024 x 1024 4.9 / 7.2, 2048 x 2048 11.9 / 11.1, 2560 x 1024 12.1 / 7.9, 1024 x 2560 14.2 / 12.6, 4096 x 4096 38.9 / 17.6
+// Rows that no vector takes (the tiles then wait for their aligned copies, the few-rows kernel loads single values):
+//   16 rows: 1001 x 2047 13.6 / 14.8, 8191 x 513 10.7 / 15.8; 32 rows: 501 x 999 10.5 / 11.0, 2047 x 1001 13.2 / 12.2,
+//            1001 x 2047 21.8 / 15.5; 64 rows: 501 x 999 19.5 / 11.2, 8191 x 513 27.6 / 15.9
+bool use_few(int64_t M, int64_t N, const Operand& a, const Operand& b) {
+  if (M > 64) return false;
+  const int64_t tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;  // of 16 rows
+  const int64_t most_k = !few_vec(a, b) ? 2048 / tiles : tiles == 1 ? 2816 : 2048;
+  return a.cols <= most_k && N <= (tiles == 1 ? 16384 : 8192 / tiles);
+}
 
 int launch_few(const GemmP& p, cudaStream_t s) {
   const unsigned g = (unsigned)((p.N + 7) / 8);
-  const bool v = p.a.tma && p.b.tma && p.K % 8 == 0;
+  const bool v = few_vec(p.a, p.b);
   if (p.M <= 16)
     v ? few_rows_kernel<1, true><<<g, 256, 0, s>>>(p) : few_rows_kernel<1, false><<<g, 256, 0, s>>>(p);
   else if (p.M <= 32)
@@ -1072,9 +1090,8 @@ int gdn_linear_workspace_bytes(const gdn_linear_args* a, size_t* bytes) {
   if (!a || !bytes) return GDN_ERR_NULL;
   const int st = check_sizes(a->M, a->N, a->K, a->act, a->keep);
   if (st != GDN_OK) return st;
-  *bytes = a->M <= FEW_ROWS ? 0
-                            : plan(a->M, a->N, a->K).part + align_bytes(operand(a->x, a->sx, a->M, a->K)) +
-                                  align_bytes(operand(a->weight, a->sw, a->N, a->K));
+  const Operand x = operand(a->x, a->sx, a->M, a->K), w = operand(a->weight, a->sw, a->N, a->K);
+  *bytes = a->M == 0 || use_few(a->M, a->N, x, w) ? 0 : plan(a->M, a->N, a->K).part + align_bytes(x) + align_bytes(w);
   return GDN_OK;
 }
 
@@ -1097,7 +1114,7 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
   p.act = a->act;
   p.slope = a->keep == GDN_LINEAR_KEEP_SLOPE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.M <= FEW_ROWS) return launch_few(p, s);
+  if (use_few(p.M, p.N, p.a, p.b)) return launch_few(p, s);
   char* ws = static_cast<char*>(a->workspace);
   st = align_operands(&p.a, &p.b, ws, s);
   return st == GDN_OK ? gemm<false, false>(p, ws, s) : st;
