@@ -87,14 +87,16 @@ Tensor row_lengths(const Opt& lengths, int64_t B, int64_t T, int64_t device) {
   return n.to(at::kInt).contiguous();
 }
 
-bool wants_grad(std::initializer_list<Tensor> ts) {
-  for (const Tensor& t : ts)  // the kernels would drop a tangent
-    if (t.defined() && C10_UNLIKELY(t._fw_grad(/*level=*/0).defined()))
+// The first of `ts` (absent ones among them) that wants a gradient, or NULL.
+using Tensors = std::initializer_list<const Tensor*>;
+const Tensor* wants_grad(Tensors ts) {
+  for (const Tensor* t : ts)  // the kernels would drop a tangent
+    if (t->defined() && C10_UNLIKELY(t->_fw_grad(/*level=*/0).defined()))
       C10_THROW_ERROR(NotImplementedError, "the kernels have no forward-mode derivative");
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor& t : ts)
-    if (t.defined() && t.requires_grad()) return true;
-  return false;
+  if (!at::GradMode::is_enabled()) return nullptr;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return t;
+  return nullptr;
 }
 
 // A kernel wrote `t` in place: a graph that keeps the old values refuses its backward.  (Tensors of inference mode are in no
@@ -115,11 +117,10 @@ struct OneTokenNode : torch::autograd::Function<OneTokenNode> {
   }
 };
 template <typename F>
-Tensor one_token(std::initializer_list<Tensor> inputs, const Tensor& state, const F& run) {
-  VALUE(!wants_grad({state}), "state is updated in place and must not require a gradient: detach it");
-  for (const Tensor& t : inputs)
-    if (wants_grad({t})) return OneTokenNode::apply(t, std::function<Tensor()>(run));
-  return run();
+Tensor one_token(Tensors inputs, const Tensor& state, const F& run) {
+  VALUE(!wants_grad({&state}), "state is updated in place and must not require a gradient: detach it");
+  const Tensor* source = wants_grad(inputs);
+  return source ? OneTokenNode::apply(*source, std::function<Tensor()>(run)) : run();
 }
 
 int activation_code(const std::optional<std::string>& a, bool gelu) {
@@ -230,7 +231,7 @@ std::pair<Tensor, Opt> causal_conv(const Tensor& x0, const Tensor& weight, const
   const int64_t st[] = {B, C, w.size(1) - 1};
   const Tensor state = dense(get(initial_state), "initial_state", st, x.scalar_type(), device), lengths = row_lengths(lengths0, B, x.size(1), device);
   Tensor y, last;
-  if (wants_grad({x, w, bias, state})) {
+  if (wants_grad({&x, &w, &bias, &state})) {
     const variable_list r = ConvNode::apply(x, w, opt(bias), opt(state), opt(lengths), (int64_t)act, output_final_state);
     y = r[0];
     if (output_final_state) last = r[1];
@@ -250,7 +251,7 @@ Tensor causal_conv_step(const Tensor& x0, const Tensor& weight, const Tensor& st
   const int64_t st[] = {B, C, w.size(1) - 1};
   VALUE(state.sizes() == at::IntArrayRef(st) && state.scalar_type() == x.scalar_type() && state.is_contiguous() && state.device() == x.device(),
         "state must be a contiguous ", at::IntArrayRef(st), " ", x.scalar_type(), " tensor on ", x.device(), ": it is updated in place");
-  return one_token({x, w, bias}, state, [&, &w = w, &bias = bias] {
+  return one_token({&x, &w, &bias}, state, [&, &w = w, &bias = bias] {
     const c10::cuda::OptionalCUDAGuard guard(x.device());
     const Tensor y = at::empty({B, C}, x.options());
     gdn_conv_args a = conv_block(x, w, bias, state, act, Tensor());
@@ -406,7 +407,7 @@ std::pair<Tensor, Opt> selective_scan(const Tensor& x, const Tensor& dt, const T
                                       const Opt& lengths) {
   const ScanIn s = scan_block_inputs(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, lengths);
   Tensor y, h;
-  if (wants_grad({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.h0})) {
+  if (wants_grad({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.D, &s.z, &s.bias, &s.h0})) {
     const variable_list r = ScanNode::apply(s.x, s.dt, s.A, s.B, s.C, opt(s.D), opt(s.z), opt(s.bias), opt(s.h0), opt(s.lengths),
                                              dt_softplus, output_final_state);
     y = r[0];
@@ -426,7 +427,7 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& A, c
   const int64_t st[] = {x.size(0), x.size(1), s.A.size(1)};
   VALUE(state.sizes() == at::IntArrayRef(st) && state.scalar_type() == at::kFloat && state.is_contiguous() && state.device() == x.device(),
         "state must be a contiguous ", at::IntArrayRef(st), " float32 tensor on ", x.device(), ": it is updated in place");
-  return one_token({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias}, state, [&] {
+  return one_token({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.D, &s.z, &s.bias}, state, [&] {
     const c10::cuda::OptionalCUDAGuard guard(x.device());
     const Tensor y = at::empty(x.sizes(), x.options());
     gdn_scan_args a = scan_block(s);
@@ -547,7 +548,7 @@ Tensor linear(const Tensor& x0, const Tensor& weight, const Opt& bias0, const st
   const LinearIn in = linear_inputs(x0, weight, bias0, residual0);
   const auto& [x, w, bias, residual] = in;
   const int act = activation_code(activation, true);
-  Tensor y = wants_grad({x, w, bias, residual}) ? LinearNode::apply(x, w, opt(bias), opt(residual), (int64_t)act)
+  Tensor y = wants_grad({&x, &w, &bias, &residual}) ? LinearNode::apply(x, w, opt(bias), opt(residual), (int64_t)act)
                                                 : linear_forward(x, w, bias, residual, act, false).first;
   if (x0.dim() == 2) return y;
   c10::SmallVector<int64_t, 5> shape(x0.sizes().begin(), x0.sizes().end());
