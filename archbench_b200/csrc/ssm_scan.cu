@@ -12,15 +12,14 @@ namespace ssm {
 constexpr int TT = 32;  // tokens per tile of the local pass; segments are whole tiles
 
 // One (row, channel block, segment) per block of 128 threads.  Each tile is staged by the threads in their
-// per-token role (CV channels of some tokens): raw values of the next tile are already in registers while this one is
+// per-token role (a channel of some tokens): raw values of the next tile are already in registers while this one is
 // computed, so no load is waited for.  In their per-state role the threads read (s, s, s x, s x) of their channel and
 // the B and C of their four states, and leave their part of C . h in shared memory; the per-token role adds the parts.
 template <typename T, int NL>
 __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p) {
-  constexpr int CV = 1;  // channels per thread and token
   constexpr int TT = NL == 2 ? 16 : 32;  // tokens per tile (shared memory)
   constexpr int CH = SCAN_THREADS / NL, NP = NL * SPL;
-  constexpr int TSTEP = SCAN_THREADS * CV / CH, PER = TT / TSTEP;  // tokens covered at once, tokens per thread
+  constexpr int TSTEP = SCAN_THREADS / CH, PER = TT / TSTEP;  // tokens covered at once, tokens per thread
   constexpr int QUADS = TT * NL / SCAN_THREADS > 0 ? TT * NL / SCAN_THREADS : 1;
   __shared__ __align__(16) float4 sS[TT][CH];
   __shared__ __align__(16) float sY[TT][SCAN_THREADS];
@@ -52,16 +51,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
       A2[i] = pack2(av[2 * i], av[2 * i + 1]);
     }
   }
-  // per-token role: channels cc .. cc + CV, tokens ct0, ct0 + TSTEP, ...
-  const int cc = tid % (CH / CV) * CV, ct0 = tid / (CH / CV);
-  const bool cok = cc < nch;  // CV divides nch
+  // per-token role: channel cc, tokens ct0, ct0 + TSTEP, ...
+  const int cc = tid % CH, ct0 = tid / CH;
+  const bool cok = cc < nch;
   const int d = d0 + (cok ? cc : 0);
-  float bias[CV], skip[CV];
-#pragma unroll
-  for (int k = 0; k < CV; ++k) {
-    bias[k] = p.dt_bias ? p.dt_bias[d + k] : 0.f;
-    skip[k] = p.Dskip ? p.Dskip[d + k] : 0.f;
-  }
+  const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.Dskip ? p.Dskip[d] : 0.f;
   const T* xp = static_cast<const T*>(p.x) + b * p.sx_b + d;
   const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt_b + d;
   const T* zp = p.z ? static_cast<const T*>(p.z) + b * p.sz_b + d : nullptr;
@@ -70,15 +64,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
   const T* Cp = static_cast<const T*>(p.Cm) + b * p.sC_b + grp * p.sC_g;
   const int nck = (p.T + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT;
 
-  Raw<T, CV> xr[PER], dr[PER], zr[PER];
+  T xr[PER], dr[PER], zr[PER];
   Quad<T> qb[QUADS], qc[QUADS];
   auto fetch = [&](int t0) {  // places past the row's tokens read its last one; their values are dropped
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int64_t t = min(t0 + ct0 + i * TSTEP, lim - 1);
-      xr[i] = load_raw<T, CV>(xp + t * p.sx_t);
-      dr[i] = load_raw<T, CV>(dtp + t * p.sdt_t);
-      if (zp) zr[i] = load_raw<T, CV>(zp + t * p.sz_t);
+      xr[i] = xp[t * p.sx_t];
+      dr[i] = dtp[t * p.sdt_t];
+      if (zp) zr[i] = zp[t * p.sz_t];
     }
 #pragma unroll
     for (int i = 0; i < QUADS; ++i) {
@@ -93,21 +87,18 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
   if (tbeg < lim) fetch(tbeg);
   int t0 = tbeg;
   for (; t0 < lim; t0 += TT) {
-    float x[PER][CV], z[PER][CV];
+    float x[PER], z[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = ct0 + i * TSTEP;
       const bool on = t0 + r < lim;
-#pragma unroll
-      for (int k = 0; k < CV; ++k) {
-        float s = to_f32(dr[i].v[k]) + bias[k];
-        if (p.softplus) s = softplus(s);
-        s = on ? s : 0.f;
-        x[i][k] = to_f32(xr[i].v[k]);
-        z[i][k] = zp ? to_f32(zr[i].v[k]) : 0.f;
-        const float u = on ? s * x[i][k] : 0.f;
-        sS[r][cc + k] = make_float4(s, s, u, u);
-      }
+      float s = to_f32(dr[i]) + bias;
+      if (p.softplus) s = softplus(s);
+      s = on ? s : 0.f;
+      x[i] = to_f32(xr[i]);
+      z[i] = zp ? to_f32(zr[i]) : 0.f;
+      const float u = on ? s * x[i] : 0.f;
+      sS[r][cc] = make_float4(s, s, u, u);
     }
 #pragma unroll
     for (int i = 0; i < QUADS; ++i) {
@@ -151,28 +142,22 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
     for (int i = 0; i < PER; ++i) {
       const int r = ct0 + i * TSTEP, t = t0 + r;
       if (!cok || t >= tend) continue;
-      float o[CV];
+      float y = 0.f;
+      const float* part = &sY[r][cc * NL];
 #pragma unroll
-      for (int k = 0; k < CV; ++k) {
-        float y = 0.f;
-        const float* part = &sY[r][(cc + k) * NL];
-#pragma unroll
-        for (int j = 0; j < NL; j += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(part + j);
-          y += v.x + v.y;
-        }
-        y = fmaf(skip[k], x[i][k], y);
-        if (zp) y *= silu(z[i][k]);
-        o[k] = t < lim ? y : 0.f;
+      for (int j = 0; j < NL; j += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(part + j);
+        y += v.x + v.y;
       }
-      store_raw<T, CV>(yp + t * p.sy_t, o);
+      y = fmaf(skip, x[i], y);
+      if (zp) y *= silu(z[i]);
+      store_as(yp + t * p.sy_t, t < lim ? y : 0.f);
     }
     // sS, sB and sC are rewritten only after every thread passed the barrier above; sY only after the next one
   }
   // past the row's tokens
-  const float zero[CV] = {};
   for (int t = t0 + ct0; t < tend; t += TSTEP)
-    if (cok) store_raw<T, CV>(yp + (int64_t)t * p.sy_t, zero);
+    if (cok) store_as(yp + (int64_t)t * p.sy_t, 0.f);
   if (p.h_out && seg == p.nseg - 1 && live) {
     const float2 lo = unpack2(h[0]), hi = unpack2(h[1]);
     const float hv[SPL] = {lo.x, lo.y, hi.x, hi.y};
@@ -306,7 +291,7 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
   const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], two ? p.Dskip[d + 1] : 0.f) : both(0.f);
   auto put_pair = [&](T* q, const float (&v)[2]) {
     if (p.pairs_out) {
-      store_raw<T, 2>(q, v);
+      store_pair(q, v);
     } else {
       store_as(q, v[0]);
       if (two) store_as(q + 1, v[1]);

@@ -40,29 +40,17 @@ struct ScanP {
   int pairs_out;      // rows of y (or dx, ddt, dz) take stores of channel pairs
 };
 
-// CV consecutive values of type T in one register image (CV = 2: one 4- or 8-byte load).
-template <typename T, int CV>
-struct Raw {
-  T v[CV];
+// Two neighbouring values in one store.
+template <typename T>
+struct __align__(2 * sizeof(T)) Pair {
+  T v[2];
 };
-template <>
-struct __align__(4) Raw<__nv_bfloat16, 2> {
-  __nv_bfloat16 v[2];
-};
-template <>
-struct __align__(8) Raw<float, 2> {
-  float v[2];
-};
-template <typename T, int CV>
-__device__ __forceinline__ Raw<T, CV> load_raw(const T* p) {
-  return *reinterpret_cast<const Raw<T, CV>*>(p);
-}
-template <typename T, int CV>
-__device__ __forceinline__ void store_raw(T* p, const float (&f)[CV]) {
-  Raw<T, CV> r;
-#pragma unroll
-  for (int i = 0; i < CV; ++i) store_as(&r.v[i], f[i]);
-  *reinterpret_cast<Raw<T, CV>*>(p) = r;
+template <typename T>
+__device__ __forceinline__ void store_pair(T* p, const float (&f)[2]) {
+  Pair<T> r;
+  store_as(&r.v[0], f[0]);
+  store_as(&r.v[1], f[1]);
+  *reinterpret_cast<Pair<T>*>(p) = r;
 }
 
 // Four consecutive states of B or C at one token: one load where rows allow, else one by one, zeros past N.

@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   const f32x2 skip = p.Dskip ? pack2(p.Dskip[d], two ? p.Dskip[d + 1] : 0.f) : both(0.f);
   auto put_pair = [&](T* q, const float (&v)[2]) {
     if (p.pairs_out) {
-      store_raw<T, 2>(q, v);
+      store_pair(q, v);
     } else {
       store_as(q, v[0]);
       if (two) store_as(q + 1, v[1]);
