@@ -8,8 +8,8 @@ causal convolution, the selective scan and their one-token forms.
                  output_final_state=False, lengths=None) -> (y, final_state | None)
   selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False) -> y  (state in place)
 
-All are reachable as ``archbench_b200.ops.<name>``.  CUDA tensors only, bf16 or fp32 token tensors with any strides;
-states and sums are fp32.  Calls that need gradients run the backward kernels through autograd (first order;
+All are reachable as ``archbench_b200.ops.<name>``.  CUDA tensors only, bf16 or fp32 token tensors with any strides, all of
+one call in x's dtype (others are converted to it); the scan's state and all sums are fp32.  Calls that need gradients run the backward kernels through autograd (first order;
 forward-mode tangents are refused).  Under
 ``torch.compile``, ``torch.export`` and ``torch.jit.trace`` they are registered operators (``traced_ops``).
 
