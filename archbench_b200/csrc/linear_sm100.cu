@@ -1013,7 +1013,8 @@ bool few_vec(const Operand& a, const Operand& b) { return a.tma && b.tma && a.co
 //   16 rows: 1024 x 1024 3.1 / 7.2, 1024 x 2816 9.6 / 9.7, 1024 x 3584 11.4 / 10.1, 256 x 8192 22.5 / 10.1,
 //            12288 x 2048 15.5 / 19.1, 16384 x 1024 12.9 / 12.2, 32768 x 1024 21.0 / 18.1
 //   32 rows: 2048 x 2048 9.8 / 11.1, 4096 x 2048 10.1 / 11.1, 6144 x 1024 10.9 / 9.2, 1024 x 2560 12.1 / 8.8
-//   64 rows: 1024 x 1024 4.9 / 7.2, 2048 x 2048 11.9 / 11.1, 2560 x 1024 12.1 / 7.9, 1024 x 2560 14.2 / 12.6, 4096 x 4096 38.9 / 17.6
+//   64 rows: 1024 x 1024 4.9 / 7.2, 1024 x 1536 8.1 / 9.1, 768 x 2048 9.9 / 10.7, 2048 x 2048 11.9 / 11.1 (16.3 / 11.1 with x out of
+//            HBM too, 1024 x 2048 15.7 / 11.0), 2560 x 1024 12.1 / 7.9, 1024 x 2560 14.2 / 12.6, 4096 x 4096 38.9 / 17.6
 // Rows that no vector takes (the tiles then wait for their aligned copies, the few-rows kernel loads single values):
 //   16 rows: 1001 x 2047 13.6 / 14.8, 8191 x 513 10.7 / 15.8; 32 rows: 501 x 999 10.5 / 11.0, 2047 x 1001 13.2 / 12.2,
 //            1001 x 2047 21.8 / 15.5; 64 rows: 501 x 999 19.5 / 11.2, 8191 x 513 27.6 / 15.9
@@ -1021,7 +1022,7 @@ bool use_few(int64_t M, int64_t N, const Operand& a, const Operand& b) {
   if (M > 64) return false;
   const int64_t tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;  // of 16 rows
   const int64_t most_k = !few_vec(a, b) ? 2048 / tiles : tiles == 1 ? 2816 : 2048;
-  return a.cols <= most_k && N <= (tiles == 1 ? 16384 : 8192 / tiles);
+  return a.cols <= most_k && N <= (tiles == 1 ? 16384 : 8192 / tiles) && (tiles < 4 || N * a.cols <= 3 << 19);
 }
 
 int launch_few(const GemmP& p, cudaStream_t s) {
