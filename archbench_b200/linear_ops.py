@@ -5,9 +5,9 @@ from __future__ import annotations
 
 import ctypes
 
-from . import ssm_ops
+from . import ssm_ops, traced_ops
 from .native import SYMBOLS
-from .ssm_ops import _P, _SZ, traceable
+from .ssm_ops import _P, _SZ, _is_compiling, _is_tracing
 
 
 class LinearArgs(ctypes.Structure):
@@ -34,11 +34,11 @@ SYMBOLS.update({
 })
 
 
-@traceable
 def linear(x, weight, bias=None, activation=None, residual=None):
     """y = act(x weight^T + bias) + residual, in one kernel where one tile pass serves it.
 
     x (..., K), weight (N, K), bias (N), residual (..., N), all bf16 with any strides; activation None, "silu" or "gelu"
     (the erf form).  fp32 accumulation and epilogue, one rounding at the end.  Differentiable in x, weight, bias and
     residual; with an activation, training keeps its slope at x weight^T + bias in fp16."""
-    return (ssm_ops._EXT or ssm_ops.extension()).linear(x, weight, bias, activation, residual)
+    m = traced_ops if _is_compiling() or _is_tracing() else ssm_ops._EXT or ssm_ops.extension()
+    return m.linear(x, weight, bias, activation, residual)

@@ -19,7 +19,6 @@ The calls themselves -- checks, allocation, autograd nodes -- are compiled (``cs
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 
 import torch
@@ -99,36 +98,26 @@ def tracing() -> bool:
     return _is_compiling() or _is_tracing()
 
 
-def traceable(fn):
-    """``fn`` itself in plain calls, its namesake among the registered operators (``traced_ops``) where a call is traced."""
-
-    @functools.wraps(fn)
-    def call(*args, **kwargs):
-        if _is_compiling() or _is_tracing():
-            return getattr(traced_ops, fn.__name__)(*args, **kwargs)
-        return fn(*args, **kwargs)
-
-    return call
+# The functions below call the extension, or where a call is traced their namesakes among the registered operators.
 
 
-@traceable
 def causal_conv(x, weight, bias=None, activation=None, initial_state=None, output_final_state=False, lengths=None):
     """Depthwise causal convolution: y_t = act(bias + sum_w weight[:, w] x_{t-W+1+w}).
 
     x (B, T, C); weight (C, W) or (C, 1, W), W 2 to 4; bias (C); activation None or "silu"; initial_state (B, C, W - 1),
     the inputs before the first token (zeros if None); lengths (B): tokens of each right-padded row (y is 0 past them).
     Returns (y, final_state or None), final_state the last W - 1 inputs, in x's dtype."""
-    return (_EXT or extension()).causal_conv(x, weight, bias, activation, initial_state, output_final_state, lengths)
+    m = traced_ops if _is_compiling() or _is_tracing() else _EXT or extension()
+    return m.causal_conv(x, weight, bias, activation, initial_state, output_final_state, lengths)
 
 
-@traceable
 def causal_conv_step(x, weight, state, bias=None, activation=None):
     """One token of ``causal_conv``: x (B, C), state (B, C, W - 1) contiguous, in x's dtype, advanced in place.  No
     gradient: a backward through its output raises, and a state that requires one is refused."""
-    return (_EXT or extension()).causal_conv_step(x, weight, state, bias, activation)
+    m = traced_ops if _is_compiling() or _is_tracing() else _EXT or extension()
+    return m.causal_conv_step(x, weight, state, bias, activation)
 
 
-@traceable
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None, output_final_state=False,
                    lengths=None):
     """Selective state space scan over a block of tokens.
@@ -140,14 +129,15 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     channels; D, dt_bias (D); initial_state (B, D, N) fp32 (zeros if None); lengths (B): tokens of each right-padded row, int32
     for no conversion (past them y is 0 and the state stays).  N <= 64.  Returns (y, final_state or None): y in x's dtype, the state fp32.
     Training keeps one state per 8 tokens."""
-    return (_EXT or extension()).selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, lengths)
+    m = traced_ops if _is_compiling() or _is_tracing() else _EXT or extension()
+    return m.selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, lengths)
 
 
-@traceable
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False):
     """One token of ``selective_scan``: x, dt, z (B, D), B, C (B, N) or (B, G, N), state (B, D, N) fp32 contiguous,
     advanced in place.  No gradient, as for ``causal_conv_step``."""
-    return (_EXT or extension()).selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
+    m = traced_ops if _is_compiling() or _is_tracing() else _EXT or extension()
+    return m.selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
 
 
 from . import traced_ops  # noqa: E402  (which calls this module's extension)
