@@ -1007,22 +1007,25 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
 // Vector loads of the few-rows kernel.
 bool few_vec(const Operand& a, const Operand& b) { return a.tma && b.tma && a.cols % 8 == 0; }
 
-// Where the few-rows kernel is the faster one.  It needs one launch and no tiles, but each of its warps walks an eighth of the
-// contraction (12.5 us for 4096 values at 16 rows) and every 8 columns read all of x again.  Few rows / tiles in us, device
-// time, weights out of HBM (N x K, aligned):
-//   16 rows: 1024 x 1024 3.1 / 7.2, 1024 x 2816 9.6 / 9.7, 1024 x 3584 11.4 / 10.1, 256 x 8192 22.5 / 10.1,
-//            12288 x 2048 15.5 / 19.1, 16384 x 1024 12.9 / 12.2, 32768 x 1024 21.0 / 18.1
-//   32 rows: 2048 x 2048 9.8 / 11.1, 4096 x 2048 10.1 / 11.1, 6144 x 1024 10.9 / 9.2, 1024 x 2560 12.1 / 8.8
-//   64 rows: 1024 x 1024 4.9 / 7.2, 1024 x 1536 8.1 / 9.1, 768 x 2048 9.9 / 10.7, 2048 x 2048 11.9 / 11.1 (16.3 / 11.1 with x out of
-//            HBM too, 1024 x 2048 15.7 / 11.0), 2560 x 1024 12.1 / 7.9, 1024 x 2560 14.2 / 12.6, 4096 x 4096 38.9 / 17.6
+// Where the few-rows kernel serves.  It needs one launch, no tensor maps and no workspace, which saves the host about 5 us a call,
+// but each of its warps walks an eighth of the contraction (12.5 us for 4096 values at 16 rows) and every 8 columns read all of x
+// again.  So the tiles take over where they save some 3 us on the device.  Few rows / tiles in us there, weights out of HBM, x in
+// L2 (N x K, aligned):
+//   16 rows: 1024 x 1024 3.1 / 7.2, 1024 x 2816 9.6 / 9.7, 1024 x 4096 12.7 / 10.4, 4096 x 4096 13.8 / 13.1, 256 x 8192 22.5 / 10.1,
+//            12288 x 2048 15.5 / 19.1, 32768 x 1024 21.0 / 18.1, 50304 x 1024 31.1 / 27.3
+//   32 rows: 2048 x 2048 9.8 / 11.1, 4096 x 2048 10.1 / 11.1, 8192 x 1024 11.5 / 10.0, 8192 x 2048 19.4 / 11.5, 1024 x 2560 12.1 / 8.8
+//            (14.7 / 8.7 with x out of HBM too)
+//   64 rows: 1024 x 1024 4.9 / 7.2, 1024 x 1536 8.1 / 9.1, 768 x 2048 9.9 / 10.7, 1024 x 2048 11.5 / 11.0 (x out of HBM: 15.7 / 11.0),
+//            2560 x 1024 12.1 / 7.9, 4096 x 4096 38.9 / 17.6
 // Rows that no vector takes (the tiles then wait for their aligned copies, the few-rows kernel loads single values):
-//   16 rows: 1001 x 2047 13.6 / 14.8, 8191 x 513 10.7 / 15.8; 32 rows: 501 x 999 10.5 / 11.0, 2047 x 1001 13.2 / 12.2,
+//   16 rows: 1001 x 2047 13.6 / 14.8, 8191 x 513 10.7 / 15.8; 32 rows: 501 x 999 10.5 / 11.0, 4095 x 1023 17.0 / 14.2,
 //            1001 x 2047 21.8 / 15.5; 64 rows: 501 x 999 19.5 / 11.2, 8191 x 513 27.6 / 15.9
 bool use_few(int64_t M, int64_t N, const Operand& a, const Operand& b) {
-  if (M > 64) return false;
-  const int64_t tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;  // of 16 rows
-  const int64_t most_k = !few_vec(a, b) ? 2048 / tiles : tiles == 1 ? 2816 : 2048;
-  return a.cols <= most_k && N <= (tiles == 1 ? 16384 : 8192 / tiles) && (tiles < 4 || N * a.cols <= 3 << 19);
+  const int64_t K = a.cols;
+  const bool vec = few_vec(a, b);
+  if (M <= 16) return K <= (vec ? 4608 : 2560) && N <= 32768;
+  if (M <= 32) return K <= (vec ? 2048 : 1280) && N * K <= 1 << 23;
+  return M <= 64 && K <= (vec ? 2048 : 640) && N * K <= 3 << 19;
 }
 
 int launch_few(const GemmP& p, cudaStream_t s) {

@@ -37,13 +37,11 @@ def _linear(x, weight, bias=None, activation=None, residual=None):
     return y if residual is None else y + residual
 
 
-_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
-
-
 def _plain(m: nn.Module) -> bool:
     """True for an ``nn.Linear`` that is its weight and bias and nothing else.  A replacement (an adapter, a quantised
     layer), a parametrised layer or one with hooks runs through its own call."""
-    return type(m) is nn.Linear and "forward" not in m.__dict__ and not any(getattr(m, h) for h in _HOOKS)
+    return type(m) is nn.Linear and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                                         or "forward" in m.__dict__)
 
 
 def _project(m: nn.Module, x, activation=None, residual=None):
