@@ -286,7 +286,9 @@ __device__ __noinline__ void box_copy_in(char* box, int lane, const bf16* p, int
   __syncwarp();
 }
 
-template <int BN, bool AMN, bool BMN, bool PAIR>
+// SLOPE: the forward of a training step, which keeps the activation's slopes.  (As a form of its own: with a choice at run time the
+// bare products took 2 % longer.)
+template <int BN, bool AMN, bool BMN, bool PAIR, bool SLOPE>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap my,
                 const __grid_constant__ CUtensorMap mpre, const __grid_constant__ CUtensorMap mres, const GemmP p) {
@@ -499,7 +501,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = 0; i < 16; ++i) v[e][i] = act_fwd2(v[e][i], act);
         };
         auto apply_with_slope = [&](int act) {  // the slopes go to the box as they are formed
-          if (p.vec) box_ready(lane);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             uint32_t w[4];
@@ -512,13 +513,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          send(&mpre, p.pre, p.N, n0 + c);
         };
-        if (p.pre && !p.slope) put(&mpre, p.pre, p.N, n0 + c, v);
-        if (p.pre && p.slope) {
-          if (p.act == GDN_ACT_SILU) apply_with_slope(GDN_ACT_SILU);
-          if (p.act == GDN_ACT_GELU) apply_with_slope(GDN_ACT_GELU);
+        if constexpr (SLOPE) {
+          if (p.vec) box_ready(lane);
+          if (p.act == GDN_ACT_SILU)
+            apply_with_slope(GDN_ACT_SILU);
+          else
+            apply_with_slope(GDN_ACT_GELU);
+          send(&mpre, p.pre, p.N, n0 + c);
         } else {
+          if (p.pre) put(&mpre, p.pre, p.N, n0 + c, v);
           if (p.act == GDN_ACT_SILU) apply(GDN_ACT_SILU);
           if (p.act == GDN_ACT_GELU) apply(GDN_ACT_GELU);
         }
@@ -822,7 +826,7 @@ int pair_count() {
   if (c) return c - 1;
   using C = Cfg<256, true>;
   static std::atomic<unsigned long long> opted{0};
-  auto k = gemm_kernel<256, false, false, true>;
+  auto k = gemm_kernel<256, false, false, true, false>;
   int n = 0;
   if (opt_in_smem(opted, {{(const void*)k, C::SMEM}})) {
     cudaLaunchConfig_t cfg = {};
@@ -880,11 +884,11 @@ Plan plan(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-template <int BN, bool AMN, bool BMN, bool PAIR>
+template <int BN, bool AMN, bool BMN, bool PAIR, bool SLOPE>
 int launch_gemm(const GemmP& p, int pairs, cudaStream_t s) {
   using C = Cfg<BN, PAIR>;
   static std::atomic<unsigned long long> opted{0};
-  auto k = gemm_kernel<BN, AMN, BMN, PAIR>;
+  auto k = gemm_kernel<BN, AMN, BMN, PAIR, SLOPE>;
   if (!opt_in_smem(opted, {{(const void*)k, C::SMEM}})) return GDN_ERR_LAUNCH;
   CUtensorMap ma, mb, my, mpre, mres;
   const bool out = p.vec && p.splits == 1;
@@ -978,6 +982,14 @@ int align_operands(Operand* first, Operand* second, char*& ws, cudaStream_t s) {
   return ssm::launched();
 }
 
+template <bool AMN, bool BMN, bool SLOPE>
+int launch_tiles(const GemmP& p, const Plan& pl, cudaStream_t s) {
+  return pl.pairs      ? launch_gemm<256, AMN, BMN, true, SLOPE>(p, pl.pairs, s)
+         : pl.bn == 256 ? launch_gemm<256, AMN, BMN, false, SLOPE>(p, 0, s)
+         : pl.bn == 128 ? launch_gemm<128, AMN, BMN, false, SLOPE>(p, 0, s)
+                        : launch_gemm<64, AMN, BMN, false, SLOPE>(p, 0, s);
+}
+
 // C[M, N] = sum_k A B with the epilogue of p; `ws` holds plan().part bytes.
 template <bool AMN, bool BMN>
 int gemm(GemmP p, void* ws, cudaStream_t s) {
@@ -993,10 +1005,11 @@ int gemm(GemmP p, void* ws, cudaStream_t s) {
   p.part = static_cast<float*>(ws);
   p.part_tma = p.splits > 1 && p.N % 4 == 0;
   p.vec = rows16(p.y, p.ldy) && p.N % 8 == 0 && (!p.bias || ssm::aligned16(p.bias)) && (!p.res || rows16(p.res, p.ldr)) && (!p.pre || rows16(p.pre, p.N));
-  const int st = pl.pairs      ? launch_gemm<256, AMN, BMN, true>(p, pl.pairs, s)
-                 : pl.bn == 256 ? launch_gemm<256, AMN, BMN, false>(p, 0, s)
-                 : pl.bn == 128 ? launch_gemm<128, AMN, BMN, false>(p, 0, s)
-                                : launch_gemm<64, AMN, BMN, false>(p, 0, s);
+  int st;
+  if constexpr (!AMN && !BMN)
+    st = p.slope && p.splits == 1 ? launch_tiles<AMN, BMN, true>(p, pl, s) : launch_tiles<AMN, BMN, false>(p, pl, s);
+  else
+    st = launch_tiles<AMN, BMN, false>(p, pl, s);
   if (st != GDN_OK || p.splits == 1) return st;
   const int64_t g = (p.M * ((p.N + 3) / 4) + 255) / 256;
   if (g > 0x7fffffff) return GDN_ERR_SHAPE;
@@ -1012,11 +1025,11 @@ bool few_vec(const Operand& a, const Operand& b) { return a.tma && b.tma && a.co
 // again.  So the tiles take over where they save some 3 us on the device.  Few rows / tiles in us there, weights out of HBM, x in
 // L2 (N x K, aligned):
 //   16 rows: 1024 x 1024 3.1 / 7.2, 1024 x 2816 9.6 / 9.7, 1024 x 4096 12.7 / 10.4, 4096 x 4096 13.8 / 13.1, 256 x 8192 22.5 / 10.1,
-//            12288 x 2048 15.5 / 19.1, 32768 x 1024 21.0 / 18.1, 50304 x 1024 31.1 / 27.3
+//            12288 x 2048 15.5 / 19.1, 32768 x 1024 21.0 / 18.1, 50304 x 1024 31.1 / 27.3, 65536 x 64 13.0 / 8.9
 //   32 rows: 2048 x 2048 9.8 / 11.1, 4096 x 2048 10.1 / 11.1, 8192 x 1024 11.5 / 10.0, 8192 x 2048 19.4 / 11.5, 1024 x 2560 12.1 / 8.8
-//            (14.7 / 8.7 with x out of HBM too)
+//            (14.7 / 8.7 with x out of HBM too), 16384 x 512 10.9 / 8.2, 32768 x 256 13.6 / 8.8
 //   64 rows: 1024 x 1024 4.9 / 7.2, 1024 x 1536 8.1 / 9.1, 768 x 2048 9.9 / 10.7, 1024 x 2048 11.5 / 11.0 (x out of HBM: 15.7 / 11.0),
-//            2560 x 1024 12.1 / 7.9, 4096 x 4096 38.9 / 17.6
+//            2560 x 1024 12.1 / 7.9, 4096 x 4096 38.9 / 17.6, 8192 x 64 6.7 / 4.4, 16384 x 64 11.1 / 4.8
 // Rows that no vector takes (the tiles then wait for their aligned copies, the few-rows kernel loads single values):
 //   16 rows: 1001 x 2047 13.6 / 14.8, 8191 x 513 10.7 / 15.8; 32 rows: 501 x 999 10.5 / 11.0, 4095 x 1023 17.0 / 14.2,
 //            1001 x 2047 21.8 / 15.5; 64 rows: 501 x 999 19.5 / 11.2, 8191 x 513 27.6 / 15.9
@@ -1024,8 +1037,8 @@ bool use_few(int64_t M, int64_t N, const Operand& a, const Operand& b) {
   const int64_t K = a.cols;
   const bool vec = few_vec(a, b);
   if (M <= 16) return K <= (vec ? 4608 : 2560) && N <= 32768;
-  if (M <= 32) return K <= (vec ? 2048 : 1280) && N * K <= 1 << 23;
-  return M <= 64 && K <= (vec ? 2048 : 640) && N * K <= 3 << 19;
+  if (M <= 32) return K <= (vec ? 2048 : 1280) && N <= 16384 && N * K <= 1 << 23;
+  return M <= 64 && K <= (vec ? 2048 : 640) && N <= 8192 && N * K <= 3 << 19;
 }
 
 int launch_few(const GemmP& p, cudaStream_t s) {
@@ -1116,7 +1129,7 @@ int gdn_linear_fwd(const gdn_linear_args* a, void* stream) {
   p.y = static_cast<bf16*>(a->y); p.ldy = a->sy; p.pre = static_cast<bf16*>(a->pre);
   p.bias = static_cast<const bf16*>(a->bias); p.res = static_cast<const bf16*>(a->residual); p.ldr = a->sr;
   p.act = a->act;
-  p.slope = a->keep == GDN_LINEAR_KEEP_SLOPE;
+  p.slope = p.pre && a->keep == GDN_LINEAR_KEEP_SLOPE && a->act != GDN_ACT_NONE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (use_few(p.M, p.N, p.a, p.b)) return launch_few(p, s);
   char* ws = static_cast<char*>(a->workspace);

@@ -527,7 +527,8 @@ int gdn_scan_bwd(const gdn_scan_bwd_args* args, void* stream);
  * y = act(x weight^T + bias) + residual; x (M, K), weight (N, K), y and residual (M, N), bias (N), all bf16 with
  * unit last strides and fp32 accumulation, one rounding at the end.  `pre`, when not NULL, receives what the backward
  * reads (contiguous, 2 bytes a value): with keep GDN_LINEAR_KEEP_PRE x weight^T + bias in bf16, with
- * GDN_LINEAR_KEEP_SLOPE act'(x weight^T + bias) in fp16, which keeps an activation's gradient to 2^-12 of itself.  Any
+ * GDN_LINEAR_KEEP_SLOPE act'(x weight^T + bias) in fp16 (without an activation, as with GDN_LINEAR_KEEP_PRE), which keeps
+ * an activation's gradient to 2^-12 of itself.  Any
  * strides and alignment; 16-byte aligned rows are faster.
  */
 typedef enum { GDN_LINEAR_KEEP_PRE = 0, GDN_LINEAR_KEEP_SLOPE = 1 } gdn_linear_keep;
