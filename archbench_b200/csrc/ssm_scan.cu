@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4) scan_fwd_kernel(const ScanP p
   __shared__ __align__(16) float sB[TT][NP], sC[TT][NP];
   const int tid = threadIdx.x;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
-  const int seg = blockIdx.y, b = p.b0 + blockIdx.z;
+  const int seg = blockIdx.y, b = blockIdx.z;
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
   const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T), lim = min(tend, len);
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(32) scan_fwd_tiled_kernel(const ScanP p) {
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
-  const int seg = blockIdx.y, b = p.b0 + blockIdx.z;
+  const int seg = blockIdx.y, b = blockIdx.z;
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
   const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T), lim = min(tend, len);
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanP p) {
   __shared__ float sSum[NL][CH];
   const int tid = threadIdx.x;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
-  const int seg = blockIdx.y, b = p.b0 + blockIdx.z;
+  const int seg = blockIdx.y, b = blockIdx.z;
   if (seg == (REV ? 0 : p.nseg - 1)) return;  // nothing enters from here
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(32) scan_carry_tiled_kernel(const ScanP p) {
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
-  const int seg = blockIdx.y, b = p.b0 + blockIdx.z;
+  const int seg = blockIdx.y, b = blockIdx.z;
   if (seg == (REV ? 0 : p.nseg - 1)) return;  // nothing enters from here
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(STEP_THREADS) scan_step_kernel(const ScanP p) 
   const int at = (blockIdx.x * STEP_THREADS + threadIdx.x) / NL;  // a channel of row b
   const int n0 = (threadIdx.x % NL) * STEP_SL, lane = threadIdx.x % 32;
   const bool live = at < p.D && n0 < p.N;
-  const int b = p.b0 + blockIdx.y, d = live ? at : 0;
+  const int b = blockIdx.y, d = live ? at : 0;
   const int grp = p.G == 1 ? 0 : d / (p.D / p.G);
   float* hp = p.h_out + ((int64_t)b * p.D + d) * p.N + n0;
   const float* Ap = p.A + (int64_t)d * p.N + n0;
@@ -968,13 +968,13 @@ ScanP scan_params(const gdn_scan_args* a) {
 }
 
 template <typename T, bool REV>
-void launch_carry_plain(ScanP p, int nl, cudaStream_t s) {
-  for_grid_rows(p, [&](unsigned rows) {
+void launch_carry_plain(const ScanP& p, int nl, cudaStream_t s) {
+  for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) {
     const dim3 g(p.dblocks * p.G, p.nseg, rows);
-    if (nl == 2) scan_carry_kernel<T, 2, REV><<<g, SCAN_THREADS, 0, s>>>(p);
-    if (nl == 4) scan_carry_kernel<T, 4, REV><<<g, SCAN_THREADS, 0, s>>>(p);
-    if (nl == 8) scan_carry_kernel<T, 8, REV><<<g, SCAN_THREADS, 0, s>>>(p);
-    if (nl == 16) scan_carry_kernel<T, 16, REV><<<g, SCAN_THREADS, 0, s>>>(p);
+    if (nl == 2) scan_carry_kernel<T, 2, REV><<<g, SCAN_THREADS, 0, s>>>(q);
+    if (nl == 4) scan_carry_kernel<T, 4, REV><<<g, SCAN_THREADS, 0, s>>>(q);
+    if (nl == 8) scan_carry_kernel<T, 8, REV><<<g, SCAN_THREADS, 0, s>>>(q);
+    if (nl == 16) scan_carry_kernel<T, 16, REV><<<g, SCAN_THREADS, 0, s>>>(q);
   });
 }
 
@@ -985,7 +985,7 @@ int launch_carry_tiled(ScanP p, cudaStream_t s) {
   auto k = scan_carry_tiled_kernel<T, NL, SL, REV>;
   if (!opt_in_smem(opted, {{(const void*)k, K::SMEM}})) return GDN_ERR_LAUNCH;
   p.dblocks = (p.D / p.G + K::CH - 1) / K::CH;
-  for_grid_rows(p, [&](unsigned rows) { k<<<dim3(p.dblocks * p.G, p.nseg, rows), 32, K::SMEM, s>>>(p); });
+  for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) { k<<<dim3(p.dblocks * p.G, p.nseg, rows), 32, K::SMEM, s>>>(q); });
   return launched();
 }
 template <typename T, bool REV>
@@ -1022,7 +1022,7 @@ int launch_tiled(ScanP p, cudaStream_t s) {
   auto k = scan_fwd_tiled_kernel<T, NL, SL>;
   if (!opt_in_smem(opted, {{(const void*)k, K::SMEM}})) return GDN_ERR_LAUNCH;
   p.dblocks = (p.D / p.G + K::CH - 1) / K::CH;
-  for_grid_rows(p, [&](unsigned rows) { k<<<dim3(p.dblocks * p.G, p.nseg, rows), 32, K::SMEM, s>>>(p); });
+  for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) { k<<<dim3(p.dblocks * p.G, p.nseg, rows), 32, K::SMEM, s>>>(q); });
   return launched();
 }
 template <typename T>
@@ -1031,28 +1031,28 @@ int launch_tiled(const ScanP& p, cudaStream_t s) {
 }
 
 template <typename T>
-int launch_plain(ScanP p, cudaStream_t s) {
+int launch_plain(const ScanP& p, cudaStream_t s) {
   const int nl = scan_lanes(p.N);
-  for_grid_rows(p, [&](unsigned rows) {
+  for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) {
     const dim3 g(p.dblocks * p.G, p.nseg, rows);
-    if (nl == 2) scan_fwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
-    if (nl == 4) scan_fwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
-    if (nl == 8) scan_fwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
-    if (nl == 16) scan_fwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
+    if (nl == 2) scan_fwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(q);
+    if (nl == 4) scan_fwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(q);
+    if (nl == 8) scan_fwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(q);
+    if (nl == 16) scan_fwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(q);
   });
   return launched();
 }
 
 template <typename T, bool VEC>
-int launch_step(ScanP p, cudaStream_t s) {
+int launch_step(const ScanP& p, cudaStream_t s) {
   int nl = 1;
   while (nl * STEP_SL < p.N) nl *= 2;
-  for_grid_rows(p, [&](unsigned rows) {
+  for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) {
     const dim3 g((unsigned)(((int64_t)p.D * nl + STEP_THREADS - 1) / STEP_THREADS), rows);
-    if (nl == 1) scan_step_kernel<T, 1, VEC><<<g, STEP_THREADS, 0, s>>>(p);
-    if (nl == 2) scan_step_kernel<T, 2, VEC><<<g, STEP_THREADS, 0, s>>>(p);
-    if (nl == 4) scan_step_kernel<T, 4, VEC><<<g, STEP_THREADS, 0, s>>>(p);
-    if (nl == 8) scan_step_kernel<T, 8, VEC><<<g, STEP_THREADS, 0, s>>>(p);
+    if (nl == 1) scan_step_kernel<T, 1, VEC><<<g, STEP_THREADS, 0, s>>>(q);
+    if (nl == 2) scan_step_kernel<T, 2, VEC><<<g, STEP_THREADS, 0, s>>>(q);
+    if (nl == 4) scan_step_kernel<T, 4, VEC><<<g, STEP_THREADS, 0, s>>>(q);
+    if (nl == 8) scan_step_kernel<T, 8, VEC><<<g, STEP_THREADS, 0, s>>>(q);
   });
   return launched();
 }

@@ -8,6 +8,8 @@
 // time, each lane keeping the sum of one token (NL - 1 shuffles for NL tokens).
 #pragma once
 
+#include <type_traits>
+
 #include "ssm_common.cuh"
 
 namespace gdn {
@@ -29,15 +31,14 @@ struct ScanP {
   float *pD;     // backward: (B * nseg, 2, D) partial sums of dDskip and ddt_bias
   int64_t sx_b, sx_t, sdt_b, sdt_t, sB_b, sB_t, sB_g, sC_b, sC_t, sC_g, sz_b, sz_t, sy_b, sy_t, sdy_b, sdy_t;
   int B, T, D, N, G;
-  int b0;  // the launch's first row
   int softplus;
   int quads;  // rows of B and C can be loaded four states at a time
-  int ckpt_quads;  // and rows of ckpt stored so
   int nseg, seg_len;  // segments of seg_len tokens (a multiple of GDN_SCAN_CKPT)
   int dblocks;        // channel blocks per group
   int xgs;            // channels from one group to the next in x, dt, z and dy (padded copies have more than D / G)
   int tiled;          // the kernels on asynchronous tiles serve it (scan_align_plan)
   int pairs_out;      // rows of y (or dx, ddt, dz) take stores of channel pairs
+  int ckpt_quads;     // rows of ckpt take stores of four states
 };
 
 // Two neighbouring values in one store.  (Written out by type: as one struct aligned to 2 * sizeof(T) the compiler ordered the
@@ -121,11 +122,26 @@ __device__ __forceinline__ int spread_sum(float (&v)[NV], int lane) {
   return first;
 }
 
-// Rows are the last dimension of a grid, which ends at 65535: launch(rows) with p.b0 set, as often as it takes.
+// Rows are the last dimension of a grid, which ends at 65535: launch(q, rows) with q moved on to the next rows, as often as it
+// takes.  (A first row that the kernels add cost them up to 7 % by another order of their instructions.)
 template <typename F>
-void for_grid_rows(ScanP& p, F launch) {
+void for_grid_rows(const ScanP& p, int es, F launch) {
   constexpr int MOST = 65535;
-  for (p.b0 = 0; p.b0 < p.B; p.b0 += MOST) launch((unsigned)(p.B - p.b0 < MOST ? p.B - p.b0 : MOST));
+  ScanP q = p;
+  for (int64_t b = 0; b < p.B; b += MOST) {
+    if (b) {
+      auto token = [&](auto*& t, int64_t step) { if (t) t = (std::remove_reference_t<decltype(t)>)((const char*)t + MOST * step * es); };
+      auto state = [&](auto*& t, int64_t step) { if (t) t += MOST * step; };
+      const int64_t td = (int64_t)p.T * p.D, dn = (int64_t)p.D * p.N, sdn = p.nseg * dn, sd = (int64_t)p.nseg * p.D;
+      token(q.x, p.sx_b); token(q.dt, p.sdt_b); token(q.Bm, p.sB_b); token(q.Cm, p.sC_b); token(q.z, p.sz_b); token(q.dy, p.sdy_b);
+      token(q.y, p.sy_b); token(q.dx, td); token(q.ddt, td); token(q.dz, td);
+      state(q.h0, dn); state(q.dh_out, dn); state(q.h_out, dn); state(q.dh0, dn); state(q.lengths, 1);
+      state(q.ckpt, (p.T + GDN_SCAN_CKPT - 1) / GDN_SCAN_CKPT * dn);
+      state(q.carry, sdn); state(q.ssum, sd); state(q.pA, sdn); state(q.pD, 2 * sd);
+      state(q.pBC, (int64_t)p.T * p.G * 2 * p.N);  // its rows lie p.B apart still
+    }
+    launch(q, (unsigned)(p.B - b < MOST ? p.B - b : MOST));
+  }
 }
 
 // Segments of time, each at least MIN_SEG tokens.

@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(ScanP p) {
   __shared__ float sR[WARPS][CK][2 * NP];    // dB, dC of each warp's channels
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
-  const int seg = blockIdx.y, b = p.b0 + blockIdx.z;
+  const int seg = blockIdx.y, b = blockIdx.z;
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
   const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T);
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) scan_bwd_tiled_kernel(const S
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int grp = blockIdx.x / p.dblocks, dblk = blockIdx.x % p.dblocks;
-  const int seg = blockIdx.y, b = p.b0 + blockIdx.z;
+  const int seg = blockIdx.y, b = blockIdx.z;
   const int dpg = p.D / p.G, d0 = grp * dpg + dblk * CH, nch = min(CH, dpg - dblk * CH);
   const int len = row_tokens(p.lengths, b, p.T);
   const int tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, p.T), lim = min(tend, len);
@@ -676,12 +676,12 @@ ScanP bwd_params(const gdn_scan_bwd_args* a) {
 }
 
 template <typename T, int NL>
-int launch_bwd_tiled(ScanP p, cudaStream_t s) {
+int launch_bwd_tiled(const ScanP& p, cudaStream_t s) {
   using K = BwdTiled<T, NL>;
   static std::atomic<unsigned long long> opted{0};
   auto k = scan_bwd_tiled_kernel<T, NL>;
   if (!opt_in_smem(opted, {{(const void*)k, K::SMEM}})) return GDN_ERR_LAUNCH;
-  for_grid_rows(p, [&](unsigned rows) { k<<<dim3(p.dblocks * p.G, p.nseg, rows), SCAN_THREADS, K::SMEM, s>>>(p); });
+  for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) { k<<<dim3(p.dblocks * p.G, p.nseg, rows), SCAN_THREADS, K::SMEM, s>>>(q); });
   return launched();
 }
 
@@ -696,12 +696,12 @@ int launch_bwd(ScanP p, const gdn_scan_bwd_args* a, cudaStream_t s) {
   if (tiled) {
     st = nl == 2 ? launch_bwd_tiled<T, 2>(p, s) : nl == 4 ? launch_bwd_tiled<T, 4>(p, s) : nl == 8 ? launch_bwd_tiled<T, 8>(p, s) : launch_bwd_tiled<T, 16>(p, s);
   } else {
-    for_grid_rows(p, [&](unsigned rows) {
+    for_grid_rows(p, sizeof(T), [&](const ScanP& q, unsigned rows) {
       const dim3 g(p.dblocks * p.G, p.nseg, rows);
-      if (nl == 2) scan_bwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(p);
-      if (nl == 4) scan_bwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(p);
-      if (nl == 8) scan_bwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(p);
-      if (nl == 16) scan_bwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(p);
+      if (nl == 2) scan_bwd_kernel<T, 2><<<g, SCAN_THREADS, 0, s>>>(q);
+      if (nl == 4) scan_bwd_kernel<T, 4><<<g, SCAN_THREADS, 0, s>>>(q);
+      if (nl == 8) scan_bwd_kernel<T, 8><<<g, SCAN_THREADS, 0, s>>>(q);
+      if (nl == 16) scan_bwd_kernel<T, 16><<<g, SCAN_THREADS, 0, s>>>(q);
     });
     st = launched();
   }

@@ -85,3 +85,29 @@ def test_unserved_sizes_raise_value_errors():
         ops.causal_conv(z, w)
     with pytest.raises(ValueError):
         ops.selective_scan_step(z[0], z[0], A, x[0], x[0], torch.zeros(1, 2 ** 24 + 1, 1, device="cuda"))
+
+
+@pytest.mark.parametrize("N", [5, 8])
+def test_scan_of_three_grids_of_rows(N):
+    """Every launch past the first starts at its own rows: bf16, the plain and the tiled kernels, two groups, odd strides."""
+    B, T, D = 2 * 65535 + 70, 1, 4
+    g = torch.Generator("cuda").manual_seed(N)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    tok = lambda *s: rnd(*s[:-1], s[-1] + 3).bfloat16()[..., 1:1 + s[-1]]
+    v = [tok(B, T, D), tok(B, T, D), -torch.rand(D, N, generator=g, device="cuda") - 0.1, tok(B, T, 2, N), tok(B, T, 2, N), rnd(D), tok(B, T, D), rnd(D), rnd(B, D, N)]
+    n = torch.randint(0, T + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    dy, dh = tok(B, T, D), rnd(B, D, N)
+    a, b = [t.detach().requires_grad_() for t in v], [t.double().cpu().requires_grad_() for t in v]
+    run = lambda f, ts, **kw: f(*ts[:5], ts[5], ts[6], ts[7], True, ts[8], **kw)
+    oa = run(ops.selective_scan, a, output_final_state=True, lengths=n)
+    ob = run(R.scan, b, lengths=n)
+    for p, q in zip(oa, ob):
+        R.close(p, q, "out", accumulated=128 + N)
+    ga, gb = torch.autograd.grad(oa, a, [dy, dh]), torch.autograd.grad(ob, b, [dy.double().cpu(), dh.double().cpu()])
+    for i, (p, q) in enumerate(zip(ga, gb)):
+        R.close(p, q, str(i), accumulated=256 + (B * T if i in (2, 5, 7) else D if i in (3, 4) else 0))
+    h = v[8].clone()
+    y = ops.selective_scan_step(v[0][:, 0], v[1][:, 0], v[2], v[3][:, 0], v[4][:, 0], h, D=v[5], z=v[6][:, 0], dt_bias=v[7], dt_softplus=True)
+    y0, h0 = run(R.scan, [t.detach() for t in b])
+    R.close(y, y0[:, 0], "step", accumulated=128)
+    R.close(h, h0, "step state", accumulated=128)
