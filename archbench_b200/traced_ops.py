@@ -77,6 +77,8 @@ _conv.register_autograd(_conv_backward, setup_context=_conv_setup)
 
 
 def causal_conv(x, weight, bias=None, activation=None, initial_state=None, output_final_state=False, lengths=None):
+    if weight.dim() == 3 and weight.shape[1] != 1:
+        raise ValueError(f"weight must be (C, W) or (C, 1, W), got {tuple(weight.shape)}")
     w = weight[:, 0] if weight.dim() == 3 else weight
     y, last = _conv(x, w, _to(bias, w.dtype), _to(initial_state, x.dtype), lengths, activation, bool(output_final_state))
     return y, last if output_final_state else None
@@ -205,7 +207,11 @@ _linear.register_autograd(_linear_backward, setup_context=_linear_setup)
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"x must be (..., K) and weight (N, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
     N, K = weight.shape
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+        raise ValueError(f"residual must be {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
     rows = lambda t, n: None if t is None else t.reshape(-1, n)  # noqa: E731
     args = (rows(x, K), weight, bias, rows(residual, N))
     y, _ = _linear(*args, activation, _wants_grad(*args))

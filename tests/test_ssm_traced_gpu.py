@@ -152,3 +152,16 @@ def test_plain_calls_after_tracing_keep_their_parameters():
         again = torch.cat([m(x[:, :3], cache), m(x[:, 3:4], cache), m(x[:, 4:], cache)], 1)
     assert not torch.equal(before, after)
     assert ((again - after).norm() <= 1e-5 * after.norm()).item()
+
+
+def test_traced_calls_refuse_what_plain_ones_refuse():
+    """Shapes that the registered forms bring to their own first: a mismatch must not be reshaped away."""
+    x, w = rnd(1, 4, 16, dtype=torch.bfloat16), rnd(2, 8, 16, dtype=torch.bfloat16)
+    c, k = rnd(3, 2, 5, 8), rnd(4, 8, 2, 4)
+    bad = [("linear", (x, w[:, :8])), ("linear", (x, w, None, None, rnd(5, 8, 4, dtype=torch.bfloat16))), ("linear", (x, w[0])),
+           ("linear", (x.float(), w.float())), ("linear", (x, w, None, "relu")), ("causal_conv", (c, k)), ("causal_conv", (c, k[:, 0], None, "gelu")),
+           ("selective_scan", (c, c[:, :3], -rnd(6, 8, 4).abs(), c[..., :4], c[..., :4]))]
+    for name, args in bad:
+        for fn in (getattr(ops, name), getattr(traced_ops, name)):
+            with pytest.raises(ValueError):
+                fn(*args)
