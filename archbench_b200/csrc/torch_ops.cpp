@@ -173,7 +173,7 @@ variable_list conv_backward(const Tensor& x, const Tensor& w, const Tensor& bias
                             Tensor dy, Tensor dlast) {
   const c10::cuda::OptionalCUDAGuard guard(x.device());
   if (x.numel() == 0)
-    return {zeros_like_dense(x), zeros_like_dense(w), zeros_like_dense(bias), !state.defined() ? Tensor() : dlast.defined() ? dlast : zeros_like_dense(state)};
+    return {zeros_like_dense(x), zeros_like_dense(w), zeros_like_dense(bias), !state.defined() ? Tensor() : dlast.defined() ? dlast.clone() : zeros_like_dense(state)};
   dy = dy.defined() ? token(dy, "dy", x.sizes(), x.scalar_type(), x.get_device()) : at::zeros(x.sizes(), x.options());
   if (dlast.defined()) dlast = dlast.contiguous();
   variable_list out = {empty_like_dense(x), empty_like_dense(w), empty_like_dense(bias), empty_like_dense(state)};
@@ -320,7 +320,7 @@ variable_list scan_backward(const ScanIn& s, const Tensor& ckpt, Tensor dy, Tens
   variable_list out(9);
   if (x.numel() == 0) {
     for (int i = 0; i < 8; ++i) out[i] = zeros_like_dense(in[i]);
-    out[8] = !s.h0.defined() ? Tensor() : dh.defined() ? dh : zeros_like_dense(s.h0);
+    out[8] = !s.h0.defined() ? Tensor() : dh.defined() ? dh.clone() : zeros_like_dense(s.h0);
     return out;
   }
   dy = dy.defined() ? token(dy, "dy", x.sizes(), x.scalar_type(), x.get_device()) : at::zeros(x.sizes(), x.options());

@@ -165,3 +165,23 @@ def test_traced_calls_refuse_what_plain_ones_refuse():
         for fn in (getattr(ops, name), getattr(traced_ops, name)):
             with pytest.raises(ValueError):
                 fn(*args)
+
+
+@pytest.mark.parametrize("B,T", [(0, 5), (2, 0)])
+def test_traced_calls_without_tokens(B, T):
+    """No outputs to compute, but gradients that pass through: of the state as its own tensor, zeros for the rest."""
+    for m in (ops, traced_ops):
+        x, w, s = (torch.zeros(*shape, device="cuda", requires_grad=True) for shape in ((B, T, 8), (8, 4), (B, 8, 3)))
+        y, last = m.causal_conv(x, w, None, "silu", s, True)
+        d = torch.full_like(last, 2.0)
+        gx, gw, gs = torch.autograd.grad([y, last], [x, w, s], [torch.zeros_like(y), d])
+        assert gx.shape == x.shape and torch.equal(gw, torch.zeros_like(w)) and torch.equal(gs, d)
+        A, h = -torch.ones(8, 4, device="cuda"), torch.zeros(B, 8, 4, device="cuda", requires_grad=True)
+        Bm = torch.zeros(B, T, 4, device="cuda")
+        y, last = m.selective_scan(x, x, A, Bm, Bm, initial_state=h, output_final_state=True)
+        d = torch.full_like(last, 3.0)
+        gx, gh = torch.autograd.grad([y, last], [x, h], [torch.zeros_like(y), d])
+        assert gx.shape == x.shape and torch.equal(gh, d)
+        v, wl = torch.zeros(B * T, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True), torch.ones(8, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        gv, gw = torch.autograd.grad(m.linear(v, wl, None, "gelu").sum(), [v, wl])
+        assert gv.shape == v.shape and torch.equal(gw, torch.zeros_like(wl))
