@@ -37,11 +37,11 @@ def _linear(x, weight, bias=None, activation=None, residual=None):
     return y if residual is None else y + residual
 
 
-def _plain(m: nn.Module) -> bool:
-    """True for an ``nn.Linear`` that is its weight and bias and nothing else.  A replacement (an adapter, a quantised
-    layer), a parametrised layer or one with hooks runs through its own call."""
-    return type(m) is nn.Linear and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
-                                         or "forward" in m.__dict__)
+def _plain(m: nn.Module, kind: type = nn.Linear) -> bool:
+    """True for an ``nn.Linear`` (``nn.Conv1d``) that is its weight and bias and nothing else.  A replacement (an adapter, a
+    quantised layer), a parametrised layer or one with hooks runs through its own call."""
+    return type(m) is kind and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                                or "forward" in m.__dict__)
 
 
 def _project(m: nn.Module, x, activation=None, residual=None):
@@ -98,24 +98,35 @@ class SelectiveSSM(nn.Module):
         return (ops._cached(self.A_log, "neg_exp", lambda t: -torch.exp(t.float())), ops._cached(self.D, "f32", lambda t: t.float()),
                 None if bias is None else ops._cached(bias, "f32", lambda t: t.float()))
 
+    def _convolve(self, u: torch.Tensor, cache: Optional[GDNCache], one: bool) -> torch.Tensor:
+        """silu(conv1d(u)) from the cache's last inputs, which move on; ``one``: in place."""
+        c, state = self.conv1d, None if cache is None else cache.conv.get("x")
+        if _plain(c, nn.Conv1d):
+            weight, bias = c.weight.to(u.dtype), None if c.bias is None else c.bias.to(u.dtype)
+            if one:
+                return ops.causal_conv_step(u[:, 0], weight, state, bias, "silu")[:, None]
+            y, last = ops.causal_conv(u, weight, bias, "silu", state, cache is not None)
+        else:  # it pads conv_size - 1 inputs on both sides, as the nn.Conv1d does
+            W, T = self.conv_size, u.shape[1]
+            past = u.new_zeros(u.shape[0], u.shape[2], W - 1) if state is None else state.to(u.dtype)
+            inputs = torch.cat([past, u.transpose(1, 2)], -1)
+            y = F.silu(c(inputs)[..., W - 1:W - 1 + T]).transpose(1, 2)
+            last = inputs[..., T:].contiguous()
+        if cache is not None:
+            _put(cache, "x", last)
+        return y
+
     def forward(self, x: torch.Tensor, cache: Optional[GDNCache] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if cache is None:
             cache = self.bound_cache
         x = _activations(x)
-        T, R, N = x.shape[1], self.dt_rank, self.state_size
-        A, D, dt_bias = self._parameters_f32(_training(x, self))
-        conv_w = self.conv1d.weight.to(x.dtype)
-        conv_b = None if self.conv1d.bias is None else self.conv1d.bias.to(x.dtype)
+        T, R, N, train = x.shape[1], self.dt_rank, self.state_size, _training(x, self)
+        A, D, dt_bias = self._parameters_f32(train)
         # the one-token forms have no gradient; where one is wanted one token takes the prompt's
         one = cache is not None and cache.state is not None and T == 1 and (
-            cache.static or not (_training(x, self) or torch.is_grad_enabled() and cache.state.requires_grad))
+            cache.static or not (train or torch.is_grad_enabled() and cache.state.requires_grad))
         u, z = _project(self.in_proj, x).chunk(2, -1)
-        if one:
-            u = ops.causal_conv_step(u[:, 0], conv_w, cache.conv["x"], conv_b, "silu")[:, None]
-        else:
-            u, last = ops.causal_conv(u, conv_w, conv_b, "silu", None if cache is None else cache.conv.get("x"), cache is not None)
-            if cache is not None:
-                _put(cache, "x", last)
+        u = self._convolve(u, cache, one)
         r, B, C = _project(self.x_proj, u).split([R, N, N], -1)
         # a plain projection's bias is added to the step sizes inside the scan, in fp32
         dt = _linear(r, self.dt_proj.weight) if dt_bias is not None else self.dt_proj(r)

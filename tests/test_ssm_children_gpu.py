@@ -100,3 +100,43 @@ def test_adapted_mixer_decodes_what_it_prefills():
         want, cache = m(x), GDNCache()
         got = torch.cat([m(x[:, :5], cache)] + [m(x[:, t:t + 1], cache) for t in range(5, 9)], 1)
     assert ((got - want).norm() <= 1e-5 * want.norm()).item()
+
+
+class Scaled(nn.Module):
+    """A convolution that is more than its weight."""
+
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return 2 * self.base(x)
+
+
+@pytest.mark.parametrize("how", ["replaced", "hooked", "parametrised"])
+def test_convolution_of_another_kind(how):
+    torch.manual_seed(9)
+    m = SelectiveSSM(64).cuda()
+    want = copy.deepcopy(m)
+    with torch.no_grad():
+        want.conv1d.weight.mul_(2)
+        if how != "parametrised":
+            want.conv1d.bias.mul_(2)
+    if how == "replaced":
+        m.conv1d = Scaled(m.conv1d)
+    elif how == "hooked":
+        m.conv1d.register_forward_hook(lambda mod, args, out: 2 * out)
+    else:
+        parametrize.register_parametrization(m.conv1d, "weight", Doubled())
+    x = rnd(10, 3, 9, 64)
+    with torch.no_grad():
+        a, b, cache = want(x), m(x), GDNCache()
+        c = torch.cat([m(x[:, :1], cache), m(x[:, 1:5], cache)] + [m(x[:, t:t + 1], cache) for t in range(5, 9)], 1)
+    for got in (b, c):
+        assert ((got - a).norm() <= 1e-5 * a.norm()).item()
+    ga = torch.autograd.grad(want(x).sum(), want.in_proj.weight)[0]
+    gb = torch.autograd.grad(m(x).sum(), m.in_proj.weight)[0]
+    assert ((ga - gb).norm() <= 1e-5 * ga.norm()).item()
